@@ -1,0 +1,885 @@
+// Sliding-window attention with sinks, forward and backward.
+//
+// Query i of a sequence of len tokens sees key j when
+//   j < len,  j <= i + right  and  (j >= i - left  or  j < sinks):
+// a band around the diagonal and the first tokens, which stay visible to every later
+// query.  o = sum_j p_ij v_j with p = softmax(scale q.k) over the visible keys, lse
+// its log-sum; tokens at or past len give o = 0 and lse = -inf.  Backward, with
+// delta = o . dO:  P = exp(scale q.k - lse),  dS = P (dO V^T - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO.
+//
+// The walk of a workgroup is arithmetic, not a list: the 64-key tiles of the sinks,
+// then those of its rows' band.  Per wave and tile the mask is one of three cases,
+// told apart by scalar compares: nothing visible (skipped), everything (no mask), or
+// a per-lane range test at the band's two edges.
+//
+// Nothing that no query of the workgroup sees is read: DMA rows outside the sinks and
+// the band are taken from a visible row instead (their scores are masked), so tokens
+// past len, and whatever they hold, cannot reach a result.
+#include "fta_common.h"
+#include "fta_host.h"
+#include "fta_tile.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+
+struct WinArgs {
+    const uint16_t *q, *k, *v, *o, *dout;
+    int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn, d_sb, d_sh, d_sn;
+    uint16_t *out0, *out1;  // o (forward), dq, or dk and dv
+    int64_t o0_sb, o0_sh, o0_sn, o1_sb, o1_sh, o1_sn;
+    const int32_t* lens;  // [B] or null
+    float* lse;           // [B][H][N]: forward output, backward input
+    float *lse2, *delta;  // [B][H][N] workspace: lse * log2(e) and delta, from dQ to dK / dV
+    float* part;          // dK / dV parts
+    int B, N, H, Hk, G, Dreal;
+    int left, right, sinks;
+    float c, scale;
+    int hw;               // forward, dQ: query heads per workgroup (they share K / V)
+    int tiles;            // forward, dQ: token tiles per head; dK / dV: 64-key tiles
+    int ts, nps, np;      // dK / dV: tiles that hold sinks, parts of each of them, parts of the others
+    int total;
+    bool kv_narrow, q_narrow, d_narrow;  // token strides that 32-bit lane offsets span
+};
+
+__device__ __forceinline__ int seq_len(const WinArgs& a, int b) {
+    return a.lens ? __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.N)) : a.N;
+}
+
+// The 64-key tiles that rows [i_lo, i_hi] see: `ns` tiles of sinks, then the band's.
+struct WinWalk {
+    int kb0, ke;   // the band's keys [kb0, ke)
+    int ns, c_lo, iters;
+    __device__ __forceinline__ WinWalk(const WinArgs& a, int len, int i_lo, int i_hi) {
+        kb0 = max(0, i_lo - a.left);
+        ke = min(len, i_hi + a.right + 1);
+        const int c_hi = (ke + 63) >> 6;
+        c_lo = kb0 >> 6;
+        ns = (min(a.sinks, ke) + 63) >> 6;
+        if (c_lo <= ns) c_lo = ns = 0;
+        iters = ns + c_hi - c_lo;
+    }
+    __device__ __forceinline__ int key(int it) const { return 64 * (it < ns ? it : c_lo + it - ns); }
+    // whether all 64 rows of the tile at kb are keys that the workgroup sees
+    __device__ __forceinline__ bool whole(const WinArgs& a, int kb) const {
+        return kb + 64 <= ke && (kb >= kb0 || kb + 64 <= a.sinks);
+    }
+    // a key that the workgroup sees in place of one that it does not
+    __device__ __forceinline__ int seen(const WinArgs& a, int t) const {
+        return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t;
+    }
+};
+
+// Mask case of the tile at kb for rows [i0, i0 + 31]: 0 nothing, 1 partly, 2 all visible.
+__device__ __forceinline__ int tile_case(const WinArgs& a, int len, int i0, int kb) {
+    const int i1 = min(i0 + 31, len - 1);
+    if (i0 >= len || kb > i1 + a.right || (kb + 63 < i0 - a.left && kb >= a.sinks)) return 0;
+    if (kb + 63 <= i0 + a.right && kb + 63 < len && (kb >= i0 + 31 - a.left || kb + 63 < a.sinks)) return 2;
+    return 1;
+}
+
+// -inf for the scores of 32 keys (tile row of register r: rel0 + c_row) that row i does not see.
+__device__ __forceinline__ void mask_scores(const WinArgs& a, int len, int i, int kb, int rel0, int lane, f32x16& s) {
+    const int hi = min(i + a.right, len - 1) - kb - rel0, lo = i - a.left - kb - rel0, sk = a.sinks - kb - rel0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int rel = c_row(r, lane);
+        s[r] = (rel <= hi && (rel >= lo || rel < sk)) ? s[r] : -FTA_INF;
+    }
+}
+
+// Workgroup -> (b, head group, token tile); late tiles first: without a window they walk the most keys.
+struct WinPlace {
+    int b, h, hk, i0, i_lo, tok;  // batch, this wave's query head, its K/V head, its first row; the workgroup's first row, rows
+    __device__ __forceinline__ WinPlace(const WinArgs& a, int nw, int wave) {
+        const int wgi = fta_xcd_remap(blockIdx.x, a.total);
+        const int groups = a.H / a.hw;
+        const int bg = fta_scalar(wgi / a.tiles), tile = a.tiles - 1 - (wgi - bg * a.tiles);
+        const int wt = fta_scalar(wave / a.hw);
+        b = fta_scalar(bg / groups);
+        h = (bg - b * groups) * a.hw + wave - wt * a.hw;
+        hk = fta_scalar(h / a.G);
+        tok = 32 * fta_scalar(nw / a.hw);
+        i_lo = tile * tok;
+        i0 = i_lo + 32 * wt;
+    }
+};
+
+// Stages of the forward and dQ: 64-key K and V tiles in LDS, NST - 1 ahead.  Eight
+// waves take the LDS of three stages (two workgroups share a CU at D = 64), four
+// waves two stages, so that more of these smaller workgroups fit.
+template <int D, int NW>
+struct WinShape {
+    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 2>::TEN_B;
+    static constexpr int NST = (NW == 8) ? 3 : 2;
+    static constexpr int PDK = D <= 64 ? 3 : 6, PDV = D <= 64 ? 2 : 4;
+};
+// waves per SIMD that the registers leave room for
+constexpr int win_fwd_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
+constexpr int win_dq_waves(int D) { return D <= 128 ? 2 : 1; }
+
+// ----------------------------------------------------------------------------
+// Forward.  NW waves of 32 rows: hw query heads that share a K/V head, NW / hw row
+// tiles each.
+// ----------------------------------------------------------------------------
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(NW * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
+    using T = FtaTile<DT, D, 2>;
+    using Sh = WinShape<D, NW>;
+    constexpr int NST = Sh::NST, LQ = FtaGather<D, NW, 64>::LQ;
+    __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const WinPlace p(a, NW, wave);
+    const int len = seq_len(a, p.b);
+    const int row = p.i0 + (lane & 31);
+    uint16_t* out = a.out0 + p.b * a.o0_sb + p.h * a.o0_sh + (int64_t)row * a.o0_sn;
+    float* lse = a.lse + ((int64_t)p.b * a.H + p.h) * a.N;
+
+    f32x16 oacc[T::DT32];
+#pragma unroll
+    for (int dt = 0; dt < T::DT32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
+    float m_run = -FTA_INF, l_run = 0.f;
+
+    if (p.i_lo < len) {  // workgroup-uniform
+        const uint16_t* kp = a.k + p.b * a.k_sb + p.hk * a.k_sh;
+        const uint16_t* vp = a.v + p.b * a.v_sb + p.hk * a.v_sh;
+        uint4 qf[T::KS];
+        T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, row < len, a.Dreal, lane, qf);
+        const WinWalk w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        FtaGather<D, NW, 64> g;
+        g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
+        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
+        const auto lo = T::lane_offsets(lane);
+        auto issue = [&](int it, int st) {
+            const int kb = w.key(it);
+            const uint32_t lds = lds0 + st * Sh::STAGE_B;
+            if (a.kv_narrow && w.whole(a, kb))
+                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds, wave);
+            else
+                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+        };
+        fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
+#pragma unroll
+        for (int k = 0; k < NST - 1; ++k)
+            if (k < w.iters) issue(k, k);
+        int cur = 0;
+        for (int it = 0; it < w.iters; ++it) {
+            if (it + NST - 2 < w.iters)
+                fta_wait_vmcnt<2 * LQ * (NST - 2)>();
+            else
+                fta_wait_vmcnt<0>();
+            __syncthreads();  // tile `it` visible; every wave is past tile it - 1
+            if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
+            const int kb = w.key(it);
+            const int mc = tile_case(a, len, p.i0, kb);
+            if (mc != 0) {
+                const uint32_t kbase = lds0 + cur * Sh::STAGE_B;
+                f32x16 s[2];
+                T::template qk<Sh::PDK>(kbase, lo, qf, s);
+                if (mc == 1) {
+                    mask_scores(a, len, row, kb, 0, lane, s[0]);
+                    mask_scores(a, len, row, kb, 32, lane, s[1]);
+                }
+                T::template softmax_pv<Sh::PDV>(kbase + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
+            }
+            cur = (cur == NST - 1) ? 0 : cur + 1;
+        }
+    }
+
+    const float L = l_run + fta_xor32(l_run);
+    if (row >= a.N) return;
+    const bool live = row < len;
+    if (lane < 32) lse[row] = live ? fmaf(m_run, a.c, fta_log2(L)) * kLn2 : -FTA_INF;
+    if (!live) {  // a padding row: exact zeros, whatever the registers hold
+#pragma unroll
+        for (int dt = 0; dt < T::DT32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
+    }
+    T::store_row(out, a.Dreal, lane, oacc, live ? 1.f / L : 0.f);
+}
+
+// ----------------------------------------------------------------------------
+// dQ, with the forward's walk: S^T and dP^T = V dO^T of 32 keys at a time,
+// dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
+// rows are at hand) and the lse in log2 units for dK / dV.
+// ----------------------------------------------------------------------------
+template <int DT, int D, int NW>
+__global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
+    using E = Elem<DT>;
+    using T = FtaTile<DT, D, 2>;
+    using Sh = WinShape<D, NW>;
+    constexpr int NST = Sh::NST, LQ = FtaGather<D, NW, 64>::LQ, KS = T::KS;
+    __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const WinPlace p(a, NW, wave);
+    const int len = seq_len(a, p.b);
+    const int row = p.i0 + (lane & 31);
+    const bool live = row < len;
+
+    f32x16 acc[T::DT32];
+#pragma unroll
+    for (int dt = 0; dt < T::DT32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+    if (p.i_lo < len) {  // workgroup-uniform
+        const uint16_t* kp = a.k + p.b * a.k_sb + p.hk * a.k_sh;
+        const uint16_t* vp = a.v + p.b * a.v_sb + p.hk * a.v_sh;
+        uint4 qf[KS], df[KS];
+        T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, live, a.Dreal, lane, qf);
+        T::load_rows(a.dout + p.b * a.d_sb + p.h * a.d_sh + (int64_t)row * a.d_sn, live, a.Dreal, lane, df);
+        float dl = 0.f, lse2 = FTA_INF;  // a padding row: every exp is exactly 0
+        {
+            const uint16_t* op = a.o + p.b * a.o_sb + p.h * a.o_sh + (int64_t)row * a.o_sn;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const int d = ks * 16 + (lane >> 5) * 8;
+                const uint4 of = (live && d < a.Dreal) ? *reinterpret_cast<const uint4*>(op + d) : fta_zero4();
+                const uint32_t x[4] = {of.x, of.y, of.z, of.w}, y[4] = {df[ks].x, df[ks].y, df[ks].z, df[ks].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dl = fmaf(E::to_f32((uint16_t)(x[e] & 0xffffu)), E::to_f32((uint16_t)(y[e] & 0xffffu)), dl);
+                    dl = fmaf(E::to_f32((uint16_t)(x[e] >> 16)), E::to_f32((uint16_t)(y[e] >> 16)), dl);
+                }
+            }
+            dl += fta_xor32(dl);
+            if (live) {
+                const int64_t at = ((int64_t)p.b * a.H + p.h) * a.N + row;
+                lse2 = a.lse[at] * kLog2e;
+                if (lane < 32) {
+                    a.delta[at] = dl;
+                    a.lse2[at] = lse2;
+                }
+            }
+        }
+        const WinWalk w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        FtaGather<D, NW, 64> g;
+        g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
+        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
+        const auto lo = T::lane_offsets(lane);
+        auto issue = [&](int it, int st) {
+            const int kb = w.key(it);
+            const uint32_t lds = lds0 + st * Sh::STAGE_B;
+            if (a.kv_narrow && w.whole(a, kb))
+                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds, wave);
+            else
+                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+        };
+        fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream
+#pragma unroll
+        for (int k = 0; k < NST - 1; ++k)
+            if (k < w.iters) issue(k, k);
+        int cur = 0;
+        for (int it = 0; it < w.iters; ++it) {
+            if (it + NST - 2 < w.iters)
+                fta_wait_vmcnt<2 * LQ * (NST - 2)>();
+            else
+                fta_wait_vmcnt<0>();
+            __syncthreads();  // tile `it` visible; every wave is past tile it - 1
+            if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
+            const int kb = w.key(it);
+            const int mc = tile_case(a, len, p.i0, kb);
+            if (mc != 0) {
+                const uint32_t kbase = lds0 + cur * Sh::STAGE_B, vbase = kbase + T::TEN_B;
+                uint4 dsf[4];
+#pragma unroll
+                for (int sb = 0; sb < 2; ++sb) {
+                    f32x16 s, dp;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+                    uint4 kf[2], vf[2];  // fragments one MFMA pair ahead
+                    kf[0] = T::row_frag(kbase, lo, sb, 0);
+                    vf[0] = T::row_frag(vbase, lo, sb, 0);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        if (ks + 1 < KS) {
+                            kf[(ks + 1) & 1] = T::row_frag(kbase, lo, sb, ks + 1);
+                            vf[(ks + 1) & 1] = T::row_frag(vbase, lo, sb, ks + 1);
+                        }
+                        s = E::mma(kf[ks & 1], qf[ks], s);
+                        dp = E::mma(vf[ks & 1], df[ks], dp);
+                    }
+                    if (mc == 1) mask_scores(a, len, row, kb, 32 * sb, lane, s);
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        float ds[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int i = 8 * k2 + e;
+                            ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
+                        }
+                        dsf[2 * sb + k2] =
+                            make_uint4(E::pack2(ds[0], ds[1]), E::pack2(ds[2], ds[3]), E::pack2(ds[4], ds[5]), E::pack2(ds[6], ds[7]));
+                    }
+                }
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+                    for (int dt = 0; dt < T::DT32; ++dt) acc[dt] = E::mma(T::tr_frag(kbase, lo, ks, dt), dsf[ks], acc[dt]);
+            }
+            cur = (cur == NST - 1) ? 0 : cur + 1;
+        }
+    }
+    if (row < a.N)
+        T::store_row(a.out0 + p.b * a.o0_sb + p.h * a.o0_sh + (int64_t)row * a.o0_sn, a.Dreal, lane, acc, a.scale);
+}
+
+// ----------------------------------------------------------------------------
+// dK / dV.  A workgroup owns 64 keys of one K/V head and walks the 32-query chunks
+// that see any of them, through all query heads of the group in one sequence, so
+// the sums over shared heads need neither atomics nor a second pass.  Wave (tt, 0)
+// holds K of 32-key tile tt and accumulates dV, wave (tt, 1) holds V and accumulates
+// dK one chunk behind; P crosses in fp32 through LDS:
+//   wave (tt, 0):  S = Q K^T,  P = 2^{c S - lse2}  -> LDS;  dV += P^T dO
+//   wave (tt, 1):  dP = dO V^T;  dS = P (dP - delta);  dK += dS^T Q
+// One barrier per step; Q two steps ahead in four tiles, dO in three.
+//
+// The tiles that hold sinks are seen by every later query: their walks are cut into
+// nps parts as long as the other tiles' walks, and on small grids every walk into np
+// parts; parts write fp32 sums that fta_window_dkv_combine_kernel adds in order.
+// ----------------------------------------------------------------------------
+template <int D>
+struct WinDkvShape {
+    static constexpr int NW = 4, NTHR = 256, QSEG = D / 8;
+    static constexpr int LQ = 32 * QSEG / NTHR;  // DMA instructions per wave and 32-row tile
+    static constexpr int TILE_B = 32 * QSEG * 16;
+    static constexpr int NQ = 4, ND = 3;
+    static constexpr int WPC = (D <= 64) ? 3 : (D <= 128) ? 2 : 1;  // workgroups per CU
+    static_assert((32 * QSEG) % NTHR == 0, "whole DMA instructions per wave");
+    static_assert((NQ + ND) * TILE_B + NQ * 256 + 2 * 2 * 32 * 32 * 4 + 64 <= 160 * 1024 / WPC, "WPC workgroups per CU");
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kernel(WinArgs a) {
+    using E = Elem<DT>;
+    using Sh = WinDkvShape<D>;
+    constexpr int NW = Sh::NW, QSEG = Sh::QSEG, LQ = Sh::LQ, TILE_B = Sh::TILE_B;
+    using SW = FtaSwz<QSEG>;
+    constexpr int KS = D / 16, DT32 = D / 32;
+    __shared__ __align__(1024) unsigned char sQ[Sh::NQ][TILE_B];
+    __shared__ __align__(1024) unsigned char sD[Sh::ND][TILE_B];
+    __shared__ __align__(1024) float sL[Sh::NQ][64];  // [lse of entry k, delta of entry k - 1] at k % 4
+    __shared__ float4 sX[2][2][4][64];                // [step parity][tile][i / 4][lane]: P of the last two steps
+
+    const int wgi = fta_xcd_remap(blockIdx.x, a.total);
+    const int per = a.ts * a.nps + (a.tiles - a.ts) * a.np;  // workgroups per (b, K/V head)
+    const int bhk = fta_scalar(wgi / per), slot = wgi - bhk * per;
+    const bool sink = slot < a.ts * a.nps;
+    const int parts = sink ? a.nps : a.np;
+    const int off = sink ? slot : slot - a.ts * a.nps;
+    const int tp = fta_scalar(off / parts);
+    const int tile = sink ? tp : a.ts + tp;
+    const int sp = off - tp * parts;
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = seq_len(a, b);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int hf = lane >> 5;
+    const int tt = wave & 1;
+    const bool hv = (wave >> 1) != 0;  // wave-uniform role: false = K / P / dV, true = V / dS / dK
+
+    const int kb = 64 * tile, kt = kb + 32 * tt;  // first key of the workgroup, of this wave's tile
+    const int key = kt + (lane & 31);             // this lane's column
+    const bool kok = key < len;
+
+    // entries [s0, s0 + U) of the sequence (query head, chunk of 32 queries)
+    int c_lo = 0, nch = 0;
+    if (kb < len) {
+        c_lo = max(0, kb - a.right) >> 5;
+        const int i_hi = kb < a.sinks ? len - 1 : min(len - 1, min(kb + 63, len - 1) + a.left);
+        nch = (i_hi >> 5) + 1 - c_lo;
+    }
+    const int all = a.G * nch;
+    const int s0 = fta_scalar((int)((int64_t)all * sp / parts));
+    const int U = fta_scalar((int)((int64_t)all * (sp + 1) / parts)) - s0;
+
+    uint4 kv[KS];  // K (role 0) or V (role 1) rows of this tile
+    {
+        const uint16_t* src = hv ? a.v + b * a.v_sb + hk * a.v_sh + (int64_t)key * a.v_sn
+                                 : a.k + b * a.k_sb + hk * a.k_sh + (int64_t)key * a.k_sn;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const int d = ks * 16 + hf * 8;
+            kv[ks] = (kok && d < a.Dreal) ? *reinterpret_cast<const uint4*>(src + d) : fta_zero4();
+        }
+    }
+    fta_wait_vmcnt<0>();  // complete the register loads: the DMAs are invisible to the compiler
+
+    uint32_t qoff[LQ], doff[LQ];
+#pragma unroll
+    for (int i = 0; i < LQ; ++i) {
+        const int r2 = (i * NW + wave) * 64 + lane;
+        const int row = r2 / QSEG;
+        int j = SW::slot(row, r2 - row * QSEG);
+        if (j * 8 >= a.Dreal) j = 0;  // columns past D: any finite data (never stored)
+        qoff[i] = 2u * (row * (uint32_t)a.q_sn + j * 8);
+        doff[i] = 2u * (row * (uint32_t)a.d_sn + j * 8);
+    }
+    const bool l_isd = (lane & 32) != 0;  // wave 0's DMA writes [lse2 32][delta 32]
+    const uint32_t aro = 2u * SW::off(lane & 31, hf);
+    const int br = 4 * hf + ((lane & 15) >> 2), bc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    const uint32_t bro = 2u * (SW::off(br, bc >> 3) + (bc & 7));
+    const uint32_t bro8 = 2u * (SW::off(br + 8, bc >> 3) + (bc & 7)) - bro;  // added: rows + 8
+    const uint32_t ldq = fta_lds_addr(&sQ[0][0]), ldd = fta_lds_addr(&sD[0][0]), ldl = fta_lds_addr(&sL[0][0]);
+    const uint16_t* q0 = a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
+    const uint16_t* d0 = a.dout + b * a.d_sb + (int64_t)hk * a.G * a.d_sh;
+    const int64_t r0 = ((int64_t)b * a.H + (int64_t)hk * a.G) * a.N;
+
+    // the rest runs in one copy per role, so each keeps only its own values live
+    auto run = [&](auto role) {
+        constexpr bool HV = decltype(role)::value;
+        f32x16 acc[DT32];  // dV (role 0) or dK / scale (role 1): rows = keys, lane column = d
+#pragma unroll
+        for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
+
+        if (U > 0) {
+            auto tile_dma = [&](const uint16_t* base, int64_t sn, bool narrow, const uint32_t* o, int c, uint32_t lds)
+                __attribute__((always_inline)) {
+                const int t0 = 32 * c;
+                if (narrow && t0 + 32 <= len) {
+                    const uint16_t* bp = base + (int64_t)t0 * sn;
+#pragma unroll
+                    for (int i = 0; i < LQ; ++i) fta_dma16_so(bp, o[i], lds + (i * NW + wave) * 1024);
+                } else {  // the sequence's last chunk repeats its last row (masked)
+                    int ln = lane;
+                    asm volatile("" : "+v"(ln));
+#pragma unroll
+                    for (int i = 0; i < LQ; ++i) {
+                        const int r2 = (i * NW + wave) * 64 + ln;
+                        const int row = r2 / QSEG;
+                        int j = SW::slot(row, r2 - row * QSEG);
+                        if (j * 8 >= a.Dreal) j = 0;
+                        const int64_t t = min(t0 + row, len - 1);
+                        fta_dma16_at(base + t * sn + j * 8, lds + (i * NW + wave) * 1024);
+                    }
+                }
+            };
+            struct Entry {
+                int g, c;
+            };
+            // entry s (past the end: the last one again, so every step issues the same number)
+            const int last = s0 + U - 1;
+            auto next = [&](Entry e, int s) __attribute__((always_inline)) {
+                if (s > last) return e;
+                return e.c + 1 < c_lo + nch ? Entry{e.g, e.c + 1} : Entry{e.g + 1, c_lo};
+            };
+            // step k - 2's gathers: Q and lse of entry eq (number kq), dO and delta of entry ed (kq - 1)
+            auto issue = [&](int kq, int dslot, Entry eq, Entry ed) __attribute__((always_inline)) {
+                tile_dma(q0 + eq.g * a.q_sh, a.q_sn, a.q_narrow, qoff, eq.c, ldq + (kq & 3) * TILE_B);
+                tile_dma(d0 + ed.g * a.d_sh, a.d_sn, a.d_narrow, doff, ed.c, ldd + dslot * TILE_B);
+                if (wave == 0) {
+                    const int t = min(32 * (l_isd ? ed.c : eq.c) + (lane & 31), len - 1);
+                    const float* src = (l_isd ? a.delta : a.lse2) + r0 + (int64_t)(l_isd ? ed.g : eq.g) * a.N;
+                    fta_dma4_at(src + t, ldl + (kq & 3) * 256);
+                }
+            };
+            // mask case of chunk c for this wave's keys
+            auto mcase = [&](int c) __attribute__((always_inline)) {
+                const int i0 = 32 * c;
+                if (kt >= len || i0 + 31 < kt - a.right || (i0 > kt + 31 + a.left && kt >= a.sinks)) return 0;
+                if (i0 >= kt + 31 - a.right && i0 + 31 < len && kt + 31 < len && (i0 + 31 <= kt + a.left || kt + 31 < a.sinks))
+                    return 2;
+                return 1;
+            };
+            const int g0 = fta_scalar(s0 / nch);
+            const Entry first{g0, c_lo + s0 - g0 * nch};
+            Entry e1 = first;
+            int mk = mcase(first.c), mkp = 0, ck = first.c;
+            issue(0, 2, e1, e1);
+            Entry e2 = next(e1, s0 + 1);
+            issue(1, 0, e2, e1);
+            e1 = e2;                   // entry k + 1
+            e2 = next(e1, s0 + 2);     // entry k + 2
+            int ds = 2;                // dO slot of entry k - 1
+            uint4 af[2];               // role 0: P_{k-1}, A operand of dV_{k-1}
+            for (int k = 0; k <= U; ++k) {
+                // step k - 2's gathers complete (wave 0 issues the lse / delta DMA as well)
+                if (wave == 0)
+                    fta_wait_vmcnt<2 * LQ + 1>();
+                else
+                    fta_wait_vmcnt<2 * LQ>();
+                // Q_k, dO_{k-1} and P_{k-1} visible; the slots of Q_{k-2}, dO_{k-2} and sX[k & 1] free
+                __syncthreads();
+                issue(k + 2, ds == 0 ? 2 : ds - 1, e2, e1);
+                const float* ld = &sL[k & 3][0];
+                const uint32_t dbase = ldd + ds * TILE_B;
+                if constexpr (!HV) {
+                    const uint32_t qb = ldq + (k & 3) * TILE_B + aro, ob = dbase + bro;
+                    if (mkp == 0) af[0] = af[1] = fta_zero4();
+                    // S_k (a dependent chain) interleaved with dV_{k-1} (independent MFMAs).
+                    // One instruction stream for every case: without a pending accumulation P is
+                    // zero and dO any finite tile; without a chain the S result is discarded.
+                    if (mk | mkp) {
+                        f32x16 own;  // S_k then P_k
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) own[i] = 0.f;
+                        uint4 fs[2], fa2[2];
+                        auto load = [&](int j, int sl) {
+                            fs[sl] = fta_lds_b128(qb ^ (j * 32));
+                            const uint32_t x = (j / DT32) * 16 * QSEG * 16;
+                            fa2[sl] = fta_lds_tr((ob ^ ((j % DT32) * 64)) + x, ((ob + bro8) ^ ((j % DT32) * 64)) + x);
+                        };
+                        load(0, 0);
+#pragma unroll
+                        for (int j = 0; j < KS; ++j) {  // KS = 2 * DT32: one accumulation MFMA per chain link
+                            if (j + 1 < KS) load(j + 1, (j + 1) & 1);
+                            own = E::mma(fs[j & 1], kv[j], own);
+                            acc[j % DT32] = E::mma(af[j / DT32], fa2[j & 1], acc[j % DT32]);
+                        }
+                        __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+                        for (int j = 0; j < KS; ++j) {
+                            if (j + 1 < KS) __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+                        }
+                        if (mk) {  // P_k = 2^{c S_k - lse2}: to LDS for role 1, packed for dV_k
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) own[i] = fta_exp2(fmaf(own[i], a.c, -ld[c_row(i, lane)]));
+                            if (mk == 1) {  // the lane's key is seen by rows [rlo, rhi] of the chunk
+                                const int rlo = key - a.right - 32 * ck;
+                                const int rhi = (kok ? min(key < a.sinks ? len - 1 : key + a.left, len - 1) : -1) - 32 * ck;
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) {
+                                    const int r = c_row(i, lane);
+                                    own[i] = (r >= rlo && r <= rhi) ? own[i] : 0.f;
+                                }
+                            }
+#pragma unroll
+                            for (int i = 0; i < 16; i += 4)
+                                sX[k & 1][tt][i / 4][lane] = make_float4(own[i], own[i + 1], own[i + 2], own[i + 3]);
+#pragma unroll
+                            for (int ks = 0; ks < 2; ++ks)
+                                af[ks] = make_uint4(E::pack2(own[8 * ks], own[8 * ks + 1]),
+                                                    E::pack2(own[8 * ks + 2], own[8 * ks + 3]),
+                                                    E::pack2(own[8 * ks + 4], own[8 * ks + 5]),
+                                                    E::pack2(own[8 * ks + 6], own[8 * ks + 7]));
+                        }
+                    }
+                } else if (mkp) {
+                    const uint32_t ob = dbase + aro, qb = ldq + ((k + 3) & 3) * TILE_B + bro;
+                    f32x16 dpv;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dpv[i] = 0.f;
+                    {
+                        constexpr int PD = 3;
+                        uint4 fr[PD + 1];
+                        auto load = [&](auto nn) __attribute__((always_inline)) {
+                            constexpr int n = decltype(nn)::value;
+                            if constexpr (n < KS) fr[n % (PD + 1)] = fta_lds_b128(ob ^ (n * 32));
+                        };
+                        auto slot_ = [&](auto nn) __attribute__((always_inline)) {
+                            constexpr int n = decltype(nn)::value;
+                            load(std::integral_constant<int, n + PD>{});
+                            dpv = E::mma(fr[n % (PD + 1)], kv[n], dpv);
+                        };
+                        fta_static_for<0, PD>(load);
+                        fta_static_for<0, KS>(slot_);
+                    }
+                    uint4 ds2[2];  // dS = P (dP - delta)
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        float dv8[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e += 4) {
+                            const int i = 8 * ks + e;
+                            const float4 pr = sX[(k + 1) & 1][tt][i / 4][lane];
+                            const float4 dl = *reinterpret_cast<const float4*>(ld + 32 + c_row(i, lane));
+                            dv8[e] = pr.x * (dpv[i] - dl.x);
+                            dv8[e + 1] = pr.y * (dpv[i + 1] - dl.y);
+                            dv8[e + 2] = pr.z * (dpv[i + 2] - dl.z);
+                            dv8[e + 3] = pr.w * (dpv[i + 3] - dl.w);
+                        }
+                        ds2[ks] = make_uint4(E::pack2(dv8[0], dv8[1]), E::pack2(dv8[2], dv8[3]), E::pack2(dv8[4], dv8[5]),
+                                             E::pack2(dv8[6], dv8[7]));
+                    }
+                    {
+                        constexpr int PD = 3;
+                        uint4 fr[PD + 1];
+                        auto load = [&](auto nn) __attribute__((always_inline)) {
+                            constexpr int n = decltype(nn)::value;
+                            if constexpr (n < KS) {
+                                constexpr int x = (n / DT32) * 16 * QSEG * 16;
+                                fr[n % (PD + 1)] = fta_lds_tr((qb ^ ((n % DT32) * 64)) + x, ((qb + bro8) ^ ((n % DT32) * 64)) + x);
+                            }
+                        };
+                        auto slot_ = [&](auto nn) __attribute__((always_inline)) {
+                            constexpr int n = decltype(nn)::value;
+                            load(std::integral_constant<int, n + PD>{});
+                            acc[n % DT32] = E::mma(ds2[n / DT32], fr[n % (PD + 1)], acc[n % DT32]);
+                        };
+                        fta_static_for<0, PD>(load);
+                        fta_static_for<0, KS>(slot_);
+                    }
+                }
+                mkp = mk;
+                mk = (k + 1 < U) ? mcase(e1.c) : 0;
+                ck = e1.c;
+                e1 = e2;
+                e2 = next(e2, s0 + k + 3);
+                ds = (ds == 2) ? 0 : ds + 1;
+            }
+            fta_wait_vmcnt<0>();  // the gathers past the walk's end
+        }
+
+        // C layout: lane column = d, rows = keys c_row(i, lane); role 0 stores dV, role 1 dK
+        if (parts > 1) {
+            float* po = a.part + ((((int64_t)(HV ? 0 : 1) * a.B * a.Hk + bhk) * (a.np > 1 ? per : a.ts * a.nps) + slot) * 64 + 32 * tt) * D;
+#pragma unroll
+            for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) po[(int64_t)c_row(i, lane) * D + dt * 32 + (lane & 31)] = acc[dt][i];
+            return;
+        }
+        uint16_t* out = HV ? a.out0 + b * a.o0_sb + hk * a.o0_sh : a.out1 + b * a.o1_sb + hk * a.o1_sh;
+        const int64_t osn = HV ? a.o0_sn : a.o1_sn;
+        const float osc = HV ? a.scale : 1.f;
+#pragma unroll
+        for (int dt = 0; dt < DT32; ++dt) {
+            const int d = dt * 32 + (lane & 31);
+            if (d >= a.Dreal) continue;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int t = kt + c_row(i, lane);
+                if (t < a.N) out[(int64_t)t * osn + d] = (uint16_t)(E::pack2(acc[dt][i] * osc, 0.f) & 0xffffu);
+            }
+        }
+    };
+    if (hv)
+        run(std::true_type{});
+    else
+        run(std::false_type{});
+}
+
+// Sum of the dK / dV parts, added in order: one thread per (tensor, b, K/V head, key
+// of a tile with parts, 8 columns); dK takes the scale here.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, int keys) {
+    using E = Elem<DT>;
+    constexpr int DC = D / 8;
+    const int64_t per = (int64_t)a.B * a.Hk * keys * DC;
+    int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (idx >= 2 * per) return;
+    const int ten = idx >= per;  // 0: dK, 1: dV
+    idx -= ten * per;
+    const int d0 = (int)(idx % DC) * 8;
+    const int64_t rest = idx / DC;
+    const int t = (int)(rest % keys), bhk = (int)(rest / keys);
+    if (d0 >= a.Dreal) return;
+    const int tile = t >> 6;
+    const int slots = a.ts * a.nps + (a.np > 1 ? (a.tiles - a.ts) * a.np : 0);
+    const int n = tile < a.ts ? a.nps : a.np;
+    const int first = tile < a.ts ? tile * a.nps : a.ts * a.nps + (tile - a.ts) * a.np;
+    if (n <= 1) return;  // written by the kernel itself
+    const float* src = a.part + ((((int64_t)ten * a.B * a.Hk + bhk) * slots + first) * 64 + (t & 63)) * D + d0;
+    float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < n; ++p, src += 64 * D) {
+        const float4 x0 = *reinterpret_cast<const float4*>(src);
+        const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
+        o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
+        o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
+    }
+    const float f = ten ? 1.f : a.scale;
+    const int b = bhk / a.Hk, hk = bhk - b * a.Hk;
+    uint16_t* op = ten ? a.out1 + b * a.o1_sb + hk * a.o1_sh + (int64_t)t * a.o1_sn + d0
+                       : a.out0 + b * a.o0_sb + hk * a.o0_sh + (int64_t)t * a.o0_sn + d0;
+    *reinterpret_cast<uint4*>(op) = make_uint4(E::pack2(o[0] * f, o[1] * f), E::pack2(o[2] * f, o[3] * f),
+                                               E::pack2(o[4] * f, o[5] * f), E::pack2(o[6] * f, o[7] * f));
+}
+
+// ---------------------------------------------------------------------- host
+
+int kernel_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+bool narrow(int64_t sn) { return sn >= 0 && sn <= (1 << 24); }
+
+// Arguments that forward and backward share; the window is clamped to the sequence.
+int win_common(WinArgs& a, const void* q, const int64_t* qs, const void* k, const int64_t* ks, const void* v,
+               const int64_t* vs, int dtype, int B, int H, int Hk, int N, int D, const int32_t* lens, int left, int right,
+               int sinks, float scale) {
+    if (B <= 0 || H <= 0 || Hk <= 0 || N <= 0 || D <= 0) return fta::arg_error("window_attn: dims must be positive");
+    if (H % Hk != 0) return fta::arg_error("window_attn: num_heads must be a multiple of num_kv_heads");
+    if (D % 16 != 0 || D > 256) return fta::arg_error("window_attn: D must be a multiple of 16 up to 256");
+    if (left < 0 || right < 0 || sinks < 0) return fta::arg_error("window_attn: window and num_sinks must be non-negative");
+    if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("window_attn: scale must be positive and finite");
+    if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("window_attn: dtype must be bf16 or fp16");
+    if (N > (1 << 29)) return fta::unsupported("window_attn: more than 2^29 tokens");
+    a = WinArgs{};
+    a.q = (const uint16_t*)q, a.q_sb = qs[0], a.q_sh = qs[1], a.q_sn = qs[2];
+    a.k = (const uint16_t*)k, a.k_sb = ks[0], a.k_sh = ks[1], a.k_sn = ks[2];
+    a.v = (const uint16_t*)v, a.v_sb = vs[0], a.v_sh = vs[1], a.v_sn = vs[2];
+    a.lens = lens;
+    a.B = B, a.N = N, a.H = H, a.Hk = Hk, a.G = H / Hk, a.Dreal = D;
+    a.left = std::min(left, N), a.right = std::min(right, N);
+    a.sinks = a.left >= N - 1 ? 0 : std::min(sinks, N);  // a window of everything has no sinks left
+    a.scale = scale;
+    a.c = scale * kLog2e;
+    a.kv_narrow = narrow(a.k_sn) && narrow(a.v_sn);
+    a.q_narrow = narrow(a.q_sn);
+    return FTA_OK;
+}
+
+// Query heads per workgroup of nw waves: as many of a K/V head's as divide both.
+int heads_per_wg(int G, int nw) {
+    int hw = 1;
+    while (hw * 2 <= nw && G % (hw * 2) == 0) hw *= 2;
+    return hw;
+}
+
+// Grid of the forward and dQ for workgroups of nw waves.
+int64_t row_grid(WinArgs& a, int nw) {
+    a.hw = heads_per_wg(a.G, nw);
+    const int tok = 32 * (nw / a.hw);
+    a.tiles = (a.N + tok - 1) / tok;
+    return (int64_t)a.B * (a.H / a.hw) * a.tiles;
+}
+
+template <int DT, int D>
+int launch_rows(WinArgs& a, bool dq, hipStream_t st) {
+    constexpr int NWL = D <= 128 ? 8 : 4;
+    int64_t grid = row_grid(a, NWL);
+    const bool small = NWL == 8 && grid < 512;
+    if (small) grid = row_grid(a, 4);
+    if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    a.total = (int)grid;
+    const dim3 g((unsigned)grid);
+    if (small) {
+        if (dq)
+            hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, 4>), g, dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_window_fwd_kernel<DT, D, 4>), g, dim3(256), 0, st, a);
+    } else {
+        if (dq)
+            hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, NWL>), g, dim3(NWL * 64), 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_window_fwd_kernel<DT, D, NWL>), g, dim3(NWL * 64), 0, st, a);
+    }
+    return fta::check_launch(dq ? "fta_window_dq_kernel" : "fta_window_fwd_kernel");
+}
+
+// Parts of the dK / dV walks.  Small grids (fewer workgroups than the chip holds) cut
+// every walk into up to 4; the tiles with sinks get parts as long as the other walks.
+void dkv_parts(WinArgs& a, int Dk) {
+    a.tiles = (a.N + 63) / 64;
+    a.ts = (a.sinks + 63) / 64;
+    const int64_t wgs = (int64_t)a.tiles * a.B * a.Hk, cap = 256 * (Dk <= 64 ? 3 : Dk <= 128 ? 2 : 1);
+    const int64_t nall = (a.N + 31) / 32;
+    const int64_t steps = a.G * std::min<int64_t>(nall, ((int64_t)64 + a.left + a.right + 31) / 32 + 1);
+    int64_t np = wgs >= cap ? 1 : std::min<int64_t>(4, cap / wgs);
+    np = std::max<int64_t>(1, std::min<int64_t>(np, steps / 4));
+    a.np = (int)np;
+    const int64_t own = std::max<int64_t>(8, steps / np);
+    a.nps = a.ts == 0 ? 1 : (int)std::max<int64_t>(np, std::min<int64_t>(128, (a.G * nall + own - 1) / own));
+}
+
+int64_t dkv_slots(const WinArgs& a) {
+    return (a.nps > 1 ? (int64_t)a.ts * a.nps : 0) + (a.np > 1 ? (int64_t)(a.tiles - a.ts) * a.np : 0);
+}
+size_t rows_bytes(int B, int H, int N) { return fta::align_up((size_t)B * H * N * sizeof(float)); }
+size_t part_bytes(const WinArgs& a, int Dk) {
+    return fta::align_up((size_t)2 * a.B * a.Hk * dkv_slots(a) * 64 * Dk * sizeof(float));
+}
+
+template <int DT, int D>
+int launch_dkv(WinArgs& a, hipStream_t st) {
+    const int64_t grid = ((int64_t)a.ts * a.nps + (int64_t)(a.tiles - a.ts) * a.np) * a.B * a.Hk;
+    if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    a.total = (int)grid;
+    hipLaunchKernelGGL((fta_window_dkv_kernel<DT, D>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    int rc = fta::check_launch("fta_window_dkv_kernel");
+    if (rc != FTA_OK || (a.np <= 1 && (a.ts == 0 || a.nps <= 1))) return rc;
+    const int keys = a.np > 1 ? a.N : std::min(a.N, a.ts * 64);
+    const int64_t threads = 2 * (int64_t)a.B * a.Hk * keys * (D / 8);
+    if ((threads + 255) / 256 > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    hipLaunchKernelGGL((fta_window_dkv_combine_kernel<DT, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a,
+                       keys);
+    return fta::check_launch("fta_window_dkv_combine_kernel");
+}
+
+template <typename F>
+int with_shape(int dtype, int D, F f) {
+    auto dim = [&](auto dt) {
+        switch (kernel_dim(D)) {
+            case 64: return f(dt, std::integral_constant<int, 64>{});
+            case 128: return f(dt, std::integral_constant<int, 128>{});
+            default: return f(dt, std::integral_constant<int, 256>{});
+        }
+    };
+    return dtype == FTA_DTYPE_BF16 ? dim(std::integral_constant<int, FTA_DTYPE_BF16>{})
+                                   : dim(std::integral_constant<int, FTA_DTYPE_F16>{});
+}
+
+}  // namespace
+
+extern "C" {
+
+int fta_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, int dtype, int B, int H, int Hk, int N, int D, const int32_t* seq_lens,
+                        int left, int right, int num_sinks, float scale, void* o, const int64_t* o_strides, float* lse,
+                        void* stream) {
+    FTA_TRY_BEGIN
+    WinArgs a;
+    int rc = win_common(a, q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, N, D, seq_lens, left, right,
+                        num_sinks, scale);
+    if (rc != FTA_OK) return rc;
+    a.out0 = (uint16_t*)o, a.o0_sb = o_strides[0], a.o0_sh = o_strides[1], a.o0_sn = o_strides[2];
+    a.lse = lse;
+    return with_shape(dtype, D, [&](auto dt, auto dk) {
+        return launch_rows<decltype(dt)::value, decltype(dk)::value>(a, false, (hipStream_t)stream);
+    });
+    FTA_TRY_END
+}
+
+size_t fta_window_attn_bwd_workspace_size(int B, int H, int Hk, int N, int D, int left, int right, int num_sinks) {
+    const int64_t none[3] = {0, 0, 0};
+    WinArgs a;
+    if (win_common(a, nullptr, none, nullptr, none, nullptr, none, FTA_DTYPE_BF16, B, H, Hk, N, D, nullptr, left, right,
+                   num_sinks, 1.f) != FTA_OK)
+        return 0;
+    dkv_parts(a, kernel_dim(D));
+    return 2 * rows_bytes(B, H, N) + part_bytes(a, kernel_dim(D));
+}
+
+int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const void* o, const int64_t* o_strides, const void* dout,
+                        const int64_t* do_strides, int dtype, int B, int H, int Hk, int N, int D, const int32_t* seq_lens,
+                        int left, int right, int num_sinks, float scale, const float* lse, void* dq,
+                        const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                        const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream) {
+    FTA_TRY_BEGIN
+    WinArgs a;
+    int rc = win_common(a, q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, N, D, seq_lens, left, right,
+                        num_sinks, scale);
+    if (rc != FTA_OK) return rc;
+    if (workspace == nullptr || workspace_bytes < fta_window_attn_bwd_workspace_size(B, H, Hk, N, D, left, right, num_sinks))
+        return fta::arg_error("window_attn_bwd: workspace too small");
+    a.o = (const uint16_t*)o, a.o_sb = o_strides[0], a.o_sh = o_strides[1], a.o_sn = o_strides[2];
+    a.dout = (const uint16_t*)dout, a.d_sb = do_strides[0], a.d_sh = do_strides[1], a.d_sn = do_strides[2];
+    a.d_narrow = narrow(a.d_sn);
+    a.lse = const_cast<float*>(lse);
+    a.lse2 = (float*)workspace;
+    a.delta = (float*)((char*)workspace + rows_bytes(B, H, N));
+    a.part = (float*)((char*)workspace + 2 * rows_bytes(B, H, N));
+    hipStream_t st = (hipStream_t)stream;
+    // dQ first: it leaves delta and the lse in log2 units for dK / dV
+    a.out0 = (uint16_t*)dq, a.o0_sb = dq_strides[0], a.o0_sh = dq_strides[1], a.o0_sn = dq_strides[2];
+    rc = with_shape(dtype, D, [&](auto dt, auto dkk) {
+        return launch_rows<decltype(dt)::value, decltype(dkk)::value>(a, true, st);
+    });
+    if (rc != FTA_OK) return rc;
+    a.out0 = (uint16_t*)dk, a.o0_sb = dk_strides[0], a.o0_sh = dk_strides[1], a.o0_sn = dk_strides[2];
+    a.out1 = (uint16_t*)dv, a.o1_sb = dv_strides[0], a.o1_sh = dv_strides[1], a.o1_sn = dv_strides[2];
+    dkv_parts(a, kernel_dim(D));
+    return with_shape(dtype, D, [&](auto dt, auto dkk) { return launch_dkv<decltype(dt)::value, decltype(dkk)::value>(a, st); });
+    FTA_TRY_END
+}
+
+}  // extern "C"

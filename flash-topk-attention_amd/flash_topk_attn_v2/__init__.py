@@ -5,6 +5,12 @@ Drop-in for the public API of the reference package ``flash_topk_attn_v2``
 ``build_qblock_topk_indices`` and ``flash_topk_attn`` (differentiable), with
 the same signatures, argument checks and return conventions.  All compute runs
 in hand-written HIP kernels (libfta_gfx950.so, C ABI in include/fta.h).
+
+Beside it, without counterpart in the reference, what a model puts around such
+attention: ``flash_qk_norm_rope`` in front of it, ``flash_window_attn`` for its local
+layers (both differentiable), and the serving forms over K/V caches
+``flash_qk_norm_rope_append``, ``flash_window_attn_decode`` and
+``flash_prefix_attn_decode``.
 """
 
 from __future__ import annotations
@@ -16,10 +22,13 @@ import torch.nn.functional as F
 
 from . import _lib
 from .block_score import _parse_block_score_args, _prepare_qk, flash_block_score
+from .cache_attn import flash_prefix_attn_decode
 from .qblock_merge import flash_qblock_merge
+from .qk_prep import flash_qk_norm_rope, flash_qk_norm_rope_append
 from .sparse_attn import FlashSparseAttnFunc, flash_sparse_attn
 from .sparse_attn_bwd import flash_build_reverse_indices, flash_sort_by_count, preprocess_delta
 from .topk_select import flash_topk_select
+from .window_attn import flash_window_attn, flash_window_attn_decode
 
 
 def flash_topk_score(
@@ -227,4 +236,9 @@ __all__ = [
     "preprocess_delta",
     "flash_build_reverse_indices",
     "flash_sort_by_count",
+    "flash_qk_norm_rope",
+    "flash_qk_norm_rope_append",
+    "flash_window_attn",
+    "flash_window_attn_decode",
+    "flash_prefix_attn_decode",
 ]

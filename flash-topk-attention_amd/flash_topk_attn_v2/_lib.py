@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from contextlib import nullcontext
 from functools import lru_cache
 from typing import Sequence
 
@@ -22,6 +23,7 @@ FTA_ERR_UNSUPPORTED = 2
 FTA_ERR_HIP = 3
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
+DTYPE_F32 = 2  # norm weights only
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
@@ -71,6 +73,21 @@ _SIGNATURES = {
     "fta_sparse_attn_bwd_noalloc": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p,
                                          _i, _i, _i, _i, _i, _i, _i, _i, _f, _p, _p, _p, _i64p, _p, _i64p, _p,
                                          _i64p, _p]),
+    "fta_qk_norm_rope": (_i, [_p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i, _i, _p, _i64, _f,
+                              _i, _p, _i64p, _p, _i64p, _p]),
+    "fta_qk_norm_rope_bwd_workspace_size": (_sz, [_i] * 5),
+    "fta_qk_norm_rope_bwd": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p,
+                                  _p, _i, _i, _p, _i64, _f, _i, _p, _i64p, _p, _i64p, _p, _p, _p, _sz, _p]),
+    "fta_qk_norm_rope_append": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
+                                     _i, _i, _f, _i, _p, _i, _p, _i64p, _p, _i64p, _p, _i64p, _p]),
+    "fta_window_attn_fwd": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _i, _i, _i, _f, _p,
+                                 _i64p, _p, _p]),
+    "fta_window_attn_bwd_workspace_size": (_sz, [_i] * 8),
+    "fta_window_attn_bwd": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p,
+                                 _i, _i, _i, _f, _p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _sz, _p]),
+    "fta_cache_attn_workspace_size": (_sz, [_i] * 9),
+    "fta_cache_attn": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _i64p, _p, _i64p, _i,
+                            _i, _i, _f, _p, _i64p, _p, _p, _sz, _p]),
 }
 
 
@@ -135,6 +152,34 @@ def dtype_code(dt: torch.dtype) -> int:
     if dt == torch.float16:
         return DTYPE_F16
     raise ValueError(f"unsupported dtype {dt}; expected bfloat16 or float16")
+
+
+def on_device(device: torch.device):
+    """Context in which ``device`` is the current one (launches go to the current device)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return nullcontext()
+    return torch.cuda.device(device)
+
+
+def check_tensors(what: str, device: torch.device, **tensors) -> None:
+    """Every given tensor has to be on ``device`` (None is skipped)."""
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+
+
+def head_counts(what: str, width: int, num_heads: int, num_kv_heads):
+    """``(H, Hk, D)`` of a ``[..., H * D]`` tensor, checked."""
+    H = int(num_heads)
+    if H <= 0 or width % H != 0 or width == 0:
+        raise ValueError(f"{what}: C ({width}) must be a positive multiple of num_heads ({H})")
+    Hk = H if num_kv_heads is None else int(num_kv_heads)
+    if Hk <= 0 or H % Hk != 0:
+        raise ValueError(f"{what}: num_heads ({H}) must be a positive multiple of num_kv_heads ({Hk})")
+    D = width // H
+    if D % 16 != 0 or D > 256:
+        raise ValueError(f"{what}: D ({D}) must be a multiple of 16 up to 256")
+    return H, Hk, D
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -41,6 +41,7 @@ extern "C" {
 
 #define FTA_DTYPE_BF16 0
 #define FTA_DTYPE_F16 1
+#define FTA_DTYPE_F32 2 /* norm weights and their gradients only */
 
 /* Message of the last failing call on this thread ("" if none). */
 const char* fta_last_error(void);
@@ -418,6 +419,102 @@ int fta_sparse_attn_bwd_noalloc(const void* q, const int64_t* q_strides, const v
                                 const float* delta, void* dq, const int64_t* dq_strides, void* dk,
                                 const int64_t* dk_strides, void* dv, const int64_t* dv_strides,
                                 void* stream);
+
+/* ---------------------------------------------------------------- queries and keys */
+
+/*
+ * Norm of every head and rotation by position in one pass (no counterpart in the
+ * reference: its callers prepare q and k by separate torch operations).  A row is one
+ * head of one token: x r w with r = 1 / sqrt(mean(x^2) + eps), then the first R
+ * columns turned pair by pair -- columns (i, i + R/2), or (2i, 2i + 1) with
+ * interleaved != 0 -- by the angle whose cos and sin are row `position` of the fp32
+ * tables cos, sin [P][R/2] (16-byte aligned rows).  positions [B][N] (int32, batch
+ * stride positions_stride_b, unit token stride) or null (the token's index, N <= P);
+ * values outside [0, P) are clamped into it.  q_weight, k_weight [D] of weight_dtype
+ * (bf16, fp16 or fp32) or null (ones).  D a multiple of 16 up to 256, R a multiple of
+ * 16 up to D, eps > 0.  Everything is formed in fp32 and rounded once.
+ */
+int fta_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype, int B,
+                     int H, int Hk, int N, int D, const void* q_weight, const void* k_weight, int weight_dtype,
+                     const float* cos, const float* sin, int P, int R, const int32_t* positions,
+                     int64_t positions_stride_b, float eps, int interleaved, void* q_out, const int64_t* qo_strides,
+                     void* k_out, const int64_t* ko_strides, void* stream);
+
+/*
+ * Backward of fta_qk_norm_rope from q, k and the gradients of its outputs.
+ * dq_weight / dk_weight [D] of weight_dtype may be null; with either the workspace
+ * (fta_qk_norm_rope_bwd_workspace_size bytes) holds the workgroups' partial sums, which
+ * are added in order (the same bits every run).
+ */
+size_t fta_qk_norm_rope_bwd_workspace_size(int B, int H, int Hk, int N, int D);
+int fta_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                         const void* dq_out, const int64_t* dqo_strides, const void* dk_out, const int64_t* dko_strides,
+                         int dtype, int B, int H, int Hk, int N, int D, const void* q_weight, const void* k_weight,
+                         int weight_dtype, const float* cos, const float* sin, int P, int R, const int32_t* positions,
+                         int64_t positions_stride_b, float eps, int interleaved, void* dq, const int64_t* dq_strides,
+                         void* dk, const int64_t* dk_strides, void* dq_weight, void* dk_weight, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * The same for T new tokens of each request, K and V written into the caches
+ * ([B][S][Hk][D] strided) in the same pass.  cache_lens[b] (int32, device) counts the
+ * cached tokens with these T: token t goes to row cache_lens[b] - T + t and takes that
+ * row plus position_offset as its position.  Rows outside [0, S) are not written.
+ */
+int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                            const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,
+                            const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                            const float* sin, int P, int R, int position_offset, float eps, int interleaved,
+                            const int32_t* cache_lens, int S, void* q_out, const int64_t* qo_strides, void* k_cache,
+                            const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides, void* stream);
+
+/* ---------------------------------------------------------------- window attention */
+
+/*
+ * Sliding-window attention with sinks (no counterpart in the reference): query i of a
+ * sequence of len tokens sees key j when j < len, j <= i + right and (j >= i - left or
+ * j < num_sinks).  seq_lens [B] (int32, device; clamped into [0, N]) or null (N); tokens
+ * at or past len give o = 0, lse = -inf and zero gradients, and what q, k, v and dout
+ * hold there is not used.  Tokens in front of len must be finite.  Layouts, head counts
+ * (H a multiple of Hk) and head dims as for fta_sparse_attn_fwd_gqa; scale > 0.
+ */
+int fta_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, int dtype, int B, int H, int Hk, int N, int D, const int32_t* seq_lens,
+                        int left, int right, int num_sinks, float scale, void* o, const int64_t* o_strides, float* lse,
+                        void* stream);
+
+/*
+ * Its backward, from the forward's o and lse: dq [B][N][H][D], dk, dv [B][N][Hk][D].
+ * No atomics; the workspace (fta_window_attn_bwd_workspace_size bytes) holds delta =
+ * o . dout, the lse in log2 units and the fp32 parts of split dK / dV walks.
+ */
+size_t fta_window_attn_bwd_workspace_size(int B, int H, int Hk, int N, int D, int left, int right, int num_sinks);
+int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                        const int64_t* v_strides, const void* o, const int64_t* o_strides, const void* dout,
+                        const int64_t* do_strides, int dtype, int B, int H, int Hk, int N, int D, const int32_t* seq_lens,
+                        int left, int right, int num_sinks, float scale, const float* lse, void* dq,
+                        const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+                        const int64_t* dv_strides, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- cache attention */
+
+/*
+ * Attention of T new tokens per request over K/V caches [B][S][Hk][D] (no counterpart in
+ * the reference).  cache_lens[b] (int32, device; clamped into [0, S]) counts the cached
+ * tokens, the new ones included; token t stands at p = cache_lens[b] - T + t and sees own
+ * key j when j <= p and (j >= p - left or j < num_sinks).  P > 0 adds a prefix that every
+ * request sees whole (k_prefix, v_prefix [P][Hk][D]; strides {unused, stride_h, stride_n}),
+ * read once for the batch; it needs left >= S (no window).  q and o are [B][T][H][D]
+ * strided, lse [B][H][T]; rows that see nothing give o = 0, lse = -inf.  Cache rows that
+ * no token sees may hold anything.  The workspace (fta_cache_attn_workspace_size bytes)
+ * holds the parts that the keys are split into.
+ */
+size_t fta_cache_attn_workspace_size(int B, int H, int Hk, int T, int S, int D, int P, int left, int num_sinks);
+int fta_cache_attn(const void* q, const int64_t* q_strides, const void* k_cache, const int64_t* kc_strides,
+                   const void* v_cache, const int64_t* vc_strides, int dtype, int B, int H, int Hk, int T, int S, int D,
+                   const int32_t* cache_lens, const void* k_prefix, const int64_t* kp_strides, const void* v_prefix,
+                   const int64_t* vp_strides, int P, int left, int num_sinks, float scale, void* o,
+                   const int64_t* o_strides, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,120 @@
+"""Refusals of the operators around the sparse attention, without a GPU: the Python
+checks raise before anything is launched, and the C entries return a status."""
+
+import pytest
+import torch
+
+import flash_topk_attn_v2 as fta
+from flash_topk_attn_v2 import _lib
+
+BF = torch.bfloat16
+
+
+
+
+def test_cpu_tensors_are_refused():
+    x, t = torch.zeros(1, 4, 64, dtype=BF), torch.zeros(4, 32)
+    n = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="CUDA"):
+        fta.flash_qk_norm_rope(x, x, 1, t, t)
+    with pytest.raises(ValueError, match="CUDA"):
+        fta.flash_qk_norm_rope_append(x, x, x, x, x, n, 1, t, t)
+    with pytest.raises(ValueError, match="CUDA"):
+        fta.flash_window_attn(x, x, x, 1, (3, 0))
+    with pytest.raises(ValueError, match="CUDA"):
+        fta.flash_window_attn_decode(x, x, x, n, 1, 3)
+    with pytest.raises(ValueError, match="CUDA"):
+        fta.flash_prefix_attn_decode(x, x[0], x[0], x, x, n, 1)
+    with pytest.raises(ValueError, match="required"):
+        fta.flash_prefix_attn_decode(x, None, None, x, x, n, 1)
+    with pytest.raises(ValueError, match="non-negative"):
+        fta.flash_window_attn_decode(x, x, x, n, 1, -1)
+
+
+def _prep(L, B=1, H=2, Hk=1, N=4, D=64, P=4, R=64, dtype=0, wt=2, eps=1e-6, append=False, S=8):
+    z = _lib.i64arr((0, 0, 0))
+    if append:
+        return L.fta_qk_norm_rope_append(None, z, None, z, None, z, dtype, B, H, Hk, N, D, None, None, wt, None, None, P, R,
+                                         0, eps, 0, None, S, None, z, None, z, None, z, None)
+    return L.fta_qk_norm_rope(None, z, None, z, dtype, B, H, Hk, N, D, None, None, wt, None, None, P, R, None, 0, eps, 0,
+                              None, z, None, z, None)
+
+
+@pytest.mark.parametrize("bad", [dict(B=0), dict(H=0), dict(N=0), dict(D=0), dict(D=24), dict(D=272), dict(R=8), dict(R=80),
+                                 dict(R=0), dict(P=0), dict(dtype=2), dict(dtype=-1), dict(wt=3), dict(eps=0.0),
+                                 dict(eps=float("nan"))])
+@pytest.mark.parametrize("append", [False, True])
+def test_prep_entry(bad, append):
+    L = _lib.lib()
+    assert _prep(L, append=append, **bad) == _lib.FTA_ERR_ARG
+    assert L.fta_last_error()
+
+
+def test_prep_entry_rows():
+    L = _lib.lib()
+    assert _prep(L, N=5, P=4) == _lib.FTA_ERR_ARG  # more tokens than table rows
+    assert _prep(L, append=True, S=0) == _lib.FTA_ERR_ARG
+    assert L.fta_qk_norm_rope_bwd_workspace_size(1, 2, 1, 4, 24) == 0
+    assert L.fta_qk_norm_rope_bwd_workspace_size(1, 2, 1, 4, 64) > 0
+
+
+def _window(L, B=1, H=4, Hk=2, N=10, D=64, left=3, right=0, sinks=0, scale=0.1, dtype=0):
+    z = _lib.i64arr((0, 0, 0))
+    return L.fta_window_attn_fwd(None, z, None, z, None, z, dtype, B, H, Hk, N, D, None, left, right, sinks, scale, None, z,
+                                 None, None)
+
+
+def _window_bwd(L, ws=0, **kw):
+    z = _lib.i64arr((0, 0, 0))
+    a = dict(B=1, H=4, Hk=2, N=10, D=64, left=3, right=0, sinks=0, scale=0.1, dtype=0) | kw
+    return L.fta_window_attn_bwd(None, z, None, z, None, z, None, z, None, z, a["dtype"], a["B"], a["H"], a["Hk"], a["N"],
+                                 a["D"], None, a["left"], a["right"], a["sinks"], a["scale"], None, None, z, None, z, None,
+                                 z, None, ws, None)
+
+
+BAD = [dict(B=0), dict(H=3), dict(Hk=0), dict(N=0), dict(N=-1), dict(D=8), dict(D=260), dict(left=-1), dict(right=-2),
+       dict(sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(dtype=2)]
+
+
+@pytest.mark.parametrize("bad", BAD)
+def test_window_entries(bad):
+    L = _lib.lib()
+    assert _window(L, **bad) == _lib.FTA_ERR_ARG
+    assert _window_bwd(L, **bad) == _lib.FTA_ERR_ARG
+
+
+def test_window_entry_sizes():
+    L = _lib.lib()
+    assert _window(L, N=(1 << 29) + 1) == _lib.FTA_ERR_UNSUPPORTED
+    assert _window_bwd(L) == _lib.FTA_ERR_ARG  # no workspace
+    assert b"workspace" in L.fta_last_error()
+    # delta and the log2 lse, then fp32 dK / dV parts of small grids and of the sinks' tiles
+    assert L.fta_window_attn_bwd_workspace_size(1, 4, 2, 10, 64, 3, 0, 0) >= 2 * 256
+    big = (1, 32, 8, 32768, 128, 1023, 0)
+    none, four = (L.fta_window_attn_bwd_workspace_size(*big, s) for s in (0, 4))
+    assert none == 2 * 4 * 32 * 32768  # 4096 workgroups: no parts
+    assert four > none and (four - none) % (2 * 8 * 64 * 128 * 4) == 0
+    assert L.fta_window_attn_bwd_workspace_size(1, 4, 3, 10, 64, 3, 0, 0) == 0
+
+
+def _cache(L, B=1, H=4, Hk=2, T=1, S=10, D=64, P=0, left=3, sinks=0, scale=0.1, dtype=0, ws=0):
+    z = _lib.i64arr((0, 0, 0))
+    return L.fta_cache_attn(None, z, None, z, None, z, dtype, B, H, Hk, T, S, D, None, None, z, None, z, P, left, sinks, scale,
+                            None, z, None, None, ws, None)
+
+
+@pytest.mark.parametrize("bad", [dict(B=0), dict(H=5), dict(Hk=-2), dict(T=0), dict(S=0), dict(D=12), dict(D=512), dict(P=-1),
+                                 dict(left=-1), dict(sinks=-1), dict(scale=0.0), dict(scale=float("nan")), dict(dtype=7)])
+def test_cache_entry(bad):
+    L = _lib.lib()
+    assert _cache(L, **bad) == _lib.FTA_ERR_ARG
+
+
+def test_cache_entry_sizes():
+    L = _lib.lib()
+    assert _cache(L, P=5) == _lib.FTA_ERR_UNSUPPORTED  # a window behind a shared prefix
+    assert _cache(L, S=(1 << 29) + 1) == _lib.FTA_ERR_UNSUPPORTED
+    assert _cache(L, P=5, left=10) == _lib.FTA_ERR_ARG  # parts without a workspace
+    assert L.fta_cache_attn_workspace_size(1, 4, 2, 1, 10, 64, 0, 3, 0) == 0  # one part: o written directly
+    assert L.fta_cache_attn_workspace_size(1, 4, 2, 1, 10, 64, 70, 10, 0) > 0
+    assert L.fta_cache_attn_workspace_size(1, 4, 3, 1, 10, 64, 0, 3, 0) == 0
