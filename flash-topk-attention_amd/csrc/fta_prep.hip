@@ -20,6 +20,9 @@
 #include "fta_common.h"
 #include "fta_host.h"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 struct PrepArgs {
@@ -42,13 +45,6 @@ struct PrepArgs {
     float eps;
 };
 
-__device__ __forceinline__ float load_w(const void* w, int dt, int i) {
-    if (w == nullptr) return 1.f;
-    if (dt == 2) return reinterpret_cast<const float*>(w)[i];
-    const uint16_t x = reinterpret_cast<const uint16_t*>(w)[i];
-    return dt == FTA_DTYPE_BF16 ? Elem<FTA_DTYPE_BF16>::to_f32(x) : Elem<FTA_DTYPE_F16>::to_f32(x);
-}
-
 template <int DT>
 __device__ __forceinline__ void unpack8(uint4 x, float* f) {
     const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -66,6 +62,23 @@ __device__ __forceinline__ uint4 pack8(const float* f) {
 __device__ __forceinline__ uint4 shfl4(uint4 x, int src) {
     return make_uint4(__shfl((int)x.x, src, 64), __shfl((int)x.y, src, 64), __shfl((int)x.z, src, 64),
                       __shfl((int)x.w, src, 64));
+}
+// Weights of columns d .. d + 7.
+__device__ __forceinline__ void load_w8(const void* w, int dt, int d, float* f) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = 1.f;
+    } else if (dt == FTA_DTYPE_F32) {
+        const float4 x = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + d);
+        const float4 y = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(w) + d + 4);
+        f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w, f[4] = y.x, f[5] = y.y, f[6] = y.z, f[7] = y.w;
+    } else {
+        const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(w) + d);
+        if (dt == FTA_DTYPE_BF16)
+            unpack8<FTA_DTYPE_BF16>(x, f);
+        else
+            unpack8<FTA_DTYPE_F16>(x, f);
+    }
 }
 template <int LG>
 __device__ __forceinline__ float row_sum(float x) {
@@ -118,8 +131,9 @@ __device__ __forceinline__ void load_angles(const PrepArgs& a, const LaneCols& c
 }
 
 // ----------------------------------------------------------------------------
-// Forward.  One wave works on U groups of 64 / LG rows of one token: their loads
-// are issued together, the angles are read once for all of them.
+// Forward.  A wave strides over (token, part) pairs; a part is U groups of 64 / LG
+// rows of one token, whose loads are issued together and share the token's angles.
+// The weights (the lane's own and its partners') stay in registers.
 // APPEND: rows past the query and key heads copy V; K and V go to cache row
 // lens[b] - N + n (not written outside [0, S)).
 // ----------------------------------------------------------------------------
@@ -127,89 +141,95 @@ template <int DT, int LG, int U, bool APPEND>
 __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
     constexpr int RW = 64 / LG;
     const int lane = threadIdx.x & 63;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (unit >= a.units) return;
-    const int64_t tok = unit / a.parts;
-    const int part = (int)(unit - tok * a.parts);
-    const int b = (int)(tok / a.N), n = (int)(tok - (int64_t)b * a.N);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const LaneCols c = lane_cols<LG>(a, lane);
     const int rows = a.H + a.Hk + (APPEND ? a.Hk : 0);
-    const int r0 = part * U * RW + lane / LG;
-
-    int crow = 0, pos;
-    if constexpr (APPEND) {
-        const int64_t at = (int64_t)a.lens[b] - a.N + n;
-        crow = (at < 0 || at >= a.S) ? -1 : (int)at;
-        const int64_t p = at + a.pos_off;
-        pos = (int)min(max(p, (int64_t)0), (int64_t)a.P - 1);
-    } else {
-        pos = a.positions ? a.positions[b * a.pos_sb + n] : n;
-        pos = min(max(pos, 0), a.P - 1);
-    }
-
-    uint4 x[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int row = r0 + u * RW;
-        x[u] = fta_zero4();
-        if (c.live && row < rows) {
-            const uint16_t* p = row < a.H ? a.q + b * a.q_sb + row * a.q_sh + n * a.q_sn
-                                          : a.k + b * a.k_sb + (row - a.H) * a.k_sh + n * a.k_sn;
-            if (APPEND && row >= a.H + a.Hk) p = a.v + b * a.v_sb + (row - a.H - a.Hk) * a.v_sh + n * a.v_sn;
-            x[u] = *reinterpret_cast<const uint4*>(p + c.d0);
-        }
-    }
-    float cs[8], sn[8];
-    load_angles(a, c, pos, cs, sn);
     const float inv_d = 1.f / (float)a.D;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const int row = r0 + u * RW;
-        const bool isq = row < a.H;
-        float f[8], y[8];
-        unpack8<DT>(x[u], f);
-        float ss = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
-        const float r = rsqrtf(fmaf(row_sum<LG>(ss), inv_d, a.eps));
-        const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
-        if (!c.live || row >= rows) continue;
-        uint16_t* out;
-        if (APPEND && row >= a.H + a.Hk) {
-            if (crow < 0) continue;
-            out = a.vo + b * a.vo_sb + (row - a.H - a.Hk) * a.vo_sh + crow * a.vo_sn;
-            *reinterpret_cast<uint4*>(out + c.d0) = x[u];
-            continue;
-        }
-        const void* w = isq ? a.qw : a.kw;
-        if (a.inter) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] *= r * load_w(w, a.w_dtype, c.d0 + e);
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
-                y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
-            }
+    float wq[8], wk[8], pq[8], pk[8];
+    {
+        const int d = c.live ? c.d0 : 0, dp = c.live ? (c.src & (LG - 1)) * 8 : 0;
+        load_w8(a.qw, a.w_dtype, d, wq);
+        load_w8(a.kw, a.w_dtype, d, wk);
+        load_w8(a.qw, a.w_dtype, dp, pq);
+        load_w8(a.kw, a.w_dtype, dp, pk);
+    }
+    for (int64_t unit = (int64_t)blockIdx.x * 4 + wave; unit < a.units; unit += (int64_t)gridDim.x * 4) {
+        const int64_t tok = unit / a.parts;
+        const int part = (int)(unit - tok * a.parts);
+        const int b = (int)(tok / a.N), n = (int)(tok - (int64_t)b * a.N);
+        const int r0 = part * U * RW + lane / LG;
+
+        int crow = 0, pos;
+        if constexpr (APPEND) {
+            const int64_t at = (int64_t)a.lens[b] - a.N + n;
+            crow = (at < 0 || at >= a.S) ? -1 : (int)at;
+            pos = (int)min(max(at + a.pos_off, (int64_t)0), (int64_t)a.P - 1);
         } else {
-            float g[8];
-            unpack8<DT>(xp, g);
-            const int dp = (c.src & (LG - 1)) * 8;
+            pos = a.positions ? a.positions[b * a.pos_sb + n] : n;
+            pos = min(max(pos, 0), a.P - 1);
+        }
+
+        uint4 x[U];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float t = f[e] * (r * load_w(w, a.w_dtype, c.d0 + e));
-                const float p = g[e] * (r * load_w(w, a.w_dtype, dp + e));
-                y[e] = fmaf(p, c.sgn * sn[e], t * cs[e]);
+        for (int u = 0; u < U; ++u) {
+            const int row = r0 + u * RW;
+            x[u] = fta_zero4();
+            if (c.live && row < rows) {
+                const uint16_t* p = row < a.H ? a.q + b * a.q_sb + row * a.q_sh + n * a.q_sn
+                                              : a.k + b * a.k_sb + (row - a.H) * a.k_sh + n * a.k_sn;
+                if (APPEND && row >= a.H + a.Hk) p = a.v + b * a.v_sb + (row - a.H - a.Hk) * a.v_sh + n * a.v_sn;
+                x[u] = *reinterpret_cast<const uint4*>(p + c.d0);
             }
         }
-        if (isq) {
-            out = a.qo + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn;
-        } else if (APPEND) {
-            if (crow < 0) continue;
-            out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + crow * a.ko_sn;
-        } else {
-            out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + n * a.ko_sn;
+        float cs[8], sn[8];
+        load_angles(a, c, pos, cs, sn);
+        if (!a.inter) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sn[e] *= c.sgn;
         }
-        *reinterpret_cast<uint4*>(out + c.d0) = pack8<DT>(y);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = r0 + u * RW;
+            const bool isq = row < a.H;
+            float f[8], y[8];
+            unpack8<DT>(x[u], f);
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+            const float r = rsqrtf(fmaf(row_sum<LG>(ss), inv_d, a.eps));
+            const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
+            if (!c.live || row >= rows) continue;
+            uint16_t* out;
+            if (APPEND && row >= a.H + a.Hk) {
+                if (crow < 0) continue;
+                out = a.vo + b * a.vo_sb + (row - a.H - a.Hk) * a.vo_sh + crow * a.vo_sn;
+                *reinterpret_cast<uint4*>(out + c.d0) = x[u];
+                continue;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] *= r * (isq ? wq[e] : wk[e]);
+            if (a.inter) {
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) {
+                    y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
+                    y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
+                }
+            } else {
+                float g[8];
+                unpack8<DT>(xp, g);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = fmaf(g[e] * (r * (isq ? pq[e] : pk[e])), sn[e], f[e] * cs[e]);
+            }
+            if (isq) {
+                out = a.qo + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn;
+            } else if (APPEND) {
+                if (crow < 0) continue;
+                out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + crow * a.ko_sn;
+            } else {
+                out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + n * a.ko_sn;
+            }
+            *reinterpret_cast<uint4*>(out + c.d0) = pack8<DT>(y);
+        }
     }
 }
 
@@ -230,11 +250,9 @@ __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
     const float inv_d = 1.f / (float)a.D;
     float dwq[8], dwk[8], wq[8], wk[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        dwq[e] = dwk[e] = 0.f;
-        wq[e] = c.live ? load_w(a.qw, a.w_dtype, c.d0 + e) : 0.f;
-        wk[e] = c.live ? load_w(a.kw, a.w_dtype, c.d0 + e) : 0.f;
-    }
+    for (int e = 0; e < 8; ++e) dwq[e] = dwk[e] = 0.f;
+    load_w8(a.qw, a.w_dtype, c.live ? c.d0 : 0, wq);
+    load_w8(a.kw, a.w_dtype, c.live ? c.d0 : 0, wk);
     for (int64_t unit = (int64_t)blockIdx.x * 4 + wave; unit < a.units; unit += (int64_t)gridDim.x * 4) {
         const int64_t tok = unit / a.parts;
         const int part = (int)(unit - tok * a.parts);
@@ -325,30 +343,35 @@ __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
     }
 }
 
-// Sum of the workgroups' partial weight gradients: 16 columns and 16 slices of the
+// Sum of the workgroups' partial weight gradients: 8 columns and 32 slices of the
 // partials per workgroup; columns [0, D) are the query weights', the rest the keys'.
 __global__ __launch_bounds__(256) void fta_norm_rope_dw_kernel(const float* part, int nwg, int D, void* dqw, void* dkw,
                                                                int w_dtype) {
-    __shared__ float s[16][17];
-    const int cx = threadIdx.x & 15, sy = threadIdx.x >> 4;
-    const int col = blockIdx.x * 16 + cx;  // 2 D is a multiple of 16
-    float t = 0.f;
-    for (int w = sy; w < nwg; w += 16) t += part[(int64_t)w * 2 * D + col];
-    s[sy][cx] = t;
+    __shared__ float s[32][9];
+    const int cx = threadIdx.x & 7, sy = threadIdx.x >> 3;
+    const int col = blockIdx.x * 8 + cx;  // D is a multiple of 16
+    float t[4] = {0.f, 0.f, 0.f, 0.f};
+    int w = sy;
+    for (; w + 96 < nwg; w += 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] += part[(int64_t)(w + 32 * i) * 2 * D + col];
+    }
+    for (; w < nwg; w += 32) t[0] += part[(int64_t)w * 2 * D + col];
+    s[sy][cx] = (t[0] + t[1]) + (t[2] + t[3]);
     __syncthreads();
     if (sy != 0) return;
-    t = 0.f;
+    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += s[i][cx];
+    for (int i = 0; i < 32; ++i) sum += s[i][cx];
     void* out = col < D ? dqw : dkw;
     const int d = col < D ? col : col - D;
     if (out == nullptr) return;
-    if (w_dtype == 2)
-        reinterpret_cast<float*>(out)[d] = t;
+    if (w_dtype == FTA_DTYPE_F32)
+        reinterpret_cast<float*>(out)[d] = sum;
     else
-        reinterpret_cast<uint16_t*>(out)[d] =
-            (uint16_t)((w_dtype == FTA_DTYPE_BF16 ? Elem<FTA_DTYPE_BF16>::pack2(t, 0.f) : Elem<FTA_DTYPE_F16>::pack2(t, 0.f)) &
-                       0xffffu);
+        reinterpret_cast<uint16_t*>(out)[d] = (uint16_t)((w_dtype == FTA_DTYPE_BF16 ? Elem<FTA_DTYPE_BF16>::pack2(sum, 0.f)
+                                                                                    : Elem<FTA_DTYPE_F16>::pack2(sum, 0.f)) &
+                                                         0xffffu);
 }
 
 // ---------------------------------------------------------------------- host
@@ -377,12 +400,10 @@ void set_units(PrepArgs& a, int B, int U, int rows) {
     a.units = (int64_t)B * a.N * a.parts;
 }
 
-constexpr int kBwdGrid = 2048;  // 8 workgroups of 4 waves per CU
+// Workgroups of 4 waves that the chip holds at once: the kernels stride over the rest.
+constexpr int kFwdGrid = 256 * 6, kBwdGrid = 256 * 4;
 
-int64_t bwd_grid(int64_t units) {
-    const int64_t g = (units + 3) / 4;
-    return g < kBwdGrid ? g : kBwdGrid;
-}
+unsigned grid_of(int64_t units, int most) { return (unsigned)std::min<int64_t>((units + 3) / 4, most); }
 
 template <typename F>
 int with_lanes(int D, F f) {
@@ -400,16 +421,16 @@ int launch_fwd(PrepArgs& a, int B, hipStream_t st) {
     const int rows = a.H + a.Hk + (APPEND ? a.Hk : 0);
     return with_lanes(a.D, [&](auto lg) {
         constexpr int LG = decltype(lg)::value;
-        set_units(a, B, 1, rows);
         // few rows: one group per wave, so that they spread over the CUs
-        const bool few = a.units <= 8192;
-        if (!few) set_units(a, B, 4, rows);
-        const int64_t wgs = (a.units + 3) / 4;
-        if (wgs > 0x7fffffff) return fta::unsupported("qk_norm_rope: too many tokens");
-        if (few)
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, APPEND>), dim3((unsigned)wgs), dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 4, APPEND>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+        set_units(a, B, 1, rows);
+        if (a.units <= 4 * kFwdGrid) {
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, APPEND>), dim3(grid_of(a.units, kFwdGrid)), dim3(256), 0, st,
+                               a);
+        } else {
+            set_units(a, B, 2, rows);
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 2, APPEND>), dim3(grid_of(a.units, kFwdGrid)), dim3(256), 0, st,
+                               a);
+        }
         return fta::check_launch("fta_norm_rope_fwd_kernel");
     });
 }
@@ -419,11 +440,11 @@ int launch_bwd(PrepArgs& a, int B, void* dqw, void* dkw, hipStream_t st) {
     return with_lanes(a.D, [&](auto lg) {
         constexpr int LG = decltype(lg)::value;
         set_units(a, B, 2, a.H + a.Hk);
-        const int64_t wgs = bwd_grid(a.units);
-        hipLaunchKernelGGL((fta_norm_rope_bwd_kernel<DT, LG, 2>), dim3((unsigned)wgs), dim3(256), 0, st, a);
+        const unsigned wgs = grid_of(a.units, kBwdGrid);
+        hipLaunchKernelGGL((fta_norm_rope_bwd_kernel<DT, LG, 2>), dim3(wgs), dim3(256), 0, st, a);
         int rc = fta::check_launch("fta_norm_rope_bwd_kernel");
         if (rc != FTA_OK || a.part == nullptr) return rc;
-        hipLaunchKernelGGL(fta_norm_rope_dw_kernel, dim3(2 * a.D / 16), dim3(256), 0, st, a.part, (int)wgs, a.D, dqw, dkw,
+        hipLaunchKernelGGL(fta_norm_rope_dw_kernel, dim3(2 * a.D / 8), dim3(256), 0, st, a.part, (int)wgs, a.D, dqw, dkw,
                            a.w_dtype);
         return fta::check_launch("fta_norm_rope_dw_kernel");
     });

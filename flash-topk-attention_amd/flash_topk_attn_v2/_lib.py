@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-from contextlib import nullcontext
 from functools import lru_cache
 from typing import Sequence
 
@@ -154,18 +153,68 @@ def dtype_code(dt: torch.dtype) -> int:
     raise ValueError(f"unsupported dtype {dt}; expected bfloat16 or float16")
 
 
-def on_device(device: torch.device):
-    """Context in which ``device`` is the current one (launches go to the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+def call(name: str, device: torch.device, *args) -> None:
+    """One entry point of the library, launched on ``device``'s current stream (appended as
+    the last argument); a failure raises as ``check`` does."""
+    fn = getattr(lib(), name)
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:  # launches go to the current device
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != FTA_OK:
+        check(rc, name)
 
 
-def check_tensors(what: str, device: torch.device, **tensors) -> None:
+@lru_cache(maxsize=4096)
+def dense_strides(shape: tuple, heads: int):
+    """Strides of a contiguous ``[B, N, heads * D]`` tensor as the library takes them."""
+    _, N, C = shape
+    return i64arr((N * C, C // heads, C))
+
+
+@lru_cache(maxsize=4096)
+def _row_strides(shape: tuple, stride: tuple, heads: int):
+    """``{stride_b, stride_h, stride_n}`` of a ``[B, N, heads * D]`` tensor, or None where its
+    rows are not contiguous or not whole 16-byte steps apart."""
+    B, N, C = shape
+    sb = stride[0] if B > 1 else 0
+    sn = stride[1] if N > 1 else C
+    if stride[2] != 1 or (sb | sn) & 7:
+        return None
+    return i64arr((sb, C // heads, sn))
+
+
+def rows(x: torch.Tensor, heads: int):
+    """``(tensor, address, strides)`` that address ``x`` ``[B, N, heads * D]`` by 16-byte
+    loads; a copy only where its layout or its address does not allow them."""
+    strides, at = _row_strides(x.shape, x.stride(), heads), x.data_ptr()
+    if strides is None or at & 15:
+        x = x.clone(memory_format=torch.contiguous_format)
+        strides, at = _row_strides(x.shape, x.stride(), heads), x.data_ptr()
+    return x, at, strides
+
+
+def rows_in_place(what: str, x: torch.Tensor, heads: int):
+    """``(address, strides)`` of a tensor that is used where it is (a cache)."""
+    strides, at = _row_strides(x.shape, x.stride(), heads), x.data_ptr()
+    if strides is None or at & 15:
+        raise ValueError(f"{what}: cache rows must be contiguous and 16-byte aligned")
+    return at, strides
+
+
+def flat(x: torch.Tensor) -> torch.Tensor:
+    """``x`` contiguous and 16-byte aligned (a table or weights)."""
+    if x.is_contiguous() and x.data_ptr() & 15 == 0:
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
+def check_device(what: str, device: torch.device, *tensors) -> None:
     """Every given tensor has to be on ``device`` (None is skipped)."""
-    for name, t in tensors.items():
+    for t in tensors:
         if t is not None and t.device != device:
-            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+            raise ValueError(f"{what}: a tensor is on {t.device}, expected {device}")
 
 
 def head_counts(what: str, width: int, num_heads: int, num_kv_heads):
@@ -180,6 +229,25 @@ def head_counts(what: str, width: int, num_heads: int, num_kv_heads):
     if D % 16 != 0 or D > 256:
         raise ValueError(f"{what}: D ({D}) must be a multiple of 16 up to 256")
     return H, Hk, D
+
+
+HALVES = (torch.float16, torch.bfloat16)
+DTYPE_CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
+
+
+def no_grad_inputs(what: str, *tensors) -> None:
+    """Refuses a call whose gradients would be lost."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
+
+
+def softmax_scale(what: str, scale, D: int) -> float:
+    scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3.0e38:
+        raise ValueError(f"{what}: scale must be positive and finite")
+    return scale
 
 
 def workspace(nbytes: int, device: torch.device) -> torch.Tensor:

@@ -6,58 +6,62 @@ No counterpart in the reference.
 
 from __future__ import annotations
 
-import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from .qk_prep import _cache_strides, _check_cache, _no_grad_inputs
+from .qk_prep import check_cache
+
+
+@lru_cache(maxsize=1024)
+def _geometry(what, q, dtype, num_heads, num_kv_heads, S, P, left, sinks, scale):
+    """``(H, Hk, D, left, scale, workspace bytes)``, checked (calls of one shape are checked once)."""
+    if len(q) != 3:
+        raise ValueError(f"{what}: q must be [B, T, num_heads * D]")
+    if dtype not in _lib.HALVES:
+        raise ValueError(f"{what}: q must be float16 or bfloat16")
+    B, T, C = q
+    H, Hk, D = _lib.head_counts(what, C, num_heads, num_kv_heads)
+    if B == 0 or T == 0:
+        raise ValueError(f"{what}: empty batch or no new tokens")
+    left = S if left is None else left
+    nbytes = int(_lib.lib().fta_cache_attn_workspace_size(B, H, Hk, T, S, D, P, left, sinks))
+    return H, Hk, D, left, _lib.softmax_scale(what, scale, D), nbytes
 
 
 def cache_attn(what, q, k_cache, v_cache, cache_lens, num_heads, num_kv_heads, k_prefix, v_prefix, left, sinks, scale):
     """Checks and the launch of ``fta_cache_attn``."""
-    if q.ndim != 3:
-        raise ValueError(f"{what}: q must be [B, T, num_heads * D]")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    if q.dtype not in (torch.float16, torch.bfloat16):
-        raise ValueError(f"{what}: q must be float16 or bfloat16")
-    _no_grad_inputs(what, q, k_cache, v_cache, k_prefix, v_prefix)
-    B, T, C = q.shape
-    H, Hk, D = _lib.head_counts(what, C, num_heads, num_kv_heads)
-    if B == 0 or T == 0:
-        raise ValueError(f"{what}: empty batch or no new tokens")
-    _check_cache(what, k_cache, v_cache, cache_lens, B, Hk, D, q)
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError(f"{what}: scale must be positive and finite")
-    S, P, kps, vps = k_cache.shape[1], 0, None, None
-    if left is None:
-        left = S
+    _lib.no_grad_inputs(what, q, k_cache, v_cache, k_prefix, v_prefix)
+    S = k_cache.shape[1] if k_cache.ndim == 3 else 0
+    P = 0 if k_prefix is None else k_prefix.shape[0]
+    H, Hk, D, left, scale, nbytes = _geometry(what, q.shape, q.dtype, num_heads, num_kv_heads, S, P, left, sinks, scale)
+    B, T, _ = q.shape
+    check_cache(what, q, k_cache, v_cache, cache_lens, B, Hk * D)
+    kpa = kps = vpa = vps = None
     if k_prefix is not None:
         if k_prefix.ndim != 2 or k_prefix.shape[1] != Hk * D or v_prefix.shape != k_prefix.shape:
             raise ValueError(f"{what}: k_prefix and v_prefix must be [P, num_kv_heads * D] = [P, {Hk * D}]")
         if k_prefix.dtype != q.dtype or v_prefix.dtype != q.dtype:
             raise ValueError(f"{what}: the prefix must have q's type")
-        _lib.check_tensors(what, q.device, k_prefix=k_prefix, v_prefix=v_prefix)
-        P = k_prefix.shape[0]
+        _lib.check_device(what, q.device, k_prefix, v_prefix)
         if P > 0:
-            kps, vps = (_cache_strides(what, x[None], D) for x in (k_prefix, v_prefix))
-    kcs, vcs = _cache_strides(what, k_cache, D), _cache_strides(what, v_cache, D)
-    dev = q.device
-    qq, qs = _lib.token_view(q, "bnc", H)
+            kpa, kps = _lib.rows_in_place(what, k_prefix[None], Hk)
+            vpa, vps = _lib.rows_in_place(what, v_prefix[None], Hk)
+    kca, kcs = _lib.rows_in_place(what, k_cache, Hk)
+    vca, vcs = _lib.rows_in_place(what, v_cache, Hk)
+    q, qa, qs = _lib.rows(q, H)
     lens = cache_lens.contiguous()
-    o = torch.empty(B, T, C, device=dev, dtype=q.dtype)
+    dev = q.device
+    o = torch.empty(q.shape, device=dev, dtype=q.dtype)
     lse = torch.empty(B, H, T, device=dev, dtype=torch.float32)
-    nbytes = _lib.size_of("fta_cache_attn_workspace_size", B, H, Hk, T, S, D, P, left, sinks)
     ws = _lib.workspace(nbytes, dev) if nbytes else None
-    with _lib.on_device(dev):
-        rc = _lib.lib().fta_cache_attn(
-            _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(k_cache), kcs, _lib.ptr(v_cache), vcs, _lib.dtype_code(q.dtype),
-            B, H, Hk, T, S, D, _lib.ptr(lens), _lib.ptr(k_prefix), kps, _lib.ptr(v_prefix), vps, P, left, sinks, scale,
-            _lib.ptr(o), _lib.i64arr((T * C, D, C)), _lib.ptr(lse), _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
-    _lib.check(rc, what)
+    _lib.call("fta_cache_attn", dev, qa, qs, kca, kcs, vca, vcs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, S, D,
+              lens.data_ptr(), kpa, kps, vpa, vps, P, left, sinks, scale, o.data_ptr(), _lib.dense_strides(q.shape, H),
+              lse.data_ptr(), _lib.ptr(ws), nbytes)
     return o, lse
 
 

@@ -8,6 +8,7 @@ operations.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -15,105 +16,91 @@ import torch
 from . import _lib
 
 
-def _check_common(what, q, k, num_heads, num_kv_heads, cos, sin, q_weight, k_weight, eps):
-    if q.ndim != 3 or k.ndim != 3:
+@lru_cache(maxsize=1024)
+def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, weight_types, num_heads, num_kv_heads, eps):
+    """``(H, Hk, D, R, weights' type code)`` from shapes and types, checked (calls of one
+    shape are checked once)."""
+    if len(q) != 3 or len(k) != 3:
         raise ValueError(f"{what}: q and k must be [B, N, heads * D]")
-    if q.device.type != "cuda":
-        raise ValueError(f"{what} requires CUDA tensors")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype:
+    if dtypes[0] not in _lib.HALVES or dtypes[1] != dtypes[0]:
         raise ValueError(f"{what}: q and k must both be float16 or bfloat16")
-    H, Hk, D = _lib.head_counts(what, q.shape[2], num_heads, num_kv_heads)
-    if tuple(k.shape) != (q.shape[0], q.shape[1], Hk * D):
-        raise ValueError(f"{what}: k must be {[q.shape[0], q.shape[1], Hk * D]}")
-    if q.shape[0] == 0 or q.shape[1] == 0:
+    H, Hk, D = _lib.head_counts(what, q[2], num_heads, num_kv_heads)
+    if tuple(k) != (q[0], q[1], Hk * D):
+        raise ValueError(f"{what}: k must be {[q[0], q[1], Hk * D]}")
+    if q[0] == 0 or q[1] == 0:
         raise ValueError(f"{what}: empty batch or sequence")
-    if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+    if len(cos) != 2 or cos != sin or table_types != (torch.float32, torch.float32):
         raise ValueError(f"{what}: cos and sin must be float32 tables [P, R / 2] of one shape")
-    if cos.requires_grad or sin.requires_grad:
-        raise ValueError(f"{what}: cos and sin are not differentiable")
-    R = 2 * cos.shape[1]
+    R = 2 * cos[1]
     if R <= 0 or R % 16 != 0 or R > D:
         raise ValueError(f"{what}: the rotated columns ({R}) must be a positive multiple of 16 up to D ({D})")
-    if cos.shape[0] == 0:
+    if cos[0] == 0:
         raise ValueError(f"{what}: cos and sin have no rows")
-    dtypes = {w.dtype for w in (q_weight, k_weight) if w is not None}
-    if len(dtypes) > 1 or not dtypes <= {torch.float32, torch.float16, torch.bfloat16}:
-        raise ValueError(f"{what}: weights must both be float32, float16 or bfloat16")
     for w in (q_weight, k_weight):
-        if w is not None and tuple(w.shape) != (D,):
+        if w is not None and tuple(w) != (D,):
             raise ValueError(f"{what}: weights must be [D] = [{D}]")
+    types = {t for t in weight_types if t is not None}
+    if len(types) > 1 or not types <= set(_lib.DTYPE_CODES):
+        raise ValueError(f"{what}: weights must both be float32, float16 or bfloat16")
     if not 0.0 < float(eps) < float("inf"):
         raise ValueError(f"{what}: eps must be positive")
-    _lib.check_tensors(what, q.device, k=k, cos=cos, sin=sin, q_weight=q_weight, k_weight=k_weight)
-    return H, Hk, D, R
+    return H, Hk, D, R, _lib.DTYPE_CODES[types.pop()] if types else _lib.DTYPE_F32
 
 
-def _table(t):
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _weights(q_weight, k_weight):
-    """Contiguous weights and the code of their type."""
-    codes = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
-    w = [None if x is None else x.contiguous() for x in (q_weight, k_weight)]
-    return w[0], w[1], next((codes[x.dtype] for x in w if x is not None), _lib.DTYPE_F32)
-
-
-def _dense(B, N, heads, D):
-    return _lib.i64arr((N * heads * D, D, heads * D))
+def _check(what, q, k, num_heads, num_kv_heads, cos, sin, qw, kw, eps):
+    if not q.is_cuda:
+        raise ValueError(f"{what} requires CUDA tensors")
+    geo = _geometry(what, q.shape, k.shape, (q.dtype, k.dtype), cos.shape, sin.shape, (cos.dtype, sin.dtype),
+                    None if qw is None else qw.shape, None if kw is None else kw.shape,
+                    (None if qw is None else qw.dtype, None if kw is None else kw.dtype), num_heads, num_kv_heads, eps)
+    if cos.requires_grad or sin.requires_grad:
+        raise ValueError(f"{what}: cos and sin are not differentiable")
+    _lib.check_device(what, q.device, k, cos, sin, qw, kw)
+    return geo
 
 
 class _QKNormRopeFunc(torch.autograd.Function):
     """Autograd function behind ``flash_qk_norm_rope``."""
 
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, H, Hk, eps, interleaved):
-        B, N, C = q.shape
-        D, dev = C // H, q.device
-        qq, qs = _lib.token_view(q, "bnc", H)
-        kk, ks = _lib.token_view(k, "bnc", Hk)
-        qw, kw, wt = _weights(q_weight, k_weight)
-        qo = torch.empty(B, N, C, device=dev, dtype=q.dtype)
-        ko = torch.empty(B, N, Hk * D, device=dev, dtype=q.dtype)
-        with _lib.on_device(dev):
-            rc = _lib.lib().fta_qk_norm_rope(
-                _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(kk), _lib.i64arr(ks), _lib.dtype_code(q.dtype), B, H, Hk, N, D,
-                _lib.ptr(qw), _lib.ptr(kw), wt, _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], 2 * cos.shape[1],
-                _lib.ptr(positions), 0 if positions is None else positions.stride(0), eps, int(interleaved),
-                _lib.ptr(qo), _dense(B, N, H, D), _lib.ptr(ko), _dense(B, N, Hk, D), _lib.stream_ptr(dev))
-        _lib.check(rc, "flash_qk_norm_rope")
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.args = H, Hk, eps, interleaved
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, geo, eps, interleaved):
+        H, Hk, D, R, wt = geo
+        B, N, _ = q.shape
+        q, qa, qs = _lib.rows(q, H)
+        k, ka, ks = _lib.rows(k, Hk)
+        qw, kw = (None if w is None else _lib.flat(w) for w in (q_weight, k_weight))
+        qo, ko = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k))
+        _lib.call("fta_qk_norm_rope", q.device, qa, qs, ka, ks, _lib.DTYPE_CODES[q.dtype], B, H, Hk, N, D, _lib.ptr(qw),
+                  _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, _lib.ptr(positions),
+                  0 if positions is None else positions.stride(0), eps, interleaved, qo.data_ptr(),
+                  _lib.dense_strides(q.shape, H), ko.data_ptr(), _lib.dense_strides(k.shape, Hk))
+        ctx.save_for_backward(q, k, qw, kw, cos, sin, positions)
+        ctx.args = geo, eps, interleaved
         return qo, ko
 
     @staticmethod
     def backward(ctx, dqo, dko):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        H, Hk, eps, interleaved = ctx.args
-        B, N, C = q.shape
-        D, dev = C // H, q.device
-        qq, qs = _lib.token_view(q, "bnc", H)
-        kk, ks = _lib.token_view(k, "bnc", Hk)
-        dqq, dqs = _lib.token_view(dqo, "bnc", H)
-        dkk, dks = _lib.token_view(dko, "bnc", Hk)
-        qw, kw, wt = _weights(q_weight, k_weight)
-        dq = torch.empty(B, N, C, device=dev, dtype=q.dtype)
-        dk = torch.empty(B, N, Hk * D, device=dev, dtype=q.dtype)
-        dqw = torch.empty_like(qw) if qw is not None and ctx.needs_input_grad[2] else None
-        dkw = torch.empty_like(kw) if kw is not None and ctx.needs_input_grad[3] else None
-        need = dqw is not None or dkw is not None
-        ws = _lib.workspace(_lib.size_of("fta_qk_norm_rope_bwd_workspace_size", B, H, Hk, N, D), dev) if need else None
-        with _lib.on_device(dev):
-            rc = _lib.lib().fta_qk_norm_rope_bwd(
-                _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(kk), _lib.i64arr(ks), _lib.ptr(dqq), _lib.i64arr(dqs),
-                _lib.ptr(dkk), _lib.i64arr(dks), _lib.dtype_code(q.dtype), B, H, Hk, N, D, _lib.ptr(qw), _lib.ptr(kw),
-                wt, _lib.ptr(cos), _lib.ptr(sin), cos.shape[0], 2 * cos.shape[1], _lib.ptr(positions),
-                0 if positions is None else positions.stride(0), eps, int(interleaved), _lib.ptr(dq),
-                _dense(B, N, H, D), _lib.ptr(dk), _dense(B, N, Hk, D), _lib.ptr(dqw), _lib.ptr(dkw), _lib.ptr(ws),
-                0 if ws is None else ws.numel(), _lib.stream_ptr(dev))
-        _lib.check(rc, "flash_qk_norm_rope backward")
-        return dq, dk, dqw, dkw, None, None, None, None, None, None, None
+        q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
+        (H, Hk, D, R, wt), eps, interleaved = ctx.args
+        B, N, _ = q.shape
+        dev = q.device
+        q, qa, qs = _lib.rows(q, H)
+        k, ka, ks = _lib.rows(k, Hk)
+        dqo, dqa, dqs = _lib.rows(dqo, H)
+        dko, dka, dks = _lib.rows(dko, Hk)
+        dq, dk = (torch.empty(x.shape, device=dev, dtype=x.dtype) for x in (q, k))
+        dqw = torch.empty(D, device=dev, dtype=qw.dtype) if qw is not None and ctx.needs_input_grad[2] else None
+        dkw = torch.empty(D, device=dev, dtype=kw.dtype) if kw is not None and ctx.needs_input_grad[3] else None
+        ws, nbytes = None, 0
+        if dqw is not None or dkw is not None:
+            nbytes = _lib.size_of("fta_qk_norm_rope_bwd_workspace_size", B, H, Hk, N, D)
+            ws = _lib.workspace(nbytes, dev)
+        _lib.call("fta_qk_norm_rope_bwd", dev, qa, qs, ka, ks, dqa, dqs, dka, dks, _lib.DTYPE_CODES[q.dtype], B, H, Hk, N,
+                  D, _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R,
+                  _lib.ptr(positions), 0 if positions is None else positions.stride(0), eps, interleaved, dq.data_ptr(),
+                  _lib.dense_strides(q.shape, H), dk.data_ptr(), _lib.dense_strides(k.shape, Hk), _lib.ptr(dqw),
+                  _lib.ptr(dkw), _lib.ptr(ws), nbytes)
+        return dq, dk, dqw, dkw, None, None, None, None, None, None
 
 
 def flash_qk_norm_rope(
@@ -148,46 +135,22 @@ def flash_qk_norm_rope(
         The prepared ``(q, k)``, shapes and type of the inputs.
     """
     what = "flash_qk_norm_rope"
-    H, Hk, D, R = _check_common(what, q, k, num_heads, num_kv_heads, cos, sin, q_weight, k_weight, eps)
-    B, N = q.shape[:2]
+    geo = _check(what, q, k, num_heads, num_kv_heads, cos, sin, q_weight, k_weight, eps)
+    B, N, _ = q.shape
     if positions is None:
         if N > cos.shape[0]:
             raise ValueError(f"{what}: cos and sin have {cos.shape[0]} rows for {N} tokens")
     else:
-        _lib.check_tensors(what, q.device, positions=positions)
+        _lib.check_device(what, q.device, positions)
         if positions.dtype not in (torch.int32, torch.int64):
             raise ValueError(f"{what}: positions must be int32 or int64")
-        if tuple(positions.shape) not in ((N,), (B, N)):
+        if positions.shape not in ((N,), (B, N)):
             raise ValueError(f"{what}: positions must be [N] or [B, N] = {[B, N]}")
         if positions.dtype == torch.int64:  # into the tables' range first: the narrow type would wrap
             positions = positions.clamp(0, cos.shape[0] - 1).to(torch.int32)
         positions = positions.contiguous().expand(B, N)
-    return _QKNormRopeFunc.apply(q, k, q_weight, k_weight, _table(cos), _table(sin), positions, H, Hk, float(eps),
-                                 bool(interleaved))
-
-
-def _check_cache(what, k_cache, v_cache, cache_lens, B, Hk, D, q):
-    if k_cache.ndim != 3 or k_cache.shape[0] != B or k_cache.shape[2] != Hk * D or k_cache.shape[1] == 0:
-        raise ValueError(f"{what}: k_cache must be [B, S, num_kv_heads * D] = [{B}, S, {Hk * D}]")
-    if v_cache.shape != k_cache.shape:
-        raise ValueError(f"{what}: v_cache must have k_cache's shape")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise ValueError(f"{what}: the caches must have q's type")
-    if cache_lens.dtype != torch.int32 or tuple(cache_lens.shape) != (B,):
-        raise ValueError(f"{what}: cache_lens must be int32 [B] = [{B}]")
-    _lib.check_tensors(what, q.device, k_cache=k_cache, v_cache=v_cache, cache_lens=cache_lens)
-
-
-def _cache_strides(what, c, D):
-    """Strides of a cache that is read or written in place."""
-    if c.stride(2) != 1 or c.data_ptr() % 16 != 0 or (c.stride(0) | c.stride(1)) & 7:
-        raise ValueError(f"{what}: cache rows must be contiguous and 16-byte aligned")
-    return _lib.i64arr((c.stride(0), D, c.stride(1)))
-
-
-def _no_grad_inputs(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{what} is not differentiable: call it under torch.no_grad()")
+    return _QKNormRopeFunc.apply(q, k, q_weight, k_weight, _lib.flat(cos), _lib.flat(sin), positions, geo, float(eps),
+                                 int(bool(interleaved)))
 
 
 def flash_qk_norm_rope_append(
@@ -221,36 +184,47 @@ def flash_qk_norm_rope_append(
     Returns the prepared q ``[B, T, num_heads * D]``.
     """
     what = "flash_qk_norm_rope_append"
-    _no_grad_inputs(what, q, k, v, q_weight, k_weight, k_cache, v_cache)
-    H, Hk, D, R = _check_common(what, q, k, num_heads, num_kv_heads, cos, sin, q_weight, k_weight, eps)
-    B, T, C = q.shape
+    _lib.no_grad_inputs(what, q, k, v, q_weight, k_weight, k_cache, v_cache)
+    H, Hk, D, R, wt = _check(what, q, k, num_heads, num_kv_heads, cos, sin, q_weight, k_weight, eps)
+    B, T, _ = q.shape
     if v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"{what}: v must have k's shape and type")
-    _check_cache(what, k_cache, v_cache, cache_lens, B, Hk, D, q)
-    _lib.check_tensors(what, q.device, v=v)
-    if any(c.stride(0) == 0 and B > 1 for c in (k_cache, v_cache)) or any(
-            c.stride(1) == 0 and c.shape[1] > 1 for c in (k_cache, v_cache)):
-        raise ValueError(f"{what}: the caches must not be expanded")
-    if not -(1 << 31) <= int(position_offset) < (1 << 31):
+    check_cache(what, q, k_cache, v_cache, cache_lens, B, Hk * D)
+    _lib.check_device(what, q.device, v)
+    kca, kcs = _lib.rows_in_place(what, k_cache, Hk)
+    vca, vcs = _lib.rows_in_place(what, v_cache, Hk)
+    if 0 in k_cache.stride() or 0 in v_cache.stride():
+        for c in (k_cache, v_cache):
+            if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
+                raise ValueError(f"{what}: the caches must not be expanded")
+    if not -(1 << 31) <= position_offset < (1 << 31):
         raise ValueError(f"{what}: position_offset out of range")
-    dev = q.device
-    qq, qs = _lib.token_view(q, "bnc", H)
-    kk, ks = _lib.token_view(k, "bnc", Hk)
-    vv, vs = _lib.token_view(v, "bnc", Hk)
-    qw, kw, wt = _weights(q_weight, k_weight)
-    cos, sin, lens = _table(cos), _table(sin), cache_lens.contiguous()
-    kcs, vcs = _cache_strides(what, k_cache, D), _cache_strides(what, v_cache, D)
-    qo = torch.empty(B, T, C, device=dev, dtype=q.dtype)
-    with _lib.on_device(dev):
-        rc = _lib.lib().fta_qk_norm_rope_append(
-            _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(kk), _lib.i64arr(ks), _lib.ptr(vv), _lib.i64arr(vs),
-            _lib.dtype_code(q.dtype), B, H, Hk, T, D, _lib.ptr(qw), _lib.ptr(kw), wt, _lib.ptr(cos), _lib.ptr(sin),
-            cos.shape[0], R, int(position_offset), float(eps), int(bool(interleaved)), _lib.ptr(lens),
-            k_cache.shape[1], _lib.ptr(qo), _dense(B, T, H, D), _lib.ptr(k_cache), kcs, _lib.ptr(v_cache), vcs,
-            _lib.stream_ptr(dev))
-    _lib.check(rc, what)
+    q, qa, qs = _lib.rows(q, H)
+    k, ka, ks = _lib.rows(k, Hk)
+    v, va, vs = _lib.rows(v, Hk)
+    qw, kw = (None if w is None else _lib.flat(w) for w in (q_weight, k_weight))
+    cos, sin, lens = _lib.flat(cos), _lib.flat(sin), cache_lens.contiguous()
+    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    _lib.call("fta_qk_norm_rope_append", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, D,
+              _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, int(position_offset),
+              float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),
+              _lib.dense_strides(q.shape, H), kca, kcs, vca, vcs)
     torch.autograd.graph.increment_version((k_cache, v_cache))
     return qo
+
+
+def check_cache(what, q, k_cache, v_cache, cache_lens, B, width):
+    """Shapes, types and devices of a pair of caches and their lengths."""
+    shape = k_cache.shape
+    if len(shape) != 3 or shape[0] != B or shape[2] != width or shape[1] == 0:
+        raise ValueError(f"{what}: k_cache must be [B, S, num_kv_heads * D] = [{B}, S, {width}]")
+    if v_cache.shape != shape:
+        raise ValueError(f"{what}: v_cache must have k_cache's shape")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise ValueError(f"{what}: the caches must have q's type")
+    if cache_lens.dtype != torch.int32 or cache_lens.shape != (B,):
+        raise ValueError(f"{what}: cache_lens must be int32 [B] = [{B}]")
+    _lib.check_device(what, q.device, k_cache, v_cache, cache_lens)
 
 
 __all__ = ["flash_qk_norm_rope", "flash_qk_norm_rope_append"]

@@ -6,7 +6,7 @@ No counterpart in the reference.
 
 from __future__ import annotations
 
-import math
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -17,59 +17,67 @@ from .cache_attn import cache_attn
 _MAX = (1 << 30) - 1  # windows past this are the same as this
 
 
-def _scale(what, scale, D):
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError(f"{what}: scale must be positive and finite")
-    return scale
+@lru_cache(maxsize=1024)
+def _geometry(what, q, k, v, dtypes, num_heads, num_kv_heads, window, num_sinks, scale):
+    """``(H, Hk, D, left, right, sinks, scale)``, checked (calls of one shape are checked once)."""
+    if len(q) != 3 or len(k) != 3 or len(v) != 3:
+        raise ValueError(f"{what}: q, k and v must be [B, N, heads * D]")
+    if dtypes[0] not in _lib.HALVES or dtypes != (dtypes[0],) * 3:
+        raise ValueError(f"{what}: q, k and v must all be float16 or all bfloat16")
+    B, N, C = q
+    H, Hk, D = _lib.head_counts(what, C, num_heads, num_kv_heads)
+    if B == 0 or N == 0:
+        raise ValueError(f"{what}: empty batch or sequence")
+    if tuple(k) != (B, N, Hk * D) or tuple(v) != (B, N, Hk * D):
+        raise ValueError(f"{what}: k and v must be [B, N, num_kv_heads * D] = {[B, N, Hk * D]}")
+    if len(window) != 2 or int(window[0]) < 0 or int(window[1]) < 0:
+        raise ValueError(f"{what}: window must be (left, right), both non-negative")
+    if int(num_sinks) < 0:
+        raise ValueError(f"{what}: num_sinks must be non-negative")
+    left, right, sinks = (min(int(x), _MAX) for x in (*window, num_sinks))
+    return H, Hk, D, left, right, sinks, _lib.softmax_scale(what, scale, D)
 
 
 class _WindowAttnFunc(torch.autograd.Function):
     """Autograd function behind ``flash_window_attn``."""
 
     @staticmethod
-    def forward(ctx, q, k, v, lens, H, Hk, left, right, sinks, scale):
-        B, N, C = q.shape
-        D, dev = C // H, q.device
-        qq, qs = _lib.token_view(q, "bnc", H)
-        kk, ks = _lib.token_view(k, "bnc", Hk)
-        vv, vs = _lib.token_view(v, "bnc", Hk)
-        o = torch.empty(B, N, C, device=dev, dtype=q.dtype)
-        lse = torch.empty(B, H, N, device=dev, dtype=torch.float32)
-        with _lib.on_device(dev):
-            rc = _lib.lib().fta_window_attn_fwd(
-                _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(kk), _lib.i64arr(ks), _lib.ptr(vv), _lib.i64arr(vs),
-                _lib.dtype_code(q.dtype), B, H, Hk, N, D, _lib.ptr(lens), left, right, sinks, scale, _lib.ptr(o),
-                _lib.i64arr((N * C, D, C)), _lib.ptr(lse), _lib.stream_ptr(dev))
-        _lib.check(rc, "flash_window_attn")
+    def forward(ctx, q, k, v, lens, geo):
+        H, Hk, D, left, right, sinks, scale = geo
+        B, N, _ = q.shape
+        q, qa, qs = _lib.rows(q, H)
+        k, ka, ks = _lib.rows(k, Hk)
+        v, va, vs = _lib.rows(v, Hk)
+        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        lse = torch.empty(B, H, N, device=q.device, dtype=torch.float32)
+        _lib.call("fta_window_attn_fwd", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, N, D,
+                  _lib.ptr(lens), left, right, sinks, scale, o.data_ptr(), _lib.dense_strides(q.shape, H),
+                  lse.data_ptr())
         ctx.save_for_backward(q, k, v, o, lse, lens)
-        ctx.args = H, Hk, left, right, sinks, scale
+        ctx.geo = geo
         ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return o, lse
 
     @staticmethod
     def backward(ctx, do, _dlse):
+        if do is None:
+            return None, None, None, None, None
         q, k, v, o, lse, lens = ctx.saved_tensors
-        H, Hk, left, right, sinks, scale = ctx.args
-        B, N, C = q.shape
-        D, dev = C // H, q.device
-        qq, qs = _lib.token_view(q, "bnc", H)
-        kk, ks = _lib.token_view(k, "bnc", Hk)
-        vv, vs = _lib.token_view(v, "bnc", Hk)
-        dd, ds = _lib.token_view(do, "bnc", H)
-        dq = torch.empty(B, N, C, device=dev, dtype=q.dtype)
-        dk = torch.empty(B, N, Hk * D, device=dev, dtype=q.dtype)
-        dv = torch.empty(B, N, Hk * D, device=dev, dtype=q.dtype)
-        sq, sk = _lib.i64arr((N * C, D, C)), _lib.i64arr((N * Hk * D, D, Hk * D))
-        ws = _lib.workspace(_lib.size_of("fta_window_attn_bwd_workspace_size", B, H, Hk, N, D, left, right, sinks), dev)
-        with _lib.on_device(dev):
-            rc = _lib.lib().fta_window_attn_bwd(
-                _lib.ptr(qq), _lib.i64arr(qs), _lib.ptr(kk), _lib.i64arr(ks), _lib.ptr(vv), _lib.i64arr(vs),
-                _lib.ptr(o), sq, _lib.ptr(dd), _lib.i64arr(ds), _lib.dtype_code(q.dtype), B, H, Hk, N, D,
-                _lib.ptr(lens), left, right, sinks, scale, _lib.ptr(lse), _lib.ptr(dq), sq, _lib.ptr(dk), sk,
-                _lib.ptr(dv), sk, _lib.ptr(ws), ws.numel(), _lib.stream_ptr(dev))
-        _lib.check(rc, "flash_window_attn backward")
-        return dq, dk, dv, None, None, None, None, None, None, None
+        H, Hk, D, left, right, sinks, scale = ctx.geo
+        B, N, _ = q.shape
+        q, qa, qs = _lib.rows(q, H)
+        k, ka, ks = _lib.rows(k, Hk)
+        v, va, vs = _lib.rows(v, Hk)
+        do, da, ds = _lib.rows(do, H)
+        dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
+        sq, sk = _lib.dense_strides(q.shape, H), _lib.dense_strides(k.shape, Hk)
+        nbytes = _lib.size_of("fta_window_attn_bwd_workspace_size", B, H, Hk, N, D, left, right, sinks)
+        ws = _lib.workspace(nbytes, q.device)
+        _lib.call("fta_window_attn_bwd", q.device, qa, qs, ka, ks, va, vs, o.data_ptr(), sq, da, ds,
+                  _lib.DTYPE_CODES[q.dtype], B, H, Hk, N, D, _lib.ptr(lens), left, right, sinks, scale, lse.data_ptr(),
+                  dq.data_ptr(), sq, dk.data_ptr(), sk, dv.data_ptr(), sk, ws.data_ptr(), nbytes)
+        return dq, dk, dv, None, None
 
 
 def flash_window_attn(
@@ -108,28 +116,16 @@ def flash_window_attn(
         is not differentiable.
     """
     what = "flash_window_attn"
-    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
-        raise ValueError(f"{what}: q, k and v must be [B, N, heads * D]")
-    if q.device.type != "cuda":
+    if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"{what}: q, k and v must all be float16 or all bfloat16")
-    B, N, C = q.shape
-    H, Hk, D = _lib.head_counts(what, C, num_heads, num_kv_heads)
-    if B == 0 or N == 0:
-        raise ValueError(f"{what}: empty batch or sequence")
-    if tuple(k.shape) != (B, N, Hk * D) or tuple(v.shape) != (B, N, Hk * D):
-        raise ValueError(f"{what}: k and v must be [B, N, num_kv_heads * D] = {[B, N, Hk * D]}")
-    if len(window) != 2 or int(window[0]) < 0 or int(window[1]) < 0:
-        raise ValueError(f"{what}: window must be (left, right), both non-negative")
-    if int(num_sinks) < 0:
-        raise ValueError(f"{what}: num_sinks must be non-negative")
-    if seq_lens is not None and (seq_lens.dtype != torch.int32 or tuple(seq_lens.shape) != (B,)):
-        raise ValueError(f"{what}: seq_lens must be int32 [B] = [{B}]")
-    _lib.check_tensors(what, q.device, k=k, v=v, seq_lens=seq_lens)
-    left, right, sinks = (min(int(x), _MAX) for x in (*window, num_sinks))
-    lens = None if seq_lens is None else seq_lens.contiguous()
-    return _WindowAttnFunc.apply(q, k, v, lens, H, Hk, left, right, sinks, _scale(what, scale, D))
+    geo = _geometry(what, q.shape, k.shape, v.shape, (q.dtype, k.dtype, v.dtype), num_heads, num_kv_heads, tuple(window),
+                    num_sinks, scale)
+    _lib.check_device(what, q.device, k, v, seq_lens)
+    if seq_lens is not None:
+        if seq_lens.dtype != torch.int32 or seq_lens.shape != q.shape[:1]:
+            raise ValueError(f"{what}: seq_lens must be int32 [B] = [{q.shape[0]}]")
+        seq_lens = seq_lens.contiguous()
+    return _WindowAttnFunc.apply(q, k, v, seq_lens, geo)
 
 
 def flash_window_attn_decode(
