@@ -106,11 +106,11 @@ __global__ __launch_bounds__(CacheShape<D>::NW * 64) void fta_cache_attn_kernel(
     if (it0 + wave < it1) {  // wave-uniform
         const uint16_t* kp = a.k + b * a.k_sb + hk * a.k_sh;
         const uint16_t* vp = a.v + b * a.v_sb + hk * a.v_sh;
-        uint4 qf[T::KS];
+        fta_frag qf[T::KS];
         T::load_rows(a.q + q_offset(a, b, hk, min(r, a.R - 1)), r < a.R, a.Dreal, lane, qf);
         FtaGather<D, 1, 32> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, 0, lane);
-        const auto lo = T::lane_offsets(lane);
+        const FtaLane lo = fta_lane_offsets<D>(lane);
         auto key = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
         auto issue = [&](int it, int st) {
             const int kb = key(it);
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefi
 
     const uint16_t* kp = a.kp + hk * a.kp_sh;
     const uint16_t* vp = a.vp + hk * a.vp_sh;
-    uint4 qf[T::KS];
+    fta_frag qf[T::KS];
     T::load_rows(a.q + q_offset(a, b, hk, r), ok, a.Dreal, lane, qf);
     f32x16 oacc[T::DT32];
 #pragma unroll
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefi
     FtaGather<D, NW, 64> g;
     g.start(a.kp_sn, a.vp_sn, a.Dreal, wave, lane);
     const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
-    const auto lo = T::lane_offsets(lane);
+    const FtaLane lo = fta_lane_offsets<D>(lane);
     auto issue = [&](int it, int st) {
         const int kb = 64 * it;
         const uint32_t lds = lds0 + st * Sh::STAGE_B;

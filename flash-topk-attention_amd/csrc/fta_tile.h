@@ -27,6 +27,55 @@ __device__ __forceinline__ void fta_static_for(F& f) {
 // instruction wrote it, and nothing sees that distance into inline asm).
 __device__ __forceinline__ int fta_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Bits [lo, hi) of a 32-bit mask; lo and hi may lie anywhere.
+__device__ __forceinline__ uint32_t fta_bits_below(int hi) { return hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u; }
+__device__ __forceinline__ uint32_t fta_bits(int lo, int hi) { return fta_bits_below(hi) & ~fta_bits_below(lo); }
+
+// An MFMA operand fragment.  A vector type all the way from its load: as a struct of four
+// words the compiler may read it word by word (two ds_read2_b32 instead of one
+// ds_read_b128, which conflict in LDS: the D = 256 forward spent two thirds of its LDS
+// cycles on that).
+typedef unsigned int fta_frag __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ f32x16 fta_mma(fta_frag a, fta_frag b, f32x16 c) {
+    if constexpr (DT == FTA_DTYPE_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(fta_bf16x8, a), __builtin_bit_cast(fta_bf16x8, b), c,
+                                                       0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(fta_f16x8, a), __builtin_bit_cast(fta_f16x8, b), c, 0,
+                                                      0, 0);
+}
+// 16 bytes of LDS, and two 8-byte transpose reads, by byte address
+__device__ __forceinline__ fta_frag fta_lds_frag(uint32_t addr) {
+    return *(__attribute__((address_space(3))) const fta_frag*)addr;
+}
+__device__ __forceinline__ fta_frag fta_lds_tr_frag(uint32_t lo, uint32_t hi) {
+    const fta_s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((fta_lds_s16x4*)lo);
+    const fta_s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((fta_lds_s16x4*)hi);
+    return __builtin_bit_cast(fta_frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+// eight fp32 values rounded to a fragment
+template <int DT>
+__device__ __forceinline__ fta_frag fta_pack_frag(const float* f) {
+    return fta_frag{Elem<DT>::pack2(f[0], f[1]), Elem<DT>::pack2(f[2], f[3]), Elem<DT>::pack2(f[4], f[5]),
+                    Elem<DT>::pack2(f[6], f[7])};
+}
+
+// Per-lane byte offsets of the operand fragments in a tile of D columns: K (or V) rows,
+// and the two halves of a transposed fragment.  Other k slices and column tiles differ by
+// an XOR of their slot bits, 16 or 32 rows down by a constant.
+struct FtaLane {
+    uint32_t row, tr0, tr1;
+};
+template <int D>
+__device__ __forceinline__ FtaLane fta_lane_offsets(int lane) {
+    using SW = FtaSwz<D / 8>;
+    const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+    return {2u * SW::off(lane & 31, lane >> 5), 2u * (SW::off(vr, vc >> 3) + (vc & 7)),
+            2u * (SW::off(vr + 8, vc >> 3) + (vc & 7))};
+}
+
 template <int DT, int D, int NH>
 struct FtaTile {
     using E = Elem<DT>;
@@ -37,29 +86,18 @@ struct FtaTile {
     static constexpr int KS = D / 16, DT32 = D / 32;
     using SW = FtaSwz<QSEG>;
 
-    // Per-lane byte offsets of the operand fragments in a tile: K (or V) rows, and
-    // the two halves of a transposed fragment.  Other k slices and column tiles
-    // differ by an XOR of their slot bits, 16 or 32 rows down by a constant.
-    struct Lane {
-        uint32_t row, tr0, tr1;
-    };
-    __device__ static __forceinline__ Lane lane_offsets(int lane) {
-        const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-        return {2u * SW::off(lane & 31, lane >> 5), 2u * (SW::off(vr, vc >> 3) + (vc & 7)),
-                2u * (SW::off(vr + 8, vc >> 3) + (vc & 7))};
+    __device__ static __forceinline__ fta_frag row_frag(uint32_t base, const FtaLane& l, int half, int ks) {
+        return fta_lds_frag(((base + l.row) ^ (ks * 32)) + half * 32 * QSEG * 16);
     }
-    __device__ static __forceinline__ uint4 row_frag(uint32_t base, const Lane& l, int half, int ks) {
-        return fta_lds_b128(((base + l.row) ^ (ks * 32)) + half * 32 * QSEG * 16);
-    }
-    __device__ static __forceinline__ uint4 tr_frag(uint32_t base, const Lane& l, int ks, int dt) {
+    __device__ static __forceinline__ fta_frag tr_frag(uint32_t base, const FtaLane& l, int ks, int dt) {
         const uint32_t x = ks * 16 * QSEG * 16;
-        return fta_lds_tr(((base + l.tr0) ^ (dt * 64)) + x, ((base + l.tr1) ^ (dt * 64)) + x);
+        return fta_lds_tr_frag(((base + l.tr0) ^ (dt * 64)) + x, ((base + l.tr1) ^ (dt * 64)) + x);
     }
 
     // s[half] = (K Q^T)[32 half .. + 31][row], fragments read PD MFMAs ahead.
     template <int PD>
-    __device__ static __forceinline__ void qk(uint32_t kbase, const Lane& l, const uint4* qf, f32x16* s) {
-        uint4 fr[PD + 1];
+    __device__ static __forceinline__ void qk(uint32_t kbase, const FtaLane& l, const fta_frag* qf, f32x16* s) {
+        fta_frag fr[PD + 1];
         auto load = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value;
             if constexpr (n < NH * KS) fr[n % (PD + 1)] = row_frag(kbase, l, n % NH, n / NH);
@@ -72,7 +110,7 @@ struct FtaTile {
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
             }
-            s[n % NH] = E::mma(fr[n % (PD + 1)], qf[n / NH], s[n % NH]);
+            s[n % NH] = fta_mma<DT>(fr[n % (PD + 1)], qf[n / NH], s[n % NH]);
         };
         fta_static_for<0, PD>(load);
         fta_static_for<0, NH * KS>(slot);
@@ -84,14 +122,18 @@ struct FtaTile {
     // P stays below 2^8 and its 16-bit rounding keeps the same relative error.  A row
     // that has seen no key yet keeps m = -inf and adds exact zeros.
     template <int PD>
-    __device__ static __forceinline__ void softmax_pv(uint32_t vbase, const Lane& l, const f32x16* s, float c,
+    __device__ static __forceinline__ void softmax_pv(uint32_t vbase, const FtaLane& l, const f32x16* s, float c,
                                                       float& m_run, float& l_run, f32x16* oacc) {
         float mx = s[0][0];
 #pragma unroll
         for (int sb = 0; sb < NH; ++sb)
 #pragma unroll
             for (int i = (sb == 0); i < 16; ++i) mx = fmaxf(mx, s[sb][i]);
-        mx = fmaxf(mx, fta_xor32(mx));
+        {
+            float x = mx, y = mx;  // the row's other half of the keys is in lane ^ 32
+            fta_swap32(x, y);
+            mx = fmaxf(x, y);
+        }
         const float mn = fmaxf(m_run, mx);
         const bool grow = (mn - m_run) * c > 8.f;
         if (__ballot(grow) != 0ull) {
@@ -106,8 +148,8 @@ struct FtaTile {
         const float mc = (m_run == -FTA_INF) ? 0.f : m_run * c;
         float ls = 0.f;
         constexpr int NM = 2 * NH * DT32;
-        uint4 fr[PD + 1];
-        uint32_t pw[4];
+        fta_frag fr[PD + 1];
+        fta_frag pf;
         auto load = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value;
             if constexpr (n < NM) fr[n % (PD + 1)] = tr_frag(vbase, l, n / DT32, n % DT32);
@@ -123,10 +165,9 @@ struct FtaTile {
                     pv[e] = fta_exp2(fmaf(s[ks >> 1][8 * (ks & 1) + e], c, -mc));
                     ls += pv[e];
                 }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) pw[e] = E::pack2(pv[2 * e], pv[2 * e + 1]);
+                pf = fta_pack_frag<DT>(pv);
             }
-            oacc[n % DT32] = E::mma(fr[n % (PD + 1)], make_uint4(pw[0], pw[1], pw[2], pw[3]), oacc[n % DT32]);
+            oacc[n % DT32] = fta_mma<DT>(fr[n % (PD + 1)], pf, oacc[n % DT32]);
         };
         fta_static_for<0, PD>(load);
         fta_static_for<0, NM>(slot);
@@ -134,12 +175,23 @@ struct FtaTile {
         l_run += ls;
     }
 
+    // -inf for the scores of 32 keys whose bit of `seen` (bit = key) is clear.
+    __device__ static __forceinline__ void mask(uint32_t seen, int lane, f32x16& s) {
+        const uint32_t m = seen >> (4 * (lane >> 5));  // register r holds key (r >> 2) * 8 + (r & 3) of these
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint32_t k = (uint32_t)(((int)(m << (31 - ((r >> 2) * 8 + (r & 3))))) >> 31);
+            const float v = s[r];
+            s[r] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & k) | (0xff800000u & ~k));
+        }
+    }
+
     // A wave's Q (or dO) rows as B operands: row `ok ? p : none` of this lane, zero past Dreal.
-    __device__ static __forceinline__ void load_rows(const uint16_t* p, bool ok, int Dreal, int lane, uint4* f) {
+    __device__ static __forceinline__ void load_rows(const uint16_t* p, bool ok, int Dreal, int lane, fta_frag* f) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = ks * 16 + (lane >> 5) * 8;
-            f[ks] = (ok && d < Dreal) ? *reinterpret_cast<const uint4*>(p + d) : fta_zero4();
+            f[ks] = (ok && d < Dreal) ? *reinterpret_cast<const fta_frag*>(p + d) : fta_frag{0u, 0u, 0u, 0u};
         }
     }
     // One row of O^T (this lane's column), scaled and rounded once.

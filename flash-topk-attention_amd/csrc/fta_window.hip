@@ -24,6 +24,11 @@
 
 namespace {
 
+// Waves per workgroup of the forward and dQ.  Eight, whose K / V tiles serve twice the rows, keep
+// a SIMD's two waves in step through each tile's barrier, so that both want the same pipe at
+// the same time; two workgroups of four drift apart (32K tokens, 32 / 8 heads of 128, window
+// 1024: forward 747 -> 733 us, dQ 1025 -> 944).  Two were slower on small grids too.
+constexpr int kRowWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
 struct WinArgs {
@@ -49,23 +54,24 @@ __device__ __forceinline__ int seq_len(const WinArgs& a, int b) {
     return a.lens ? __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.N)) : a.N;
 }
 
-// The 64-key tiles that rows [i_lo, i_hi] see: `ns` tiles of sinks, then the band's.
+// The tiles of KEYS keys that rows [i_lo, i_hi] see: `ns` tiles of sinks, then the band's.
+template <int KEYS>
 struct WinWalk {
     int kb0, ke;   // the band's keys [kb0, ke)
     int ns, c_lo, iters;
     __device__ __forceinline__ WinWalk(const WinArgs& a, int len, int i_lo, int i_hi) {
         kb0 = max(0, i_lo - a.left);
         ke = min(len, i_hi + a.right + 1);
-        const int c_hi = (ke + 63) >> 6;
-        c_lo = kb0 >> 6;
-        ns = (min(a.sinks, ke) + 63) >> 6;
+        const int c_hi = (ke + KEYS - 1) / KEYS;
+        c_lo = kb0 / KEYS;
+        ns = (min(a.sinks, ke) + KEYS - 1) / KEYS;
         if (c_lo <= ns) c_lo = ns = 0;
         iters = ns + c_hi - c_lo;
     }
-    __device__ __forceinline__ int key(int it) const { return 64 * (it < ns ? it : c_lo + it - ns); }
-    // whether all 64 rows of the tile at kb are keys that the workgroup sees
+    __device__ __forceinline__ int key(int it) const { return KEYS * (it < ns ? it : c_lo + it - ns); }
+    // whether all rows of the tile at kb are keys that the workgroup sees
     __device__ __forceinline__ bool whole(const WinArgs& a, int kb) const {
-        return kb + 64 <= ke && (kb >= kb0 || kb + 64 <= a.sinks);
+        return kb + KEYS <= ke && (kb >= kb0 || kb + KEYS <= a.sinks);
     }
     // a key that the workgroup sees in place of one that it does not
     __device__ __forceinline__ int seen(const WinArgs& a, int t) const {
@@ -73,28 +79,23 @@ struct WinWalk {
     }
 };
 
-// Mask case of the tile at kb for rows [i0, i0 + 31]: 0 nothing, 1 partly, 2 all visible.
+// Mask case of the 32 keys at kb for rows [i0, i0 + 31]: 0 nothing, 1 partly, 2 all visible.
 __device__ __forceinline__ int tile_case(const WinArgs& a, int len, int i0, int kb) {
-    const int i1 = min(i0 + 31, len - 1);
-    if (i0 >= len || kb > i1 + a.right || (kb + 63 < i0 - a.left && kb >= a.sinks)) return 0;
-    if (kb + 63 <= i0 + a.right && kb + 63 < len && (kb >= i0 + 31 - a.left || kb + 63 < a.sinks)) return 2;
+    const int i1 = min(i0 + 31, len - 1), k1 = kb + 31;
+    if (i0 >= len || kb > i1 + a.right || (k1 < i0 - a.left && kb >= a.sinks)) return 0;
+    if (k1 <= i0 + a.right && k1 < len && (kb >= i0 + 31 - a.left || k1 < a.sinks)) return 2;
     return 1;
 }
 
-// -inf for the scores of 32 keys (tile row of register r: rel0 + c_row) that row i does not see.
-__device__ __forceinline__ void mask_scores(const WinArgs& a, int len, int i, int kb, int rel0, int lane, f32x16& s) {
-    const int hi = min(i + a.right, len - 1) - kb - rel0, lo = i - a.left - kb - rel0, sk = a.sinks - kb - rel0;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int rel = c_row(r, lane);
-        s[r] = (rel <= hi && (rel >= lo || rel < sk)) ? s[r] : -FTA_INF;
-    }
+// Which of the 32 keys at kb row i sees (bit = key).
+__device__ __forceinline__ uint32_t seen_keys(const WinArgs& a, int len, int i, int kb) {
+    return fta_bits_below(min(i + a.right, len - 1) + 1 - kb) & (~fta_bits_below(i - a.left - kb) | fta_bits_below(a.sinks - kb));
 }
 
 // Workgroup -> (b, head group, token tile); late tiles first: without a window they walk the most keys.
 struct WinPlace {
     int b, h, hk, i0, i_lo, tok;  // batch, this wave's query head, its K/V head, its first row; the workgroup's first row, rows
-    __device__ __forceinline__ WinPlace(const WinArgs& a, int nw, int wave) {
+    __device__ __forceinline__ WinPlace(const WinArgs& a, int wave) {
         const int wgi = fta_xcd_remap(blockIdx.x, a.total);
         const int groups = a.H / a.hw;
         const int bg = fta_scalar(wgi / a.tiles), tile = a.tiles - 1 - (wgi - bg * a.tiles);
@@ -102,38 +103,44 @@ struct WinPlace {
         b = fta_scalar(bg / groups);
         h = (bg - b * groups) * a.hw + wave - wt * a.hw;
         hk = fta_scalar(h / a.G);
-        tok = 32 * fta_scalar(nw / a.hw);
+        tok = 32 * fta_scalar(kRowWaves / a.hw);
         i_lo = tile * tok;
         i0 = i_lo + 32 * wt;
     }
 };
 
-// Stages of the forward and dQ: 64-key K and V tiles in LDS, NST - 1 ahead.  Eight
-// waves take the LDS of three stages (two workgroups share a CU at D = 64), four
-// waves two stages, so that more of these smaller workgroups fit.
-template <int D, int NW>
+// Stages of the forward and dQ: tiles of 32 NH keys of K and V, two in LDS.
+template <int D, int NH>
 struct WinShape {
-    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 2>::TEN_B;
-    static constexpr int NST = (NW == 8) ? 3 : 2;
-    static constexpr int PDK = D <= 64 ? 3 : 6, PDV = D <= 64 ? 2 : 4;
+    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, NH>::TEN_B;
+    static constexpr int NST = 2;
 };
 // waves per SIMD that the registers leave room for
-constexpr int win_fwd_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
-constexpr int win_dq_waves(int D) { return D <= 128 ? 2 : 1; }
+constexpr int win_fwd_waves(int D) { return D <= 64 ? 4 : 2; }
+constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 
 // ----------------------------------------------------------------------------
-// Forward.  NW waves of 32 rows: hw query heads that share a K/V head, NW / hw row
-// tiles each.
+// Forward.  Four waves of 32 rows: hw query heads that share a K/V head, 4 / hw row
+// tiles each; 64-key tiles of K and V (32 at D = 256), worked on 32 keys at a time so
+// that the half tiles at the band's edges and the sinks' tile cost what they hold.
+// What bounds it: neither pipe alone.  N32768, 32 / 8 heads of 128, window 1024, 4 sinks:
+// 730 us, 835 TFLOP/s with the masked scores (65% of a large library product on the same
+// card); matrix units 38% busy, vector units 35%, LDS 45%; more waves per SIMD (three, by
+// 32-key stages) and other prefetch distances or wave priorities change it by under 4%.
+// D = 256 is held to 256 registers, two workgroups per CU: with 512 the compiler moved the
+// whole accumulator through copies at every tile (N4096, 16 / 2 heads, window 512: 150 ->
+// 107 us).
 // ----------------------------------------------------------------------------
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(NW * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
-    using T = FtaTile<DT, D, 2>;
-    using Sh = WinShape<D, NW>;
-    constexpr int NST = Sh::NST, LQ = FtaGather<D, NW, 64>::LQ;
+template <int DT, int D, int NH>
+__global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
+    using T = FtaTile<DT, D, 1>;
+    using Sh = WinShape<D, NH>;
+    constexpr int PD = D <= 128 ? 3 : 2;  // fragments read ahead
+    constexpr int NST = Sh::NST, KEYS = 32 * NH, LQ = FtaGather<D, kRowWaves, KEYS>::LQ;
     __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const WinPlace p(a, NW, wave);
+    const WinPlace p(a, wave);
     const int len = seq_len(a, p.b);
     const int row = p.i0 + (lane & 31);
     uint16_t* out = a.out0 + p.b * a.o0_sb + p.h * a.o0_sh + (int64_t)row * a.o0_sn;
@@ -149,13 +156,13 @@ __global__ __launch_bounds__(NW * 64, win_fwd_waves(D)) void fta_window_fwd_kern
     if (p.i_lo < len) {  // workgroup-uniform
         const uint16_t* kp = a.k + p.b * a.k_sb + p.hk * a.k_sh;
         const uint16_t* vp = a.v + p.b * a.v_sb + p.hk * a.v_sh;
-        uint4 qf[T::KS];
+        fta_frag qf[T::KS];
         T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, row < len, a.Dreal, lane, qf);
-        const WinWalk w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
-        FtaGather<D, NW, 64> g;
+        const WinWalk<KEYS> w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        FtaGather<D, kRowWaves, KEYS> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
         const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
-        const auto lo = T::lane_offsets(lane);
+        const FtaLane lo = fta_lane_offsets<D>(lane);
         auto issue = [&](int it, int st) {
             const int kb = w.key(it);
             const uint32_t lds = lds0 + st * Sh::STAGE_B;
@@ -177,16 +184,16 @@ __global__ __launch_bounds__(NW * 64, win_fwd_waves(D)) void fta_window_fwd_kern
             __syncthreads();  // tile `it` visible; every wave is past tile it - 1
             if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
             const int kb = w.key(it);
-            const int mc = tile_case(a, len, p.i0, kb);
-            if (mc != 0) {
-                const uint32_t kbase = lds0 + cur * Sh::STAGE_B;
-                f32x16 s[2];
-                T::template qk<Sh::PDK>(kbase, lo, qf, s);
-                if (mc == 1) {
-                    mask_scores(a, len, row, kb, 0, lane, s[0]);
-                    mask_scores(a, len, row, kb, 32, lane, s[1]);
-                }
-                T::template softmax_pv<Sh::PDV>(kbase + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
+            const uint32_t kbase = lds0 + cur * Sh::STAGE_B;
+#pragma unroll
+            for (int sb = 0; sb < NH; ++sb) {
+                const int mc = tile_case(a, len, p.i0, kb + 32 * sb);
+                if (mc == 0) continue;
+                const uint32_t hbase = kbase + sb * T::TEN_B;
+                f32x16 s[1];
+                T::template qk<PD>(hbase, lo, qf, s);
+                if (mc == 1) T::mask(seen_keys(a, len, row, kb + 32 * sb), lane, s[0]);
+                T::template softmax_pv<PD>(hbase + NH * T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
             }
             cur = (cur == NST - 1) ? 0 : cur + 1;
         }
@@ -210,16 +217,16 @@ __global__ __launch_bounds__(NW * 64, win_fwd_waves(D)) void fta_window_fwd_kern
 // dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
 // rows are at hand) and the lse in log2 units for dK / dV.
 // ----------------------------------------------------------------------------
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
+template <int DT, int D, int NH>
+__global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
     using E = Elem<DT>;
-    using T = FtaTile<DT, D, 2>;
-    using Sh = WinShape<D, NW>;
-    constexpr int NST = Sh::NST, LQ = FtaGather<D, NW, 64>::LQ, KS = T::KS;
+    using T = FtaTile<DT, D, NH>;
+    using Sh = WinShape<D, NH>;
+    constexpr int NST = Sh::NST, KEYS = 32 * NH, LQ = FtaGather<D, kRowWaves, KEYS>::LQ, KS = T::KS;
     __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const WinPlace p(a, NW, wave);
+    const WinPlace p(a, wave);
     const int len = seq_len(a, p.b);
     const int row = p.i0 + (lane & 31);
     const bool live = row < len;
@@ -233,7 +240,7 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
     if (p.i_lo < len) {  // workgroup-uniform
         const uint16_t* kp = a.k + p.b * a.k_sb + p.hk * a.k_sh;
         const uint16_t* vp = a.v + p.b * a.v_sb + p.hk * a.v_sh;
-        uint4 qf[KS], df[KS];
+        fta_frag qf[KS], df[KS];
         T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, live, a.Dreal, lane, qf);
         T::load_rows(a.dout + p.b * a.d_sb + p.h * a.d_sh + (int64_t)row * a.d_sn, live, a.Dreal, lane, df);
         float dl = 0.f, lse2 = FTA_INF;  // a padding row: every exp is exactly 0
@@ -242,12 +249,11 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const int d = ks * 16 + (lane >> 5) * 8;
-                const uint4 of = (live && d < a.Dreal) ? *reinterpret_cast<const uint4*>(op + d) : fta_zero4();
-                const uint32_t x[4] = {of.x, of.y, of.z, of.w}, y[4] = {df[ks].x, df[ks].y, df[ks].z, df[ks].w};
+                const fta_frag of = (live && d < a.Dreal) ? *reinterpret_cast<const fta_frag*>(op + d) : fta_frag{0u, 0u, 0u, 0u};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    dl = fmaf(E::to_f32((uint16_t)(x[e] & 0xffffu)), E::to_f32((uint16_t)(y[e] & 0xffffu)), dl);
-                    dl = fmaf(E::to_f32((uint16_t)(x[e] >> 16)), E::to_f32((uint16_t)(y[e] >> 16)), dl);
+                    dl = fmaf(E::to_f32((uint16_t)(of[e] & 0xffffu)), E::to_f32((uint16_t)(df[ks][e] & 0xffffu)), dl);
+                    dl = fmaf(E::to_f32((uint16_t)(of[e] >> 16)), E::to_f32((uint16_t)(df[ks][e] >> 16)), dl);
                 }
             }
             dl += fta_xor32(dl);
@@ -260,11 +266,11 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
                 }
             }
         }
-        const WinWalk w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
-        FtaGather<D, NW, 64> g;
+        const WinWalk<KEYS> w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        FtaGather<D, kRowWaves, KEYS> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
         const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
-        const auto lo = T::lane_offsets(lane);
+        const FtaLane lo = fta_lane_offsets<D>(lane);
         auto issue = [&](int it, int st) {
             const int kb = w.key(it);
             const uint32_t lds = lds0 + st * Sh::STAGE_B;
@@ -286,16 +292,17 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
             __syncthreads();  // tile `it` visible; every wave is past tile it - 1
             if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
             const int kb = w.key(it);
-            const int mc = tile_case(a, len, p.i0, kb);
-            if (mc != 0) {
-                const uint32_t kbase = lds0 + cur * Sh::STAGE_B, vbase = kbase + T::TEN_B;
-                uint4 dsf[4];
+            const uint32_t kbase = lds0 + cur * Sh::STAGE_B, vbase = kbase + T::TEN_B;
+            {
 #pragma unroll
-                for (int sb = 0; sb < 2; ++sb) {
+                for (int sb = 0; sb < NH; ++sb) {
+                    const int mc = tile_case(a, len, p.i0, kb + 32 * sb);
+                    if (mc == 0) continue;
+                    fta_frag dsf[2];
                     f32x16 s, dp;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-                    uint4 kf[2], vf[2];  // fragments one MFMA pair ahead
+                    fta_frag kf[2], vf[2];  // fragments one MFMA pair ahead
                     kf[0] = T::row_frag(kbase, lo, sb, 0);
                     vf[0] = T::row_frag(vbase, lo, sb, 0);
 #pragma unroll
@@ -304,10 +311,10 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
                             kf[(ks + 1) & 1] = T::row_frag(kbase, lo, sb, ks + 1);
                             vf[(ks + 1) & 1] = T::row_frag(vbase, lo, sb, ks + 1);
                         }
-                        s = E::mma(kf[ks & 1], qf[ks], s);
-                        dp = E::mma(vf[ks & 1], df[ks], dp);
+                        s = fta_mma<DT>(kf[ks & 1], qf[ks], s);
+                        dp = fta_mma<DT>(vf[ks & 1], df[ks], dp);
                     }
-                    if (mc == 1) mask_scores(a, len, row, kb, 32 * sb, lane, s);
+                    if (mc == 1) T::mask(seen_keys(a, len, row, kb + 32 * sb), lane, s);
 #pragma unroll
                     for (int k2 = 0; k2 < 2; ++k2) {
                         float ds[8];
@@ -316,14 +323,14 @@ __global__ __launch_bounds__(NW * 64, win_dq_waves(D)) void fta_window_dq_kernel
                             const int i = 8 * k2 + e;
                             ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
                         }
-                        dsf[2 * sb + k2] =
-                            make_uint4(E::pack2(ds[0], ds[1]), E::pack2(ds[2], ds[3]), E::pack2(ds[4], ds[5]), E::pack2(ds[6], ds[7]));
+                        dsf[k2] = fta_pack_frag<DT>(ds);
                     }
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                        for (int dt = 0; dt < T::DT32; ++dt)
+                            acc[dt] = fta_mma<DT>(T::tr_frag(kbase, lo, 2 * sb + ks, dt), dsf[ks], acc[dt]);
                 }
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-                    for (int dt = 0; dt < T::DT32; ++dt) acc[dt] = E::mma(T::tr_frag(kbase, lo, ks, dt), dsf[ks], acc[dt]);
             }
             cur = (cur == NST - 1) ? 0 : cur + 1;
         }
@@ -401,14 +408,14 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
     const int s0 = fta_scalar((int)((int64_t)all * sp / parts));
     const int U = fta_scalar((int)((int64_t)all * (sp + 1) / parts)) - s0;
 
-    uint4 kv[KS];  // K (role 0) or V (role 1) rows of this tile
+    fta_frag kv[KS];  // K (role 0) or V (role 1) rows of this tile
     {
         const uint16_t* src = hv ? a.v + b * a.v_sb + hk * a.v_sh + (int64_t)key * a.v_sn
                                  : a.k + b * a.k_sb + hk * a.k_sh + (int64_t)key * a.k_sn;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             const int d = ks * 16 + hf * 8;
-            kv[ks] = (kok && d < a.Dreal) ? *reinterpret_cast<const uint4*>(src + d) : fta_zero4();
+            kv[ks] = (kok && d < a.Dreal) ? *reinterpret_cast<const fta_frag*>(src + d) : fta_frag{0u, 0u, 0u, 0u};
         }
     }
     fta_wait_vmcnt<0>();  // complete the register loads: the DMAs are invisible to the compiler
@@ -443,13 +450,12 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
             for (int i = 0; i < 16; ++i) acc[dt][i] = 0.f;
 
         if (U > 0) {
+            // the 32 rows from `base`, chunk c of their head
             auto tile_dma = [&](const uint16_t* base, int64_t sn, bool narrow, const uint32_t* o, int c, uint32_t lds)
                 __attribute__((always_inline)) {
-                const int t0 = 32 * c;
-                if (narrow && t0 + 32 <= len) {
-                    const uint16_t* bp = base + (int64_t)t0 * sn;
+                if (narrow && 32 * c + 32 <= len) {
 #pragma unroll
-                    for (int i = 0; i < LQ; ++i) fta_dma16_so(bp, o[i], lds + (i * NW + wave) * 1024);
+                    for (int i = 0; i < LQ; ++i) fta_dma16_so(base, o[i], lds + (i * NW + wave) * 1024);
                 } else {  // the sequence's last chunk repeats its last row (masked)
                     int ln = lane;
                     asm volatile("" : "+v"(ln));
@@ -459,28 +465,38 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                         const int row = r2 / QSEG;
                         int j = SW::slot(row, r2 - row * QSEG);
                         if (j * 8 >= a.Dreal) j = 0;
-                        const int64_t t = min(t0 + row, len - 1);
+                        const int64_t t = min(row, len - 1 - 32 * c);
                         fta_dma16_at(base + t * sn + j * 8, lds + (i * NW + wave) * 1024);
                     }
                 }
             };
+            // A (query head, chunk) entry of the walk: the chunk, its Q and dO rows, and the row of
+            // its lse and delta.  The addresses are stepped, not multiplied out: at 128 scalar
+            // instructions a step the scalar unit was as busy as the matrix unit.
             struct Entry {
-                int g, c;
+                int c;
+                const uint16_t *q, *d;
+                int64_t r;
             };
-            // entry s (past the end: the last one again, so every step issues the same number)
-            const int last = s0 + U - 1;
+            const int c_end = c_lo + nch, last = s0 + U - 1;
+            const int64_t q_step = 32 * a.q_sn, d_step = 32 * a.d_sn;
+            const int64_t q_turn = a.q_sh - (nch - 1) * q_step, d_turn = a.d_sh - (nch - 1) * d_step;
+            const int64_t r_turn = a.N - 32 * (int64_t)(nch - 1);
+            // entry s after entry s - 1 (past the end: the last one again, so every step issues the same number)
             auto next = [&](Entry e, int s) __attribute__((always_inline)) {
                 if (s > last) return e;
-                return e.c + 1 < c_lo + nch ? Entry{e.g, e.c + 1} : Entry{e.g + 1, c_lo};
+                const bool turn = e.c + 1 == c_end;  // on to the next query head's first chunk
+                return Entry{turn ? c_lo : e.c + 1, e.q + (turn ? q_turn : q_step), e.d + (turn ? d_turn : d_step),
+                             e.r + (turn ? r_turn : 32)};
             };
             // step k - 2's gathers: Q and lse of entry eq (number kq), dO and delta of entry ed (kq - 1)
-            auto issue = [&](int kq, int dslot, Entry eq, Entry ed) __attribute__((always_inline)) {
-                tile_dma(q0 + eq.g * a.q_sh, a.q_sn, a.q_narrow, qoff, eq.c, ldq + (kq & 3) * TILE_B);
-                tile_dma(d0 + ed.g * a.d_sh, a.d_sn, a.d_narrow, doff, ed.c, ldd + dslot * TILE_B);
+            auto issue = [&](int kq, int dslot, const Entry& eq, const Entry& ed) __attribute__((always_inline)) {
+                tile_dma(eq.q, a.q_sn, a.q_narrow, qoff, eq.c, ldq + (kq & 3) * TILE_B);
+                tile_dma(ed.d, a.d_sn, a.d_narrow, doff, ed.c, ldd + dslot * TILE_B);
                 if (wave == 0) {
-                    const int t = min(32 * (l_isd ? ed.c : eq.c) + (lane & 31), len - 1);
-                    const float* src = (l_isd ? a.delta : a.lse2) + r0 + (int64_t)(l_isd ? ed.g : eq.g) * a.N;
-                    fta_dma4_at(src + t, ldl + (kq & 3) * 256);
+                    const int c = l_isd ? ed.c : eq.c;
+                    const float* src = l_isd ? a.delta + ed.r : a.lse2 + eq.r;
+                    fta_dma4_at(src + min(lane & 31, len - 1 - 32 * c), ldl + (kq & 3) * 256);
                 }
             };
             // mask case of chunk c for this wave's keys
@@ -492,16 +508,16 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                 return 1;
             };
             const int g0 = fta_scalar(s0 / nch);
-            const Entry first{g0, c_lo + s0 - g0 * nch};
-            Entry e1 = first;
-            int mk = mcase(first.c), mkp = 0, ck = first.c;
+            const int c0 = c_lo + s0 - g0 * nch;
+            Entry e1{c0, q0 + g0 * a.q_sh + c0 * q_step, d0 + g0 * a.d_sh + c0 * d_step, r0 + (int64_t)g0 * a.N + 32 * (int64_t)c0};
+            int mk = mcase(c0), mkp = 0, ck = c0;
             issue(0, 2, e1, e1);
             Entry e2 = next(e1, s0 + 1);
             issue(1, 0, e2, e1);
             e1 = e2;                   // entry k + 1
             e2 = next(e1, s0 + 2);     // entry k + 2
             int ds = 2;                // dO slot of entry k - 1
-            uint4 af[2];               // role 0: P_{k-1}, A operand of dV_{k-1}
+            fta_frag af[2];               // role 0: P_{k-1}, A operand of dV_{k-1}
             for (int k = 0; k <= U; ++k) {
                 // step k - 2's gathers complete (wave 0 issues the lse / delta DMA as well)
                 if (wave == 0)
@@ -515,7 +531,7 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                 const uint32_t dbase = ldd + ds * TILE_B;
                 if constexpr (!HV) {
                     const uint32_t qb = ldq + (k & 3) * TILE_B + aro, ob = dbase + bro;
-                    if (mkp == 0) af[0] = af[1] = fta_zero4();
+                    if (mkp == 0) af[0] = af[1] = fta_frag{0u, 0u, 0u, 0u};
                     // S_k (a dependent chain) interleaved with dV_{k-1} (independent MFMAs).
                     // One instruction stream for every case: without a pending accumulation P is
                     // zero and dO any finite tile; without a chain the S result is discarded.
@@ -523,18 +539,18 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                         f32x16 own;  // S_k then P_k
 #pragma unroll
                         for (int i = 0; i < 16; ++i) own[i] = 0.f;
-                        uint4 fs[2], fa2[2];
+                        fta_frag fs[2], fa2[2];
                         auto load = [&](int j, int sl) {
-                            fs[sl] = fta_lds_b128(qb ^ (j * 32));
+                            fs[sl] = fta_lds_frag(qb ^ (j * 32));
                             const uint32_t x = (j / DT32) * 16 * QSEG * 16;
-                            fa2[sl] = fta_lds_tr((ob ^ ((j % DT32) * 64)) + x, ((ob + bro8) ^ ((j % DT32) * 64)) + x);
+                            fa2[sl] = fta_lds_tr_frag((ob ^ ((j % DT32) * 64)) + x, ((ob + bro8) ^ ((j % DT32) * 64)) + x);
                         };
                         load(0, 0);
 #pragma unroll
                         for (int j = 0; j < KS; ++j) {  // KS = 2 * DT32: one accumulation MFMA per chain link
                             if (j + 1 < KS) load(j + 1, (j + 1) & 1);
-                            own = E::mma(fs[j & 1], kv[j], own);
-                            acc[j % DT32] = E::mma(af[j / DT32], fa2[j & 1], acc[j % DT32]);
+                            own = fta_mma<DT>(fs[j & 1], kv[j], own);
+                            acc[j % DT32] = fta_mma<DT>(af[j / DT32], fa2[j & 1], acc[j % DT32]);
                         }
                         __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
 #pragma unroll
@@ -558,11 +574,12 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                             for (int i = 0; i < 16; i += 4)
                                 sX[k & 1][tt][i / 4][lane] = make_float4(own[i], own[i + 1], own[i + 2], own[i + 3]);
 #pragma unroll
-                            for (int ks = 0; ks < 2; ++ks)
-                                af[ks] = make_uint4(E::pack2(own[8 * ks], own[8 * ks + 1]),
-                                                    E::pack2(own[8 * ks + 2], own[8 * ks + 3]),
-                                                    E::pack2(own[8 * ks + 4], own[8 * ks + 5]),
-                                                    E::pack2(own[8 * ks + 6], own[8 * ks + 7]));
+                            for (int ks = 0; ks < 2; ++ks) {
+                                float p8[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) p8[e] = own[8 * ks + e];
+                                af[ks] = fta_pack_frag<DT>(p8);
+                            }
                         }
                     }
                 } else if (mkp) {
@@ -572,20 +589,20 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                     for (int i = 0; i < 16; ++i) dpv[i] = 0.f;
                     {
                         constexpr int PD = 3;
-                        uint4 fr[PD + 1];
+                        fta_frag fr[PD + 1];
                         auto load = [&](auto nn) __attribute__((always_inline)) {
                             constexpr int n = decltype(nn)::value;
-                            if constexpr (n < KS) fr[n % (PD + 1)] = fta_lds_b128(ob ^ (n * 32));
+                            if constexpr (n < KS) fr[n % (PD + 1)] = fta_lds_frag(ob ^ (n * 32));
                         };
                         auto slot_ = [&](auto nn) __attribute__((always_inline)) {
                             constexpr int n = decltype(nn)::value;
                             load(std::integral_constant<int, n + PD>{});
-                            dpv = E::mma(fr[n % (PD + 1)], kv[n], dpv);
+                            dpv = fta_mma<DT>(fr[n % (PD + 1)], kv[n], dpv);
                         };
                         fta_static_for<0, PD>(load);
                         fta_static_for<0, KS>(slot_);
                     }
-                    uint4 ds2[2];  // dS = P (dP - delta)
+                    fta_frag ds2[2];  // dS = P (dP - delta)
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks) {
                         float dv8[8];
@@ -599,23 +616,22 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
                             dv8[e + 2] = pr.z * (dpv[i + 2] - dl.z);
                             dv8[e + 3] = pr.w * (dpv[i + 3] - dl.w);
                         }
-                        ds2[ks] = make_uint4(E::pack2(dv8[0], dv8[1]), E::pack2(dv8[2], dv8[3]), E::pack2(dv8[4], dv8[5]),
-                                             E::pack2(dv8[6], dv8[7]));
+                        ds2[ks] = fta_pack_frag<DT>(dv8);
                     }
                     {
                         constexpr int PD = 3;
-                        uint4 fr[PD + 1];
+                        fta_frag fr[PD + 1];
                         auto load = [&](auto nn) __attribute__((always_inline)) {
                             constexpr int n = decltype(nn)::value;
                             if constexpr (n < KS) {
                                 constexpr int x = (n / DT32) * 16 * QSEG * 16;
-                                fr[n % (PD + 1)] = fta_lds_tr((qb ^ ((n % DT32) * 64)) + x, ((qb + bro8) ^ ((n % DT32) * 64)) + x);
+                                fr[n % (PD + 1)] = fta_lds_tr_frag((qb ^ ((n % DT32) * 64)) + x, ((qb + bro8) ^ ((n % DT32) * 64)) + x);
                             }
                         };
                         auto slot_ = [&](auto nn) __attribute__((always_inline)) {
                             constexpr int n = decltype(nn)::value;
                             load(std::integral_constant<int, n + PD>{});
-                            acc[n % DT32] = E::mma(ds2[n / DT32], fr[n % (PD + 1)], acc[n % DT32]);
+                            acc[n % DT32] = fta_mma<DT>(ds2[n / DT32], fr[n % (PD + 1)], acc[n % DT32]);
                         };
                         fta_static_for<0, PD>(load);
                         fta_static_for<0, KS>(slot_);
@@ -660,40 +676,51 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
         run(std::false_type{});
 }
 
-// Sum of the dK / dV parts, added in order: one thread per (tensor, b, K/V head, key
-// of a tile with parts, 8 columns); dK takes the scale here.
-template <int DT, int D>
+// Sum of the dK / dV parts: SL threads per (tensor, b, K/V head, key of a tile with parts,
+// 8 columns) add every SL-th part and then their sums, always in the same order; dK takes
+// the scale here.  (One thread for all of a sink tile's 58 parts took 17.6 us at N 32768.)
+template <int DT, int D, int SL>
 __global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, int keys) {
     using E = Elem<DT>;
-    constexpr int DC = D / 8;
-    const int64_t per = (int64_t)a.B * a.Hk * keys * DC;
-    int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (idx >= 2 * per) return;
-    const int ten = idx >= per;  // 0: dK, 1: dV
-    idx -= ten * per;
-    const int d0 = (int)(idx % DC) * 8;
-    const int64_t rest = idx / DC;
-    const int t = (int)(rest % keys), bhk = (int)(rest / keys);
-    if (d0 >= a.Dreal) return;
-    const int tile = t >> 6;
+    constexpr int DC = D / 8, ROWS = 256 / (DC * SL);
+    __shared__ float so[SL][ROWS * D];
+    const int dc = threadIdx.x % DC, sl = threadIdx.x / DC % SL, rr = threadIdx.x / (DC * SL);
+    const int64_t rows = (int64_t)a.B * a.Hk * keys;
+    int64_t row = (int64_t)blockIdx.x * ROWS + rr;
+    const bool ok = row < 2 * rows;
+    const int ten = row >= rows;  // 0: dK, 1: dV
+    row = ok ? row - ten * rows : 0;
+    const int t = (int)(row % keys), bhk = (int)(row / keys);
+    const int tile = t >> 6, d0 = dc * 8;
     const int slots = a.ts * a.nps + (a.np > 1 ? (a.tiles - a.ts) * a.np : 0);
     const int n = tile < a.ts ? a.nps : a.np;
     const int first = tile < a.ts ? tile * a.nps : a.ts * a.nps + (tile - a.ts) * a.np;
-    if (n <= 1) return;  // written by the kernel itself
-    const float* src = a.part + ((((int64_t)ten * a.B * a.Hk + bhk) * slots + first) * 64 + (t & 63)) * D + d0;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < n; ++p, src += 64 * D) {
-        const float4 x0 = *reinterpret_cast<const float4*>(src);
-        const float4 x1 = *reinterpret_cast<const float4*>(src + 4);
-        o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
-        o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
+    if (ok && n > 1) {
+        const float* src = a.part + ((((int64_t)ten * a.B * a.Hk + bhk) * slots + first) * 64 + (t & 63)) * D + d0;
+        for (int p = sl; p < n; p += SL) {
+            const float4 x0 = *reinterpret_cast<const float4*>(src + (int64_t)p * 64 * D);
+            const float4 x1 = *reinterpret_cast<const float4*>(src + (int64_t)p * 64 * D + 4);
+            o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
+            o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
+        }
     }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) so[sl][rr * D + d0 + e] = o[e];
+    __syncthreads();
+    if (sl != 0 || !ok || n <= 1 || d0 >= a.Dreal) return;  // n <= 1: written by the kernel itself
     const float f = ten ? 1.f : a.scale;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int i = 1; i < SL; ++i) o[e] += so[i][rr * D + d0 + e];
+        o[e] *= f;
+    }
     const int b = bhk / a.Hk, hk = bhk - b * a.Hk;
     uint16_t* op = ten ? a.out1 + b * a.o1_sb + hk * a.o1_sh + (int64_t)t * a.o1_sn + d0
                        : a.out0 + b * a.o0_sb + hk * a.o0_sh + (int64_t)t * a.o0_sn + d0;
-    *reinterpret_cast<uint4*>(op) = make_uint4(E::pack2(o[0] * f, o[1] * f), E::pack2(o[2] * f, o[3] * f),
-                                               E::pack2(o[4] * f, o[5] * f), E::pack2(o[6] * f, o[7] * f));
+    *reinterpret_cast<uint4*>(op) = make_uint4(E::pack2(o[0], o[1]), E::pack2(o[2], o[3]), E::pack2(o[4], o[5]),
+                                               E::pack2(o[6], o[7]));
 }
 
 // ---------------------------------------------------------------------- host
@@ -727,54 +754,40 @@ int win_common(WinArgs& a, const void* q, const int64_t* qs, const void* k, cons
     return FTA_OK;
 }
 
-// Query heads per workgroup of nw waves: as many of a K/V head's as divide both.
-int heads_per_wg(int G, int nw) {
-    int hw = 1;
-    while (hw * 2 <= nw && G % (hw * 2) == 0) hw *= 2;
-    return hw;
-}
-
-// Grid of the forward and dQ for workgroups of nw waves.
-int64_t row_grid(WinArgs& a, int nw) {
-    a.hw = heads_per_wg(a.G, nw);
-    const int tok = 32 * (nw / a.hw);
+// Grid of the forward and dQ: a workgroup takes as many query heads of a K/V head as
+// divide both its waves and the group.
+int64_t row_grid(WinArgs& a) {
+    a.hw = 1;
+    while (a.hw * 2 <= kRowWaves && a.G % (a.hw * 2) == 0) a.hw *= 2;
+    const int tok = 32 * (kRowWaves / a.hw);
     a.tiles = (a.N + tok - 1) / tok;
     return (int64_t)a.B * (a.H / a.hw) * a.tiles;
 }
 
 template <int DT, int D>
 int launch_rows(WinArgs& a, bool dq, hipStream_t st) {
-    constexpr int NWL = D <= 128 ? 8 : 4;
-    int64_t grid = row_grid(a, NWL);
-    const bool small = NWL == 8 && grid < 512;
-    if (small) grid = row_grid(a, 4);
+    const int64_t grid = row_grid(a);
     if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
     a.total = (int)grid;
-    const dim3 g((unsigned)grid);
-    if (small) {
-        if (dq)
-            hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, 4>), g, dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((fta_window_fwd_kernel<DT, D, 4>), g, dim3(256), 0, st, a);
-    } else {
-        if (dq)
-            hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, NWL>), g, dim3(NWL * 64), 0, st, a);
-        else
-            hipLaunchKernelGGL((fta_window_fwd_kernel<DT, D, NWL>), g, dim3(NWL * 64), 0, st, a);
-    }
+    if (dq)
+        hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, 2>), dim3((unsigned)grid), dim3(kRowWaves * 64), 0, st, a);
+    else
+        hipLaunchKernelGGL((fta_window_fwd_kernel<DT, D, (D <= 128 ? 2 : 1)>), dim3((unsigned)grid), dim3(kRowWaves * 64), 0, st, a);
     return fta::check_launch(dq ? "fta_window_dq_kernel" : "fta_window_fwd_kernel");
 }
 
-// Parts of the dK / dV walks.  Small grids (fewer workgroups than the chip holds) cut
-// every walk into up to 4; the tiles with sinks get parts as long as the other walks.
-void dkv_parts(WinArgs& a, int Dk) {
+// Parts of the dK / dV walks.  Grids that leave CUs idle cut every walk into up to 4 parts of
+// at least 4 steps (N1024, 4 heads of 128, causal: 20.4 us whole, 15.6 + 4.5 with their sum in
+// 4; N2048, 8 on 2 heads of 64, window 256: 24.9 -> 16.5 + 9), but not ones that have a
+// workgroup for each CU (N2048, 8 heads of 128, window 256: 22 + 4.5 whole, 21.5 + 11.6 in 2).
+// The tiles with sinks get parts as long as the other walks.
+void dkv_parts(WinArgs& a) {
     a.tiles = (a.N + 63) / 64;
     a.ts = (a.sinks + 63) / 64;
-    const int64_t wgs = (int64_t)a.tiles * a.B * a.Hk, cap = 256 * (Dk <= 64 ? 3 : Dk <= 128 ? 2 : 1);
+    const int64_t wgs = (int64_t)a.tiles * a.B * a.Hk;
     const int64_t nall = (a.N + 31) / 32;
     const int64_t steps = a.G * std::min<int64_t>(nall, ((int64_t)64 + a.left + a.right + 31) / 32 + 1);
-    int64_t np = wgs >= cap ? 1 : std::min<int64_t>(4, cap / wgs);
-    np = std::max<int64_t>(1, std::min<int64_t>(np, steps / 4));
+    const int64_t np = std::max<int64_t>(1, std::min<int64_t>({4, 256 / wgs, steps / 4}));
     a.np = (int)np;
     const int64_t own = std::max<int64_t>(8, steps / np);
     a.nps = a.ts == 0 ? 1 : (int)std::max<int64_t>(np, std::min<int64_t>(128, (a.G * nall + own - 1) / own));
@@ -797,10 +810,15 @@ int launch_dkv(WinArgs& a, hipStream_t st) {
     int rc = fta::check_launch("fta_window_dkv_kernel");
     if (rc != FTA_OK || (a.np <= 1 && (a.ts == 0 || a.nps <= 1))) return rc;
     const int keys = a.np > 1 ? a.N : std::min(a.N, a.ts * 64);
-    const int64_t threads = 2 * (int64_t)a.B * a.Hk * keys * (D / 8);
-    if ((threads + 255) / 256 > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
-    hipLaunchKernelGGL((fta_window_dkv_combine_kernel<DT, D>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a,
-                       keys);
+    // many parts of few keys (the sinks alone), or a few parts of every key
+    constexpr int SLF = 256 / (D / 8) < 16 ? 256 / (D / 8) : 16;
+    const int sl = a.np > 1 ? 4 : SLF, per = 256 / (D / 8 * sl);
+    const int64_t wgs = (2 * (int64_t)a.B * a.Hk * keys + per - 1) / per;
+    if (wgs > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    if (a.np > 1)
+        hipLaunchKernelGGL((fta_window_dkv_combine_kernel<DT, D, 4>), dim3((unsigned)wgs), dim3(256), 0, st, a, keys);
+    else
+        hipLaunchKernelGGL((fta_window_dkv_combine_kernel<DT, D, SLF>), dim3((unsigned)wgs), dim3(256), 0, st, a, keys);
     return fta::check_launch("fta_window_dkv_combine_kernel");
 }
 
@@ -844,7 +862,7 @@ size_t fta_window_attn_bwd_workspace_size(int B, int H, int Hk, int N, int D, in
     if (win_common(a, nullptr, none, nullptr, none, nullptr, none, FTA_DTYPE_BF16, B, H, Hk, N, D, nullptr, left, right,
                    num_sinks, 1.f) != FTA_OK)
         return 0;
-    dkv_parts(a, kernel_dim(D));
+    dkv_parts(a);
     return 2 * rows_bytes(B, H, N) + part_bytes(a, kernel_dim(D));
 }
 
@@ -877,7 +895,7 @@ int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, 
     if (rc != FTA_OK) return rc;
     a.out0 = (uint16_t*)dk, a.o0_sb = dk_strides[0], a.o0_sh = dk_strides[1], a.o0_sn = dk_strides[2];
     a.out1 = (uint16_t*)dv, a.o1_sb = dv_strides[0], a.o1_sh = dv_strides[1], a.o1_sn = dv_strides[2];
-    dkv_parts(a, kernel_dim(D));
+    dkv_parts(a);
     return with_shape(dtype, D, [&](auto dt, auto dkk) { return launch_dkv<decltype(dt)::value, decltype(dkk)::value>(a, st); });
     FTA_TRY_END
 }
