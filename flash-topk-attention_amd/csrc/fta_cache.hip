@@ -40,7 +40,7 @@ struct CacheArgs {
     int row_tiles, ns;        // own keys: 32-row tiles of R, parts
     int pre_tiles, pre_ns;    // prefix: row tiles of B * R, parts
     int64_t rows;             // B * Hk * R
-    int total;
+    int total, pre_total;     // workgroups of either
     bool narrow, pre_narrow;
 };
 
@@ -56,28 +56,30 @@ __device__ __forceinline__ void write_row4(const CacheArgs& a, int slot, int64_t
 
 template <int D>
 struct CacheShape {
-    static constexpr int NW = D <= 128 ? 4 : 2;  // waves, each with its own stages
-    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 1>::TEN_B;
-    static constexpr int NST = 2;
+    static constexpr int NW = 4;                                           // waves
+    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 1>::TEN_B;  // 32 keys, each wave's own
+    static constexpr int PRE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, D <= 128 ? 2 : 1>::TEN_B;  // prefix: 64 (or 32) keys, shared
     static constexpr int OROW = D + 4;  // floats per row of the merge buffer
-    static constexpr int LDS_B = NW * NST * STAGE_B;
-    static_assert(NW * 32 * OROW * 4 <= LDS_B, "the merge buffer reuses the stages");
+    static constexpr int OWN_B = NW * (STAGE_B > 32 * OROW * 4 ? STAGE_B : 32 * OROW * 4);  // the merge buffer reuses the stages
+    static constexpr int LDS_B = OWN_B > 2 * PRE_B ? OWN_B : 2 * PRE_B;
 };
 
 // ----------------------------------------------------------------------------
-// Own keys.  Workgroup = (b, K/V head, row tile, part).
+// Own keys.  Workgroup = (b, K/V head, row tile, part).  A wave loads its next tile as soon
+// as it has read the last one, into the same stage: the other waves of the CU (eight at
+// D = 128, 128 KB of loads in all) cover its wait, and a second stage changed nothing.
+// What bounds it: memory.  128 requests, 32 / 8 heads of 128, 4096 of 8192 cached tokens:
+// 363 to 376 us, 5.7 to 5.9 TB/s (a large copy moves 5.15); one request: 8 us and 4 for the
+// join, latencies.
 // ----------------------------------------------------------------------------
 template <int DT, int D>
-__global__ __launch_bounds__(CacheShape<D>::NW * 64) void fta_cache_attn_kernel(CacheArgs a) {
+__device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, float2 (*sML)[32]) {
     using E = Elem<DT>;
     using T = FtaTile<DT, D, 1>;
     using Sh = CacheShape<D>;
-    constexpr int NW = Sh::NW, LQ = FtaGather<D, 1, 32>::LQ;
-    __shared__ __align__(1024) unsigned char sStage[Sh::LDS_B];
-    __shared__ float2 sML[NW][32];
+    constexpr int NW = Sh::NW;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wgi = fta_xcd_remap(blockIdx.x, a.total);
     const int rest = fta_scalar(wgi / a.ns), sp = wgi - rest * a.ns;
     const int bhk = fta_scalar(rest / a.row_tiles), rt = rest - bhk * a.row_tiles;
     const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
@@ -102,7 +104,7 @@ __global__ __launch_bounds__(CacheShape<D>::NW * 64) void fta_cache_attn_kernel(
         for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
     float m_run = -FTA_INF, l_run = 0.f;
 
-    const uint32_t lds0 = fta_lds_addr(&sStage[wave * Sh::NST * Sh::STAGE_B]);
+    const uint32_t lds0 = fta_lds_addr(sStage + wave * Sh::STAGE_B);
     if (it0 + wave < it1) {  // wave-uniform
         const uint16_t* kp = a.k + b * a.k_sb + hk * a.k_sh;
         const uint16_t* vp = a.v + b * a.v_sb + hk * a.v_sh;
@@ -112,42 +114,30 @@ __global__ __launch_bounds__(CacheShape<D>::NW * 64) void fta_cache_attn_kernel(
         g.start(a.k_sn, a.v_sn, a.Dreal, 0, lane);
         const FtaLane lo = fta_lane_offsets<D>(lane);
         auto key = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
-        auto issue = [&](int it, int st) {
+        auto issue = [&](int it) {
             const int kb = key(it);
-            const uint32_t lds = lds0 + st * Sh::STAGE_B;
             if (a.narrow && kb + 32 <= ke && (kb >= kb0 || kb + 32 <= a.sinks))
-                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds, 0);
+                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds0, 0);
             else  // keys that no row sees are taken from one that is seen (masked)
-                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds, 0, lane,
+                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds0, 0, lane,
                          [&](int t) { return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t; });
         };
         fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
-        issue(it0 + wave, 0);
-        int st = 0;
+        issue(it0 + wave);
         for (int it = it0 + wave; it < it1; it += NW) {
-            if (it + NW < it1) {
-                // every LDS read of the other stage has returned: its MFMAs were issued
-                __builtin_amdgcn_sched_barrier(0);
-                issue(it + NW, st ^ 1);
-                fta_wait_vmcnt<2 * LQ>();
-            } else {
-                fta_wait_vmcnt<0>();
-            }
+            fta_wait_vmcnt<0>();
             asm volatile("" ::: "memory");
             const int kb = key(it);
-            const uint32_t kbase = lds0 + st * Sh::STAGE_B;
             f32x16 s[1];
-            T::template qk<3>(kbase, lo, qf, s);
-            if (!(kb + 31 <= p0 && (kb >= p1 - a.left || kb + 31 < a.sinks) && r_n == 32)) {
-                const int hi = pos - kb, lw = pos - a.left - kb, sk = a.sinks - kb;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int rel = c_row(i, lane);
-                    s[0][i] = (rel <= hi && (rel >= lw || rel < sk)) ? s[0][i] : -FTA_INF;
-                }
+            T::template qk<3>(lds0, lo, qf, s);
+            if (!(kb + 31 <= p0 && (kb >= p1 - a.left || kb + 31 < a.sinks)))  // (rows past R are never written)
+                T::mask(fta_bits_below(pos + 1 - kb) & (~fta_bits_below(pos - a.left - kb) | fta_bits_below(a.sinks - kb)),
+                        lane, s[0]);
+            T::template softmax_pv<3>(lds0 + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
+            if (it + NW < it1) {  // every LDS read has returned: its MFMAs were issued
+                __builtin_amdgcn_sched_barrier(0);
+                issue(it + NW);
             }
-            T::template softmax_pv<3>(kbase + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
-            st ^= 1;
         }
     }
 
@@ -200,27 +190,19 @@ __global__ __launch_bounds__(CacheShape<D>::NW * 64) void fta_cache_attn_kernel(
 
 // ----------------------------------------------------------------------------
 // Shared prefix.  Workgroup = (K/V head, 32 NW rows of the batch's B * R, part):
-// 64-key stages shared by its waves, no mask but at the prefix's end.
+// 64-key stages (32 at D = 256) shared by its waves, no mask but at the prefix's end.
 // ----------------------------------------------------------------------------
-template <int D>
-struct PrefixShape {
-    static constexpr int NW = 4;
-    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 2>::TEN_B;
-    static constexpr int PDK = D <= 64 ? 3 : 6, PDV = D <= 64 ? 2 : 4;
-};
-
 template <int DT, int D>
-__global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefix_attn_kernel(CacheArgs a) {
-    using T = FtaTile<DT, D, 2>;
-    using Sh = PrefixShape<D>;
+__device__ void cache_prefix(const CacheArgs& a, int wgi, unsigned char* sStage) {
+    constexpr int NH = D <= 128 ? 2 : 1, KEYS = 32 * NH, PD = D <= 128 ? 3 : 2;
+    using T = FtaTile<DT, D, 1>;
+    using Sh = CacheShape<D>;
     constexpr int NW = Sh::NW;
-    __shared__ __align__(1024) unsigned char sStage[2][Sh::STAGE_B];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wgi = fta_xcd_remap(blockIdx.x, a.total);
     const int rest = fta_scalar(wgi / a.pre_tiles), rt = wgi - rest * a.pre_tiles;
     const int hk = fta_scalar(rest / a.pre_ns), sp = rest - hk * a.pre_ns;
-    const int all = (a.P + 63) >> 6;
+    const int all = (a.P + KEYS - 1) / KEYS;
     const int it0 = fta_scalar((int)((int64_t)all * sp / a.pre_ns));
     const int it1 = fta_scalar((int)((int64_t)all * (sp + 1) / a.pre_ns));
     const int64_t rows = (int64_t)a.B * a.R;
@@ -238,14 +220,14 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefi
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[dt][i] = 0.f;
     float m_run = -FTA_INF, l_run = 0.f;
-    FtaGather<D, NW, 64> g;
+    FtaGather<D, NW, KEYS> g;
     g.start(a.kp_sn, a.vp_sn, a.Dreal, wave, lane);
-    const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
+    const uint32_t lds0 = fta_lds_addr(sStage);
     const FtaLane lo = fta_lane_offsets<D>(lane);
     auto issue = [&](int it, int st) {
-        const int kb = 64 * it;
-        const uint32_t lds = lds0 + st * Sh::STAGE_B;
-        if (a.pre_narrow && kb + 64 <= a.P)
+        const int kb = KEYS * it;
+        const uint32_t lds = lds0 + st * Sh::PRE_B;
+        if (a.pre_narrow && kb + KEYS <= a.P)
             g.whole(kp, vp, a.kp_sn, a.vp_sn, kb, lds, wave);
         else
             g.mapped(kp, vp, a.kp_sn, a.vp_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return min(t, a.P - 1); });
@@ -258,17 +240,17 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefi
         __syncthreads();  // tile `it` visible; every wave is past tile it - 1
         if (it + 1 < it1) issue(it + 1, st ^ 1);
         if (f0 < rows) {  // wave-uniform
-            const uint32_t kbase = lds0 + st * Sh::STAGE_B;
-            f32x16 s[2];
-            T::template qk<Sh::PDK>(kbase, lo, qf, s);
-            const int hi = a.P - 64 * it;
-            if (hi < 64) {
+            const uint32_t kbase = lds0 + st * Sh::PRE_B;
 #pragma unroll
-                for (int sb = 0; sb < 2; ++sb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) s[sb][i] = (32 * sb + c_row(i, lane) < hi) ? s[sb][i] : -FTA_INF;
+            for (int sb = 0; sb < NH; ++sb) {
+                const int hi = a.P - KEYS * it - 32 * sb;  // keys left
+                if (hi <= 0) continue;
+                const uint32_t hbase = kbase + sb * T::TEN_B;
+                f32x16 s[1];
+                T::template qk<PD>(hbase, lo, qf, s);
+                if (hi < 32) T::mask(fta_bits_below(hi), lane, s[0]);
+                T::template softmax_pv<PD>(hbase + NH * T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
             }
-            T::template softmax_pv<Sh::PDV>(kbase + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
         }
         st ^= 1;
     }
@@ -282,6 +264,29 @@ __global__ __launch_bounds__(256, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_prefi
         for (int i = 0; i < 16; i += 4)
             write_row4(a, sp, row, D, dt * 32 + c_row(i, lane),
                        make_float4(oacc[dt][i], oacc[dt][i + 1], oacc[dt][i + 2], oacc[dt][i + 3]));
+}
+
+// One launch for both: the prefix's workgroups, bound by the matrix units for many rows, and
+// the own keys', bound by memory, are spread evenly over the block ids, so that a CU holds
+// some of each.  64 requests, 32 / 8 heads of 128, a prefix of 32768 and 768 own tokens on
+// average: 47 + 47 us as two launches, 84 as one; prefix first or last is 3 to 5% slower.
+// Each CU holds two workgroups (registers and LDS), so the mix hides less than it could.
+template <int DT, int D>
+__global__ __launch_bounds__(CacheShape<D>::NW * 64, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_cache_attn_kernel(CacheArgs a) {
+    using Sh = CacheShape<D>;
+    __shared__ __align__(1024) unsigned char sStage[Sh::LDS_B];
+    __shared__ float2 sML[Sh::NW][32];
+    if (a.pre_total == 0) {
+        cache_own<DT, D>(a, fta_xcd_remap(blockIdx.x, a.total), sStage, sML);
+        return;
+    }
+    const int64_t all = a.pre_total + a.total;
+    const int before = fta_scalar((int)((int64_t)blockIdx.x * a.pre_total / all));
+    const bool pre = fta_scalar((int)((int64_t)(blockIdx.x + 1) * a.pre_total / all)) > before;
+    if (pre)
+        cache_prefix<DT, D>(a, fta_xcd_remap(before, a.pre_total), sStage);
+    else
+        cache_own<DT, D>(a, fta_xcd_remap(blockIdx.x - before, a.total), sStage, sML);
 }
 
 // Join of the parts, one workgroup per row: D / 8 column groups x 2048 / D slices of
@@ -365,15 +370,15 @@ int cache_plan(CacheArgs& a, int B, int H, int Hk, int T, int S, int D, int P, i
     const int64_t wgs = (int64_t)B * Hk * a.row_tiles;
     // keys a row tile can see, in 32-key tiles: at least one tile per wave and part
     const int64_t span = std::min<int64_t>(S, (int64_t)a.left + T + a.sinks);
-    const int64_t tiles = (span + 31) / 32, nw = kernel_dim(D) <= 128 ? 4 : 2;
-    a.ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, tiles / nw));
+    const int64_t tiles = (span + 31) / 32;
+    a.ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, tiles / 4));
     if (P > 0) {
         const int64_t pt = ((int64_t)B * a.R + 127) / 128;
         if (pt > (1 << 24)) return fta::unsupported("cache_attn: too many rows");
         a.pre_tiles = (int)pt;
         a.pre_ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + pt * Hk - 1) / (pt * Hk), ((int64_t)P + 255) / 256));
     }
-    if (wgs * a.ns > 0x7fffffff || a.rows > 0x7fffffff || (int64_t)Hk * a.pre_tiles * std::max(a.pre_ns, 1) > 0x7fffffff)
+    if (a.rows > 0x7fffffff || wgs * a.ns + (int64_t)Hk * a.pre_tiles * a.pre_ns > 0x7fffffff)
         return fta::unsupported("cache_attn: too many rows");
     return FTA_OK;
 }
@@ -388,13 +393,10 @@ size_t cache_bytes(const CacheArgs& a, int Dk) {
 template <int DT, int D>
 int launch_cache(CacheArgs& a, hipStream_t st) {
     int rc;
-    if (a.P > 0) {
-        a.total = a.Hk * a.pre_tiles * a.pre_ns;
-        hipLaunchKernelGGL((fta_prefix_attn_kernel<DT, D>), dim3(a.total), dim3(256), 0, st, a);
-        if ((rc = fta::check_launch("fta_prefix_attn_kernel")) != FTA_OK) return rc;
-    }
+    a.pre_total = a.Hk * a.pre_tiles * a.pre_ns;
     a.total = a.B * a.Hk * a.row_tiles * a.ns;
-    hipLaunchKernelGGL((fta_cache_attn_kernel<DT, D>), dim3(a.total), dim3(CacheShape<D>::NW * 64), 0, st, a);
+    hipLaunchKernelGGL((fta_cache_attn_kernel<DT, D>), dim3((unsigned)(a.pre_total + a.total)), dim3(CacheShape<D>::NW * 64), 0,
+                       st, a);
     if ((rc = fta::check_launch("fta_cache_attn_kernel")) != FTA_OK || cache_slots(a) <= 1) return rc;
     hipLaunchKernelGGL((fta_cache_combine_kernel<DT, D>), dim3((unsigned)a.rows), dim3(256), 0, st, a, cache_slots(a));
     return fta::check_launch("fta_cache_combine_kernel");

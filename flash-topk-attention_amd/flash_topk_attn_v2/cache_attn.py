@@ -56,7 +56,7 @@ def cache_attn(what, q, k_cache, v_cache, cache_lens, num_heads, num_kv_heads, k
     q, qa, qs = _lib.rows(q, H)
     lens = cache_lens.contiguous()
     dev = q.device
-    o = torch.empty(q.shape, device=dev, dtype=q.dtype)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty(B, H, T, device=dev, dtype=torch.float32)
     ws = _lib.workspace(nbytes, dev) if nbytes else None
     _lib.call("fta_cache_attn", dev, qa, qs, kca, kcs, vca, vcs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, S, D,

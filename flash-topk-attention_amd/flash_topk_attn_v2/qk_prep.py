@@ -69,7 +69,7 @@ class _QKNormRopeFunc(torch.autograd.Function):
         q, qa, qs = _lib.rows(q, H)
         k, ka, ks = _lib.rows(k, Hk)
         qw, kw = (None if w is None else _lib.flat(w) for w in (q_weight, k_weight))
-        qo, ko = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k))
+        qo, ko = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
         _lib.call("fta_qk_norm_rope", q.device, qa, qs, ka, ks, _lib.DTYPE_CODES[q.dtype], B, H, Hk, N, D, _lib.ptr(qw),
                   _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, _lib.ptr(positions),
                   0 if positions is None else positions.stride(0), eps, interleaved, qo.data_ptr(),
@@ -88,7 +88,7 @@ class _QKNormRopeFunc(torch.autograd.Function):
         k, ka, ks = _lib.rows(k, Hk)
         dqo, dqa, dqs = _lib.rows(dqo, H)
         dko, dka, dks = _lib.rows(dko, Hk)
-        dq, dk = (torch.empty(x.shape, device=dev, dtype=x.dtype) for x in (q, k))
+        dq, dk = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
         dqw = torch.empty(D, device=dev, dtype=qw.dtype) if qw is not None and ctx.needs_input_grad[2] else None
         dkw = torch.empty(D, device=dev, dtype=kw.dtype) if kw is not None and ctx.needs_input_grad[3] else None
         ws, nbytes = None, 0
@@ -204,7 +204,7 @@ def flash_qk_norm_rope_append(
     v, va, vs = _lib.rows(v, Hk)
     qw, kw = (None if w is None else _lib.flat(w) for w in (q_weight, k_weight))
     cos, sin, lens = _lib.flat(cos), _lib.flat(sin), cache_lens.contiguous()
-    qo = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     _lib.call("fta_qk_norm_rope_append", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, D,
               _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, int(position_offset),
               float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),

@@ -48,7 +48,7 @@ class _WindowAttnFunc(torch.autograd.Function):
         q, qa, qs = _lib.rows(q, H)
         k, ka, ks = _lib.rows(k, Hk)
         v, va, vs = _lib.rows(v, Hk)
-        o = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = torch.empty(B, H, N, device=q.device, dtype=torch.float32)
         _lib.call("fta_window_attn_fwd", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, N, D,
                   _lib.ptr(lens), left, right, sinks, scale, o.data_ptr(), _lib.dense_strides(q.shape, H),
@@ -70,7 +70,7 @@ class _WindowAttnFunc(torch.autograd.Function):
         k, ka, ks = _lib.rows(k, Hk)
         v, va, vs = _lib.rows(v, Hk)
         do, da, ds = _lib.rows(do, H)
-        dq, dk, dv = (torch.empty(x.shape, device=x.device, dtype=x.dtype) for x in (q, k, v))
+        dq, dk, dv = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k, v))
         sq, sk = _lib.dense_strides(q.shape, H), _lib.dense_strides(k.shape, Hk)
         nbytes = _lib.size_of("fta_window_attn_bwd_workspace_size", B, H, Hk, N, D, left, right, sinks)
         ws = _lib.workspace(nbytes, q.device)
