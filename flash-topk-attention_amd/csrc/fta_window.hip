@@ -45,6 +45,7 @@ struct WinArgs {
     float c, scale;
     int hw;               // forward, dQ: query heads per workgroup (they share K / V)
     int tiles;            // forward, dQ: token tiles per head; dK / dV: 64-key tiles
+    int kt_keys;          // dK / dV: keys per tile
     int ts, nps, np;      // dK / dV: tiles that hold sinks, parts of each of them, parts of the others
     int total;
     bool kv_narrow, q_narrow, d_narrow;  // token strides that 32-bit lane offsets span
@@ -340,34 +341,34 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
 }
 
 // ----------------------------------------------------------------------------
-// dK / dV.  A workgroup owns 64 keys of one K/V head and walks the 32-query chunks
-// that see any of them, through all query heads of the group in one sequence, so
-// the sums over shared heads need neither atomics nor a second pass.  Wave (tt, 0)
-// holds K of 32-key tile tt and accumulates dV, wave (tt, 1) holds V and accumulates
-// dK one chunk behind; P crosses in fp32 through LDS:
+// dK / dV at D = 256, where one wave's keys' rows and both accumulators would take every
+// register: a workgroup owns 64 keys of one K/V head, wave (tt, 0) holds K of 32-key tile
+// tt and accumulates dV, wave (tt, 1) holds V and accumulates dK one chunk behind; P
+// crosses in fp32 through LDS:
 //   wave (tt, 0):  S = Q K^T,  P = 2^{c S - lse2}  -> LDS;  dV += P^T dO
 //   wave (tt, 1):  dP = dO V^T;  dS = P (dP - delta);  dK += dS^T Q
 // One barrier per step; Q two steps ahead in four tiles, dO in three.
 //
-// The tiles that hold sinks are seen by every later query: their walks are cut into
-// nps parts as long as the other tiles' walks, and on small grids every walk into np
-// parts; parts write fp32 sums that fta_window_dkv_combine_kernel adds in order.
+// This kernel and the next walk the 32-query chunks that see any of the workgroup's keys,
+// through all query heads of the group in one sequence, so the sums over shared heads need
+// neither atomics nor a second pass.  The tiles that hold sinks are seen by every later
+// query: their walks are cut into nps parts as long as the other tiles' walks, and on small
+// grids every walk into np parts; parts write fp32 sums that
+// fta_window_dkv_combine_kernel adds in order.
 // ----------------------------------------------------------------------------
 template <int D>
-struct WinDkvShape {
+struct WinDkvSplitShape {
     static constexpr int NW = 4, NTHR = 256, QSEG = D / 8;
     static constexpr int LQ = 32 * QSEG / NTHR;  // DMA instructions per wave and 32-row tile
     static constexpr int TILE_B = 32 * QSEG * 16;
     static constexpr int NQ = 4, ND = 3;
-    static constexpr int WPC = (D <= 64) ? 3 : (D <= 128) ? 2 : 1;  // workgroups per CU
     static_assert((32 * QSEG) % NTHR == 0, "whole DMA instructions per wave");
-    static_assert((NQ + ND) * TILE_B + NQ * 256 + 2 * 2 * 32 * 32 * 4 + 64 <= 160 * 1024 / WPC, "WPC workgroups per CU");
 };
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kernel(WinArgs a) {
+__global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a) {
     using E = Elem<DT>;
-    using Sh = WinDkvShape<D>;
+    using Sh = WinDkvSplitShape<D>;
     constexpr int NW = Sh::NW, QSEG = Sh::QSEG, LQ = Sh::LQ, TILE_B = Sh::TILE_B;
     using SW = FtaSwz<QSEG>;
     constexpr int KS = D / 16, DT32 = D / 32;
@@ -676,6 +677,256 @@ __global__ __launch_bounds__(256, WinDkvShape<D>::WPC) void fta_window_dkv_kerne
         run(std::false_type{});
 }
 
+// ----------------------------------------------------------------------------
+// dK / dV up to D = 128: four waves of 32 keys, each with its keys' K and V rows and both
+// accumulators in registers, so a 32-query chunk of Q and dO serves 128 keys and P never
+// leaves the wave:
+//   S = Q K^T,  dP = dO V^T,  P = 2^{c S - lse2},  dS = P (dP - delta),
+//   dV += P^T dO,  dK += dS^T Q.
+// At D = 128 that is 254 registers, two workgroups per CU; 154 and three at D = 64.  Against
+// 64 keys a workgroup with the work of a tile split over two waves (the kernel above):
+// half the gathers and barriers, no exchange of P.  N32768, 32 / 8 heads of 128, window
+// 1024: 1510 -> 1290 us (870 TFLOP/s with the masked scores); N10000 twice, 12 / 4 heads of
+// 64, 300 to both sides: 175 -> 126.  Three stages instead of two change nothing.
+// ----------------------------------------------------------------------------
+template <int D>
+struct WinDkvShape {
+    static constexpr int NW = 4, KEYS = 128, QSEG = D / 8, NST = 2;
+    static constexpr int LQ = 32 * QSEG / 256;
+    static constexpr int TILE_B = 32 * QSEG * 16;
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(WinArgs a) {
+    using E = Elem<DT>;
+    using Sh = WinDkvShape<D>;
+    using T = FtaTile<DT, D, 1>;
+    constexpr int NW = Sh::NW, QSEG = Sh::QSEG, LQ = Sh::LQ, TILE_B = Sh::TILE_B, NST = Sh::NST;
+    using SW = FtaSwz<QSEG>;
+    constexpr int KS = D / 16, DT32 = D / 32;
+    __shared__ __align__(1024) unsigned char sQ[NST][TILE_B];
+    __shared__ __align__(1024) unsigned char sD[NST][TILE_B];
+    __shared__ __align__(1024) float sL[NST][64];  // lse2, delta
+
+    const int wgi = fta_xcd_remap(blockIdx.x, a.total);
+    const int per = a.ts * a.nps + (a.tiles - a.ts) * a.np;  // workgroups per (b, K/V head)
+    const int bhk = fta_scalar(wgi / per), slot = wgi - bhk * per;
+    const bool sink = slot < a.ts * a.nps;
+    const int parts = sink ? a.nps : a.np;
+    const int off = sink ? slot : slot - a.ts * a.nps;
+    const int tp = fta_scalar(off / parts);
+    const int tile = sink ? tp : a.ts + tp;
+    const int sp = off - tp * parts;
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = seq_len(a, b);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kb = Sh::KEYS * tile, kt = kb + 32 * wave;
+
+    int c_lo = 0, nch = 0;
+    if (kb < len) {
+        c_lo = max(0, kb - a.right) >> 5;
+        const int i_hi = kb < a.sinks ? len - 1 : min(len - 1, min(kb + Sh::KEYS - 1, len - 1) + a.left);
+        nch = (i_hi >> 5) + 1 - c_lo;
+    }
+    const int all = a.G * nch;
+    const int s0 = fta_scalar((int)((int64_t)all * sp / parts));
+    const int U = fta_scalar((int)((int64_t)all * (sp + 1) / parts)) - s0;
+
+    f32x16 dk[DT32], dv[DT32];
+#pragma unroll
+    for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[dt][i] = dv[dt][i] = 0.f;
+
+    if (U > 0) {
+        fta_frag kf[KS], vf[KS];
+        const int key = kt + (lane & 31);
+        const bool kok = key < len;
+        T::load_rows(a.k + b * a.k_sb + hk * a.k_sh + (int64_t)key * a.k_sn, kok, a.Dreal, lane, kf);
+        T::load_rows(a.v + b * a.v_sb + hk * a.v_sh + (int64_t)key * a.v_sn, kok, a.Dreal, lane, vf);
+        fta_wait_vmcnt<0>();
+        // Per-lane DMA source: instruction 0 fills row drow; the others lie 256 / QSEG rows down
+        // each, a multiple of 16, where the swizzle repeats: the same lane offset from a base
+        // further down.
+        constexpr int STEP = 256 / QSEG;
+        static_assert(STEP % 16 == 0, "the swizzle repeats");
+        const int drow = (wave * 64 + lane) / QSEG;
+        int dcol = SW::slot(drow, (wave * 64 + lane) % QSEG) * 8;
+        if (dcol >= a.Dreal) dcol = 0;  // columns past D: any finite data (never stored)
+        const uint32_t qoff = 2u * (drow * (uint32_t)a.q_sn + dcol), doff = 2u * (drow * (uint32_t)a.d_sn + dcol);
+        const bool l_isd = (lane & 32) != 0;
+        const FtaLane lo = fta_lane_offsets<D>(lane);
+        const uint32_t ldq = fta_lds_addr(&sQ[0][0]), ldd = fta_lds_addr(&sD[0][0]), ldl = fta_lds_addr(&sL[0][0]);
+        const int64_t q_step = 32 * a.q_sn, d_step = 32 * a.d_sn;
+        const int64_t q_turn = a.q_sh - (nch - 1) * q_step, d_turn = a.d_sh - (nch - 1) * d_step;
+        const int64_t r_turn = a.N - 32 * (int64_t)(nch - 1);
+        const int g0 = fta_scalar(s0 / nch), c_end = c_lo + nch;
+        int ci = c_lo + s0 - g0 * nch, cc = ci;  // chunk to gather, chunk to work on
+        const uint16_t* qp = a.q + b * a.q_sb + ((int64_t)hk * a.G + g0) * a.q_sh + ci * q_step;
+        const uint16_t* dp = a.dout + b * a.d_sb + ((int64_t)hk * a.G + g0) * a.d_sh + ci * d_step;
+        int64_t rp = ((int64_t)b * a.H + (int64_t)hk * a.G + g0) * a.N + 32 * (int64_t)ci;
+
+        // 32 rows of chunk ci from `base`
+        auto tile_dma = [&](const uint16_t* base, int64_t sn, bool narrow, uint32_t o, uint32_t lds)
+            __attribute__((always_inline)) {
+            if (narrow && 32 * ci + 32 <= len) {
+#pragma unroll
+                for (int i = 0; i < LQ; ++i) fta_dma16_so(base + i * STEP * sn, o, lds + (i * NW + wave) * 1024);
+            } else {  // the sequence's last chunk repeats its last row (masked); formed here, kept nowhere
+                int ln = lane;
+                asm volatile("" : "+v"(ln));
+#pragma unroll
+                for (int i = 0; i < LQ; ++i) {
+                    const int r2 = (i * NW + wave) * 64 + ln;
+                    const int row = r2 / QSEG;
+                    int j = SW::slot(row, r2 - row * QSEG);
+                    if (j * 8 >= a.Dreal) j = 0;
+                    const int64_t t = min(row, len - 1 - 32 * ci);
+                    fta_dma16_at(base + t * sn + j * 8, lds + (i * NW + wave) * 1024);
+                }
+            }
+        };
+        auto issue = [&](int st) __attribute__((always_inline)) {
+            tile_dma(qp, a.q_sn, a.q_narrow, qoff, ldq + st * TILE_B);
+            tile_dma(dp, a.d_sn, a.d_narrow, doff, ldd + st * TILE_B);
+            if (wave == 0) {
+                const float* src = l_isd ? a.delta + rp : a.lse2 + rp;
+                fta_dma4_at(src + min(lane & 31, len - 1 - 32 * ci), ldl + st * 256);
+            }
+            const bool turn = ci + 1 == c_end;  // on to the next query head's first chunk
+            ci = turn ? c_lo : ci + 1;
+            qp += turn ? q_turn : q_step;
+            dp += turn ? d_turn : d_step;
+            rp += turn ? r_turn : 32;
+        };
+#pragma unroll
+        for (int k = 0; k < NST - 1; ++k)
+            if (k < U) issue(k);
+        int st = 0;
+        for (int k = 0; k < U; ++k) {
+            if (k + NST - 2 < U) {
+                if (wave == 0)
+                    fta_wait_vmcnt<(2 * LQ + 1) * (NST - 2)>();
+                else
+                    fta_wait_vmcnt<2 * LQ * (NST - 2)>();
+            } else {
+                fta_wait_vmcnt<0>();
+            }
+            __syncthreads();  // chunk k visible; every wave is past chunk k - 1
+            if (k + NST - 1 < U) issue(st == 0 ? NST - 1 : st - 1);
+            const int i0 = 32 * cc;
+            cc = cc + 1 == c_end ? c_lo : cc + 1;
+            const bool some = kt < len && i0 + 31 >= kt - a.right && (i0 <= kt + 31 + a.left || kt < a.sinks);
+            if (some) {
+                const bool whole = i0 >= kt + 31 - a.right && i0 + 31 < len && kt + 31 < len &&
+                                   (i0 + 31 <= kt + a.left || kt + 31 < a.sinks);
+                const uint32_t qb = ldq + st * TILE_B, ob = ldd + st * TILE_B;
+                const float* ld = &sL[st][0];
+                f32x16 s, dpv;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = dpv[i] = 0.f;
+                {
+                    fta_frag fq[2], fo[2];
+                    fq[0] = T::row_frag(qb, lo, 0, 0);
+                    fo[0] = T::row_frag(ob, lo, 0, 0);
+#pragma unroll
+                    for (int ks = 0; ks < KS; ++ks) {
+                        if (ks + 1 < KS) {
+                            fq[(ks + 1) & 1] = T::row_frag(qb, lo, 0, ks + 1);
+                            fo[(ks + 1) & 1] = T::row_frag(ob, lo, 0, ks + 1);
+                        }
+                        s = fta_mma<DT>(fq[ks & 1], kf[ks], s);
+                        dpv = fta_mma<DT>(fo[ks & 1], vf[ks], dpv);
+                    }
+                }
+                if (!whole) {
+                    // query rows [rlo, rhi] of the chunk see this lane's key: bit = row
+                    int ln = lane;
+                    asm volatile("" : "+v"(ln));
+                    const int key = kt + (ln & 31);
+                    const int rlo = key - a.right - i0;
+                    const int rhi = (key < len ? min(key < a.sinks ? len - 1 : key + a.left, len - 1) : -1) - i0;
+                    T::mask(fta_bits_below(rhi + 1) & ~fta_bits_below(rlo), lane, s);
+                }
+                fta_frag pf[2], df[2];
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    float p8[8], d8[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 4) {
+                        const int i = 8 * ks + e;
+                        const float4 l4 = *reinterpret_cast<const float4*>(ld + c_row(i, lane));
+                        const float4 e4 = *reinterpret_cast<const float4*>(ld + 32 + c_row(i, lane));
+                        p8[e] = fta_exp2(fmaf(s[i], a.c, -l4.x));
+                        p8[e + 1] = fta_exp2(fmaf(s[i + 1], a.c, -l4.y));
+                        p8[e + 2] = fta_exp2(fmaf(s[i + 2], a.c, -l4.z));
+                        p8[e + 3] = fta_exp2(fmaf(s[i + 3], a.c, -l4.w));
+                        d8[e] = p8[e] * (dpv[i] - e4.x);
+                        d8[e + 1] = p8[e + 1] * (dpv[i + 1] - e4.y);
+                        d8[e + 2] = p8[e + 2] * (dpv[i + 2] - e4.z);
+                        d8[e + 3] = p8[e + 3] * (dpv[i + 3] - e4.w);
+                    }
+                    pf[ks] = fta_pack_frag<DT>(p8);
+                    df[ks] = fta_pack_frag<DT>(d8);
+                }
+                {
+                    constexpr int PD = 2, NM = 4 * DT32;  // dV and dK in turn
+                    fta_frag fr[PD + 1];
+                    auto load = [&](auto nn) __attribute__((always_inline)) {
+                        constexpr int n = decltype(nn)::value;
+                        if constexpr (n < NM) fr[n % (PD + 1)] = T::tr_frag((n & 1) ? qb : ob, lo, n / 2 / DT32, n / 2 % DT32);
+                    };
+                    auto slot_ = [&](auto nn) __attribute__((always_inline)) {
+                        constexpr int n = decltype(nn)::value, ks = n / 2 / DT32, dt = n / 2 % DT32;
+                        if constexpr (n % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+                        load(std::integral_constant<int, n + PD>{});
+                        if constexpr ((n & 1) == 0)
+                            dv[dt] = fta_mma<DT>(pf[ks], fr[n % (PD + 1)], dv[dt]);
+                        else
+                            dk[dt] = fta_mma<DT>(df[ks], fr[n % (PD + 1)], dk[dt]);
+                    };
+                    fta_static_for<0, PD>(load);
+                    fta_static_for<0, NM>(slot_);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            st = st == NST - 1 ? 0 : st + 1;
+        }
+    }
+
+    // C layout: lane column = d, rows = keys c_row(i, lane)
+    if (parts > 1) {
+        const int64_t slots = a.np > 1 ? per : a.ts * a.nps;
+        float* pk = a.part + (((int64_t)bhk * slots + slot) * Sh::KEYS + 32 * wave) * D;
+        float* pv = pk + (int64_t)a.B * a.Hk * slots * Sh::KEYS * D;
+#pragma unroll
+        for (int dt = 0; dt < DT32; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t at = (int64_t)c_row(i, lane) * D + dt * 32 + (lane & 31);
+                pk[at] = dk[dt][i];
+                pv[at] = dv[dt][i];
+            }
+        return;
+    }
+    uint16_t* ok = a.out0 + b * a.o0_sb + hk * a.o0_sh;
+    uint16_t* ov = a.out1 + b * a.o1_sb + hk * a.o1_sh;
+#pragma unroll
+    for (int dt = 0; dt < DT32; ++dt) {
+        const int d = dt * 32 + (lane & 31);
+        if (d >= a.Dreal) continue;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int t = kt + c_row(i, lane);
+            if (t >= a.N) continue;
+            const uint32_t pk = E::pack2(dk[dt][i] * a.scale, dv[dt][i]);
+            ok[(int64_t)t * a.o0_sn + d] = (uint16_t)(pk & 0xffffu);
+            ov[(int64_t)t * a.o1_sn + d] = (uint16_t)(pk >> 16);
+        }
+    }
+}
+
 // Sum of the dK / dV parts: SL threads per (tensor, b, K/V head, key of a tile with parts,
 // 8 columns) add every SL-th part and then their sums, always in the same order; dK takes
 // the scale here.  (One thread for all of a sink tile's 58 parts took 17.6 us at N 32768.)
@@ -691,16 +942,17 @@ __global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, 
     const int ten = row >= rows;  // 0: dK, 1: dV
     row = ok ? row - ten * rows : 0;
     const int t = (int)(row % keys), bhk = (int)(row / keys);
-    const int tile = t >> 6, d0 = dc * 8;
+    constexpr int KEYS = D <= 128 ? 128 : 64;  // of a tile
+    const int tile = t / KEYS, d0 = dc * 8;
     const int slots = a.ts * a.nps + (a.np > 1 ? (a.tiles - a.ts) * a.np : 0);
     const int n = tile < a.ts ? a.nps : a.np;
     const int first = tile < a.ts ? tile * a.nps : a.ts * a.nps + (tile - a.ts) * a.np;
     float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (ok && n > 1) {
-        const float* src = a.part + ((((int64_t)ten * a.B * a.Hk + bhk) * slots + first) * 64 + (t & 63)) * D + d0;
+        const float* src = a.part + ((((int64_t)ten * a.B * a.Hk + bhk) * slots + first) * KEYS + t % KEYS) * D + d0;
         for (int p = sl; p < n; p += SL) {
-            const float4 x0 = *reinterpret_cast<const float4*>(src + (int64_t)p * 64 * D);
-            const float4 x1 = *reinterpret_cast<const float4*>(src + (int64_t)p * 64 * D + 4);
+            const float4 x0 = *reinterpret_cast<const float4*>(src + (int64_t)p * KEYS * D);
+            const float4 x1 = *reinterpret_cast<const float4*>(src + (int64_t)p * KEYS * D + 4);
             o[0] += x0.x, o[1] += x0.y, o[2] += x0.z, o[3] += x0.w;
             o[4] += x1.x, o[5] += x1.y, o[6] += x1.z, o[7] += x1.w;
         }
@@ -777,17 +1029,18 @@ int launch_rows(WinArgs& a, bool dq, hipStream_t st) {
 }
 
 // Parts of the dK / dV walks.  Grids that leave CUs idle cut every walk into up to 4 parts of
-// at least 4 steps (N1024, 4 heads of 128, causal: 20.4 us whole, 15.6 + 4.5 with their sum in
-// 4; N2048, 8 on 2 heads of 64, window 256: 24.9 -> 16.5 + 9), but not ones that have a
-// workgroup for each CU (N2048, 8 heads of 128, window 256: 22 + 4.5 whole, 21.5 + 11.6 in 2).
-// The tiles with sinks get parts as long as the other walks.
+// at least 8 steps (N1024, 4 heads of 128, causal: 47 us whole, 19.4 + 5 with their sum in
+// 4; N2048, 8 on 2 heads of 64, window 256: 52 + 4.6 -> 18.4 + 5.4), but not shorter ones
+// (N2048, 8 heads of 128, window 256, 13 steps: 26.9 + 4.8 whole, 21.4 + 12.4 in 2).  The
+// tiles with sinks get parts as long as the other walks.
 void dkv_parts(WinArgs& a) {
-    a.tiles = (a.N + 63) / 64;
-    a.ts = (a.sinks + 63) / 64;
+    a.kt_keys = a.Dreal <= 128 ? 128 : 64;
+    a.tiles = (a.N + a.kt_keys - 1) / a.kt_keys;
+    a.ts = (a.sinks + a.kt_keys - 1) / a.kt_keys;
     const int64_t wgs = (int64_t)a.tiles * a.B * a.Hk;
     const int64_t nall = (a.N + 31) / 32;
-    const int64_t steps = a.G * std::min<int64_t>(nall, ((int64_t)64 + a.left + a.right + 31) / 32 + 1);
-    const int64_t np = std::max<int64_t>(1, std::min<int64_t>({4, 256 / wgs, steps / 4}));
+    const int64_t steps = a.G * std::min<int64_t>(nall, ((int64_t)a.kt_keys + a.left + a.right + 31) / 32 + 1);
+    const int64_t np = std::max<int64_t>(1, std::min<int64_t>({4, 256 / wgs, steps / 8}));
     a.np = (int)np;
     const int64_t own = std::max<int64_t>(8, steps / np);
     a.nps = a.ts == 0 ? 1 : (int)std::max<int64_t>(np, std::min<int64_t>(128, (a.G * nall + own - 1) / own));
@@ -798,7 +1051,7 @@ int64_t dkv_slots(const WinArgs& a) {
 }
 size_t rows_bytes(int B, int H, int N) { return fta::align_up((size_t)B * H * N * sizeof(float)); }
 size_t part_bytes(const WinArgs& a, int Dk) {
-    return fta::align_up((size_t)2 * a.B * a.Hk * dkv_slots(a) * 64 * Dk * sizeof(float));
+    return fta::align_up((size_t)2 * a.B * a.Hk * dkv_slots(a) * a.kt_keys * Dk * sizeof(float));
 }
 
 template <int DT, int D>
@@ -806,10 +1059,13 @@ int launch_dkv(WinArgs& a, hipStream_t st) {
     const int64_t grid = ((int64_t)a.ts * a.nps + (int64_t)(a.tiles - a.ts) * a.np) * a.B * a.Hk;
     if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
     a.total = (int)grid;
-    hipLaunchKernelGGL((fta_window_dkv_kernel<DT, D>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    if constexpr (D <= 128)
+        hipLaunchKernelGGL((fta_window_dkv_kernel<DT, D>), dim3((unsigned)grid), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((fta_window_dkv_split_kernel<DT, D>), dim3((unsigned)grid), dim3(256), 0, st, a);
     int rc = fta::check_launch("fta_window_dkv_kernel");
     if (rc != FTA_OK || (a.np <= 1 && (a.ts == 0 || a.nps <= 1))) return rc;
-    const int keys = a.np > 1 ? a.N : std::min(a.N, a.ts * 64);
+    const int keys = a.np > 1 ? a.N : std::min(a.N, a.ts * a.kt_keys);
     // many parts of few keys (the sinks alone), or a few parts of every key
     constexpr int SLF = 256 / (D / 8) < 16 ? 256 / (D / 8) : 16;
     const int sl = a.np > 1 ? 4 : SLF, per = 256 / (D / 8 * sl);
