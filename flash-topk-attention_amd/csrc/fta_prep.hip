@@ -40,7 +40,8 @@ struct PrepArgs {
     const int32_t* lens;            // append: tokens in the cache, the new ones included
     int S, pos_off;                 // append: rows of the cache, table row of cache row 0
     float* part;                    // backward: [workgroup][2][D] partial weight gradients, or null
-    int N, H, Hk, D, R, P, inter, parts;
+    int N, H, Hk, D, R, P, inter;
+    int parts, per;                 // parts of a token's row groups, groups in each
     int64_t units;                  // (token, part) pairs
     float eps;
 };
@@ -79,6 +80,21 @@ __device__ __forceinline__ void load_w8(const void* w, int dt, int d, float* f) 
         else
             unpack8<FTA_DTYPE_F16>(x, f);
     }
+}
+// 16 bytes that are read or written once: past the caches where the call streams more than
+// they hold (NT; 32K tokens, 32 + 8 heads of 128: backward 229 -> 203 us).
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <bool NT>
+__device__ __forceinline__ uint4 load16(const uint16_t* p) {
+    if constexpr (NT) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(p)));
+    return *reinterpret_cast<const uint4*>(p);
+}
+template <bool NT>
+__device__ __forceinline__ void store16(uint16_t* p, uint4 v) {
+    if constexpr (NT)
+        __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(p));
+    else
+        *reinterpret_cast<uint4*>(p) = v;
 }
 template <int LG>
 __device__ __forceinline__ float row_sum(float x) {
@@ -137,7 +153,7 @@ __device__ __forceinline__ void load_angles(const PrepArgs& a, const LaneCols& c
 // APPEND: rows past the query and key heads copy V; K and V go to cache row
 // lens[b] - N + n (not written outside [0, S)).
 // ----------------------------------------------------------------------------
-template <int DT, int LG, int U, bool APPEND>
+template <int DT, int LG, int U, bool APPEND, bool NT>
 __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
     constexpr int RW = 64 / LG;
     const int lane = threadIdx.x & 63;
@@ -157,7 +173,7 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
         const int64_t tok = unit / a.parts;
         const int part = (int)(unit - tok * a.parts);
         const int b = (int)(tok / a.N), n = (int)(tok - (int64_t)b * a.N);
-        const int r0 = part * U * RW + lane / LG;
+        const int r0 = part * a.per * RW + lane / LG;
 
         int crow = 0, pos;
         if constexpr (APPEND) {
@@ -174,11 +190,11 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
         for (int u = 0; u < U; ++u) {
             const int row = r0 + u * RW;
             x[u] = fta_zero4();
-            if (c.live && row < rows) {
+            if (c.live && row < rows && u < a.per) {
                 const uint16_t* p = row < a.H ? a.q + b * a.q_sb + row * a.q_sh + n * a.q_sn
                                               : a.k + b * a.k_sb + (row - a.H) * a.k_sh + n * a.k_sn;
                 if (APPEND && row >= a.H + a.Hk) p = a.v + b * a.v_sb + (row - a.H - a.Hk) * a.v_sh + n * a.v_sn;
-                x[u] = *reinterpret_cast<const uint4*>(p + c.d0);
+                x[u] = load16<NT>(p + c.d0);
             }
         }
         float cs[8], sn[8];
@@ -198,12 +214,12 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
             for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
             const float r = rsqrtf(fmaf(row_sum<LG>(ss), inv_d, a.eps));
             const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
-            if (!c.live || row >= rows) continue;
+            if (!c.live || row >= rows || u >= a.per) continue;
             uint16_t* out;
             if (APPEND && row >= a.H + a.Hk) {
                 if (crow < 0) continue;
                 out = a.vo + b * a.vo_sb + (row - a.H - a.Hk) * a.vo_sh + crow * a.vo_sn;
-                *reinterpret_cast<uint4*>(out + c.d0) = x[u];
+                store16<NT>(out + c.d0, x[u]);
                 continue;
             }
 #pragma unroll
@@ -228,7 +244,7 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
             } else {
                 out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + n * a.ko_sn;
             }
-            *reinterpret_cast<uint4*>(out + c.d0) = pack8<DT>(y);
+            store16<NT>(out + c.d0, pack8<DT>(y));
         }
     }
 }
@@ -239,7 +255,7 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
 // workgroup adds its lanes' and writes one partial, and fta_norm_rope_dw_kernel
 // adds the partials in order: no atomics, the same bits every run of a shape.
 // ----------------------------------------------------------------------------
-template <int DT, int LG, int U>
+template <int DT, int LG, int U, bool NT>
 __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
     constexpr int RW = 64 / LG;
     __shared__ float sw[4][2][LG * 8];
@@ -259,21 +275,21 @@ __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
         const int b = (int)(tok / a.N), n = (int)(tok - (int64_t)b * a.N);
         int pos = a.positions ? a.positions[b * a.pos_sb + n] : n;
         pos = min(max(pos, 0), a.P - 1);
-        const int r0 = part * U * RW + lane / LG;
+        const int r0 = part * a.per * RW + lane / LG;
         uint4 x[U], dy[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int row = r0 + u * RW;
             x[u] = dy[u] = fta_zero4();
-            if (c.live && row < rows) {
+            if (c.live && row < rows && u < a.per) {
                 const bool isq = row < a.H;
                 const int h = isq ? row : row - a.H;
                 const uint16_t* p = isq ? a.q + b * a.q_sb + h * a.q_sh + n * a.q_sn
                                         : a.k + b * a.k_sb + h * a.k_sh + n * a.k_sn;
                 const uint16_t* g = isq ? a.dqo + b * a.dq_sb + h * a.dq_sh + n * a.dq_sn
                                         : a.dko + b * a.dk_sb + h * a.dk_sh + n * a.dk_sn;
-                x[u] = *reinterpret_cast<const uint4*>(p + c.d0);
-                dy[u] = *reinterpret_cast<const uint4*>(g + c.d0);
+                x[u] = load16<NT>(p + c.d0);
+                dy[u] = load16<NT>(g + c.d0);
             }
         }
         float cs[8], sn[8];
@@ -306,7 +322,7 @@ __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
             for (int e = 0; e < 8; ++e) {
                 f[e] *= r;  // n
                 const float gn = g[e] * f[e];
-                if (row < rows) {
+                if (row < rows && u < a.per) {
                     dwq[e] += isq ? gn : 0.f;
                     dwk[e] += isq ? 0.f : gn;
                 }
@@ -314,13 +330,13 @@ __global__ __launch_bounds__(256) void fta_norm_rope_bwd_kernel(PrepArgs a) {
                 hn = fmaf(g[e], f[e], hn);
             }
             const float m = row_sum<LG>(hn) * inv_d;
-            if (!c.live || row >= rows) continue;
+            if (!c.live || row >= rows || u >= a.per) continue;
 #pragma unroll
             for (int e = 0; e < 8; ++e) d[e] = r * (g[e] - f[e] * m);
             const int h = isq ? row : row - a.H;
             uint16_t* out = isq ? a.qo + b * a.qo_sb + h * a.qo_sh + n * a.qo_sn
                                 : a.ko + b * a.ko_sb + h * a.ko_sh + n * a.ko_sn;
-            *reinterpret_cast<uint4*>(out + c.d0) = pack8<DT>(d);
+            store16<NT>(out + c.d0, pack8<DT>(d));
         }
     }
     if (a.part == nullptr) return;
@@ -392,18 +408,30 @@ int prep_geometry(int B, int H, int Hk, int N, int D, int R, int P) {
     return FTA_OK;
 }
 
-// The (token, part) pairs: parts of U groups of 64 / LG rows.
+// The (token, part) pairs: the 64 / LG-row groups of a token in even parts of at most U.
 void set_units(PrepArgs& a, int B, int U, int rows) {
     const int rw = 64 / lanes_per_row(a.D);
     const int groups = (rows + rw - 1) / rw;
     a.parts = (groups + U - 1) / U;
+    a.per = (groups + a.parts - 1) / a.parts;
     a.units = (int64_t)B * a.N * a.parts;
 }
 
-// Workgroups of 4 waves that the chip holds at once: the kernels stride over the rest.
-constexpr int kFwdGrid = 256 * 6, kBwdGrid = 256 * 4;
+// Groups per wave and grids, measured at 32K tokens, 32 + 8 heads of 128 (ten groups a token):
+//  * forward, 671 MB: two groups a wave 166 us, four 150, five 132, ten 127; five with twice
+//    the workgroups that run at once (the kernel strides over the rest) and past the caches
+//    120 us, 5.6 TB/s.
+//  * backward, 1.0 GB: one 328, two 229, four 260, five 252; past the caches two 204, three
+//    203 (5.0 TB/s), five 197 with twice the partial sums.
+// Few rows (a step of a serving batch) take one group a wave, so that they spread over the CUs.
+constexpr int kFwdGroups = 5, kFwdGrid = 256 * 12, kBwdGroups = 3, kBwdGrid = 256 * 4;
+// Bytes of one tensor from which a call is taken to stream past the caches (4 MB of L2 a die,
+// 256 MB behind them, shared with what the caller does next).
+constexpr int64_t kStream = 64 << 20;
 
 unsigned grid_of(int64_t units, int most) { return (unsigned)std::min<int64_t>((units + 3) / 4, most); }
+
+bool streams(const PrepArgs& a, int B) { return (int64_t)B * a.N * a.H * a.D * 2 >= kStream; }
 
 template <typename F>
 int with_lanes(int D, F f) {
@@ -421,16 +449,16 @@ int launch_fwd(PrepArgs& a, int B, hipStream_t st) {
     const int rows = a.H + a.Hk + (APPEND ? a.Hk : 0);
     return with_lanes(a.D, [&](auto lg) {
         constexpr int LG = decltype(lg)::value;
-        // few rows: one group per wave, so that they spread over the CUs
         set_units(a, B, 1, rows);
-        if (a.units <= 4 * kFwdGrid) {
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, APPEND>), dim3(grid_of(a.units, kFwdGrid)), dim3(256), 0, st,
-                               a);
-        } else {
-            set_units(a, B, 2, rows);
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 2, APPEND>), dim3(grid_of(a.units, kFwdGrid)), dim3(256), 0, st,
-                               a);
-        }
+        const bool few = a.units <= 4 * kFwdGrid, nt = streams(a, B);
+        if (!few) set_units(a, B, kFwdGroups, rows);
+        const dim3 g(grid_of(a.units, kFwdGrid)), t(256);
+        if (few)
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, APPEND, false>), g, t, 0, st, a);
+        else if (nt && !APPEND)
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, kFwdGroups, APPEND, !APPEND>), g, t, 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, kFwdGroups, APPEND, false>), g, t, 0, st, a);
         return fta::check_launch("fta_norm_rope_fwd_kernel");
     });
 }
@@ -439,9 +467,12 @@ template <int DT>
 int launch_bwd(PrepArgs& a, int B, void* dqw, void* dkw, hipStream_t st) {
     return with_lanes(a.D, [&](auto lg) {
         constexpr int LG = decltype(lg)::value;
-        set_units(a, B, 2, a.H + a.Hk);
+        set_units(a, B, kBwdGroups, a.H + a.Hk);
         const unsigned wgs = grid_of(a.units, kBwdGrid);
-        hipLaunchKernelGGL((fta_norm_rope_bwd_kernel<DT, LG, 2>), dim3(wgs), dim3(256), 0, st, a);
+        if (streams(a, B))
+            hipLaunchKernelGGL((fta_norm_rope_bwd_kernel<DT, LG, kBwdGroups, true>), dim3(wgs), dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_norm_rope_bwd_kernel<DT, LG, kBwdGroups, false>), dim3(wgs), dim3(256), 0, st, a);
         int rc = fta::check_launch("fta_norm_rope_bwd_kernel");
         if (rc != FTA_OK || a.part == nullptr) return rc;
         hipLaunchKernelGGL(fta_norm_rope_dw_kernel, dim3(2 * a.D / 8), dim3(256), 0, st, a.part, (int)wgs, a.D, dqw, dkw,

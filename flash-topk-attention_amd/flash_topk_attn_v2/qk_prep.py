@@ -12,6 +12,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -79,6 +80,7 @@ class _QKNormRopeFunc(torch.autograd.Function):
         return qo, ko
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dqo, dko):
         q, k, qw, kw, cos, sin, positions = ctx.saved_tensors
         (H, Hk, D, R, wt), eps, interleaved = ctx.args
@@ -209,7 +211,9 @@ def flash_qk_norm_rope_append(
               _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, int(position_offset),
               float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),
               _lib.dense_strides(q.shape, H), kca, kcs, vca, vcs)
-    torch.autograd.graph.increment_version((k_cache, v_cache))
+    for c in (k_cache, v_cache):
+        if not c.is_inference():  # written in place (inference tensors keep no version)
+            torch.autograd.graph.increment_version(c)
     return qo
 
 

@@ -10,6 +10,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .cache_attn import cache_attn
@@ -60,6 +61,7 @@ class _WindowAttnFunc(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do, _dlse):
         if do is None:
             return None, None, None, None, None

@@ -290,3 +290,57 @@ def test_serving_step_in_a_graph(gpu):
             for _, out, state in sets:
                 for x, y in zip((*want, *eager), (*out, *state)):
                     assert torch.equal(x, y), i
+
+
+def test_refusals(gpu):
+    import flash_topk_attn_v2 as fta
+
+    B, T, H, Hk, D, S = 2, 2, 4, 2, 64, 20
+    q, kc, vc, ln = _state(gpu, BF, B, T, H, Hk, D, S, None)
+    good = dict(q=q, k_cache=kc, v_cache=vc, cache_lens=ln, num_heads=H, num_kv_heads=Hk)
+    bad = [dict(q=q[0]), dict(q=q.float()), dict(q=q[:1]), dict(q=q[:, :0]), dict(k_cache=kc.half()), dict(v_cache=vc[:, :3]),
+           dict(num_heads=3), dict(num_kv_heads=4), dict(num_kv_heads=3), dict(cache_lens=ln.long()), dict(cache_lens=ln.cpu()),
+           dict(scale=0.0), dict(scale=float("nan")), dict(k_cache=kc.transpose(1, 2)),
+           dict(k_cache=torch.zeros(B, S, 2 * Hk * D, device=gpu, dtype=BF)[..., ::2])]
+    win, pre = dict(window_left=5, num_sinks=2), dict(k_prefix=kc[0], v_prefix=vc[0])
+    fta.flash_window_attn_decode(**good, **win)
+    fta.flash_prefix_attn_decode(**good, **pre)
+    for b in bad:
+        with pytest.raises(ValueError):
+            fta.flash_window_attn_decode(**(good | b), **win)
+        with pytest.raises(ValueError):
+            fta.flash_prefix_attn_decode(**(good | b), **pre)
+    for b in (dict(window_left=-1), dict(num_sinks=-1)):
+        with pytest.raises(ValueError):
+            fta.flash_window_attn_decode(**good, **(win | b))
+    for b in (dict(k_prefix=kc), dict(v_prefix=vc[0, :3]), dict(k_prefix=kc[0].half()), dict(k_prefix=kc[0].cpu()),
+              dict(k_prefix=kc[0, :, :64]), dict(k_prefix=None)):
+        with pytest.raises(ValueError):
+            fta.flash_prefix_attn_decode(**good, **(pre | b))
+    g = good | dict(q=q.clone().requires_grad_(True))
+    with pytest.raises(ValueError, match="not differentiable"):
+        fta.flash_window_attn_decode(**g, **win)
+    with torch.no_grad():
+        fta.flash_window_attn_decode(**g, **win)
+
+
+@pytest.mark.parametrize("case", range(12))
+def test_drawn_shapes(gpu, case):
+    """Shapes over the whole range, odd ones among them, both forms on the same caches."""
+    import random
+
+    import flash_topk_attn_v2 as fta
+
+    r = random.Random(100 + case)
+    dtype, D = r.choice([BF, FP]), r.choice([16, 64, 80, 128, 176, 256])
+    Hk, G = r.choice([1, 2, 3, 8]), r.choice([1, 2, 3, 4, 8])
+    B, T, S, P = r.choice([1, 2, 3, 20]), r.choice([1, 1, 2, 5, 9]), r.randrange(1, 900), r.randrange(1, 900)
+    left, sinks = r.randrange(0, 400), r.choice([0, 1, 4, 33, 150])
+    lens = [r.randrange(0, S + 1) for _ in range(B)]
+    say("cache drawn", case, dtype, B, T, Hk * G, Hk, D, S, P, left, sinks, lens)
+    q, kc, vc, ln = _state(gpu, dtype, B, T, Hk * G, Hk, D, S, lens, seed=2000 + case)
+    kp, vp = (rand((P, Hk * D), 3000 + i, dtype, gpu) for i in (0, 1))
+    o, lse = fta.flash_window_attn_decode(q, kc, vc, ln, Hk * G, left, sinks, num_kv_heads=Hk)
+    R.check({"o": o, "lse": lse}, R.cache(q, kc, vc, lens, Hk * G, Hk, left, sinks, D ** -0.5), ("o", "lse"))
+    o, lse = fta.flash_prefix_attn_decode(q, kp, vp, kc, vc, ln, Hk * G, num_kv_heads=Hk)
+    R.check({"o": o, "lse": lse}, R.cache(q, kc, vc, lens, Hk * G, Hk, S, 0, D ** -0.5, kp, vp), ("o", "lse"))

@@ -49,6 +49,8 @@ CASES = [
     (BF, FP, 1, 40, 5, 5, 144, 48, False, None),
     (FP, BF, 2, 100, 4, 2, 256, 256, False, "long"),
     (BF, F32, 1, 3000, 2, 1, 64, 32, False, None),
+    (BF, F32, 1, 4200, 64, 8, 128, 128, False, None),  # 69 MB: streamed past the caches
+    (FP, F32, 2, 2100, 32, 8, 256, 64, True, "row"),
 ]
 
 
@@ -143,7 +145,8 @@ def test_layouts_streams_and_same_bits(gpu):
 
 @pytest.mark.parametrize("dtype,B,T,H,Hk,D,Rc,S,inter,offset", [
     (BF, 1, 1, 8, 8, 64, 64, 40, False, 0), (FP, 5, 3, 4, 2, 128, 64, 64, True, 7), (BF, 130, 1, 32, 8, 128, 128, 33, False, 100),
-    (FP, 4, 2, 3, 1, 80, 32, 9, False, 0), (BF, 2, 70, 4, 2, 256, 256, 100, False, 3)])
+    (FP, 4, 2, 3, 1, 80, 32, 9, False, 0), (BF, 2, 70, 4, 2, 256, 256, 100, False, 3),
+    (BF, 130, 10, 32, 8, 128, 128, 33, False, 0)])
 def test_append(gpu, dtype, B, T, H, Hk, D, Rc, S, inter, offset):
     import flash_topk_attn_v2 as fta
 
@@ -187,3 +190,78 @@ def test_append_into_views(gpu):
     a = fta.flash_qk_norm_rope_append(q, k, v, kd, vd, lens, H, cos, sin)
     b = fta.flash_qk_norm_rope_append(q, k, v, kc, vc, lens, H, cos, sin)
     assert torch.equal(a, b) and torch.equal(kd, kc) and torch.equal(vd, vc)
+
+
+def test_unaligned_addresses(gpu):
+    """Contiguous tensors whose first element is off the 16-byte grid."""
+    import flash_topk_attn_v2 as fta
+
+    def shifted(x):
+        y = torch.empty(x.numel() + 3, device=gpu, dtype=x.dtype)[3:].view(x.shape)
+        return y.copy_(x)
+
+    q, k = rand((2, 9, 128), 1, BF, gpu), rand((2, 9, 64), 2, BF, gpu)
+    cos, sin = _tables(9, 32, gpu)
+    w = _weight(64, 4, FP, gpu)
+    want = fta.flash_qk_norm_rope(q, k, 2, cos, sin, w, w, num_kv_heads=1)
+    got = fta.flash_qk_norm_rope(shifted(q), shifted(k), 2, shifted(cos), shifted(sin), shifted(w), w, num_kv_heads=1)
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+    kc = torch.zeros(2, 20, 64, device=gpu, dtype=BF)
+    lens = torch.tensor([9, 20], dtype=torch.int32, device=gpu)
+    with pytest.raises(ValueError, match="16-byte aligned"):
+        fta.flash_qk_norm_rope_append(q, k, k, shifted(kc), kc, lens, 2, cos, sin, num_kv_heads=1)
+
+
+def test_modes(gpu):
+    """Inference mode, a second derivative (refused) and calls that would lose a gradient (refused)."""
+    import flash_topk_attn_v2 as fta
+
+    cos, sin = _tables(8, 64, gpu)
+    lens = torch.tensor([4], dtype=torch.int32, device=gpu)
+    with torch.inference_mode():
+        x = rand((1, 4, 64), 1, BF, gpu)
+        c = torch.zeros(1, 8, 64, device=gpu, dtype=BF)
+        out = fta.flash_qk_norm_rope_append(x, x, x, c, c.clone(), lens, 1, cos, sin)
+        a, b = fta.flash_qk_norm_rope(x, x, 1, cos, sin)
+        assert torch.equal(out, a) and torch.equal(c[:, :4], b)
+    q = rand((1, 4, 64), 1, BF, gpu).requires_grad_(True)
+    a, _ = fta.flash_qk_norm_rope(q, q.detach(), 1, cos, sin)
+    g, = torch.autograd.grad(a.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+    c = torch.zeros(1, 8, 64, device=gpu, dtype=BF)
+    with pytest.raises(ValueError, match="not differentiable"):
+        fta.flash_qk_norm_rope_append(q, q, q, c, c.clone(), lens, 1, cos, sin)
+
+
+def test_refusals(gpu):
+    import flash_topk_attn_v2 as fta
+
+    q, k = (torch.zeros(2, 5, n * 64, device=gpu, dtype=BF) for n in (4, 2))
+    cos, sin = _tables(6, 64, gpu)
+    w = torch.ones(64, device=gpu)
+    good = dict(q=q, k=k, num_heads=4, cos=cos, sin=sin, q_weight=w, k_weight=w, num_kv_heads=2)
+    fta.flash_qk_norm_rope(**good)
+    bad = [dict(q=q[0]), dict(q=q.float()), dict(k=k.half()), dict(k=k[:, :4]), dict(k=q), dict(num_heads=3), dict(num_heads=0),
+           dict(num_kv_heads=3), dict(num_heads=32, num_kv_heads=16), dict(cos=cos[:4], sin=sin[:4]), dict(cos=cos[:, :3]),
+           dict(cos=cos.half(), sin=sin.half()), dict(cos=cos[:, :4], sin=sin[:, :4]), dict(cos=cos.cpu()), dict(eps=0.0),
+           dict(eps=float("nan")), dict(q_weight=w[:32]), dict(q_weight=w.half()), dict(q_weight=w.double(), k_weight=w.double()),
+           dict(q_weight=w.cpu()), dict(cos=cos.clone().requires_grad_(True)),
+           dict(positions=torch.zeros(2, 4, device=gpu, dtype=torch.int32)), dict(positions=torch.zeros(2, 5, device=gpu)),
+           dict(positions=torch.zeros(2, 5, dtype=torch.int32)), dict(q=q[:0], k=k[:0])]
+    for b in bad:
+        with pytest.raises(ValueError):
+            fta.flash_qk_norm_rope(**(good | b))
+    kc, vc = (torch.zeros(2, 9, 128, device=gpu, dtype=BF) for _ in range(2))
+    lens = torch.tensor([5, 9], dtype=torch.int32, device=gpu)
+    good |= dict(v=k, k_cache=kc, v_cache=vc, cache_lens=lens)
+    with torch.no_grad():
+        fta.flash_qk_norm_rope_append(**good)
+        bad = [dict(v=q), dict(v=k.half()), dict(k_cache=kc[:1]), dict(v_cache=vc[:, :8]), dict(k_cache=kc.half()),
+               dict(cache_lens=lens.long()), dict(cache_lens=lens[:1]), dict(cache_lens=lens.cpu()),
+               dict(k_cache=kc[:1].expand(2, -1, -1)), dict(v_cache=vc[:, :1].expand(-1, 9, -1)), dict(position_offset=1 << 40),
+               dict(k_cache=torch.zeros(2, 9, 256, device=gpu, dtype=BF)[..., ::2]), dict(k_cache=kc[:, :0], v_cache=vc[:, :0])]
+        for b in bad:
+            with pytest.raises(ValueError):
+                fta.flash_qk_norm_rope_append(**(good | b))

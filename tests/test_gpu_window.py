@@ -228,3 +228,52 @@ def test_gradient_by_differences(gpu):
     exact = sum(float((ref[n] * d).sum()) for n, d in zip(("dq", "dk", "dv"), dirs))
     assert abs(exact - slope) <= 1e-5 * (1 + abs(slope))  # second-order term of a central difference at 1e-4
     assert abs(along - slope) <= tol + 1e-5 * (1 + abs(slope))
+
+
+def test_unused_output_and_second_derivative(gpu):
+    import flash_topk_attn_v2 as fta
+
+    q, k, v, do = _inputs(gpu, BF, 1, 50, 2, 2, 64)
+    q.requires_grad_(True)
+    o, lse = fta.flash_window_attn(q, k, v, 2, (9, 0))
+    assert o.requires_grad and not lse.requires_grad
+    g, = torch.autograd.grad(o.float().square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+    with torch.no_grad():
+        o2, _ = fta.flash_window_attn(q, k, v, 2, (9, 0))
+    assert not o2.requires_grad and torch.equal(o.detach(), o2)
+
+
+def test_refusals(gpu):
+    import flash_topk_attn_v2 as fta
+
+    q, k = (torch.zeros(2, 5, n * 64, device=gpu, dtype=BF) for n in (4, 2))
+    lens = torch.tensor([5, 3], dtype=torch.int32, device=gpu)
+    good = dict(q=q, k=k, v=k, num_heads=4, window=(3, 0), num_kv_heads=2, seq_lens=lens)
+    fta.flash_window_attn(**good)
+    bad = [dict(q=q[0]), dict(q=q.float()), dict(v=k.half()), dict(k=k[:, :4]), dict(v=q), dict(num_heads=3), dict(num_kv_heads=4),
+           dict(num_heads=32, num_kv_heads=16), dict(window=(-1, 0)), dict(window=(0, -2)), dict(window=(1, 2, 3)),
+           dict(num_sinks=-1), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(seq_lens=lens.long()),
+           dict(seq_lens=lens[:1]), dict(seq_lens=lens.cpu()), dict(k=k.cpu()), dict(q=q[:, :0], k=k[:, :0], v=k[:, :0])]
+    for b in bad:
+        with pytest.raises(ValueError):
+            fta.flash_window_attn(**(good | b))
+
+
+@pytest.mark.parametrize("case", range(12))
+def test_drawn_shapes(gpu, case):
+    """Shapes over the whole range, odd ones among them."""
+    import random
+
+    r = random.Random(case)
+    dtype, D = r.choice([BF, FP]), r.choice([16, 64, 80, 128, 176, 256])
+    Hk, G = r.choice([1, 2, 3]), r.choice([1, 2, 3, 4, 8])
+    B, N = r.choice([1, 2, 3]), r.randrange(1, 900)
+    left, right, sinks = r.randrange(0, 400), r.choice([0, 0, r.randrange(0, 300)]), r.choice([0, 1, 4, 33, 150])
+    lens = [r.randrange(0, N + 1) for _ in range(B)] if r.random() < 0.5 else None
+    say("window drawn", case, dtype, B, N, Hk * G, Hk, D, left, right, sinks, lens)
+    q, k, v, do = _inputs(gpu, dtype, B, N, Hk * G, Hk, D, seed=1000 + case)
+    ln = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=gpu)
+    got = _run(q, k, v, do, Hk * G, Hk, (left, right), sinks, ln)
+    R.check(got, R.window(q, k, v, Hk * G, Hk, left, right, sinks, D ** -0.5, lens, do), ALL)
