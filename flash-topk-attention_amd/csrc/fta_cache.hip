@@ -57,8 +57,8 @@ __device__ __forceinline__ void write_row4(const CacheArgs& a, int slot, int64_t
 template <int D>
 struct CacheShape {
     static constexpr int NW = 4;                                           // waves
-    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, 1>::TEN_B;  // 32 keys, each wave's own
-    static constexpr int PRE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, D <= 128 ? 2 : 1>::TEN_B;  // prefix: 64 (or 32) keys, shared
+    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D>::TEN_B;  // 32 keys, each wave's own
+    static constexpr int PRE_B = (D <= 128 ? 2 : 1) * STAGE_B;  // prefix: 64 (or 32) keys, shared
     static constexpr int OROW = D + 4;  // floats per row of the merge buffer
     static constexpr int OWN_B = NW * (STAGE_B > 32 * OROW * 4 ? STAGE_B : 32 * OROW * 4);  // the merge buffer reuses the stages
     static constexpr int LDS_B = OWN_B > 2 * PRE_B ? OWN_B : 2 * PRE_B;
@@ -75,7 +75,7 @@ struct CacheShape {
 template <int DT, int D>
 __device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, float2 (*sML)[32]) {
     using E = Elem<DT>;
-    using T = FtaTile<DT, D, 1>;
+    using T = FtaTile<DT, D>;
     using Sh = CacheShape<D>;
     constexpr int NW = Sh::NW;
     const int lane = threadIdx.x & 63;
@@ -112,12 +112,12 @@ __device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, fl
         T::load_rows(a.q + q_offset(a, b, hk, min(r, a.R - 1)), r < a.R, a.Dreal, lane, qf);
         FtaGather<D, 1, 32> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, 0, lane);
-        const FtaLane lo = fta_lane_offsets<D>(lane);
+        const FtaAddr<D> ad0(lds0, lane);
         auto key = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
         auto issue = [&](int it) {
             const int kb = key(it);
             if (a.narrow && kb + 32 <= ke && (kb >= kb0 || kb + 32 <= a.sinks))
-                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds0, 0);
+                g.whole(kp + (int64_t)kb * a.k_sn, vp + (int64_t)kb * a.v_sn, lds0);
             else  // keys that no row sees are taken from one that is seen (masked)
                 g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds0, 0, lane,
                          [&](int t) { return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t; });
@@ -128,12 +128,13 @@ __device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, fl
             fta_wait_vmcnt<0>();
             asm volatile("" ::: "memory");
             const int kb = key(it);
-            f32x16 s[1];
-            T::template qk<3>(lds0, lo, qf, s);
+            const FtaAddr<D> ad = ad0.here();
+            f32x16 s;
+            T::template qk<3>(ad, 0, qf, s);
             if (!(kb + 31 <= p0 && (kb >= p1 - a.left || kb + 31 < a.sinks)))  // (rows past R are never written)
                 T::mask(fta_bits_below(pos + 1 - kb) & (~fta_bits_below(pos - a.left - kb) | fta_bits_below(a.sinks - kb)),
-                        lane, s[0]);
-            T::template softmax_pv<3>(lds0 + T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
+                        lane, s);
+            T::template softmax_pv<3>(ad, T::TEN_B, s, a.c, m_run, l_run, oacc);
             if (it + NW < it1) {  // every LDS read has returned: its MFMAs were issued
                 __builtin_amdgcn_sched_barrier(0);
                 issue(it + NW);
@@ -195,7 +196,7 @@ __device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, fl
 template <int DT, int D>
 __device__ void cache_prefix(const CacheArgs& a, int wgi, unsigned char* sStage) {
     constexpr int NH = D <= 128 ? 2 : 1, KEYS = 32 * NH, PD = D <= 128 ? 3 : 2;
-    using T = FtaTile<DT, D, 1>;
+    using T = FtaTile<DT, D>;
     using Sh = CacheShape<D>;
     constexpr int NW = Sh::NW;
     const int lane = threadIdx.x & 63;
@@ -222,37 +223,40 @@ __device__ void cache_prefix(const CacheArgs& a, int wgi, unsigned char* sStage)
     float m_run = -FTA_INF, l_run = 0.f;
     FtaGather<D, NW, KEYS> g;
     g.start(a.kp_sn, a.vp_sn, a.Dreal, wave, lane);
-    const uint32_t lds0 = fta_lds_addr(sStage);
-    const FtaLane lo = fta_lane_offsets<D>(lane);
-    auto issue = [&](int it, int st) {
+    const uint32_t lds0 = fta_lds_addr(sStage), ldsw = lds0 + 1024 * wave;
+    const FtaAddr<D> ad0(lds0, lane);
+    auto issue = [&](int it, int st) __attribute__((always_inline)) {
         const int kb = KEYS * it;
-        const uint32_t lds = lds0 + st * Sh::PRE_B;
+        const uint32_t lds = ldsw + st * Sh::PRE_B;
         if (a.pre_narrow && kb + KEYS <= a.P)
-            g.whole(kp, vp, a.kp_sn, a.vp_sn, kb, lds, wave);
+            g.whole(kp + (int64_t)kb * a.kp_sn, vp + (int64_t)kb * a.vp_sn, lds);
         else
             g.mapped(kp, vp, a.kp_sn, a.vp_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return min(t, a.P - 1); });
     };
     fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
+    int it = it0;
     if (it0 < it1) issue(it0, 0);
-    int st = 0;
-    for (int it = it0; it < it1; ++it) {
+    auto tile = [&](auto st) __attribute__((always_inline)) {
+        constexpr int ST = decltype(st)::value;
         fta_wait_vmcnt<0>();
         __syncthreads();  // tile `it` visible; every wave is past tile it - 1
-        if (it + 1 < it1) issue(it + 1, st ^ 1);
-        if (f0 < rows) {  // wave-uniform
-            const uint32_t kbase = lds0 + st * Sh::PRE_B;
+        const int left = a.P - KEYS * it;
+        if (++it < it1) issue(it, ST ^ 1);
+        if (f0 >= rows) return;  // wave-uniform
 #pragma unroll
-            for (int sb = 0; sb < NH; ++sb) {
-                const int hi = a.P - KEYS * it - 32 * sb;  // keys left
-                if (hi <= 0) continue;
-                const uint32_t hbase = kbase + sb * T::TEN_B;
-                f32x16 s[1];
-                T::template qk<PD>(hbase, lo, qf, s);
-                if (hi < 32) T::mask(fta_bits_below(hi), lane, s[0]);
-                T::template softmax_pv<PD>(hbase + NH * T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
-            }
+        for (int sb = 0; sb < NH; ++sb) {
+            const int hi = left - 32 * sb;  // keys left
+            if (hi <= 0) continue;
+            const FtaAddr<D> ad = ad0.here();
+            f32x16 s;
+            T::template qk<PD>(ad, ST * Sh::PRE_B + sb * T::TEN_B, qf, s);
+            if (hi < 32) T::mask(fta_bits_below(hi), lane, s);
+            T::template softmax_pv<PD>(ad, ST * Sh::PRE_B + (NH + sb) * T::TEN_B, s, a.c, m_run, l_run, oacc);
         }
-        st ^= 1;
+    };
+    while (it < it1) {
+        tile(std::integral_constant<int, 0>{});
+        if (it < it1) tile(std::integral_constant<int, 1>{});
     }
     const float L = l_run + fta_xor32(l_run);
     if (!ok) return;

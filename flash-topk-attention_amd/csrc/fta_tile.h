@@ -1,9 +1,9 @@
-// Attention of 32 query rows against tiles of 32 NH keys in LDS: the inner step of the
+// Attention of 32 query rows against tiles of 32 keys in LDS: the inner step of the
 // window and cache kernels.
 //
-// K and V tiles are row-major ([32 NH][D], rows swizzled by FtaSwz) and filled by LDS
-// DMA.  A wave owns 32 query rows as the columns of S^T = K Q^T (32x32x16 MFMA, NH
-// 32-key parts), so a row's scores are 16 registers each of lanes l and l + 32 and
+// K and V tiles are row-major ([32][D], rows swizzled by FtaSwz) and filled by LDS
+// DMA.  A wave owns 32 query rows as the columns of S^T = K Q^T (32x32x16 MFMA),
+// so a row's scores are 16 registers each of lanes l and l + 32 and
 // its maximum and sum are lane values; P^T in that layout is the B operand of
 // O^T += V^T P^T as it stands, V^T coming from LDS transpose reads.
 #pragma once
@@ -62,73 +62,87 @@ __device__ __forceinline__ fta_frag fta_pack_frag(const float* f) {
                     Elem<DT>::pack2(f[6], f[7])};
 }
 
-// Per-lane byte offsets of the operand fragments in a tile of D columns: K (or V) rows,
-// and the two halves of a transposed fragment.  Other k slices and column tiles differ by
-// an XOR of their slot bits, 16 or 32 rows down by a constant.
-struct FtaLane {
-    uint32_t row, tr0, tr1;
-};
-template <int D>
-__device__ __forceinline__ FtaLane fta_lane_offsets(int lane) {
-    using SW = FtaSwz<D / 8>;
-    const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-    return {2u * SW::off(lane & 31, lane >> 5), 2u * (SW::off(vr, vc >> 3) + (vc & 7)),
-            2u * (SW::off(vr + 8, vc >> 3) + (vc & 7))};
-}
+// Per-lane LDS addresses of the operand fragments of a 32-row tile of D columns at `base`
+// (a multiple of 1024): rows (K or V as they stand), and the two halves of a transposed
+// fragment.  k slices and column tiles differ by an XOR of their slot bits; 16 rows, other
+// tiles and other stages by constants that go into the instructions' offsets.  KEPT: every
+// XOR is formed once and held; else at each use, where registers are short.
+template <int D, bool KEPT = (D <= 128)>
+struct FtaAddr {
+    static constexpr int KS = D / 16, DT32 = D / 32;
+    uint32_t row_[KEPT ? KS : 1], tr0_[KEPT ? DT32 : 1], tr1_[KEPT ? DT32 : 1];
 
-template <int DT, int D, int NH>
+    __device__ __forceinline__ FtaAddr(uint32_t base, int lane) {
+        using SW = FtaSwz<D / 8>;
+        const int vr = 4 * (lane >> 5) + ((lane & 15) >> 2), vc = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+        const uint32_t r = base + 2u * SW::off(lane & 31, lane >> 5);
+        const uint32_t t0 = base + 2u * (SW::off(vr, vc >> 3) + (vc & 7));
+        const uint32_t t1 = base + 2u * (SW::off(vr + 8, vc >> 3) + (vc & 7));
+#pragma unroll
+        for (int k = 0; k < (KEPT ? KS : 1); ++k) row_[k] = r ^ (k * 32);
+#pragma unroll
+        for (int d = 0; d < (KEPT ? DT32 : 1); ++d) {
+            tr0_[d] = t0 ^ (d * 64);
+            tr1_[d] = t1 ^ (d * 64);
+        }
+    }
+    // Where the XORs are not kept: the same addresses, opaque to the compiler, which would else
+    // form every XOR ahead of the loop all the same, and spill.
+    __device__ __forceinline__ FtaAddr here() const {
+        FtaAddr x = *this;
+        if constexpr (!KEPT) asm volatile("" : "+v"(x.row_[0]), "+v"(x.tr0_[0]), "+v"(x.tr1_[0]));
+        return x;
+    }
+    // rows 0 .. 31 of the tile `off` bytes further on, columns 16 ks .. 16 ks + 15
+    __device__ __forceinline__ fta_frag row(uint32_t off, int ks) const {
+        return fta_lds_frag((KEPT ? row_[KEPT ? ks : 0] : row_[0] ^ (ks * 32)) + off);
+    }
+    // its rows 16 ks .. 16 ks + 15 transposed, columns 32 dt .. 32 dt + 31
+    __device__ __forceinline__ fta_frag tr(uint32_t off, int ks, int dt) const {
+        const uint32_t x = off + ks * 16 * (D / 8) * 16;
+        return fta_lds_tr_frag((KEPT ? tr0_[KEPT ? dt : 0] : tr0_[0] ^ (dt * 64)) + x,
+                               (KEPT ? tr1_[KEPT ? dt : 0] : tr1_[0] ^ (dt * 64)) + x);
+    }
+};
+
+template <int DT, int D>
 struct FtaTile {
     using E = Elem<DT>;
-    static constexpr int QSEG = D / 8;         // 16-byte slots per row
-    static constexpr int KEYS = 32 * NH;
-    static constexpr int SLOTS = KEYS * QSEG;  // per tile
-    static constexpr int TEN_B = SLOTS * 16;   // bytes per tile
+    static constexpr int QSEG = D / 8;            // 16-byte slots per row
+    static constexpr int TEN_B = 32 * QSEG * 16;  // bytes per 32-row tile
     static constexpr int KS = D / 16, DT32 = D / 32;
-    using SW = FtaSwz<QSEG>;
 
-    __device__ static __forceinline__ fta_frag row_frag(uint32_t base, const FtaLane& l, int half, int ks) {
-        return fta_lds_frag(((base + l.row) ^ (ks * 32)) + half * 32 * QSEG * 16);
-    }
-    __device__ static __forceinline__ fta_frag tr_frag(uint32_t base, const FtaLane& l, int ks, int dt) {
-        const uint32_t x = ks * 16 * QSEG * 16;
-        return fta_lds_tr_frag(((base + l.tr0) ^ (dt * 64)) + x, ((base + l.tr1) ^ (dt * 64)) + x);
-    }
-
-    // s[half] = (K Q^T)[32 half .. + 31][row], fragments read PD MFMAs ahead.
-    template <int PD>
-    __device__ static __forceinline__ void qk(uint32_t kbase, const FtaLane& l, const fta_frag* qf, f32x16* s) {
+    // s = (K Q^T)[key][row] of the 32 keys at `off`, fragments read PD MFMAs ahead.
+    template <int PD, typename A>
+    __device__ static __forceinline__ void qk(const A& ad, uint32_t off, const fta_frag* qf, f32x16& s) {
         fta_frag fr[PD + 1];
         auto load = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value;
-            if constexpr (n < NH * KS) fr[n % (PD + 1)] = row_frag(kbase, l, n % NH, n / NH);
+            if constexpr (n < KS) fr[n % (PD + 1)] = ad.row(off, n);
         };
         auto slot = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value;
             if constexpr (n % 2 == 0) __builtin_amdgcn_sched_barrier(0);
             load(std::integral_constant<int, n + PD>{});
-            if constexpr (n < NH) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[n][i] = 0.f;
-            }
-            s[n % NH] = fta_mma<DT>(fr[n % (PD + 1)], qf[n / NH], s[n % NH]);
+            s = fta_mma<DT>(fr[n % (PD + 1)], qf[n], s);
         };
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 0.f;
         fta_static_for<0, PD>(load);
-        fta_static_for<0, NH * KS>(slot);
+        fta_static_for<0, KS>(slot);
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    // Online softmax of the tile's scores (masked ones are -inf) and O^T += V^T P^T.
+    // Online softmax of those scores (masked ones are -inf) and O^T += V^T P^T, V at `off`.
     // The accumulators are rescaled only when a row's maximum grows by more than 2^8:
     // P stays below 2^8 and its 16-bit rounding keeps the same relative error.  A row
     // that has seen no key yet keeps m = -inf and adds exact zeros.
-    template <int PD>
-    __device__ static __forceinline__ void softmax_pv(uint32_t vbase, const FtaLane& l, const f32x16* s, float c,
-                                                      float& m_run, float& l_run, f32x16* oacc) {
-        float mx = s[0][0];
+    template <int PD, typename A>
+    __device__ static __forceinline__ void softmax_pv(const A& ad, uint32_t off, const f32x16& s, float c, float& m_run,
+                                                      float& l_run, f32x16* oacc) {
+        float mx = s[0];
 #pragma unroll
-        for (int sb = 0; sb < NH; ++sb)
-#pragma unroll
-            for (int i = (sb == 0); i < 16; ++i) mx = fmaxf(mx, s[sb][i]);
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i]);
         {
             float x = mx, y = mx;  // the row's other half of the keys is in lane ^ 32
             fta_swap32(x, y);
@@ -147,12 +161,12 @@ struct FtaTile {
         }
         const float mc = (m_run == -FTA_INF) ? 0.f : m_run * c;
         float ls = 0.f;
-        constexpr int NM = 2 * NH * DT32;
+        constexpr int NM = 2 * DT32;
         fta_frag fr[PD + 1];
         fta_frag pf;
         auto load = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value;
-            if constexpr (n < NM) fr[n % (PD + 1)] = tr_frag(vbase, l, n / DT32, n % DT32);
+            if constexpr (n < NM) fr[n % (PD + 1)] = ad.tr(off, n / DT32, n % DT32);
         };
         auto slot = [&](auto nn) __attribute__((always_inline)) {
             constexpr int n = decltype(nn)::value, ks = n / DT32;
@@ -162,7 +176,7 @@ struct FtaTile {
                 float pv[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    pv[e] = fta_exp2(fmaf(s[ks >> 1][8 * (ks & 1) + e], c, -mc));
+                    pv[e] = fta_exp2(fmaf(s[8 * ks + e], c, -mc));
                     ls += pv[e];
                 }
                 pf = fta_pack_frag<DT>(pv);
@@ -175,9 +189,9 @@ struct FtaTile {
         l_run += ls;
     }
 
-    // -inf for the scores of 32 keys whose bit of `seen` (bit = key) is clear.
+    // -inf for the scores whose bit of `seen` (bit = key, or query row) is clear.
     __device__ static __forceinline__ void mask(uint32_t seen, int lane, f32x16& s) {
-        const uint32_t m = seen >> (4 * (lane >> 5));  // register r holds key (r >> 2) * 8 + (r & 3) of these
+        const uint32_t m = seen >> (4 * (lane >> 5));  // register r holds (r >> 2) * 8 + (r & 3) of these
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const uint32_t k = (uint32_t)(((int)(m << (31 - ((r >> 2) * 8 + (r & 3))))) >> 31);
@@ -186,7 +200,7 @@ struct FtaTile {
         }
     }
 
-    // A wave's Q (or dO) rows as B operands: row `ok ? p : none` of this lane, zero past Dreal.
+    // A wave's Q (or dO) rows as B operands: this lane's row at p, zero past Dreal and where !ok.
     __device__ static __forceinline__ void load_rows(const uint16_t* p, bool ok, int Dreal, int lane, fta_frag* f) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
@@ -207,6 +221,13 @@ struct FtaTile {
             }
     }
 };
+
+// One wave-wide LDS DMA (fta_dma16_so) to `lds` + a constant, the sum formed in M0 itself.
+template <int OFF>
+__device__ __forceinline__ void fta_dma16_to(const void* base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(base),
+                 "s"(__builtin_amdgcn_readfirstlane(lds)), "i"(OFF) : "memory", "m0", "scc");
+}
 
 // Fills one K and one V tile of KEYS rows by LDS DMA, NW waves together: LQ instructions
 // per wave and tensor, instruction i of a wave writing the 1 KB block i * NW + wave.
@@ -229,18 +250,20 @@ struct FtaGather {
             voff[i] = 2u * (row * (uint32_t)v_sn + j * 8);
         }
     }
-    // rows kb .. kb + KEYS - 1, all of them inside the tensor
-    __device__ __forceinline__ void whole(const uint16_t* kp, const uint16_t* vp, int64_t k_sn, int64_t v_sn, int kb,
-                                          uint32_t lds, int wave) const {
-        const uint16_t* kbp = kp + (int64_t)kb * k_sn;
-        const uint16_t* vbp = vp + (int64_t)kb * v_sn;
-#pragma unroll
-        for (int i = 0; i < LQ; ++i) fta_dma16_so(kbp, koff[i], lds + (i * NW + wave) * 1024);
-#pragma unroll
-        for (int i = 0; i < LQ; ++i) fta_dma16_so(vbp, voff[i], lds + TEN_B + (i * NW + wave) * 1024);
+    // the KEYS rows from kp and vp, all of them inside the tensor; lds: this wave's first block
+    // (the tile's address + 1024 * wave)
+    __device__ __forceinline__ void whole(const uint16_t* kp, const uint16_t* vp, uint32_t lds) const {
+        auto one = [&](auto ii) __attribute__((always_inline)) {
+            constexpr int i = decltype(ii)::value;
+            if constexpr (i < LQ)
+                fta_dma16_to<i * NW * 1024>(kp, koff[i], lds);
+            else
+                fta_dma16_to<TEN_B + (i - LQ) * NW * 1024>(vp, voff[i - LQ], lds);
+        };
+        fta_static_for<0, 2 * LQ>(one);
     }
-    // rows row_of(kb), row_of(kb + 1), ...: 64-bit addresses, formed here so that this
-    // rarer case keeps nothing live
+    // rows row_of(kb), row_of(kb + 1), ... of the sequence at kp and vp: 64-bit addresses,
+    // formed here so that this rarer case keeps nothing live
     template <typename F>
     __device__ __forceinline__ void mapped(const uint16_t* kp, const uint16_t* vp, int64_t k_sn, int64_t v_sn, int kb,
                                            int Dreal, uint32_t lds, int wave, int lane, F row_of) const {
@@ -252,8 +275,8 @@ struct FtaGather {
             int j = SW::slot(row, sidx - row * QSEG);
             if (j * 8 >= Dreal) j = 0;
             const int64_t t = row_of(kb + row);
-            fta_dma16_at(kp + t * k_sn + j * 8, lds + (i * NW + wave) * 1024);
-            fta_dma16_at(vp + t * v_sn + j * 8, lds + TEN_B + (i * NW + wave) * 1024);
+            fta_dma16_at(kp + t * k_sn + j * 8, lds + i * NW * 1024);
+            fta_dma16_at(vp + t * v_sn + j * 8, lds + TEN_B + i * NW * 1024);
         }
     }
 };

@@ -69,7 +69,6 @@ struct WinWalk {
         if (c_lo <= ns) c_lo = ns = 0;
         iters = ns + c_hi - c_lo;
     }
-    __device__ __forceinline__ int key(int it) const { return KEYS * (it < ns ? it : c_lo + it - ns); }
     // whether all rows of the tile at kb are keys that the workgroup sees
     __device__ __forceinline__ bool whole(const WinArgs& a, int kb) const {
         return kb + KEYS <= ke && (kb >= kb0 || kb + KEYS <= a.sinks);
@@ -80,13 +79,37 @@ struct WinWalk {
     }
 };
 
-// Mask case of the 32 keys at kb for rows [i0, i0 + 31]: 0 nothing, 1 partly, 2 all visible.
-__device__ __forceinline__ int tile_case(const WinArgs& a, int len, int i0, int kb) {
-    const int i1 = min(i0 + 31, len - 1), k1 = kb + 31;
-    if (i0 >= len || kb > i1 + a.right || (k1 < i0 - a.left && kb >= a.sinks)) return 0;
-    if (k1 <= i0 + a.right && k1 < len && (kb >= i0 + 31 - a.left || k1 < a.sinks)) return 2;
-    return 1;
-}
+// Walks the tiles in order: first key and its K and V rows, stepped (the multiplications were
+// a good part of the scalar instructions of a tile).
+template <int KEYS>
+struct WinCursor {
+    int it, kb;
+    const uint16_t *k, *v;
+    __device__ __forceinline__ WinCursor(const WinWalk<KEYS>& w, const WinArgs& a, const uint16_t* kp, const uint16_t* vp)
+        : it(0), kb(w.ns > 0 ? 0 : w.c_lo * KEYS), k(kp + (int64_t)kb * a.k_sn), v(vp + (int64_t)kb * a.v_sn) {}
+    __device__ __forceinline__ void next(const WinWalk<KEYS>& w, const WinArgs& a) {
+        int d = KEYS;
+        if (++it == w.ns) d = w.c_lo * KEYS - kb;  // from the sinks to the band
+        kb += d;
+        k += d * a.k_sn;
+        v += d * a.v_sn;
+    }
+};
+
+// What rows [i0, i0 + 31] see of the 32 keys at kb.
+struct WinRows {
+    int full_lo, full_hi;  // everything, for kb in [full_lo, full_hi]
+    int any_lo, any_hi;    // something, for kb in [any_lo, any_hi] (or a sink)
+    __device__ __forceinline__ WinRows(const WinArgs& a, int len, int i0) {
+        full_lo = i0 + 31 - a.left;
+        full_hi = min(i0 + a.right, len - 1) - 31;
+        any_lo = i0 - a.left - 31;
+        any_hi = min(i0 + 31, len - 1) + a.right;
+        if (i0 >= len) full_hi = any_hi = -1;  // padding rows see nothing
+    }
+    __device__ __forceinline__ bool full(int kb) const { return kb >= full_lo && kb <= full_hi; }
+    __device__ __forceinline__ bool none(const WinArgs& a, int kb) const { return kb > any_hi || (kb < any_lo && kb >= a.sinks); }
+};
 
 // Which of the 32 keys at kb row i sees (bit = key).
 __device__ __forceinline__ uint32_t seen_keys(const WinArgs& a, int len, int i, int kb) {
@@ -113,8 +136,7 @@ struct WinPlace {
 // Stages of the forward and dQ: tiles of 32 NH keys of K and V, two in LDS.
 template <int D, int NH>
 struct WinShape {
-    static constexpr int STAGE_B = 2 * FtaTile<FTA_DTYPE_BF16, D, NH>::TEN_B;
-    static constexpr int NST = 2;
+    static constexpr int STAGE_B = 2 * NH * FtaTile<FTA_DTYPE_BF16, D>::TEN_B;
 };
 // waves per SIMD that the registers leave room for
 constexpr int win_fwd_waves(int D) { return D <= 64 ? 4 : 2; }
@@ -134,11 +156,11 @@ constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
-    using T = FtaTile<DT, D, 1>;
+    using T = FtaTile<DT, D>;
     using Sh = WinShape<D, NH>;
     constexpr int PD = D <= 128 ? 3 : 2;  // fragments read ahead
-    constexpr int NST = Sh::NST, KEYS = 32 * NH, LQ = FtaGather<D, kRowWaves, KEYS>::LQ;
-    __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
+    constexpr int KEYS = 32 * NH;
+    __shared__ __align__(1024) unsigned char sStage[2][Sh::STAGE_B];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const WinPlace p(a, wave);
@@ -160,43 +182,49 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
         fta_frag qf[T::KS];
         T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, row < len, a.Dreal, lane, qf);
         const WinWalk<KEYS> w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        const WinRows rows(a, len, p.i0);
         FtaGather<D, kRowWaves, KEYS> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
-        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
-        const FtaLane lo = fta_lane_offsets<D>(lane);
-        auto issue = [&](int it, int st) {
-            const int kb = w.key(it);
-            const uint32_t lds = lds0 + st * Sh::STAGE_B;
-            if (a.kv_narrow && w.whole(a, kb))
-                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds, wave);
+        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]), ldsw = lds0 + 1024 * wave;
+        const FtaAddr<D> ad0(lds0, lane);
+        WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
+        auto issue = [&](int st) __attribute__((always_inline)) {
+            const uint32_t lds = ldsw + st * Sh::STAGE_B;
+            if (a.kv_narrow && w.whole(a, at.kb))
+                g.whole(at.k, at.v, lds);
             else
-                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+            at.next(w, a);
         };
-        fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
-#pragma unroll
-        for (int k = 0; k < NST - 1; ++k)
-            if (k < w.iters) issue(k, k);
-        int cur = 0;
-        for (int it = 0; it < w.iters; ++it) {
-            if (it + NST - 2 < w.iters)
-                fta_wait_vmcnt<2 * LQ * (NST - 2)>();
-            else
-                fta_wait_vmcnt<0>();
+        fta_wait_vmcnt<0>();  // register loads complete before the DMA stream, which the compiler does not count
+        int kb = at.kb, it = 0;
+        issue(0);
+        // one tile, in stage ST: the stages alternate in the code, so that every LDS address is a
+        // kept register and a constant
+        auto tile = [&](auto st) __attribute__((always_inline)) {
+            constexpr int ST = decltype(st)::value;
+            fta_wait_vmcnt<0>();
             __syncthreads();  // tile `it` visible; every wave is past tile it - 1
-            if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
-            const int kb = w.key(it);
-            const uint32_t kbase = lds0 + cur * Sh::STAGE_B;
+            const int next = at.kb;
+            if (++it < w.iters) issue(ST ^ 1);
 #pragma unroll
             for (int sb = 0; sb < NH; ++sb) {
-                const int mc = tile_case(a, len, p.i0, kb + 32 * sb);
-                if (mc == 0) continue;
-                const uint32_t hbase = kbase + sb * T::TEN_B;
-                f32x16 s[1];
-                T::template qk<PD>(hbase, lo, qf, s);
-                if (mc == 1) T::mask(seen_keys(a, len, row, kb + 32 * sb), lane, s[0]);
-                T::template softmax_pv<PD>(hbase + NH * T::TEN_B, lo, s, a.c, m_run, l_run, oacc);
+                const int kh = kb + 32 * sb;
+                const bool full = rows.full(kh);
+                if (!full && rows.none(a, kh)) continue;
+                constexpr uint32_t KO = ST * Sh::STAGE_B, VO = KO + NH * T::TEN_B;
+                const uint32_t ho = sb * T::TEN_B;
+                const FtaAddr<D> ad = ad0.here();
+                f32x16 s;
+                T::template qk<PD>(ad, KO + ho, qf, s);
+                if (!full) T::mask(seen_keys(a, len, row, kh), lane, s);
+                T::template softmax_pv<PD>(ad, VO + ho, s, a.c, m_run, l_run, oacc);
             }
-            cur = (cur == NST - 1) ? 0 : cur + 1;
+            kb = next;
+        };
+        while (it < w.iters) {
+            tile(std::integral_constant<int, 0>{});
+            if (it < w.iters) tile(std::integral_constant<int, 1>{});
         }
     }
 
@@ -221,10 +249,10 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
     using E = Elem<DT>;
-    using T = FtaTile<DT, D, NH>;
+    using T = FtaTile<DT, D>;
     using Sh = WinShape<D, NH>;
-    constexpr int NST = Sh::NST, KEYS = 32 * NH, LQ = FtaGather<D, kRowWaves, KEYS>::LQ, KS = T::KS;
-    __shared__ __align__(1024) unsigned char sStage[NST][Sh::STAGE_B];
+    constexpr int KEYS = 32 * NH, KS = T::KS;
+    __shared__ __align__(1024) unsigned char sStage[2][Sh::STAGE_B];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const WinPlace p(a, wave);
@@ -268,72 +296,75 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
             }
         }
         const WinWalk<KEYS> w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        const WinRows rows(a, len, p.i0);
         FtaGather<D, kRowWaves, KEYS> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
-        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]);
-        const FtaLane lo = fta_lane_offsets<D>(lane);
-        auto issue = [&](int it, int st) {
-            const int kb = w.key(it);
-            const uint32_t lds = lds0 + st * Sh::STAGE_B;
-            if (a.kv_narrow && w.whole(a, kb))
-                g.whole(kp, vp, a.k_sn, a.v_sn, kb, lds, wave);
+        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]), ldsw = lds0 + 1024 * wave;
+        const FtaAddr<D> ad0(lds0, lane);
+        WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
+        auto issue = [&](int st) __attribute__((always_inline)) {
+            const uint32_t lds = ldsw + st * Sh::STAGE_B;
+            if (a.kv_narrow && w.whole(a, at.kb))
+                g.whole(at.k, at.v, lds);
             else
-                g.mapped(kp, vp, a.k_sn, a.v_sn, kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+            at.next(w, a);
         };
-        fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream
-#pragma unroll
-        for (int k = 0; k < NST - 1; ++k)
-            if (k < w.iters) issue(k, k);
-        int cur = 0;
-        for (int it = 0; it < w.iters; ++it) {
-            if (it + NST - 2 < w.iters)
-                fta_wait_vmcnt<2 * LQ * (NST - 2)>();
-            else
-                fta_wait_vmcnt<0>();
+        fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream, which the compiler does not count
+        int kb = at.kb, it = 0;
+        issue(0);
+        // one tile, in stage ST: the stages alternate in the code, so that every LDS address is a
+        // kept register and a constant
+        auto tile = [&](auto st) __attribute__((always_inline)) {
+            constexpr int ST = decltype(st)::value;
+            fta_wait_vmcnt<0>();
             __syncthreads();  // tile `it` visible; every wave is past tile it - 1
-            if (it + NST - 1 < w.iters) issue(it + NST - 1, cur == 0 ? NST - 1 : cur - 1);
-            const int kb = w.key(it);
-            const uint32_t kbase = lds0 + cur * Sh::STAGE_B, vbase = kbase + T::TEN_B;
-            {
+            const int next = at.kb;
+            if (++it < w.iters) issue(ST ^ 1);
 #pragma unroll
-                for (int sb = 0; sb < NH; ++sb) {
-                    const int mc = tile_case(a, len, p.i0, kb + 32 * sb);
-                    if (mc == 0) continue;
-                    fta_frag dsf[2];
-                    f32x16 s, dp;
+            for (int sb = 0; sb < NH; ++sb) {
+                const int kh = kb + 32 * sb;
+                const bool full = rows.full(kh);
+                if (!full && rows.none(a, kh)) continue;
+                constexpr uint32_t KO = ST * Sh::STAGE_B, VO = KO + NH * T::TEN_B;
+                const uint32_t ho = sb * T::TEN_B;
+                const FtaAddr<D> ad = ad0.here();
+                f32x16 s, dp;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-                    fta_frag kf[2], vf[2];  // fragments one MFMA pair ahead
-                    kf[0] = T::row_frag(kbase, lo, sb, 0);
-                    vf[0] = T::row_frag(vbase, lo, sb, 0);
+                for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+                fta_frag kf[2], vf[2], dsf[2];  // K and V fragments one MFMA pair ahead
+                kf[0] = ad.row(KO + ho, 0);
+                vf[0] = ad.row(VO + ho, 0);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        if (ks + 1 < KS) {
-                            kf[(ks + 1) & 1] = T::row_frag(kbase, lo, sb, ks + 1);
-                            vf[(ks + 1) & 1] = T::row_frag(vbase, lo, sb, ks + 1);
-                        }
-                        s = fta_mma<DT>(kf[ks & 1], qf[ks], s);
-                        dp = fta_mma<DT>(vf[ks & 1], df[ks], dp);
+                for (int ks = 0; ks < KS; ++ks) {
+                    if (ks + 1 < KS) {
+                        kf[(ks + 1) & 1] = ad.row(KO + ho, ks + 1);
+                        vf[(ks + 1) & 1] = ad.row(VO + ho, ks + 1);
                     }
-                    if (mc == 1) T::mask(seen_keys(a, len, row, kb + 32 * sb), lane, s);
-#pragma unroll
-                    for (int k2 = 0; k2 < 2; ++k2) {
-                        float ds[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const int i = 8 * k2 + e;
-                            ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
-                        }
-                        dsf[k2] = fta_pack_frag<DT>(ds);
-                    }
-#pragma unroll
-                    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                        for (int dt = 0; dt < T::DT32; ++dt)
-                            acc[dt] = fta_mma<DT>(T::tr_frag(kbase, lo, 2 * sb + ks, dt), dsf[ks], acc[dt]);
+                    s = fta_mma<DT>(kf[ks & 1], qf[ks], s);
+                    dp = fta_mma<DT>(vf[ks & 1], df[ks], dp);
                 }
+                if (!full) T::mask(seen_keys(a, len, row, kh), lane, s);
+#pragma unroll
+                for (int k2 = 0; k2 < 2; ++k2) {
+                    float ds[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int i = 8 * k2 + e;
+                        ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
+                    }
+                    dsf[k2] = fta_pack_frag<DT>(ds);
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                    for (int dt = 0; dt < T::DT32; ++dt) acc[dt] = fta_mma<DT>(ad.tr(KO + ho, ks, dt), dsf[ks], acc[dt]);
             }
-            cur = (cur == NST - 1) ? 0 : cur + 1;
+            kb = next;
+        };
+        while (it < w.iters) {
+            tile(std::integral_constant<int, 0>{});
+            if (it < w.iters) tile(std::integral_constant<int, 1>{});
         }
     }
     if (row < a.N)
@@ -691,7 +722,7 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
 // ----------------------------------------------------------------------------
 template <int D>
 struct WinDkvShape {
-    static constexpr int NW = 4, KEYS = 128, QSEG = D / 8, NST = 2;
+    static constexpr int NW = 4, KEYS = 128, QSEG = D / 8;
     static constexpr int LQ = 32 * QSEG / 256;
     static constexpr int TILE_B = 32 * QSEG * 16;
 };
@@ -700,13 +731,12 @@ template <int DT, int D>
 __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(WinArgs a) {
     using E = Elem<DT>;
     using Sh = WinDkvShape<D>;
-    using T = FtaTile<DT, D, 1>;
-    constexpr int NW = Sh::NW, QSEG = Sh::QSEG, LQ = Sh::LQ, TILE_B = Sh::TILE_B, NST = Sh::NST;
+    using T = FtaTile<DT, D>;
+    constexpr int NW = Sh::NW, QSEG = Sh::QSEG, LQ = Sh::LQ, TILE_B = Sh::TILE_B;
     using SW = FtaSwz<QSEG>;
     constexpr int KS = D / 16, DT32 = D / 32;
-    __shared__ __align__(1024) unsigned char sQ[NST][TILE_B];
-    __shared__ __align__(1024) unsigned char sD[NST][TILE_B];
-    __shared__ __align__(1024) float sL[NST][64];  // lse2, delta
+    __shared__ __align__(1024) unsigned char sStage[2][2 * TILE_B];  // Q, dO
+    __shared__ __align__(1024) float sL[2][64];                       // lse2, delta
 
     const int wgi = fta_xcd_remap(blockIdx.x, a.total);
     const int per = a.ts * a.nps + (a.tiles - a.ts) * a.np;  // workgroups per (b, K/V head)
@@ -756,8 +786,8 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
         if (dcol >= a.Dreal) dcol = 0;  // columns past D: any finite data (never stored)
         const uint32_t qoff = 2u * (drow * (uint32_t)a.q_sn + dcol), doff = 2u * (drow * (uint32_t)a.d_sn + dcol);
         const bool l_isd = (lane & 32) != 0;
-        const FtaLane lo = fta_lane_offsets<D>(lane);
-        const uint32_t ldq = fta_lds_addr(&sQ[0][0]), ldd = fta_lds_addr(&sD[0][0]), ldl = fta_lds_addr(&sL[0][0]);
+        const uint32_t lds0 = fta_lds_addr(&sStage[0][0]), ldsw = lds0 + 1024 * wave, ldl = fta_lds_addr(&sL[0][0]);
+        const FtaAddr<D, (D <= 64)> ad0(lds0, lane);
         const int64_t q_step = 32 * a.q_sn, d_step = 32 * a.d_sn;
         const int64_t q_turn = a.q_sh - (nch - 1) * q_step, d_turn = a.d_sh - (nch - 1) * d_step;
         const int64_t r_turn = a.N - 32 * (int64_t)(nch - 1);
@@ -771,8 +801,11 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
         auto tile_dma = [&](const uint16_t* base, int64_t sn, bool narrow, uint32_t o, uint32_t lds)
             __attribute__((always_inline)) {
             if (narrow && 32 * ci + 32 <= len) {
-#pragma unroll
-                for (int i = 0; i < LQ; ++i) fta_dma16_so(base + i * STEP * sn, o, lds + (i * NW + wave) * 1024);
+                auto one = [&](auto ii) __attribute__((always_inline)) {
+                    constexpr int i = decltype(ii)::value;
+                    fta_dma16_to<i * NW * 1024>(base + i * STEP * sn, o, lds);
+                };
+                fta_static_for<0, LQ>(one);
             } else {  // the sequence's last chunk repeats its last row (masked); formed here, kept nowhere
                 int ln = lane;
                 asm volatile("" : "+v"(ln));
@@ -783,13 +816,13 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
                     int j = SW::slot(row, r2 - row * QSEG);
                     if (j * 8 >= a.Dreal) j = 0;
                     const int64_t t = min(row, len - 1 - 32 * ci);
-                    fta_dma16_at(base + t * sn + j * 8, lds + (i * NW + wave) * 1024);
+                    fta_dma16_at(base + t * sn + j * 8, lds + i * NW * 1024);
                 }
             }
         };
         auto issue = [&](int st) __attribute__((always_inline)) {
-            tile_dma(qp, a.q_sn, a.q_narrow, qoff, ldq + st * TILE_B);
-            tile_dma(dp, a.d_sn, a.d_narrow, doff, ldd + st * TILE_B);
+            tile_dma(qp, a.q_sn, a.q_narrow, qoff, ldsw + st * 2 * TILE_B);
+            tile_dma(dp, a.d_sn, a.d_narrow, doff, ldsw + st * 2 * TILE_B + TILE_B);
             if (wave == 0) {
                 const float* src = l_isd ? a.delta + rp : a.lse2 + rp;
                 fta_dma4_at(src + min(lane & 31, len - 1 - 32 * ci), ldl + st * 256);
@@ -800,41 +833,38 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
             dp += turn ? d_turn : d_step;
             rp += turn ? r_turn : 32;
         };
-#pragma unroll
-        for (int k = 0; k < NST - 1; ++k)
-            if (k < U) issue(k);
-        int st = 0;
-        for (int k = 0; k < U; ++k) {
-            if (k + NST - 2 < U) {
-                if (wave == 0)
-                    fta_wait_vmcnt<(2 * LQ + 1) * (NST - 2)>();
-                else
-                    fta_wait_vmcnt<2 * LQ * (NST - 2)>();
-            } else {
-                fta_wait_vmcnt<0>();
-            }
+        // rows [32 c, 32 c + 31] see all of this wave's keys for c in [full_lo, full_hi], some of them
+        // for c in [any_lo, any_hi] (any later ones too where the keys hold sinks)
+        const int full_lo = (max(kt + 31 - a.right, 0) + 31) >> 5, any_lo = max(kt - a.right, 0) >> 5;
+        const int full_hi = kt + 31 < len ? (min(kt + 31 < a.sinks ? len - 1 : kt + a.left, len - 1) - 31) >> 5 : -1;
+        const int any_hi = kt >= len ? -1 : kt < a.sinks ? len >> 5 : (kt + 31 + a.left) >> 5;
+        int k = 0;
+        issue(0);
+        auto chunk = [&](auto st_) __attribute__((always_inline)) {
+            constexpr int ST = decltype(st_)::value;
+            constexpr uint32_t QO = ST * 2 * TILE_B, OO = QO + TILE_B;
+            fta_wait_vmcnt<0>();
             __syncthreads();  // chunk k visible; every wave is past chunk k - 1
-            if (k + NST - 1 < U) issue(st == 0 ? NST - 1 : st - 1);
-            const int i0 = 32 * cc;
-            cc = cc + 1 == c_end ? c_lo : cc + 1;
-            const bool some = kt < len && i0 + 31 >= kt - a.right && (i0 <= kt + 31 + a.left || kt < a.sinks);
-            if (some) {
-                const bool whole = i0 >= kt + 31 - a.right && i0 + 31 < len && kt + 31 < len &&
-                                   (i0 + 31 <= kt + a.left || kt + 31 < a.sinks);
-                const uint32_t qb = ldq + st * TILE_B, ob = ldd + st * TILE_B;
-                const float* ld = &sL[st][0];
+            const int c = cc;
+            cc = ci;
+            if (++k < U) issue(ST ^ 1);
+            if (c >= any_lo && c <= any_hi) {
+                const bool whole = c >= full_lo && c <= full_hi;
+                const int i0 = 32 * c;
+                const float* ld = &sL[ST][0];
+                const auto ad = ad0.here();
                 f32x16 s, dpv;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] = dpv[i] = 0.f;
                 {
                     fta_frag fq[2], fo[2];
-                    fq[0] = T::row_frag(qb, lo, 0, 0);
-                    fo[0] = T::row_frag(ob, lo, 0, 0);
+                    fq[0] = ad.row(QO, 0);
+                    fo[0] = ad.row(OO, 0);
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         if (ks + 1 < KS) {
-                            fq[(ks + 1) & 1] = T::row_frag(qb, lo, 0, ks + 1);
-                            fo[(ks + 1) & 1] = T::row_frag(ob, lo, 0, ks + 1);
+                            fq[(ks + 1) & 1] = ad.row(QO, ks + 1);
+                            fo[(ks + 1) & 1] = ad.row(OO, ks + 1);
                         }
                         s = fta_mma<DT>(fq[ks & 1], kf[ks], s);
                         dpv = fta_mma<DT>(fo[ks & 1], vf[ks], dpv);
@@ -875,7 +905,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
                     fta_frag fr[PD + 1];
                     auto load = [&](auto nn) __attribute__((always_inline)) {
                         constexpr int n = decltype(nn)::value;
-                        if constexpr (n < NM) fr[n % (PD + 1)] = T::tr_frag((n & 1) ? qb : ob, lo, n / 2 / DT32, n / 2 % DT32);
+                        if constexpr (n < NM) fr[n % (PD + 1)] = ad.tr((n & 1) ? QO : OO, n / 2 / DT32, n / 2 % DT32);
                     };
                     auto slot_ = [&](auto nn) __attribute__((always_inline)) {
                         constexpr int n = decltype(nn)::value, ks = n / 2 / DT32, dt = n / 2 % DT32;
@@ -891,7 +921,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            st = st == NST - 1 ? 0 : st + 1;
+        };
+        while (k < U) {
+            chunk(std::integral_constant<int, 0>{});
+            if (k < U) chunk(std::integral_constant<int, 1>{});
         }
     }
 
