@@ -382,7 +382,9 @@ int cache_plan(CacheArgs& a, int B, int H, int Hk, int T, int S, int D, int P, i
         a.pre_tiles = (int)pt;
         a.pre_ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + pt * Hk - 1) / (pt * Hk), ((int64_t)P + 255) / 256));
     }
-    if (a.rows > 0x7fffffff || wgs * a.ns + (int64_t)Hk * a.pre_tiles * a.pre_ns > 0x7fffffff)
+    // workgroups of 256 threads: fewer than 2^32 threads a launch
+    const int64_t most = (1 << 24) - 1;
+    if (a.rows > most || wgs * a.ns + (int64_t)Hk * a.pre_tiles * a.pre_ns > most)
         return fta::unsupported("cache_attn: too many rows");
     return FTA_OK;
 }
@@ -429,6 +431,9 @@ int fta_cache_attn(const void* q, const int64_t* q_strides, const void* k_cache,
     if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("cache_attn: scale must be positive and finite");
     const size_t need = cache_bytes(a, kernel_dim(D));
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fta::arg_error("cache_attn: workspace too small");
+    if (!fta::all_set(q, q_strides, k_cache, kc_strides, v_cache, vc_strides, cache_lens, o, o_strides, lse) ||
+        (P > 0 && !fta::all_set(k_prefix, kp_strides, v_prefix, vp_strides)))
+        return fta::arg_error("cache_attn: a required pointer is null");
     a.q = (const uint16_t*)q, a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sn = q_strides[2];
     a.k = (const uint16_t*)k_cache, a.k_sb = kc_strides[0], a.k_sh = kc_strides[1], a.k_sn = kc_strides[2];
     a.v = (const uint16_t*)v_cache, a.v_sb = vc_strides[0], a.v_sh = vc_strides[1], a.v_sn = vc_strides[2];

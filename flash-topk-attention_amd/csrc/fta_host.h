@@ -19,6 +19,12 @@ inline int arg_error(const char* msg) {
     set_error(msg);
     return FTA_ERR_ARG;
 }
+
+// Whether every pointer is set.
+template <typename... P>
+inline bool all_set(const P*... p) {
+    return ((p != nullptr) && ...);
+}
 inline int unsupported(const char* msg) {
     set_error(msg);
     return FTA_ERR_UNSUPPORTED;

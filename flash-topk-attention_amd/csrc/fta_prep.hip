@@ -508,6 +508,8 @@ int fta_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, con
     if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
     if (!(eps > 0.f)) return fta::arg_error("qk_norm_rope: eps must be positive");
     if (positions == nullptr && N > P) return fta::arg_error("qk_norm_rope: cos and sin have fewer rows than tokens");
+    if (!fta::all_set(q, q_strides, k, k_strides, cos, sin, q_out, qo_strides, k_out, ko_strides))
+        return fta::arg_error("qk_norm_rope: a required pointer is null");
     PrepArgs a = {};
     a.q = (const uint16_t*)q;
     a.k = (const uint16_t*)k;
@@ -546,6 +548,9 @@ int fta_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k,
     const bool dw = dq_weight != nullptr || dk_weight != nullptr;
     if (dw && (workspace == nullptr || workspace_bytes < fta_qk_norm_rope_bwd_workspace_size(B, H, Hk, N, D)))
         return fta::arg_error("qk_norm_rope_bwd: workspace too small");
+    if (!fta::all_set(q, q_strides, k, k_strides, dq_out, dqo_strides, dk_out, dko_strides, cos, sin, dq, dq_strides, dk,
+                      dk_strides))
+        return fta::arg_error("qk_norm_rope_bwd: a required pointer is null");
     PrepArgs a = {};
     a.q = (const uint16_t*)q;
     a.k = (const uint16_t*)k;
@@ -581,6 +586,9 @@ int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void*
     if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
     if (!(eps > 0.f)) return fta::arg_error("qk_norm_rope: eps must be positive");
     if (S <= 0) return fta::arg_error("qk_norm_rope_append: the caches must have rows");
+    if (!fta::all_set(q, q_strides, k, k_strides, v, v_strides, cos, sin, cache_lens, q_out, qo_strides, k_cache, kc_strides,
+                      v_cache, vc_strides))
+        return fta::arg_error("qk_norm_rope_append: a required pointer is null");
     PrepArgs a = {};
     a.q = (const uint16_t*)q;
     a.k = (const uint16_t*)k;

@@ -1010,6 +1010,8 @@ __global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, 
 
 // ---------------------------------------------------------------------- host
 
+constexpr int64_t kMaxGrid = (1 << 24) - 1;  // workgroups of 256 threads: fewer than 2^32 threads a launch
+
 int kernel_dim(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
 bool narrow(int64_t sn) { return sn >= 0 && sn <= (1 << 24); }
 
@@ -1024,6 +1026,7 @@ int win_common(WinArgs& a, const void* q, const int64_t* qs, const void* k, cons
     if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("window_attn: scale must be positive and finite");
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("window_attn: dtype must be bf16 or fp16");
     if (N > (1 << 29)) return fta::unsupported("window_attn: more than 2^29 tokens");
+    if (!fta::all_set(qs, ks, vs)) return fta::arg_error("window_attn: strides are null");
     a = WinArgs{};
     a.q = (const uint16_t*)q, a.q_sb = qs[0], a.q_sh = qs[1], a.q_sn = qs[2];
     a.k = (const uint16_t*)k, a.k_sb = ks[0], a.k_sh = ks[1], a.k_sn = ks[2];
@@ -1052,7 +1055,7 @@ int64_t row_grid(WinArgs& a) {
 template <int DT, int D>
 int launch_rows(WinArgs& a, bool dq, hipStream_t st) {
     const int64_t grid = row_grid(a);
-    if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    if (grid > kMaxGrid) return fta::unsupported("window_attn: too many tokens");
     a.total = (int)grid;
     if (dq)
         hipLaunchKernelGGL((fta_window_dq_kernel<DT, D, 2>), dim3((unsigned)grid), dim3(kRowWaves * 64), 0, st, a);
@@ -1090,7 +1093,7 @@ size_t part_bytes(const WinArgs& a, int Dk) {
 template <int DT, int D>
 int launch_dkv(WinArgs& a, hipStream_t st) {
     const int64_t grid = ((int64_t)a.ts * a.nps + (int64_t)(a.tiles - a.ts) * a.np) * a.B * a.Hk;
-    if (grid > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    if (grid > kMaxGrid) return fta::unsupported("window_attn: too many tokens");
     a.total = (int)grid;
     if constexpr (D <= 128)
         hipLaunchKernelGGL((fta_window_dkv_kernel<DT, D>), dim3((unsigned)grid), dim3(256), 0, st, a);
@@ -1103,7 +1106,7 @@ int launch_dkv(WinArgs& a, hipStream_t st) {
     constexpr int SLF = 256 / (D / 8) < 16 ? 256 / (D / 8) : 16;
     const int sl = a.np > 1 ? 4 : SLF, per = 256 / (D / 8 * sl);
     const int64_t wgs = (2 * (int64_t)a.B * a.Hk * keys + per - 1) / per;
-    if (wgs > 0x7fffffff) return fta::unsupported("window_attn: too many tokens");
+    if (wgs > kMaxGrid) return fta::unsupported("window_attn: too many tokens");
     if (a.np > 1)
         hipLaunchKernelGGL((fta_window_dkv_combine_kernel<DT, D, 4>), dim3((unsigned)wgs), dim3(256), 0, st, a, keys);
     else
@@ -1137,6 +1140,8 @@ int fta_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, 
     int rc = win_common(a, q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, N, D, seq_lens, left, right,
                         num_sinks, scale);
     if (rc != FTA_OK) return rc;
+    if (!fta::all_set(q, k, v, o, o_strides, lse))
+        return fta::arg_error("window_attn: a required pointer is null");
     a.out0 = (uint16_t*)o, a.o0_sb = o_strides[0], a.o0_sh = o_strides[1], a.o0_sn = o_strides[2];
     a.lse = lse;
     return with_shape(dtype, D, [&](auto dt, auto dk) {
@@ -1168,6 +1173,8 @@ int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, 
     if (rc != FTA_OK) return rc;
     if (workspace == nullptr || workspace_bytes < fta_window_attn_bwd_workspace_size(B, H, Hk, N, D, left, right, num_sinks))
         return fta::arg_error("window_attn_bwd: workspace too small");
+    if (!fta::all_set(q, k, v, o, o_strides, dout, do_strides, lse, dq, dq_strides, dk, dk_strides, dv, dv_strides))
+        return fta::arg_error("window_attn_bwd: a required pointer is null");
     a.o = (const uint16_t*)o, a.o_sb = o_strides[0], a.o_sh = o_strides[1], a.o_sn = o_strides[2];
     a.dout = (const uint16_t*)dout, a.d_sb = do_strides[0], a.d_sh = do_strides[1], a.d_sn = do_strides[2];
     a.d_narrow = narrow(a.d_sn);

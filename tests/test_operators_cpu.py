@@ -118,3 +118,45 @@ def test_cache_entry_sizes():
     assert L.fta_cache_attn_workspace_size(1, 4, 2, 1, 10, 64, 0, 3, 0) == 0  # one part: o written directly
     assert L.fta_cache_attn_workspace_size(1, 4, 2, 1, 10, 64, 70, 10, 0) > 0
     assert L.fta_cache_attn_workspace_size(1, 4, 3, 1, 10, 64, 0, 3, 0) == 0
+
+
+def _pointers(entry):
+    """Entry, its arguments as a list, and the places of the pointers it requires.  Every
+    pointer is some address that nothing reads: with one of them null the entry returns
+    before any launch."""
+    L = _lib.lib()
+    z, x = _lib.i64arr((0, 0, 0)), 4096
+    if entry == "prep":
+        args = [x, z, x, z, 0, 1, 2, 1, 4, 64, None, None, 2, x, x, 4, 64, None, 0, 1e-6, 0, x, z, x, z, None]
+        return L.fta_qk_norm_rope, args, (0, 1, 2, 3, 13, 14, 21, 22, 23, 24)
+    if entry == "prep_bwd":
+        args = [x, z, x, z, x, z, x, z, 0, 1, 2, 1, 4, 64, None, None, 2, x, x, 4, 64, None, 0, 1e-6, 0, x, z, x, z,
+                None, None, None, 0, None]
+        return L.fta_qk_norm_rope_bwd, args, (*range(8), 17, 18, 25, 26, 27, 28)
+    if entry == "append":
+        args = [x, z, x, z, x, z, 0, 1, 2, 1, 4, 64, None, None, 2, x, x, 4, 64, 0, 1e-6, 0, x, 8, x, z, x, z, x, z, None]
+        return L.fta_qk_norm_rope_append, args, (*range(6), 15, 16, 22, *range(24, 30))
+    if entry == "window":
+        args = [x, z, x, z, x, z, 0, 1, 4, 2, 10, 64, None, 3, 0, 0, 0.1, x, z, x, None]
+        return L.fta_window_attn_fwd, args, (*range(6), 17, 18, 19)
+    if entry == "window_bwd":
+        size = L.fta_window_attn_bwd_workspace_size(1, 4, 2, 10, 64, 3, 0, 0)
+        args = [x, z, x, z, x, z, x, z, x, z, 0, 1, 4, 2, 10, 64, None, 3, 0, 0, 0.1, x, x, z, x, z, x, z, x, size, None]
+        return L.fta_window_attn_bwd, args, (*range(10), *range(21, 29))
+    size = L.fta_cache_attn_workspace_size(1, 4, 2, 1, 10, 64, 5, 10, 0)
+    args = [x, z, x, z, x, z, 0, 1, 4, 2, 1, 10, 64, x, x, z, x, z, 5, 10, 0, 0.1, x, z, x, x, size, None]
+    return L.fta_cache_attn, args, (*range(6), *range(13, 18), *range(22, 26))
+
+
+@pytest.mark.parametrize("entry", ["prep", "prep_bwd", "append", "window", "window_bwd", "cache"])
+def test_null_pointers(entry):
+    call, args, required = _pointers(entry)
+    assert len(args) == len(call.argtypes)
+    for i in required:
+        assert call(*(args[:i] + [None] + args[i + 1:])) == _lib.FTA_ERR_ARG, i
+
+
+def test_launch_limits():
+    L = _lib.lib()
+    assert L.fta_cache_attn_workspace_size(1 << 24, 1, 1, 1, 10, 64, 0, 3, 0) == 0  # 2^32 threads
+    assert _cache(L, B=1 << 24, H=1, Hk=1) == _lib.FTA_ERR_UNSUPPORTED
