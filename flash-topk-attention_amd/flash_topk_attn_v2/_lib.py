@@ -231,6 +231,17 @@ def head_counts(what: str, width: int, num_heads: int, num_kv_heads):
     return H, Hk, D
 
 
+def int_sizes(what: str, *sizes: int) -> None:
+    """Refuses sizes that the library's 32-bit ints do not hold (ctypes would wrap them)."""
+    if max(sizes) >= 1 << 31:
+        raise NotImplementedError(f"{what}: a size of {max(sizes)}; sizes must be below 2^31")
+
+
+def scalars(num_heads, num_kv_heads, real):
+    """Head counts and a real number as Python numbers: what a cached check may be keyed by."""
+    return int(num_heads), None if num_kv_heads is None else int(num_kv_heads), None if real is None else float(real)
+
+
 HALVES = (torch.float16, torch.bfloat16)
 DTYPE_CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
 

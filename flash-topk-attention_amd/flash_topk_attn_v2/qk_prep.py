@@ -30,6 +30,7 @@ def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, wei
         raise ValueError(f"{what}: k must be {[q[0], q[1], Hk * D]}")
     if q[0] == 0 or q[1] == 0:
         raise ValueError(f"{what}: empty batch or sequence")
+    _lib.int_sizes(what, q[0], q[1], *cos)
     if len(cos) != 2 or cos != sin or table_types != (torch.float32, torch.float32):
         raise ValueError(f"{what}: cos and sin must be float32 tables [P, R / 2] of one shape")
     R = 2 * cos[1]
@@ -43,7 +44,7 @@ def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, wei
     types = {t for t in weight_types if t is not None}
     if len(types) > 1 or not types <= set(_lib.DTYPE_CODES):
         raise ValueError(f"{what}: weights must both be float32, float16 or bfloat16")
-    if not 0.0 < float(eps) < float("inf"):
+    if not 0.0 < eps < float("inf"):
         raise ValueError(f"{what}: eps must be positive")
     return H, Hk, D, R, _lib.DTYPE_CODES[types.pop()] if types else _lib.DTYPE_F32
 
@@ -51,6 +52,7 @@ def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, wei
 def _check(what, q, k, num_heads, num_kv_heads, cos, sin, qw, kw, eps):
     if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
+    num_heads, num_kv_heads, eps = _lib.scalars(num_heads, num_kv_heads, eps)
     geo = _geometry(what, q.shape, k.shape, (q.dtype, k.dtype), cos.shape, sin.shape, (cos.dtype, sin.dtype),
                     None if qw is None else qw.shape, None if kw is None else kw.shape,
                     (None if qw is None else qw.dtype, None if kw is None else kw.dtype), num_heads, num_kv_heads, eps)
@@ -222,6 +224,7 @@ def check_cache(what, q, k_cache, v_cache, cache_lens, B, width):
     shape = k_cache.shape
     if len(shape) != 3 or shape[0] != B or shape[2] != width or shape[1] == 0:
         raise ValueError(f"{what}: k_cache must be [B, S, num_kv_heads * D] = [{B}, S, {width}]")
+    _lib.int_sizes(what, shape[1])
     if v_cache.shape != shape:
         raise ValueError(f"{what}: v_cache must have k_cache's shape")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:

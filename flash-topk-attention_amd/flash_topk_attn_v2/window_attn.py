@@ -31,11 +31,12 @@ def _geometry(what, q, k, v, dtypes, num_heads, num_kv_heads, window, num_sinks,
         raise ValueError(f"{what}: empty batch or sequence")
     if tuple(k) != (B, N, Hk * D) or tuple(v) != (B, N, Hk * D):
         raise ValueError(f"{what}: k and v must be [B, N, num_kv_heads * D] = {[B, N, Hk * D]}")
-    if len(window) != 2 or int(window[0]) < 0 or int(window[1]) < 0:
+    _lib.int_sizes(what, B, N)
+    if len(window) != 2 or min(window) < 0:
         raise ValueError(f"{what}: window must be (left, right), both non-negative")
-    if int(num_sinks) < 0:
+    if num_sinks < 0:
         raise ValueError(f"{what}: num_sinks must be non-negative")
-    left, right, sinks = (min(int(x), _MAX) for x in (*window, num_sinks))
+    left, right, sinks = (min(x, _MAX) for x in (*window, num_sinks))
     return H, Hk, D, left, right, sinks, _lib.softmax_scale(what, scale, D)
 
 
@@ -120,8 +121,9 @@ def flash_window_attn(
     what = "flash_window_attn"
     if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    geo = _geometry(what, q.shape, k.shape, v.shape, (q.dtype, k.dtype, v.dtype), num_heads, num_kv_heads, tuple(window),
-                    num_sinks, scale)
+    num_heads, num_kv_heads, scale = _lib.scalars(num_heads, num_kv_heads, scale)
+    geo = _geometry(what, q.shape, k.shape, v.shape, (q.dtype, k.dtype, v.dtype), num_heads, num_kv_heads,
+                    tuple(map(int, window)), int(num_sinks), scale)
     _lib.check_device(what, q.device, k, v, seq_lens)
     if seq_lens is not None:
         if seq_lens.dtype != torch.int32 or seq_lens.shape != q.shape[:1]:

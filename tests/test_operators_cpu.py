@@ -160,3 +160,18 @@ def test_launch_limits():
     L = _lib.lib()
     assert L.fta_cache_attn_workspace_size(1 << 24, 1, 1, 1, 10, 64, 0, 3, 0) == 0  # 2^32 threads
     assert _cache(L, B=1 << 24, H=1, Hk=1) == _lib.FTA_ERR_UNSUPPORTED
+
+
+def test_sizes_past_32_bits():
+    """They are refused before they would wrap."""
+    from flash_topk_attn_v2 import cache_attn, qk_prep, window_attn
+
+    n, f = 1 << 31, torch.float32
+    prep = ("prep", (1, n, 64), (1, n, 64), (BF, BF), (n, 32), (n, 32), (f, f), None, None, (None, None), 1, 1, 1e-6)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        qk_prep._geometry(*prep)
+    with pytest.raises(NotImplementedError, match="2\\^31"):
+        window_attn._geometry("window", (1, n, 64), (1, n, 64), (1, n, 64), (BF, BF, BF), 1, 1, (3, 0), 0, None)
+    for S, P in ((n, 0), (4, n)):
+        with pytest.raises(NotImplementedError, match="2\\^31"):
+            cache_attn._geometry("cache", (1, 1, 64), BF, 1, 1, S, P, None, 0, None)
