@@ -58,25 +58,19 @@ __device__ __forceinline__ int seq_len(const WinArgs& a, int b) {
 // The tiles of KEYS keys that rows [i_lo, i_hi] see: `ns` tiles of sinks, then the band's.
 template <int KEYS>
 struct WinWalk {
-    int kb0, ke;   // the band's keys [kb0, ke)
-    int ns, c_lo, iters;
-    __device__ __forceinline__ WinWalk(const WinArgs& a, int len, int i_lo, int i_hi) {
-        kb0 = max(0, i_lo - a.left);
-        ke = min(len, i_hi + a.right + 1);
+    int len, ns, c_lo, iters;
+    __device__ __forceinline__ WinWalk(const WinArgs& a, int len_, int i_lo, int i_hi) : len(len_) {
+        const int kb0 = max(0, i_lo - a.left), ke = min(len, i_hi + a.right + 1);  // the band's keys [kb0, ke)
         const int c_hi = (ke + KEYS - 1) / KEYS;
         c_lo = kb0 / KEYS;
         ns = (min(a.sinks, ke) + KEYS - 1) / KEYS;
         if (c_lo <= ns) c_lo = ns = 0;
         iters = ns + c_hi - c_lo;
     }
-    // whether all rows of the tile at kb are keys that the workgroup sees
-    __device__ __forceinline__ bool whole(const WinArgs& a, int kb) const {
-        return kb + KEYS <= ke && (kb >= kb0 || kb + KEYS <= a.sinks);
-    }
-    // a key that the workgroup sees in place of one that it does not
-    __device__ __forceinline__ int seen(const WinArgs& a, int t) const {
-        return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t;
-    }
+    // whether all rows of the tile at kb are tokens in front of len
+    __device__ __forceinline__ bool whole(int kb) const { return kb + KEYS <= len; }
+    // a token in front of len in place of one that is not
+    __device__ __forceinline__ int seen(int t) const { return min(t, len - 1); }
 };
 
 // Walks the tiles in order: first key and its K and V rows, stepped (the multiplications were
@@ -190,10 +184,10 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
         WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
         auto issue = [&](int st) __attribute__((always_inline)) {
             const uint32_t lds = ldsw + st * Sh::STAGE_B;
-            if (a.kv_narrow && w.whole(a, at.kb))
+            if (a.kv_narrow && w.whole(at.kb))
                 g.whole(at.k, at.v, lds);
             else
-                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(t); });
             at.next(w, a);
         };
         fta_wait_vmcnt<0>();  // register loads complete before the DMA stream, which the compiler does not count
@@ -304,10 +298,10 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
         WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
         auto issue = [&](int st) __attribute__((always_inline)) {
             const uint32_t lds = ldsw + st * Sh::STAGE_B;
-            if (a.kv_narrow && w.whole(a, at.kb))
+            if (a.kv_narrow && w.whole(at.kb))
                 g.whole(at.k, at.v, lds);
             else
-                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(a, t); });
+                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(t); });
             at.next(w, a);
         };
         fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream, which the compiler does not count
