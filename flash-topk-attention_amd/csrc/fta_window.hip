@@ -10,12 +10,13 @@
 //
 // The walk of a workgroup is arithmetic, not a list: the 64-key tiles of the sinks,
 // then those of its rows' band.  Per wave and tile the mask is one of three cases,
-// told apart by scalar compares: nothing visible (skipped), everything (no mask), or
-// a per-lane range test at the band's two edges.
+// told apart by scalar compares: nothing visible (skipped), everything (no mask), or,
+// at the band's two edges, a word per row whose bits are the visible keys.
 //
-// Nothing that no query of the workgroup sees is read: DMA rows outside the sinks and
-// the band are taken from a visible row instead (their scores are masked), so tokens
-// past len, and whatever they hold, cannot reach a result.
+// Rows at or past len are never read: a tile that reaches them takes token len - 1 in
+// their place (its scores are masked), so what padding holds cannot reach a result.
+// Tiles inside the sequence are gathered whole, whether or not a row of the workgroup
+// sees all their keys.
 #include "fta_common.h"
 #include "fta_host.h"
 #include "fta_tile.h"
@@ -44,7 +45,7 @@ struct WinArgs {
     int left, right, sinks;
     float c, scale;
     int hw;               // forward, dQ: query heads per workgroup (they share K / V)
-    int tiles;            // forward, dQ: token tiles per head; dK / dV: 64-key tiles
+    int tiles;            // forward, dQ: token tiles per head; dK / dV: tiles of kt_keys keys
     int kt_keys;          // dK / dV: keys per tile
     int ts, nps, np;      // dK / dV: tiles that hold sinks, parts of each of them, parts of the others
     int total;
@@ -140,13 +141,18 @@ constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 // Forward.  Four waves of 32 rows: hw query heads that share a K/V head, 4 / hw row
 // tiles each; 64-key tiles of K and V (32 at D = 256), worked on 32 keys at a time so
 // that the half tiles at the band's edges and the sinks' tile cost what they hold.
-// What bounds it: neither pipe alone.  N32768, 32 / 8 heads of 128, window 1024, 4 sinks:
-// 730 us, 835 TFLOP/s with the masked scores (65% of a large library product on the same
-// card); matrix units 38% busy, vector units 35%, LDS 45%; more waves per SIMD (three, by
-// 32-key stages) and other prefetch distances or wave priorities change it by under 4%.
+// What bounds it at D = 128: power, then neither pipe alone.  N32768, 32 / 8 heads of 128,
+// window 1024, 4 sinks: 681 us at a clock of 1.95 GHz (914 us in a run that held 1.44), 844
+// TFLOP/s with the masked scores, 66% of a large library product on the same card; matrix
+// units 44% busy, vector units 40%, LDS 45%; more waves per SIMD (three, by 32-key stages)
+// and other prefetch distances or wave priorities change it by under 4%.  Gathering the edge
+// tiles whole took 74.6 -> 71.3 us at D = 64 (N10000 twice, 12 / 4 heads, 300 to both sides)
+// and 705 -> 681 here.  At D = 64 the vector unit bounds it: of 84 vector instructions per 32
+// x 32 scores (four cycles each, the 16 exp2 more) 64 are the fma, exp2, sum and packing of
+// the softmax and 8 its maximum, against 8 MFMAs.
 // D = 256 is held to 256 registers, two workgroups per CU: with 512 the compiler moved the
-// whole accumulator through copies at every tile (N4096, 16 / 2 heads, window 512: 150 ->
-// 107 us).
+// whole accumulator through copies at every tile (N4096 twice, 16 / 2 heads, window 512: 150
+// -> 101 us, 643 TFLOP/s without the masked scores).
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
@@ -239,6 +245,8 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 // dQ, with the forward's walk: S^T and dP^T = V dO^T of 32 keys at a time,
 // dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
 // rows are at hand) and the lse in log2 units for dK / dV.
+// Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 905 us, 953 TFLOP/s
+// with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 89 us.
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
@@ -372,7 +380,9 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
 // crosses in fp32 through LDS:
 //   wave (tt, 0):  S = Q K^T,  P = 2^{c S - lse2}  -> LDS;  dV += P^T dO
 //   wave (tt, 1):  dP = dO V^T;  dS = P (dP - delta);  dK += dS^T Q
-// One barrier per step; Q two steps ahead in four tiles, dO in three.
+// One barrier per step; Q two steps ahead in four tiles, dO in three.  One workgroup per CU,
+// so each step waits out its own barrier and LDS latencies: N4096, 8 heads of 256, window
+// 512: 100 us; N8192, causal: 765 us, 720 TFLOP/s.
 //
 // This kernel and the next walk the 32-query chunks that see any of the workgroup's keys,
 // through all query heads of the group in one sequence, so the sums over shared heads need
@@ -708,11 +718,12 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
 // leaves the wave:
 //   S = Q K^T,  dP = dO V^T,  P = 2^{c S - lse2},  dS = P (dP - delta),
 //   dV += P^T dO,  dK += dS^T Q.
-// At D = 128 that is 254 registers, two workgroups per CU; 154 and three at D = 64.  Against
+// At D = 128 that is 250 registers, two workgroups per CU; 158 and three at D = 64.  Against
 // 64 keys a workgroup with the work of a tile split over two waves (the kernel above):
 // half the gathers and barriers, no exchange of P.  N32768, 32 / 8 heads of 128, window
-// 1024: 1510 -> 1290 us (870 TFLOP/s with the masked scores); N10000 twice, 12 / 4 heads of
-// 64, 300 to both sides: 175 -> 126.  Three stages instead of two change nothing.
+// 1024: 1510 -> 1150 us, 1000 TFLOP/s with the masked scores at a clock of 1.65 GHz (power);
+// N10000 twice, 12 / 4 heads of 64, 300 to both sides: 175 -> 113.  Three stages instead of
+// two change nothing.
 // ----------------------------------------------------------------------------
 template <int D>
 struct WinDkvShape {
