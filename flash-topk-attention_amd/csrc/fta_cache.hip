@@ -69,7 +69,7 @@ struct CacheShape {
 // as it has read the last one, into the same stage: the other waves of the CU (eight at
 // D = 128, 128 KB of loads in all) cover its wait, and a second stage changed nothing.
 // What bounds it: memory.  128 requests, 32 / 8 heads of 128, 4096 of 8192 cached tokens:
-// 363 to 376 us, 5.7 to 5.9 TB/s (a large copy moves 5.15); one request: 8 us and 4 for the
+// 356 to 361 us, 6.0 TB/s (a large copy moves 5.15); one request: 7 us and 4 for the
 // join, latencies.
 // ----------------------------------------------------------------------------
 template <int DT, int D>
@@ -277,13 +277,16 @@ __device__ void cache_prefix(const CacheArgs& a, int wgi, unsigned char* sStage)
 // some of each.  64 requests, 32 / 8 heads of 128, a prefix of 32768 and 768 own tokens on
 // average: 47 + 47 us as two launches, 84 as one; prefix first or last is 3 to 5% slower.
 // Each CU holds two workgroups (registers and LDS), so the mix hides less than it could.
+// The own keys' workgroups go to the XCDs in turn: parts of one cache share no keys, and
+// runs of requests on one XCD would leave it with the longest (128 requests of 256 to 4096
+// tokens: 273 -> 212 us; of 4096 out of 8192: 370 -> 358).
 template <int DT, int D>
 __global__ __launch_bounds__(CacheShape<D>::NW * 64, D <= 64 ? 4 : D <= 128 ? 2 : 1) void fta_cache_attn_kernel(CacheArgs a) {
     using Sh = CacheShape<D>;
     __shared__ __align__(1024) unsigned char sStage[Sh::LDS_B];
     __shared__ float2 sML[Sh::NW][32];
     if (a.pre_total == 0) {
-        cache_own<DT, D>(a, fta_xcd_remap(blockIdx.x, a.total), sStage, sML);
+        cache_own<DT, D>(a, blockIdx.x, sStage, sML);
         return;
     }
     const int64_t all = a.pre_total + a.total;
@@ -292,7 +295,7 @@ __global__ __launch_bounds__(CacheShape<D>::NW * 64, D <= 64 ? 4 : D <= 128 ? 2 
     if (pre)
         cache_prefix<DT, D>(a, fta_xcd_remap(before, a.pre_total), sStage);
     else
-        cache_own<DT, D>(a, fta_xcd_remap(blockIdx.x - before, a.total), sStage, sML);
+        cache_own<DT, D>(a, blockIdx.x - before, sStage, sML);
 }
 
 // Join of the parts, one workgroup per row: D / 8 column groups x 2048 / D slices of

@@ -68,7 +68,7 @@ def test_forward_and_gradients(gpu, case):
 @pytest.mark.parametrize("dtype,B,N,H,Hk,D,left,sinks", [
     (BF, 1, 4200, 32, 8, 128, 500, 4), (FP, 2, 4100, 16, 16, 64, 127, 1), (BF, 1, 4099, 32, 4, 64, 1023, 70)])
 def test_grids_that_fill_the_card(gpu, dtype, B, N, H, Hk, D, left, sinks):
-    """The workgroups of eight waves, whose heads share K and V."""
+    """Many workgroups, whose heads share K and V."""
     say("window large", dtype, B, N, H, Hk, D)
     q, k, v, do = _inputs(gpu, dtype, B, N, H, Hk, D)
     got = _run(q, k, v, do, H, Hk, (left, 0), sinks)
