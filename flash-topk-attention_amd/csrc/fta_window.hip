@@ -151,8 +151,8 @@ constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 // TFLOP/s with the masked scores, 66% of a large library product on the same card; matrix
 // units 44% busy, vector units 40%, LDS 45%; more waves per SIMD (three, by 32-key stages)
 // and other prefetch distances or wave priorities change it by under 4%.  Gathering the edge
-// tiles whole took 74.6 -> 71.3 us at D = 64 (N10000 twice, 12 / 4 heads, 300 to both sides)
-// and 705 -> 681 here.  At D = 64 the vector unit bounds it: of 84 vector instructions per 32
+// tiles whole took 74.6 -> 71.3 us at D = 64 (N10000 twice, 12 / 4 heads, 300 to both sides;
+// 68 with the heads outermost) and 705 -> 681 here.  At D = 64 the vector unit bounds it: of 84 vector instructions per 32
 // x 32 scores (four cycles each, the 16 exp2 more) 64 are the fma, exp2, sum and packing of
 // the softmax and 8 its maximum, against 8 MFMAs.
 // D = 256 is held to 256 registers, two workgroups per CU: with 512 the compiler moved the
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 // dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
 // rows are at hand) and the lse in log2 units for dK / dV.
 // Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 905 us, 953 TFLOP/s
-// with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 89 us.
+// with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 85 us.
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
@@ -728,7 +728,7 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
 // 64 keys a workgroup with the work of a tile split over two waves (the kernel above):
 // half the gathers and barriers, no exchange of P.  N32768, 32 / 8 heads of 128, window
 // 1024: 1510 -> 1150 us, 1000 TFLOP/s with the masked scores at a clock of 1.65 GHz (power);
-// N10000 twice, 12 / 4 heads of 64, 300 to both sides: 175 -> 113.  Three stages instead of
+// N10000 twice, 12 / 4 heads of 64, 300 to both sides: 175 -> 110.  Three stages instead of
 // two change nothing.
 // ----------------------------------------------------------------------------
 template <int D>
