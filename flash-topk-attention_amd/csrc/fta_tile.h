@@ -29,7 +29,6 @@ __device__ __forceinline__ int fta_scalar(int x) { return __builtin_amdgcn_readf
 
 // Bits [lo, hi) of a 32-bit mask; lo and hi may lie anywhere.
 __device__ __forceinline__ uint32_t fta_bits_below(int hi) { return hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u; }
-__device__ __forceinline__ uint32_t fta_bits(int lo, int hi) { return fta_bits_below(hi) & ~fta_bits_below(lo); }
 
 // An MFMA operand fragment.  A vector type all the way from its load: as a struct of four
 // words the compiler may read it word by word (two ds_read2_b32 instead of one

@@ -1080,7 +1080,8 @@ int launch_rows(WinArgs& a, bool dq, hipStream_t st) {
 // at least 8 steps (N1024, 4 heads of 128, causal: 47 us whole, 19.4 + 5 with their sum in
 // 4; N2048, 8 on 2 heads of 64, window 256: 52 + 4.6 -> 18.4 + 5.4), but not shorter ones
 // (N2048, 8 heads of 128, window 256, 13 steps: 26.9 + 4.8 whole, 21.4 + 12.4 in 2).  The
-// tiles with sinks get parts as long as the other walks.
+// tiles with sinks get parts as long as the other walks, 2048 in all (268 MB of parts at D =
+// 128), which is what fills the card several times over.
 void dkv_parts(WinArgs& a) {
     a.kt_keys = a.Dreal <= 128 ? 128 : 64;
     a.tiles = (a.N + a.kt_keys - 1) / a.kt_keys;
@@ -1091,7 +1092,9 @@ void dkv_parts(WinArgs& a) {
     const int64_t np = std::max<int64_t>(1, std::min<int64_t>({4, 256 / wgs, steps / 8}));
     a.np = (int)np;
     const int64_t own = std::max<int64_t>(8, steps / np);
-    a.nps = a.ts == 0 ? 1 : (int)std::max<int64_t>(np, std::min<int64_t>(128, (a.G * nall + own - 1) / own));
+    const int64_t sink_wgs = (int64_t)a.ts * a.B * a.Hk;
+    a.nps = a.ts == 0 ? 1
+                      : (int)std::max<int64_t>(np, std::min<int64_t>({128, (a.G * nall + own - 1) / own, 2048 / sink_wgs}));
 }
 
 int64_t dkv_slots(const WinArgs& a) {

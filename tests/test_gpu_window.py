@@ -66,7 +66,8 @@ def test_forward_and_gradients(gpu, case):
 
 
 @pytest.mark.parametrize("dtype,B,N,H,Hk,D,left,sinks", [
-    (BF, 1, 4200, 32, 8, 128, 500, 4), (FP, 2, 4100, 16, 16, 64, 127, 1), (BF, 1, 4099, 32, 4, 64, 1023, 70)])
+    (BF, 1, 4200, 32, 8, 128, 500, 4), (FP, 2, 4100, 16, 16, 64, 127, 1), (BF, 1, 4099, 32, 4, 64, 1023, 70),
+    (FP, 4, 1000, 16, 16, 16, 40, 900), (BF, 5, 600, 32, 16, 256, 9, 500)])  # more tiles of sinks than parts for each
 def test_grids_that_fill_the_card(gpu, dtype, B, N, H, Hk, D, left, sinks):
     """Many workgroups, whose heads share K and V."""
     say("window large", dtype, B, N, H, Hk, D)

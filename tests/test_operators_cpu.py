@@ -175,3 +175,12 @@ def test_sizes_past_32_bits():
     for S, P in ((n, 0), (4, n)):
         with pytest.raises(NotImplementedError, match="2\\^31"):
             cache_attn._geometry("cache", (1, 1, 64), BF, 1, 1, S, P, None, 0, None)
+
+
+def test_window_workspace_of_many_sinks():
+    """The parts of the sinks' walks stay a few hundred MB, however many sinks and sequences."""
+    L = _lib.lib()
+    for B, H, Hk, N, D, left, sinks in ((1, 32, 8, 32768, 128, 1023, 16384), (1, 32, 32, 32768, 256, 15, 8192),
+                                        (64, 16, 16, 4096, 128, 63, 100), (8, 4, 1, 100000, 64, 0, 99000)):
+        rows = 2 * 4 * B * H * N
+        assert 0 < L.fta_window_attn_bwd_workspace_size(B, H, Hk, N, D, left, 0, sinks) <= rows + 512 + (300 << 20)
