@@ -249,7 +249,10 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 // ----------------------------------------------------------------------------
 // dQ, with the forward's walk: S^T and dP^T = V dO^T of 32 keys at a time,
 // dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
-// rows are at hand) and the lse in log2 units for dK / dV.
+// rows are at hand) and the lse in log2 units for dK / dV.  delta is summed in fp32 from the
+// rounded o: dQ and dK are off by 1.5 times a rounding of the exact ones (2.3 times for rows that
+// see two keys), against 1.4 times from the rounding of dS alone; an o of more bits would cost
+// every training step another tensor of its size.
 // Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 905 us, 953 TFLOP/s
 // with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 85 us.
 // ----------------------------------------------------------------------------
