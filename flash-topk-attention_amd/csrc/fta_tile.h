@@ -27,7 +27,7 @@ __device__ __forceinline__ void fta_static_for(F& f) {
 // instruction wrote it, and nothing sees that distance into inline asm).
 __device__ __forceinline__ int fta_scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-// Bits [lo, hi) of a 32-bit mask; lo and hi may lie anywhere.
+// A 32-bit mask of the bits below hi, which may lie anywhere.
 __device__ __forceinline__ uint32_t fta_bits_below(int hi) { return hi >= 32 ? 0xffffffffu : hi <= 0 ? 0u : (1u << hi) - 1u; }
 
 // An MFMA operand fragment.  A vector type all the way from its load: as a struct of four
