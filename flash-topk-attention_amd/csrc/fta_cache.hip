@@ -367,6 +367,7 @@ int cache_plan(CacheArgs& a, int B, int H, int Hk, int T, int S, int D, int P, i
     if (P < 0 || left < 0 || sinks < 0) return fta::arg_error("cache_attn: prefix, window and num_sinks must be non-negative");
     if (S > (1 << 29) || T > (1 << 20) || P > (1 << 29) || H > (1 << 20))
         return fta::unsupported("cache_attn: sizes past 2^29 keys, 2^20 new tokens or heads");
+    if (!fta::size_fits(B, T, H, D)) return fta::unsupported("cache_attn: 2^60 elements and more");
     if (P > 0 && left < S) return fta::unsupported("cache_attn: a window behind a shared prefix");
     a = CacheArgs{};
     a.B = B, a.T = T, a.H = H, a.Hk = Hk, a.G = H / Hk, a.S = S, a.P = P, a.Dreal = D;

@@ -30,6 +30,11 @@ inline int unsupported(const char* msg) {
     return FTA_ERR_UNSUPPORTED;
 }
 
+// Whether the elements of [B][N][heads][D] leave room for 64-bit arithmetic on their
+// number.  No tensor that exists fails this, but sizes alone reach the entry points, and
+// a product that wraps to zero would be divided by.
+inline bool size_fits(int B, int N, int64_t heads, int D) { return (double)B * N * (double)heads * D < 0x1p60; }
+
 inline int check_launch(const char* what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) {

@@ -405,6 +405,7 @@ int prep_geometry(int B, int H, int Hk, int N, int D, int R, int P) {
         return fta::arg_error("qk_norm_rope: the rotated columns must be a positive multiple of 16 up to D");
     if (P <= 0) return fta::arg_error("qk_norm_rope: cos and sin must have rows");
     if (H > (1 << 20) || Hk > (1 << 20)) return fta::unsupported("qk_norm_rope: too many heads");
+    if (!fta::size_fits(B, N, (int64_t)H + 2 * Hk, D)) return fta::unsupported("qk_norm_rope: 2^60 elements and more");
     return FTA_OK;
 }
 

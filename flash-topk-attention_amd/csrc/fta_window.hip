@@ -1041,6 +1041,7 @@ int win_common(WinArgs& a, const void* q, const int64_t* qs, const void* k, cons
     if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("window_attn: scale must be positive and finite");
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("window_attn: dtype must be bf16 or fp16");
     if (N > (1 << 29)) return fta::unsupported("window_attn: more than 2^29 tokens");
+    if (!fta::size_fits(B, N, H, D)) return fta::unsupported("window_attn: 2^60 elements and more");
     if (!fta::all_set(qs, ks, vs)) return fta::arg_error("window_attn: strides are null");
     a = WinArgs{};
     a.q = (const uint16_t*)q, a.q_sb = qs[0], a.q_sh = qs[1], a.q_sn = qs[2];
