@@ -203,6 +203,40 @@ def rows_in_place(what: str, x: torch.Tensor, heads: int):
     return at, strides
 
 
+def _rows_meet(shape: tuple, stride: tuple, delta: int) -> bool:
+    """Whether a row of ``[B, N, C]`` and one of the same layout ``delta`` elements on share an
+    element (``delta`` 0: two different rows of the one)."""
+    (B, N, C), (sb, sn, _) = shape, stride
+    for db in range(1 - B, B):
+        x = delta + db * sb
+        near = -x // sn if sn else 0  # the token distances that bring the rows closest
+        for ds in (near, near + 1):
+            ds = min(max(ds, 1 - N), N - 1)
+            if abs(x + ds * sn) < C and (delta or db or ds):
+                return True
+    return False
+
+
+@lru_cache(maxsize=4096)
+def _caches_meet(shape: tuple, k_stride: tuple, v_stride: tuple, delta: int) -> bool:
+    """Whether two rows of a pair of caches ``[B, N, C]``, v ``delta`` elements behind k, share
+    an element (layouts that differ and lie within each other are taken to)."""
+    if _rows_meet(shape, k_stride, 0) or _rows_meet(shape, v_stride, 0):
+        return True
+    k_end, v_end = (sum((n - 1) * s for n, s in zip(shape, st)) for st in (k_stride, v_stride))
+    if delta > k_end or -delta > v_end:
+        return False
+    dims = [i for i, n in enumerate(shape) if n > 1]
+    return any(k_stride[i] != v_stride[i] for i in dims) or _rows_meet(shape, k_stride, delta) or delta == 0
+
+
+def check_written(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
+    """Refuses caches whose rows share memory: what they would hold depends on which of two
+    writes is the last."""
+    if _caches_meet(k.shape, k.stride(), v.stride(), (v.data_ptr() - k.data_ptr()) // k.element_size()):
+        raise ValueError(f"{what}: rows of the caches share memory (an expanded cache, or one that overlaps the other)")
+
+
 def flat(x: torch.Tensor) -> torch.Tensor:
     """``x`` contiguous and 16-byte aligned (a table or weights)."""
     if x.is_contiguous() and x.data_ptr() & 15 == 0:

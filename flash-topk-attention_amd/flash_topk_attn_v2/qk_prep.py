@@ -179,7 +179,7 @@ def flash_qk_norm_rope_append(
 
     ``q`` is ``[B, T, num_heads * D]``, ``k`` and ``v`` ``[B, T, num_kv_heads * D]``,
     the caches ``[B, S, num_kv_heads * D]`` (any batch and token stride that keeps rows
-    16-byte aligned).  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host)
+    16-byte aligned; no two rows, of one cache or of both, may share memory).  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host)
     counts each request's cached tokens with these T: token t is written to row
     ``cache_lens[b] - T + t`` and turned as position ``row + position_offset`` (the
     length of a shared prefix, for instance).  Rows outside ``[0, S)`` are not written.
@@ -197,10 +197,7 @@ def flash_qk_norm_rope_append(
     _lib.check_device(what, q.device, v)
     kca, kcs = _lib.rows_in_place(what, k_cache, Hk)
     vca, vcs = _lib.rows_in_place(what, v_cache, Hk)
-    if 0 in k_cache.stride() or 0 in v_cache.stride():
-        for c in (k_cache, v_cache):
-            if any(st == 0 and n > 1 for st, n in zip(c.stride(), c.shape)):
-                raise ValueError(f"{what}: the caches must not be expanded")
+    _lib.check_written(what, k_cache, v_cache)
     if not -(1 << 31) <= position_offset < (1 << 31):
         raise ValueError(f"{what}: position_offset out of range")
     q, qa, qs = _lib.rows(q, H)

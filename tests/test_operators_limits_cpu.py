@@ -1,6 +1,9 @@
 """Limits of the operators around the sparse attention that are checked without a GPU."""
 
+import itertools
+
 import pytest
+import torch
 
 from flash_topk_attn_v2 import _lib
 
@@ -20,3 +23,36 @@ def test_sizes_whose_products_wrap(B, H, Hk, N, D):
     assert rc == _lib.FTA_ERR_UNSUPPORTED
     rc = L.fta_qk_norm_rope(x, z, x, z, 0, B, H, Hk, N, D, None, None, 2, x, x, N, 16, None, 0, 1e-6, 0, x, z, x, z, None)
     assert rc == _lib.FTA_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("B,S,W,st", [(1, 1, 16, (0, 0)), (2, 3, 16, (48, 16)), (2, 3, 16, (96, 32)), (3, 2, 16, (32, 96)),
+                                      (2, 3, 16, (48, 8)), (2, 3, 16, (40, 16)), (2, 3, 16, (0, 16)), (2, 3, 16, (48, 0)),
+                                      (3, 4, 16, (16, 56)), (3, 4, 16, (160, 40)), (1, 4, 16, (8, 16)), (4, 1, 16, (16, 8))])
+def test_rows_that_share_memory(B, S, W, st):
+    """The rule that refuses caches whose rows share memory, against every pair of elements."""
+    own = [{b * st[0] + s * st[1] + i for i in range(W)} for b in range(B) for s in range(S)]
+    alone = sum(map(len, own)) == len(set().union(*own))
+    for delta in range(-200, 201, 8):
+        other = [{x + delta for x in row} for row in own]
+        apart = alone and set().union(*own).isdisjoint(set().union(*other))
+        assert _lib._caches_meet((B, S, W), (*st, 1), (*st, 1), delta) == (not apart), delta
+
+
+def test_caches_of_the_usual_layouts():
+    B, S, W = 3, 5, 32
+    pairs = [torch.zeros(S, B, 2 * W).transpose(0, 1).split(W, -1), torch.zeros(B, S, 2, W).unbind(2),
+             torch.zeros(B, 2, S, W).unbind(1), torch.zeros(2, B, S, W).unbind(0), (torch.zeros(B, S, W), torch.zeros(B, S, W)),
+             torch.zeros(B, 2 * S, W).split(S, 1)]
+    for pair in pairs:
+        for k, v in itertools.permutations(pair):
+            _lib.check_written("caches", k, v)
+    one = torch.zeros(B, S, W)
+    wide = torch.zeros(B, S, W + 16)
+    for k, v in ((one, one), (one[:1].expand(B, -1, -1), torch.zeros(B, S, W)), (torch.zeros(B, S, W), one[:, :1].expand(-1, S, -1)),
+                 (wide[..., :W], wide[..., 16:]), (torch.zeros(B, S + 1, W)[:, :-1], one.as_strided((B, S, W), (16, W, 1))),
+                 (one, one.transpose(0, 1).reshape(B, S, W).as_strided((B, S, W), (W, W, 1)))):
+        with pytest.raises(ValueError, match="share memory"):
+            _lib.check_written("caches", k, v)
+    with pytest.raises(ValueError, match="share memory"):  # rows of a cache moved by one token
+        both = torch.zeros(B, S + 1, W)
+        _lib.check_written("caches", both[:, :-1], both[:, 1:])
