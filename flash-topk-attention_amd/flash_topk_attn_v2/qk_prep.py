@@ -121,7 +121,9 @@ def flash_qk_norm_rope(
     interleaved: bool = False,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
     """RMS norm of every query and key head and rotation by position, in one pass
-    (differentiable in q, k and the weights).
+    (differentiable in q, k and the weights).  A head whose output's gradient is zero, as
+    behind ``seq_lens`` of ``flash_window_attn``, adds nothing to any gradient, whatever
+    it holds.
 
     Args:
         q: ``[B, N, num_heads * D]`` float16 or bfloat16, D a multiple of 16 up to 256.

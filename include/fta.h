@@ -444,7 +444,8 @@ int fta_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, con
  * Backward of fta_qk_norm_rope from q, k and the gradients of its outputs.
  * dq_weight / dk_weight [D] of weight_dtype may be null; with either the workspace
  * (fta_qk_norm_rope_bwd_workspace_size bytes) holds the workgroups' partial sums, which
- * are added in order (the same bits every run).
+ * are added in order (the same bits every run).  A row whose gradient is zero gives dx = 0
+ * and adds nothing to the weights' gradients, whatever q and k hold there.
  */
 size_t fta_qk_norm_rope_bwd_workspace_size(int B, int H, int Hk, int N, int D);
 int fta_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
