@@ -8,6 +8,7 @@ operations.
 
 from __future__ import annotations
 
+import warnings
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -60,6 +61,15 @@ def _check(what, q, k, num_heads, num_kv_heads, cos, sin, qw, kw, eps):
         raise ValueError(f"{what}: cos and sin are not differentiable")
     _lib.check_device(what, q.device, k, cos, sin, qw, kw)
     return geo
+
+
+@lru_cache(maxsize=1024)
+def _warn_of_short_tables(what, P, S, offset):
+    """The lengths are on the device, so a position without a table row can only be foreseen:
+    once per geometry."""
+    if offset < 0 or S + offset > P:
+        warnings.warn(f"{what}: cos and sin have rows for positions 0 .. {P - 1}, rows of the cache stand at {offset} .. "
+                      f"{S + offset - 1}: tokens outside the tables are turned as the nearest row", stacklevel=3)
 
 
 class _QKNormRopeFunc(torch.autograd.Function):
@@ -185,6 +195,8 @@ def flash_qk_norm_rope_append(
     counts each request's cached tokens with these T: token t is written to row
     ``cache_lens[b] - T + t`` and turned as position ``row + position_offset`` (the
     length of a shared prefix, for instance).  Rows outside ``[0, S)`` are not written.
+    Positions outside the tables take their nearest row, which turns those tokens wrongly; a
+    call whose cache has such rows (tables of fewer than ``S + position_offset``) warns once.
     Other arguments as for ``flash_qk_norm_rope``.  Not differentiable.
 
     Returns the prepared q ``[B, T, num_heads * D]``.
@@ -202,6 +214,7 @@ def flash_qk_norm_rope_append(
     _lib.check_written(what, k_cache, v_cache)
     if not -(1 << 31) <= position_offset < (1 << 31):
         raise ValueError(f"{what}: position_offset out of range")
+    _warn_of_short_tables(what, cos.shape[0], k_cache.shape[1], int(position_offset))
     q, qa, qs = _lib.rows(q, H)
     k, ka, ks = _lib.rows(k, Hk)
     v, va, vs = _lib.rows(v, Hk)

@@ -460,7 +460,8 @@ int fta_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k,
  * The same for T new tokens of each request, K and V written into the caches
  * ([B][S][Hk][D] strided) in the same pass.  cache_lens[b] (int32, device) counts the
  * cached tokens with these T: token t goes to row cache_lens[b] - T + t and takes that
- * row plus position_offset as its position.  Rows outside [0, S) are not written.
+ * row plus position_offset as its position (clamped into [0, P): tables of S +
+ * position_offset rows hold every cached position).  Rows outside [0, S) are not written.
  */
 int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                             const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,

@@ -1,6 +1,7 @@
 """Calls of the operators around the sparse attention that are refused, or were once wrong, on the card."""
 
 import math
+import warnings
 
 import pytest
 import torch
@@ -92,3 +93,23 @@ def test_zero_gradients_in_some_rows_and_columns(gpu):
         one = torch.autograd.grad(fta.flash_qk_norm_rope(a, b, H, cos, sin, num_kv_heads=1, positions=pos), (a, b),
                                   (dq[:, n:n + 1], dk[:, n:n + 1]))
         assert torch.equal(one[0], got[0][:, n:n + 1]) and torch.equal(one[1], got[1][:, n:n + 1])
+
+
+def test_append_warns_of_short_tables(gpu):
+    """A cache that is longer than the tables: the tokens past them are turned as the last row, with a warning."""
+    import flash_topk_attn_v2 as fta
+    from flash_topk_attn_v2 import qk_prep
+
+    H, D, S = 1, 64, 9
+    q, k, v = (rand((1, 1, H * D), i, BF, gpu) for i in range(3))
+    kc, vc = (torch.zeros(1, S, H * D, device=gpu, dtype=BF) for _ in range(2))
+    lens = torch.tensor([S], dtype=torch.int32, device=gpu)
+    cos, sin = _tables(S, D, gpu)
+    qk_prep._warn_of_short_tables.cache_clear()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        full = fta.flash_qk_norm_rope_append(q, k, v, kc, vc, lens, H, cos, sin)
+    with pytest.warns(UserWarning, match="nearest row"):
+        short = fta.flash_qk_norm_rope_append(q, k, v, kc, vc, lens, H, cos[:S - 1], sin[:S - 1])
+    last = fta.flash_qk_norm_rope(q, k, H, cos, sin, positions=torch.tensor([S - 2], dtype=torch.int32, device=gpu))[0]
+    assert torch.equal(short, last) and not torch.equal(full, short)

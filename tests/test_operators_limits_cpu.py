@@ -1,11 +1,12 @@
 """Limits of the operators around the sparse attention that are checked without a GPU."""
 
 import itertools
+import warnings
 
 import pytest
 import torch
 
-from flash_topk_attn_v2 import _lib
+from flash_topk_attn_v2 import _lib, qk_prep
 
 
 @pytest.mark.parametrize("B,H,Hk,N,D", [(1 << 30, 4096, 4096, 1 << 29, 64), (1 << 30, 1 << 20, 1 << 16, 1 << 20, 64),
@@ -56,3 +57,17 @@ def test_caches_of_the_usual_layouts():
     with pytest.raises(ValueError, match="share memory"):  # rows of a cache moved by one token
         both = torch.zeros(B, S + 1, W)
         _lib.check_written("caches", both[:, :-1], both[:, 1:])
+
+
+def test_tables_shorter_than_the_cache():
+    """Warned of once per geometry; tables that hold every cached position are not."""
+    check = qk_prep._warn_of_short_tables
+    check.cache_clear()
+    for P, S, offset in ((7, 8, 0), (107, 8, 100), (8, 8, -1), (1, 1, 1)):
+        with pytest.warns(UserWarning, match="nearest row"):
+            check("append", P, S, offset)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        check("append", 7, 8, 0)  # already said
+        for P, S, offset in ((8, 8, 0), (108, 8, 100), (1, 1, 0), (1 << 20, 8, 5)):
+            check("append", P, S, offset)
