@@ -271,9 +271,23 @@ def int_sizes(what: str, *sizes: int) -> None:
         raise NotImplementedError(f"{what}: a size of {max(sizes)}; sizes must be below 2^31")
 
 
-def scalars(num_heads, num_kv_heads, real):
+def whole(what: str, x) -> int:
+    """``x`` as a Python integer; anything that is not a whole number is refused."""
+    if type(x) is int:
+        return x
+    try:
+        i = int(x)
+    except (TypeError, ValueError, OverflowError):
+        raise ValueError(f"{what}: {x!r} is not a whole number") from None
+    if i != x:
+        raise ValueError(f"{what}: {x!r} is not a whole number")
+    return i
+
+
+def scalars(what: str, num_heads, num_kv_heads, real):
     """Head counts and a real number as Python numbers: what a cached check may be keyed by."""
-    return int(num_heads), None if num_kv_heads is None else int(num_kv_heads), None if real is None else float(real)
+    return (whole(what, num_heads), None if num_kv_heads is None else whole(what, num_kv_heads),
+            None if real is None else float(real))
 
 
 HALVES = (torch.float16, torch.bfloat16)

@@ -39,7 +39,7 @@ def cache_attn(what, q, k_cache, v_cache, cache_lens, num_heads, num_kv_heads, k
     _lib.no_grad_inputs(what, q, k_cache, v_cache, k_prefix, v_prefix)
     S = k_cache.shape[1] if k_cache.ndim == 3 else 0
     P = 0 if k_prefix is None else k_prefix.shape[0]
-    num_heads, num_kv_heads, scale = _lib.scalars(num_heads, num_kv_heads, scale)
+    num_heads, num_kv_heads, scale = _lib.scalars(what, num_heads, num_kv_heads, scale)
     H, Hk, D, left, scale, nbytes = _geometry(what, q.shape, q.dtype, num_heads, num_kv_heads, S, P, left, sinks, scale)
     B, T, _ = q.shape
     check_cache(what, q, k_cache, v_cache, cache_lens, B, Hk * D)

@@ -53,7 +53,7 @@ def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, wei
 def _check(what, q, k, num_heads, num_kv_heads, cos, sin, qw, kw, eps):
     if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    num_heads, num_kv_heads, eps = _lib.scalars(num_heads, num_kv_heads, eps)
+    num_heads, num_kv_heads, eps = _lib.scalars(what, num_heads, num_kv_heads, eps)
     geo = _geometry(what, q.shape, k.shape, (q.dtype, k.dtype), cos.shape, sin.shape, (cos.dtype, sin.dtype),
                     None if qw is None else qw.shape, None if kw is None else kw.shape,
                     (None if qw is None else qw.dtype, None if kw is None else kw.dtype), num_heads, num_kv_heads, eps)
@@ -212,9 +212,10 @@ def flash_qk_norm_rope_append(
     kca, kcs = _lib.rows_in_place(what, k_cache, Hk)
     vca, vcs = _lib.rows_in_place(what, v_cache, Hk)
     _lib.check_written(what, k_cache, v_cache)
+    position_offset = _lib.whole(what, position_offset)
     if not -(1 << 31) <= position_offset < (1 << 31):
         raise ValueError(f"{what}: position_offset out of range")
-    _warn_of_short_tables(what, cos.shape[0], k_cache.shape[1], int(position_offset))
+    _warn_of_short_tables(what, cos.shape[0], k_cache.shape[1], position_offset)
     q, qa, qs = _lib.rows(q, H)
     k, ka, ks = _lib.rows(k, Hk)
     v, va, vs = _lib.rows(v, Hk)
@@ -222,7 +223,7 @@ def flash_qk_norm_rope_append(
     cos, sin, lens = _lib.flat(cos), _lib.flat(sin), cache_lens.contiguous()
     qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     _lib.call("fta_qk_norm_rope_append", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, D,
-              _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, int(position_offset),
+              _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, position_offset,
               float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),
               _lib.dense_strides(q.shape, H), kca, kcs, vca, vcs)
     for c in (k_cache, v_cache):

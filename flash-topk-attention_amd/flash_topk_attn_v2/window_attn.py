@@ -121,9 +121,9 @@ def flash_window_attn(
     what = "flash_window_attn"
     if not q.is_cuda:
         raise ValueError(f"{what} requires CUDA tensors")
-    num_heads, num_kv_heads, scale = _lib.scalars(num_heads, num_kv_heads, scale)
+    num_heads, num_kv_heads, scale = _lib.scalars(what, num_heads, num_kv_heads, scale)
     geo = _geometry(what, q.shape, k.shape, v.shape, (q.dtype, k.dtype, v.dtype), num_heads, num_kv_heads,
-                    tuple(map(int, window)), int(num_sinks), scale)
+                    tuple(_lib.whole(what, x) for x in window), _lib.whole(what, num_sinks), scale)
     _lib.check_device(what, q.device, k, v, seq_lens)
     if seq_lens is not None:
         if seq_lens.dtype != torch.int32 or seq_lens.shape != q.shape[:1]:
@@ -159,10 +159,11 @@ def flash_window_attn_decode(
     Returns ``(output [B, T, num_heads * D], lse [B, num_heads, T] float32)``.
     """
     what = "flash_window_attn_decode"
-    if int(window_left) < 0 or int(num_sinks) < 0:
+    window_left, num_sinks = _lib.whole(what, window_left), _lib.whole(what, num_sinks)
+    if window_left < 0 or num_sinks < 0:
         raise ValueError(f"{what}: window_left and num_sinks must be non-negative")
     return cache_attn(what, q, k_cache, v_cache, cache_lens, num_heads, num_kv_heads, None, None,
-                      min(int(window_left), _MAX), min(int(num_sinks), _MAX), scale)
+                      min(window_left, _MAX), min(num_sinks, _MAX), scale)
 
 
 __all__ = ["flash_window_attn", "flash_window_attn_decode"]

@@ -113,3 +113,27 @@ def test_append_warns_of_short_tables(gpu):
         short = fta.flash_qk_norm_rope_append(q, k, v, kc, vc, lens, H, cos[:S - 1], sin[:S - 1])
     last = fta.flash_qk_norm_rope(q, k, H, cos, sin, positions=torch.tensor([S - 2], dtype=torch.int32, device=gpu))[0]
     assert torch.equal(short, last) and not torch.equal(full, short)
+
+
+def test_fractions_are_refused(gpu):
+    import flash_topk_attn_v2 as fta
+
+    x = torch.zeros(1, 5, 128, device=gpu, dtype=BF)
+    cos, sin = _tables(5, 64, gpu)
+    lens = torch.tensor([5], dtype=torch.int32, device=gpu)
+    calls = [(fta.flash_window_attn, dict(q=x, k=x, v=x, num_heads=2, window=(3, 0), num_sinks=1, num_kv_heads=2),
+              [dict(num_heads=2.5), dict(num_kv_heads=1.5), dict(window=(3.9, 0)), dict(window=(3, 0.1)), dict(num_sinks=0.5)]),
+             (fta.flash_qk_norm_rope, dict(q=x, k=x, num_heads=2, cos=cos, sin=sin, num_kv_heads=2),
+              [dict(num_heads=2.5), dict(num_kv_heads=2.5)]),
+             (fta.flash_qk_norm_rope_append, dict(q=x, k=x, v=x, k_cache=x.clone(), v_cache=x.clone(), cache_lens=lens,
+                                                  num_heads=2, cos=cos, sin=sin), [dict(num_heads=2.5), dict(position_offset=0.5)]),
+             (fta.flash_window_attn_decode, dict(q=x, k_cache=x, v_cache=x, cache_lens=lens, num_heads=2, window_left=3),
+              [dict(num_heads=2.5), dict(window_left=2.5), dict(num_sinks=1.5)]),
+             (fta.flash_prefix_attn_decode, dict(q=x, k_prefix=x[0], v_prefix=x[0], k_cache=x, v_cache=x, cache_lens=lens,
+                                                 num_heads=2), [dict(num_heads=2.5), dict(num_kv_heads=0.5)])]
+    for call, good, bad in calls:
+        call(**good)
+        call(**(good | dict(num_heads=2.0)))
+        for b in bad:
+            with pytest.raises(ValueError, match="whole number"):
+                call(**(good | b))

@@ -3,9 +3,11 @@
 import itertools
 import warnings
 
+import numpy as np
 import pytest
 import torch
 
+import flash_topk_attn_v2 as fta
 from flash_topk_attn_v2 import _lib, qk_prep
 
 
@@ -71,3 +73,19 @@ def test_tables_shorter_than_the_cache():
         check("append", 7, 8, 0)  # already said
         for P, S, offset in ((8, 8, 0), (108, 8, 100), (1, 1, 0), (1 << 20, 8, 5)):
             check("append", P, S, offset)
+
+
+def test_fractions_are_not_sizes():
+    """Sizes were cut to whole numbers: a window of 3.9 tokens was one of 3."""
+    for x in (4, 4.0, np.int32(4), np.float64(4), torch.tensor(4), torch.tensor(4.0), True + 3):
+        got = _lib.whole("sizes", x)
+        assert type(got) is int and got == 4
+    for x in (3.9, -0.5, float("nan"), float("inf"), np.float32(0.1), torch.tensor(1.5), None, "four"):
+        with pytest.raises(ValueError, match="whole number"):
+            _lib.whole("sizes", x)
+    with pytest.raises(ValueError, match="whole number"):
+        _lib.scalars("sizes", 4, 2.5, None)
+    x, n = torch.zeros(1, 4, 64, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    for bad in (dict(window_left=3.5), dict(num_sinks=0.5)):  # refused in front of the look at the tensors
+        with pytest.raises(ValueError, match="whole number"):
+            fta.flash_window_attn_decode(x, x, x, n, 1, **(dict(window_left=3) | bad))
