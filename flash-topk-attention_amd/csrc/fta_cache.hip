@@ -434,7 +434,8 @@ int fta_cache_attn(const void* q, const int64_t* q_strides, const void* k_cache,
     int rc = cache_plan(a, B, H, Hk, T, S, D, P, left, num_sinks);
     if (rc != FTA_OK) return rc;
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("cache_attn: dtype must be bf16 or fp16");
-    if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("cache_attn: scale must be positive and finite");
+    if (!(scale > 0.f) || scale > 2.0e38f)  // times log2(e) still finite
+        return fta::arg_error("cache_attn: scale must be positive and at most 2e38");
     const size_t need = cache_bytes(a, kernel_dim(D));
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fta::arg_error("cache_attn: workspace too small");
     if (!fta::all_set(q, q_strides, k_cache, kc_strides, v_cache, vc_strides, cache_lens, o, o_strides, lse) ||

@@ -524,7 +524,7 @@ int fta_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, con
     FTA_TRY_BEGIN
     int rc = prep_geometry(B, H, Hk, N, D, R, P);
     if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
-    if (!(eps > 0.f)) return fta::arg_error("qk_norm_rope: eps must be positive");
+    if (!(eps > 0.f) || eps > 3.0e38f) return fta::arg_error("qk_norm_rope: eps must be positive and finite");
     if (positions == nullptr && N > P) return fta::arg_error("qk_norm_rope: cos and sin have fewer rows than tokens");
     if (!fta::all_set(q, q_strides, k, k_strides, cos, sin, q_out, qo_strides, k_out, ko_strides))
         return fta::arg_error("qk_norm_rope: a required pointer is null");
@@ -561,7 +561,7 @@ int fta_qk_norm_rope_bwd(const void* q, const int64_t* q_strides, const void* k,
     FTA_TRY_BEGIN
     int rc = prep_geometry(B, H, Hk, N, D, R, P);
     if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
-    if (!(eps > 0.f)) return fta::arg_error("qk_norm_rope: eps must be positive");
+    if (!(eps > 0.f) || eps > 3.0e38f) return fta::arg_error("qk_norm_rope: eps must be positive and finite");
     if (positions == nullptr && N > P) return fta::arg_error("qk_norm_rope: cos and sin have fewer rows than tokens");
     const bool dw = dq_weight != nullptr || dk_weight != nullptr;
     if (dw && (workspace == nullptr || workspace_bytes < fta_qk_norm_rope_bwd_workspace_size(B, H, Hk, N, D)))
@@ -602,7 +602,7 @@ int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void*
     FTA_TRY_BEGIN
     int rc = prep_geometry(B, H, Hk, T, D, R, P);
     if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
-    if (!(eps > 0.f)) return fta::arg_error("qk_norm_rope: eps must be positive");
+    if (!(eps > 0.f) || eps > 3.0e38f) return fta::arg_error("qk_norm_rope: eps must be positive and finite");
     if (S <= 0) return fta::arg_error("qk_norm_rope_append: the caches must have rows");
     if (!fta::all_set(q, q_strides, k, k_strides, v, v_strides, cos, sin, cache_lens, q_out, qo_strides, k_cache, kc_strides,
                       v_cache, vc_strides))

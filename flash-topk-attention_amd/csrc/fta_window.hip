@@ -1038,7 +1038,8 @@ int win_common(WinArgs& a, const void* q, const int64_t* qs, const void* k, cons
     if (H % Hk != 0) return fta::arg_error("window_attn: num_heads must be a multiple of num_kv_heads");
     if (D % 16 != 0 || D > 256) return fta::arg_error("window_attn: D must be a multiple of 16 up to 256");
     if (left < 0 || right < 0 || sinks < 0) return fta::arg_error("window_attn: window and num_sinks must be non-negative");
-    if (!(scale > 0.f) || scale > 3.0e38f) return fta::arg_error("window_attn: scale must be positive and finite");
+    if (!(scale > 0.f) || scale > 2.0e38f)  // times log2(e) still finite
+        return fta::arg_error("window_attn: scale must be positive and at most 2e38");
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("window_attn: dtype must be bf16 or fp16");
     if (N > (1 << 29)) return fta::unsupported("window_attn: more than 2^29 tokens");
     if (!fta::size_fits(B, N, H, D)) return fta::unsupported("window_attn: 2^60 elements and more");

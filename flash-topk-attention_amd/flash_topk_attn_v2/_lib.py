@@ -294,6 +294,9 @@ HALVES = (torch.float16, torch.bfloat16)
 DTYPE_CODES = {torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.float32: DTYPE_F32}
 
 
+SCALE_MAX = 2.0e38  # times log2(e) still a float32
+
+
 def no_grad_inputs(what: str, *tensors) -> None:
     """Refuses a call whose gradients would be lost."""
     if torch.is_grad_enabled():
@@ -304,8 +307,8 @@ def no_grad_inputs(what: str, *tensors) -> None:
 
 def softmax_scale(what: str, scale, D: int) -> float:
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError(f"{what}: scale must be positive and finite")
+    if not 0.0 < scale <= SCALE_MAX:
+        raise ValueError(f"{what}: scale must be positive and at most {SCALE_MAX}")
     return scale
 
 

@@ -45,8 +45,8 @@ def _geometry(what, q, k, dtypes, cos, sin, table_types, q_weight, k_weight, wei
     types = {t for t in weight_types if t is not None}
     if len(types) > 1 or not types <= set(_lib.DTYPE_CODES):
         raise ValueError(f"{what}: weights must both be float32, float16 or bfloat16")
-    if not 0.0 < eps < float("inf"):
-        raise ValueError(f"{what}: eps must be positive")
+    if not 0.0 < eps <= 3.0e38:
+        raise ValueError(f"{what}: eps must be positive and a float32")
     return H, Hk, D, R, _lib.DTYPE_CODES[types.pop()] if types else _lib.DTYPE_F32
 
 

@@ -478,7 +478,7 @@ int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void*
  * j < num_sinks).  seq_lens [B] (int32, device; clamped into [0, N]) or null (N); tokens
  * at or past len give o = 0, lse = -inf and zero gradients, and what q, k, v and dout
  * hold there is not used.  Tokens in front of len must be finite.  Layouts, head counts
- * (H a multiple of Hk) and head dims as for fta_sparse_attn_fwd_gqa; scale > 0.
+ * (H a multiple of Hk) and head dims as for fta_sparse_attn_fwd_gqa; 0 < scale <= 2e38.
  */
 int fta_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
                         const int64_t* v_strides, int dtype, int B, int H, int Hk, int N, int D, const int32_t* seq_lens,

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import flash_topk_attn_v2 as fta
-from flash_topk_attn_v2 import _lib, qk_prep
+from flash_topk_attn_v2 import _lib, cache_attn, qk_prep, window_attn
 
 
 @pytest.mark.parametrize("B,H,Hk,N,D", [(1 << 30, 4096, 4096, 1 << 29, 64), (1 << 30, 1 << 20, 1 << 16, 1 << 20, 64),
@@ -89,3 +89,34 @@ def test_fractions_are_not_sizes():
     for bad in (dict(window_left=3.5), dict(num_sinks=0.5)):  # refused in front of the look at the tensors
         with pytest.raises(ValueError, match="whole number"):
             fta.flash_window_attn_decode(x, x, x, n, 1, **(dict(window_left=3) | bad))
+
+
+def test_reals_past_float32():
+    """A scale whose product with log2(e) is infinite made every score NaN, an infinite eps every row zero."""
+    BF, f = torch.bfloat16, torch.float32
+    shape, table = (1, 4, 64), (4, 32)
+
+    def prep(eps):
+        return qk_prep._geometry("prep", shape, shape, (BF, BF), table, table, (f, f), None, None, (None, None), 1, None, eps)
+
+    def window(scale):
+        return window_attn._geometry("window", shape, shape, shape, (BF,) * 3, 1, None, (3, 0), 0, scale)
+
+    def cache(scale):
+        return cache_attn._geometry("cache", shape, BF, 1, None, 10, 0, 3, 0, scale)
+
+    for x in (1e-30, 1.0, 1e30, 2e38):
+        prep(x), window(x), cache(x)
+    for call, bad in ((prep, 1e39), (prep, float("inf")), (window, 2.5e38), (window, 1e39), (cache, 2.5e38), (cache, 1e39)):
+        with pytest.raises(ValueError, match="positive"):
+            call(bad)
+    L, z, x = _lib.lib(), _lib.i64arr((0, 0, 0)), 4096  # an address that nothing reads
+    for v in (2.5e38, float("inf")):
+        assert L.fta_window_attn_fwd(x, z, x, z, x, z, 0, 1, 1, 1, 4, 64, None, 3, 0, 0, v, None, z, x, None) == _lib.FTA_ERR_ARG
+        assert b"scale" in L.fta_last_error()
+        assert L.fta_cache_attn(x, z, x, z, x, z, 0, 1, 1, 1, 1, 10, 64, x, None, z, None, z, 0, 3, 0, v, None, z, x, None, 0,
+                                None) == _lib.FTA_ERR_ARG
+        assert b"scale" in L.fta_last_error()
+    assert L.fta_qk_norm_rope(x, z, x, z, 0, 1, 1, 1, 4, 64, None, None, 2, x, x, 4, 64, None, 0, float("inf"), 0, None, z, x, z,
+                              None) == _lib.FTA_ERR_ARG
+    assert b"eps" in L.fta_last_error()
