@@ -1,0 +1,61 @@
+"""Gradients of the window attention against differences along the gradient itself, and against the formula
+with delta from the kernel's own output, in float64."""
+
+import itertools
+
+import pytest
+import torch
+
+import _gradient_ref as G
+import _operators_ref as R
+from _helpers import say
+
+pytestmark = pytest.mark.gpu
+
+ids = lambda c: "-".join(str(x) for x in c[1:9])  # noqa: E731
+
+
+def _run(case, q, k, v, do, wanted=(True, True, True)):
+    import flash_topk_attn_v2 as fta
+
+    dtype, B, N, H, Hk, D, left, right, sinks, lens = case
+    x = [t.detach().requires_grad_(w) for t, w in zip((q, k, v), wanted)]
+    ln = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=q.device)
+    o, _ = fta.flash_window_attn(*x, H, (left, right), sinks, num_kv_heads=Hk, seq_lens=ln)
+    grads = iter(torch.autograd.grad(o, [t for t in x if t.requires_grad], do))
+    return o.detach(), [next(grads) if w else None for w in wanted]
+
+
+@pytest.mark.parametrize("case", G.CASES, ids=ids)
+def test_gradients_with_delta_of_the_own_output(gpu, case):
+    dtype, B, N, H, Hk, D, left, right, sinks, lens = case
+    say("own delta", case)
+    q, k, v, do = G.inputs(case, gpu)
+    o, (dq, dk, _) = _run(case, q, k, v, do)
+    ref = G.window(q, k, v, o, do, H, Hk, left, right, sinks, D ** -0.5, lens)
+    R.check({"dq": dq, "dk": dk}, ref, ("dq", "dk"), str(case))
+
+
+@pytest.mark.parametrize("case", G.CASES, ids=ids)
+def test_slopes_along_the_gradients(gpu, case):
+    """Each gradient alone, along itself: the slope is several times the worst error."""
+    dtype, B, N, H, Hk, D, left, right, sinks, lens = case
+    say("slopes", case)
+    q, k, v, do = G.inputs(case, gpu)
+    _, grads = _run(case, q, k, v, do)
+    ref = R.window(q, k, v, H, Hk, left, right, sinks, D ** -0.5, lens, do)
+    for name, got in zip(("dq", "dk", "dv"), grads):
+        d, slope, tol = G.along(case, q, k, v, do, ref, name)
+        got = float((got.double() * d).sum())
+        assert abs(got - slope) <= tol + 1e-6 * slope, (name, got, slope, tol)
+
+
+@pytest.mark.parametrize("case", G.CASES[:3] + G.CASES[6:7], ids=ids)
+def test_some_gradients_are_the_full_ones(gpu, case):
+    """Frozen inputs change no other gradient's bits."""
+    q, k, v, do = G.inputs(case, gpu)
+    _, full = _run(case, q, k, v, do)
+    for wanted in itertools.product((True, False), repeat=3):
+        if any(wanted):
+            for w, x, y in zip(wanted, full, _run(case, q, k, v, do, wanted)[1]):
+                assert not w or torch.equal(x, y), wanted
