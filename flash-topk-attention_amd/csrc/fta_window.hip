@@ -111,6 +111,13 @@ __device__ __forceinline__ uint32_t seen_keys(const WinArgs& a, int len, int i, 
     return fta_bits_below(min(i + a.right, len - 1) + 1 - kb) & (~fta_bits_below(i - a.left - kb) | fta_bits_below(a.sinks - kb));
 }
 
+// How many keys token i sees (sinks in front of the window and the window).
+__device__ __forceinline__ int seen_count(const WinArgs& a, int len, int i) {
+    return min(i + a.right, len - 1) - max(i - a.left, 0) + 1 + max(min(a.sinks, i - a.left), 0);
+}
+// Rows that see fewer keys than this take delta from their scores, see the dQ kernel.
+constexpr int kFewKeys = 64;
+
 // Workgroup -> (K/V head, b, head group, token tile).  An XCD takes an eighth of that order: heads
 // outermost, so that it holds some of every sequence, however their lengths differ (8 sequences
 // of 512 to 8192 tokens, 8 heads of 128, window 512: forward 216 -> 143 us, dQ 292 -> 196, dK /
@@ -248,11 +255,15 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 
 // ----------------------------------------------------------------------------
 // dQ, with the forward's walk: S^T and dP^T = V dO^T of 32 keys at a time,
-// dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta = o . dO (both
-// rows are at hand) and the lse in log2 units for dK / dV.  delta is summed in fp32 from the
-// rounded o: dQ and dK are off by 1.5 times a rounding of the exact ones (2.3 times for rows that
-// see two keys), against 1.4 times from the rounding of dS alone; an o of more bits would cost
-// every training step another tensor of its size.
+// dS^T = P^T (dP^T - delta), dQ^T += K^T dS^T.  It also forms delta and the lse in log2 units
+// for dK / dV.
+//
+// delta = o . dO, summed in fp32 from the rounded o (both rows are at hand): its error, a rounding
+// of o, is in every dS of the row alike and shrinks with the number n of keys that the row sees:
+// dQ and dK are off by 2.3 times a rounding of the exact ones for n = 2, 1.6 for 8, 1.5 for 32
+// and 1.43 to 1.47 from 64 on, of which 1.41 are the rounding of dS.  A workgroup with rows of
+// fewer than 64 keys forms delta = sum_j P_ij dP_ij in fp32 instead, by a first walk over its keys
+// without dQ's product (1.41 for every n); in a causal sequence that is the first tile of each head.
 // Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 905 us, 953 TFLOP/s
 // with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 85 us.
 // ----------------------------------------------------------------------------
@@ -282,8 +293,12 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
         fta_frag qf[KS], df[KS];
         T::load_rows(a.q + p.b * a.q_sb + p.h * a.q_sh + (int64_t)row * a.q_sn, live, a.Dreal, lane, qf);
         T::load_rows(a.dout + p.b * a.d_sb + p.h * a.d_sh + (int64_t)row * a.d_sn, live, a.Dreal, lane, df);
-        float dl = 0.f, lse2 = FTA_INF;  // a padding row: every exp is exactly 0
-        {
+        const int64_t at_row = ((int64_t)p.b * a.H + p.h) * a.N + row;
+        const float lse2 = live ? a.lse[at_row] * kLog2e : FTA_INF;  // a padding row: every exp is exactly 0
+        float dl = 0.f;
+        const int i_hi = min(p.i_lo + p.tok, len) - 1;
+        const bool few = min(seen_count(a, len, p.i_lo), seen_count(a, len, i_hi)) < kFewKeys;  // workgroup-uniform
+        if (!few) {
             const uint16_t* op = a.o + p.b * a.o_sb + p.h * a.o_sh + (int64_t)row * a.o_sn;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
@@ -296,86 +311,97 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
                 }
             }
             dl += fta_xor32(dl);
-            if (live) {
-                const int64_t at = ((int64_t)p.b * a.H + p.h) * a.N + row;
-                lse2 = a.lse[at] * kLog2e;
-                if (lane < 32) {
-                    a.delta[at] = dl;
-                    a.lse2[at] = lse2;
-                }
-            }
         }
-        const WinWalk<KEYS> w(a, len, p.i_lo, min(p.i_lo + p.tok, len) - 1);
+        const WinWalk<KEYS> w(a, len, p.i_lo, i_hi);
         const WinRows rows(a, len, p.i0);
         FtaGather<D, kRowWaves, KEYS> g;
         g.start(a.k_sn, a.v_sn, a.Dreal, wave, lane);
         const uint32_t lds0 = fta_lds_addr(&sStage[0][0]), ldsw = lds0 + 1024 * wave;
         const FtaAddr<D> ad0(lds0, lane);
-        WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
-        auto issue = [&](int st) __attribute__((always_inline)) {
-            const uint32_t lds = ldsw + st * Sh::STAGE_B;
-            if (a.kv_narrow && w.whole(at.kb))
-                g.whole(at.k, at.v, lds);
-            else
-                g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(t); });
-            at.next(w, a);
-        };
-        fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream, which the compiler does not count
-        int kb = at.kb, it = 0;
-        issue(0);
-        // one tile, in stage ST: the stages alternate in the code, so that every LDS address is a
-        // kept register and a constant
-        auto tile = [&](auto st) __attribute__((always_inline)) {
-            constexpr int ST = decltype(st)::value;
-            fta_wait_vmcnt<0>();
-            __syncthreads();  // tile `it` visible; every wave is past tile it - 1
-            const int next = at.kb;
-            if (++it < w.iters) issue(ST ^ 1);
+        // the walk; FIRST: it only sums delta = sum over keys of P dP
+        auto walk = [&](auto first) __attribute__((always_inline)) {
+            constexpr bool FIRST = decltype(first)::value;
+            WinCursor<KEYS> at(w, a, kp, vp);  // the tile to gather
+            auto issue = [&](int st) __attribute__((always_inline)) {
+                const uint32_t lds = ldsw + st * Sh::STAGE_B;
+                if (a.kv_narrow && w.whole(at.kb))
+                    g.whole(at.k, at.v, lds);
+                else
+                    g.mapped(kp, vp, a.k_sn, a.v_sn, at.kb, a.Dreal, lds, wave, lane, [&](int t) { return w.seen(t); });
+                at.next(w, a);
+            };
+            fta_wait_vmcnt<0>();  // register loads and stores complete before the DMA stream, which the compiler does not count
+            int kb = at.kb, it = 0;
+            issue(0);
+            // one tile, in stage ST: the stages alternate in the code, so that every LDS address is a
+            // kept register and a constant
+            auto tile = [&](auto st) __attribute__((always_inline)) {
+                constexpr int ST = decltype(st)::value;
+                fta_wait_vmcnt<0>();
+                __syncthreads();  // tile `it` visible; every wave is past tile it - 1
+                const int next = at.kb;
+                if (++it < w.iters) issue(ST ^ 1);
 #pragma unroll
-            for (int sb = 0; sb < NH; ++sb) {
-                const int kh = kb + 32 * sb;
-                const bool full = rows.full(kh);
-                if (!full && rows.none(a, kh)) continue;
-                constexpr uint32_t KO = ST * Sh::STAGE_B, VO = KO + NH * T::TEN_B;
-                const uint32_t ho = sb * T::TEN_B;
-                const FtaAddr<D> ad = ad0.here();
-                f32x16 s, dp;
+                for (int sb = 0; sb < NH; ++sb) {
+                    const int kh = kb + 32 * sb;
+                    const bool full = rows.full(kh);
+                    if (!full && rows.none(a, kh)) continue;
+                    constexpr uint32_t KO = ST * Sh::STAGE_B, VO = KO + NH * T::TEN_B;
+                    const uint32_t ho = sb * T::TEN_B;
+                    const FtaAddr<D> ad = ad0.here();
+                    f32x16 s, dp;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-                fta_frag kf[2], vf[2], dsf[2];  // K and V fragments one MFMA pair ahead
-                kf[0] = ad.row(KO + ho, 0);
-                vf[0] = ad.row(VO + ho, 0);
+                    for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+                    fta_frag kf[2], vf[2], dsf[2];  // K and V fragments one MFMA pair ahead
+                    kf[0] = ad.row(KO + ho, 0);
+                    vf[0] = ad.row(VO + ho, 0);
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    if (ks + 1 < KS) {
-                        kf[(ks + 1) & 1] = ad.row(KO + ho, ks + 1);
-                        vf[(ks + 1) & 1] = ad.row(VO + ho, ks + 1);
+                    for (int ks = 0; ks < KS; ++ks) {
+                        if (ks + 1 < KS) {
+                            kf[(ks + 1) & 1] = ad.row(KO + ho, ks + 1);
+                            vf[(ks + 1) & 1] = ad.row(VO + ho, ks + 1);
+                        }
+                        s = fta_mma<DT>(kf[ks & 1], qf[ks], s);
+                        dp = fta_mma<DT>(vf[ks & 1], df[ks], dp);
                     }
-                    s = fta_mma<DT>(kf[ks & 1], qf[ks], s);
-                    dp = fta_mma<DT>(vf[ks & 1], df[ks], dp);
-                }
-                if (!full) T::mask(seen_keys(a, len, row, kh), lane, s);
+                    if (!full) T::mask(seen_keys(a, len, row, kh), lane, s);
+                    if constexpr (FIRST) {
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                    float ds[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int i = 8 * k2 + e;
-                        ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
+                        for (int i = 0; i < 16; ++i) dl = fmaf(fta_exp2(fmaf(s[i], a.c, -lse2)), dp[i], dl);
+                        continue;
                     }
-                    dsf[k2] = fta_pack_frag<DT>(ds);
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        float ds[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const int i = 8 * k2 + e;
+                            ds[e] = fta_exp2(fmaf(s[i], a.c, -lse2)) * (dp[i] - dl);
+                        }
+                        dsf[k2] = fta_pack_frag<DT>(ds);
+                    }
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                        for (int dt = 0; dt < T::DT32; ++dt) acc[dt] = fta_mma<DT>(ad.tr(KO + ho, ks, dt), dsf[ks], acc[dt]);
                 }
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                    for (int dt = 0; dt < T::DT32; ++dt) acc[dt] = fta_mma<DT>(ad.tr(KO + ho, ks, dt), dsf[ks], acc[dt]);
+                kb = next;
+            };
+            while (it < w.iters) {
+                tile(std::integral_constant<int, 0>{});
+                if (it < w.iters) tile(std::integral_constant<int, 1>{});
             }
-            kb = next;
         };
-        while (it < w.iters) {
-            tile(std::integral_constant<int, 0>{});
-            if (it < w.iters) tile(std::integral_constant<int, 1>{});
+        if (few) {
+            walk(std::true_type{});
+            dl += fta_xor32(dl);
+            __syncthreads();  // every wave has read the last tile
         }
+        if (live && lane < 32) {
+            a.delta[at_row] = dl;
+            a.lse2[at_row] = lse2;
+        }
+        walk(std::false_type{});
     }
     if (row < a.N)
         T::store_row(a.out0 + p.b * a.o0_sb + p.h * a.o0_sh + (int64_t)row * a.o0_sn, a.Dreal, lane, acc, a.scale);
