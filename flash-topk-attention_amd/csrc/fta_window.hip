@@ -32,6 +32,15 @@ namespace {
 constexpr int kRowWaves = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
 
+// The power of two that P carries into dV's product: the probabilities of long walks fall below
+// fp16's normal range (2^-14) and would lose bits one by one; P <= 1 leaves room for 2^14 more.
+// dK / dV read the lse less 14 and delta times 2^-14, so that P comes out scaled and dS does
+// not; dV is scaled back in fp32.  bf16 has fp32's range.
+template <int DT>
+constexpr int kPBits = DT == FTA_DTYPE_F16 ? 14 : 0;
+template <int DT>
+constexpr float kPUnit = DT == FTA_DTYPE_F16 ? 0x1p-14f : 1.f;
+
 struct WinArgs {
     const uint16_t *q, *k, *v, *o, *dout;
     int64_t q_sb, q_sh, q_sn, k_sb, k_sh, k_sn, v_sb, v_sh, v_sn, o_sb, o_sh, o_sn, d_sb, d_sh, d_sn;
@@ -39,7 +48,7 @@ struct WinArgs {
     int64_t o0_sb, o0_sh, o0_sn, o1_sb, o1_sh, o1_sn;
     const int32_t* lens;  // [B] or null
     float* lse;           // [B][H][N]: forward output, backward input
-    float *lse2, *delta;  // [B][H][N] workspace: lse * log2(e) and delta, from dQ to dK / dV
+    float *lse2, *delta;  // [B][H][N] workspace: lse * log2(e) - kPBits and delta * kPUnit, from dQ to dK / dV
     float* part;          // dK / dV parts
     int B, N, H, Hk, G, Dreal;
     int left, right, sinks;
@@ -398,8 +407,8 @@ __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq
             __syncthreads();  // every wave has read the last tile
         }
         if (live && lane < 32) {
-            a.delta[at_row] = dl;
-            a.lse2[at_row] = lse2;
+            a.delta[at_row] = dl * kPUnit<DT>;
+            a.lse2[at_row] = lse2 - kPBits<DT>;
         }
         walk(std::false_type{});
     }
@@ -682,10 +691,10 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
                             const int i = 8 * ks + e;
                             const float4 pr = sX[(k + 1) & 1][tt][i / 4][lane];
                             const float4 dl = *reinterpret_cast<const float4*>(ld + 32 + c_row(i, lane));
-                            dv8[e] = pr.x * (dpv[i] - dl.x);
-                            dv8[e + 1] = pr.y * (dpv[i + 1] - dl.y);
-                            dv8[e + 2] = pr.z * (dpv[i + 2] - dl.z);
-                            dv8[e + 3] = pr.w * (dpv[i + 3] - dl.w);
+                            dv8[e] = pr.x * fmaf(dpv[i], kPUnit<DT>, -dl.x);
+                            dv8[e + 1] = pr.y * fmaf(dpv[i + 1], kPUnit<DT>, -dl.y);
+                            dv8[e + 2] = pr.z * fmaf(dpv[i + 2], kPUnit<DT>, -dl.z);
+                            dv8[e + 3] = pr.w * fmaf(dpv[i + 3], kPUnit<DT>, -dl.w);
                         }
                         ds2[ks] = fta_pack_frag<DT>(dv8);
                     }
@@ -729,7 +738,7 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
         }
         uint16_t* out = HV ? a.out0 + b * a.o0_sb + hk * a.o0_sh : a.out1 + b * a.o1_sb + hk * a.o1_sh;
         const int64_t osn = HV ? a.o0_sn : a.o1_sn;
-        const float osc = HV ? a.scale : 1.f;
+        const float osc = HV ? a.scale : kPUnit<DT>;
 #pragma unroll
         for (int dt = 0; dt < DT32; ++dt) {
             const int d = dt * 32 + (lane & 31);
@@ -751,7 +760,7 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
 // dK / dV up to D = 128: four waves of 32 keys, each with its keys' K and V rows and both
 // accumulators in registers, so a 32-query chunk of Q and dO serves 128 keys and P never
 // leaves the wave:
-//   S = Q K^T,  dP = dO V^T,  P = 2^{c S - lse2},  dS = P (dP - delta),
+//   S = Q K^T,  dP = dO V^T,  P = 2^{c S - lse2},  dS = P (dP - delta)  (P and delta in kPUnit),
 //   dV += P^T dO,  dK += dS^T Q.
 // At D = 128 that is 250 registers, two workgroups per CU; 158 and three at D = 64.  Against
 // 64 keys a workgroup with the work of a tile split over two waves (the kernel above):
@@ -933,10 +942,10 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
                         p8[e + 1] = fta_exp2(fmaf(s[i + 1], a.c, -l4.y));
                         p8[e + 2] = fta_exp2(fmaf(s[i + 2], a.c, -l4.z));
                         p8[e + 3] = fta_exp2(fmaf(s[i + 3], a.c, -l4.w));
-                        d8[e] = p8[e] * (dpv[i] - e4.x);
-                        d8[e + 1] = p8[e + 1] * (dpv[i + 1] - e4.y);
-                        d8[e + 2] = p8[e + 2] * (dpv[i + 2] - e4.z);
-                        d8[e + 3] = p8[e + 3] * (dpv[i + 3] - e4.w);
+                        d8[e] = p8[e] * fmaf(dpv[i], kPUnit<DT>, -e4.x);
+                        d8[e + 1] = p8[e + 1] * fmaf(dpv[i + 1], kPUnit<DT>, -e4.y);
+                        d8[e + 2] = p8[e + 2] * fmaf(dpv[i + 2], kPUnit<DT>, -e4.z);
+                        d8[e + 3] = p8[e + 3] * fmaf(dpv[i + 3], kPUnit<DT>, -e4.w);
                     }
                     pf[ks] = fta_pack_frag<DT>(p8);
                     df[ks] = fta_pack_frag<DT>(d8);
@@ -994,7 +1003,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
         for (int i = 0; i < 16; ++i) {
             const int t = kt + c_row(i, lane);
             if (t >= a.N) continue;
-            const uint32_t pk = E::pack2(dk[dt][i] * a.scale, dv[dt][i]);
+            const uint32_t pk = E::pack2(dk[dt][i] * a.scale, dv[dt][i] * kPUnit<DT>);
             ok[(int64_t)t * a.o0_sn + d] = (uint16_t)(pk & 0xffffu);
             ov[(int64_t)t * a.o1_sn + d] = (uint16_t)(pk >> 16);
         }
@@ -1035,7 +1044,7 @@ __global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, 
     for (int e = 0; e < 8; ++e) so[sl][rr * D + d0 + e] = o[e];
     __syncthreads();
     if (sl != 0 || !ok || n <= 1 || d0 >= a.Dreal) return;  // n <= 1: written by the kernel itself
-    const float f = ten ? 1.f : a.scale;
+    const float f = ten ? kPUnit<DT> : a.scale;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
 #pragma unroll

@@ -89,3 +89,24 @@ def test_rows_that_see_few_keys(gpu, dtype, B, N, H, Hk, D, left, right, sinks, 
         off = (got.double() - want).norm()
         assert off <= 1.5 * rounding, (name, float(off / rounding))
     R.check(dict(zip(("dq", "dk", "dv"), grads)), ref, ("dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("dtype,N,D,left,right", [(torch.float16, 40000, 64, 40000, 40000), (torch.float16, 70000, 128, 70000, 0),
+                                                  (torch.float16, 33000, 256, 33000, 33000), (torch.bfloat16, 33000, 64, 33000, 0)])
+def test_long_sequences_keep_small_probabilities(gpu, dtype, N, D, left, right):
+    """dV where every probability is below fp16's normal range (the mean is 1 / N).
+
+    P and dV are each rounded once, independently: sqrt(2) times what rounding the exact dV costs, and 6%
+    for the sample.  P in fp16 as it stands would be 2.1 (32768 keys) to 6.5 times (131072).
+    """
+    say("long", dtype, N, D, left, right)
+    q, k, v, do = G.inputs((dtype, 1, N, 1, 1, D), gpu)
+    _, (_, _, dv) = _run((dtype, 1, N, 1, 1, D, left, right, 0, None), q, k, v, do)
+    want = torch.zeros(N, D, device=gpu, dtype=torch.float64)
+    kd, j = k[0].double(), torch.arange(N, device=gpu)
+    for i in range(0, N, 1024):
+        rows = torch.arange(i, min(N, i + 1024), device=gpu)[:, None]
+        s = (q[0, i:i + 1024].double() @ kd.T * D ** -0.5).masked_fill_((j > rows + right) | (j < rows - left), -float("inf"))
+        want += torch.softmax(s, -1).T @ do[0, i:i + 1024].double()
+    off, rounding = (dv[0].double() - want).norm(), (want.to(dtype).double() - want).norm()
+    assert off <= 1.5 * rounding, float(off / rounding)
