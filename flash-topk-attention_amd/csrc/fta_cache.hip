@@ -69,8 +69,8 @@ struct CacheShape {
 // as it has read the last one, into the same stage: the other waves of the CU (eight at
 // D = 128, 128 KB of loads in all) cover its wait, and a second stage changed nothing.
 // What bounds it: memory.  128 requests, 32 / 8 heads of 128, 4096 of 8192 cached tokens:
-// 356 to 361 us, 6.0 TB/s (a large copy moves 5.15); one request: 7 us and 4 for the
-// join, latencies.
+// 365 us, 5.9 TB/s (a large copy moves 5.15); one request: 7 us and 4 for the join,
+// latencies.
 // ----------------------------------------------------------------------------
 template <int DT, int D>
 __device__ void cache_own(const CacheArgs& a, int wgi, unsigned char* sStage, float2 (*sML)[32]) {
@@ -378,7 +378,13 @@ int cache_plan(CacheArgs& a, int B, int H, int Hk, int T, int S, int D, int P, i
     a.rows = (int64_t)B * Hk * a.R;
     a.row_tiles = (a.R + 31) / 32;
     const int64_t wgs = (int64_t)B * Hk * a.row_tiles;
-    // keys a row tile can see, in 32-key tiles: at least one tile per wave and part
+    // Keys a row tile can see, in 32-key tiles: at least one tile per wave and part.  About 512
+    // workgroups in all (two a CU at D = 128), by shapes alone, as the lengths are on the device.
+    // Target 256 / 512 / 1024 / 2048, us, 32 / 8 heads of 128, 4096 tokens each: 8 requests 27 / 28 /
+    // 29 / 34, 64 requests 185 / 185 / 192 / 195, 65 (a second round of workgroups) 224 / 225 / 212
+    // / 205, 128 362 / 362 / 362 / 374.  What it costs is a batch with one long request, whose
+    // part is walked by one workgroup: 63 requests of 1024 tokens and one of 32768, 375 / 374 /
+    // 223 / 146.
     const int64_t span = std::min<int64_t>(S, (int64_t)a.left + T + a.sinks);
     const int64_t tiles = (span + 31) / 32;
     a.ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, tiles / 4));

@@ -82,7 +82,7 @@ __device__ __forceinline__ void load_w8(const void* w, int dt, int d, float* f) 
     }
 }
 // 16 bytes that are read or written once: past the caches where the call streams more than
-// they hold (NT; 32K tokens, 32 + 8 heads of 128: backward 229 -> 203 us).
+// they hold (see kStream).
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 template <bool NT>
 __device__ __forceinline__ uint4 load16(const uint16_t* p) {
@@ -441,10 +441,18 @@ void set_units(PrepArgs& a, int B, int U, int rows) {
 //    120 us, 5.6 TB/s.
 //  * backward, 1.0 GB: one 328, two 229, four 260, five 252; past the caches two 204, three
 //    203 (5.0 TB/s), five 197 with twice the partial sums.
-// Few rows (a step of a serving batch) take one group a wave, so that they spread over the CUs.
+// Few rows (a step of a serving batch, up to 4 kFwdGrid groups) take one group a wave, so that
+// they spread over the CUs.  One group / five groups a wave, us of the kernel: 32 + 8 heads of
+// 128, 16 tokens 3.3 / 5.3, 256 tokens 4.3 / 5.6, 512 tokens 6.2 / 6.9, 1228 tokens (the
+// border) 12.0 / 9.6, 8192 tokens 53 / 35; 8 + 8 heads of 64, 1024 tokens 3.8 / 4.5, 2048
+// tokens 5.5 / 5.8, 8192 tokens (past the border of 6144) 13.8 / 12.8.
 constexpr int kFwdGroups = 5, kFwdGrid = 256 * 12, kBwdGroups = 3, kBwdGrid = 256 * 4;
-// Bytes of one tensor from which a call is taken to stream past the caches (4 MB of L2 a die,
-// 256 MB behind them, shared with what the caller does next).
+// Bytes of q from which a call is taken to stream past the caches (4 MB of L2 a die, 256 MB
+// behind them, shared with what the caller does next).  Past them / through them, us, every call
+// on other tensors: forward and backward, 32 + 8 heads of 128, q of 32 MB 66 / 66, 64 MB
+// 87 / 94, 128 MB 166 / 184, 256 MB 321 / 357; 16 + 16 heads of 64, 64 MB 142 / 155, 512 MB
+// 1096 / 1196.  Forward with the window attention that reads its outputs: 16 MB 36.8 / 35.9
+// (heads of 64, 32 MB: 74.9 / 73.0), 64 MB 94.9 / 94.8, 128 MB 176 / 178, 256 MB 336 / 340.
 constexpr int64_t kStream = 64 << 20;
 
 unsigned grid_of(int64_t units, int most) { return (unsigned)std::min<int64_t>((units + 3) / 4, most); }

@@ -134,8 +134,11 @@ struct FtaTile {
 
     // Online softmax of those scores (masked ones are -inf) and O^T += V^T P^T, V at `off`.
     // The accumulators are rescaled only when a row's maximum grows by more than 2^8:
-    // P stays below 2^8 and its 16-bit rounding keeps the same relative error.  A row
-    // that has seen no key yet keeps m = -inf and adds exact zeros.
+    // P stays below 2^8 and its 16-bit rounding keeps the same relative error.  That rounding
+    // is what the matrix instructions of 16-bit V take, and as large as the rounding of o
+    // itself: o is off by up to sqrt(2) times the latter (the sum l adds the unrounded P; P as
+    // a sum of two 16-bit numbers would be half as many products again).  A row that has seen
+    // no key yet keeps m = -inf and adds exact zeros.
     template <int PD, typename A>
     __device__ static __forceinline__ void softmax_pv(const A& ad, uint32_t off, const f32x16& s, float c, float& m_run,
                                                       float& l_run, f32x16* oacc) {

@@ -163,17 +163,18 @@ constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 // tiles each; 64-key tiles of K and V (32 at D = 256), worked on 32 keys at a time so
 // that the half tiles at the band's edges and the sinks' tile cost what they hold.
 // What bounds it at D = 128: power, then neither pipe alone.  N32768, 32 / 8 heads of 128,
-// window 1024, 4 sinks: 681 us at a clock of 1.95 GHz (914 us in a run that held 1.44), 844
-// TFLOP/s with the masked scores, 66% of a large library product on the same card; matrix
-// units 44% busy, vector units 40%, LDS 45%; more waves per SIMD (three, by 32-key stages)
+// window 1024, 4 sinks: 680 us, 845 TFLOP/s with the masked scores, 66% of a large library
+// product on the same card; in one pass of 703 us at a clock of 1.88 GHz the matrix units
+// were busy 44% of the cycles, the vector units 44%; more waves per SIMD (three, by 32-key stages)
 // and other prefetch distances or wave priorities change it by under 4%.  Gathering the edge
 // tiles whole took 74.6 -> 71.3 us at D = 64 (N10000 twice, 12 / 4 heads, 300 to both sides;
-// 68 with the heads outermost) and 705 -> 681 here.  At D = 64 the vector unit bounds it: of 84 vector instructions per 32
+// 65 with the heads outermost) and 705 -> 681 here.  At D = 64 the vector instructions weigh
+// most (67% of the cycles, the products 33%, so that the two hardly overlap): of 84 per 32
 // x 32 scores (four cycles each, the 16 exp2 more) 64 are the fma, exp2, sum and packing of
 // the softmax and 8 its maximum, against 8 MFMAs.
 // D = 256 is held to 256 registers, two workgroups per CU: with 512 the compiler moved the
 // whole accumulator through copies at every tile (N4096 twice, 16 / 2 heads, window 512: 150
-// -> 101 us, 643 TFLOP/s without the masked scores).
+// -> 94 us, 690 TFLOP/s without the masked scores).
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_fwd_kernel(WinArgs a) {
@@ -273,8 +274,9 @@ __global__ __launch_bounds__(kRowWaves * 64, win_fwd_waves(D)) void fta_window_f
 // and 1.43 to 1.47 from 64 on, of which 1.41 are the rounding of dS.  A workgroup with rows of
 // fewer than 64 keys forms delta = sum_j P_ij dP_ij in fp32 instead, by a first walk over its keys
 // without dQ's product (1.41 for every n); in a causal sequence that is the first tile of each head.
-// Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 905 us, 953 TFLOP/s
-// with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 85 us.
+// dS is rounded to 16 bits for its product with K (in dK's kernel with Q), as P is in the forward.
+// Bound as the forward is: N32768, 32 / 8 heads of 128, window 1024: 886 us, 973 TFLOP/s
+// with the masked scores; N10000 twice, 12 / 4 heads of 64, 300 to both sides: 82 us.
 // ----------------------------------------------------------------------------
 template <int DT, int D, int NH>
 __global__ __launch_bounds__(kRowWaves * 64, win_dq_waves(D)) void fta_window_dq_kernel(WinArgs a) {
@@ -765,9 +767,8 @@ __global__ __launch_bounds__(256, 1) void fta_window_dkv_split_kernel(WinArgs a)
 // At D = 128 that is 250 registers, two workgroups per CU; 158 and three at D = 64.  Against
 // 64 keys a workgroup with the work of a tile split over two waves (the kernel above):
 // half the gathers and barriers, no exchange of P.  N32768, 32 / 8 heads of 128, window
-// 1024: 1510 -> 1150 us, 1000 TFLOP/s with the masked scores at a clock of 1.65 GHz (power);
-// N10000 twice, 12 / 4 heads of 64, 300 to both sides: 175 -> 110.  Three stages instead of
-// two change nothing.
+// 1024: 1510 -> 1150 us, 1000 TFLOP/s with the masked scores; N10000 twice, 12 / 4 heads of 64,
+// 300 to both sides: 175 -> 104.  Three stages instead of two change nothing.
 // ----------------------------------------------------------------------------
 template <int D>
 struct WinDkvShape {
@@ -1012,7 +1013,7 @@ __global__ __launch_bounds__(256, D <= 64 ? 3 : 2) void fta_window_dkv_kernel(Wi
 
 // Sum of the dK / dV parts: SL threads per (tensor, b, K/V head, key of a tile with parts,
 // 8 columns) add every SL-th part and then their sums, always in the same order; dK takes
-// the scale here.  (One thread for all of a sink tile's 58 parts took 17.6 us at N 32768.)
+// the scale here.  (One thread for all parts of a tile took 17.6 us for 58 parts.)
 template <int DT, int D, int SL>
 __global__ __launch_bounds__(256) void fta_window_dkv_combine_kernel(WinArgs a, int keys) {
     using E = Elem<DT>;

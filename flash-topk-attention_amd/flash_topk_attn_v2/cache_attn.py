@@ -86,7 +86,8 @@ def flash_prefix_attn_decode(
     prefix.  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host) counts each
     request's own tokens with these T; values outside ``[0, S]`` are clamped.  Token t sees
     the whole prefix and own key j when ``j <= cache_lens[b] - T + t``; one that sees
-    nothing gives o = 0, lse = -inf.  Cache rows that no token sees may hold anything.  Not
+    nothing gives o = 0, lse = -inf.  Cache rows that no token sees may hold anything.
+    Probabilities are rounded to the inputs' type, as in ``flash_window_attn``.  Not
     differentiable.
 
     Returns ``(output [B, T, num_heads * D], lse [B, num_heads, T] float32)``.

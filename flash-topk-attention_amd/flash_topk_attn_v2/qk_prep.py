@@ -140,6 +140,7 @@ def flash_qk_norm_rope(
         k: ``[B, N, num_kv_heads * D]``, the same type.
         cos, sin: float32 tables ``[P, R / 2]`` of the angles of positions ``0 .. P - 1``;
             the first ``R`` columns of a head are turned, ``R`` a multiple of 16 up to D.
+            Tables that are not contiguous are copied at every call.
         q_weight, k_weight: norm weights ``[D]`` (float32, float16 or bfloat16), or None for ones.
         eps: added to the mean square.
         num_kv_heads: heads of k, default ``num_heads``.
@@ -191,7 +192,8 @@ def flash_qk_norm_rope_append(
 
     ``q`` is ``[B, T, num_heads * D]``, ``k`` and ``v`` ``[B, T, num_kv_heads * D]``,
     the caches ``[B, S, num_kv_heads * D]`` (any batch and token stride that keeps rows
-    16-byte aligned; no two rows, of one cache or of both, may share memory).  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host)
+    16-byte aligned; no two rows, of one cache or of both, may share memory, and q, k and v
+    may lie in them only where a row is written to itself).  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host)
     counts each request's cached tokens with these T: token t is written to row
     ``cache_lens[b] - T + t`` and turned as position ``row + position_offset`` (the
     length of a shared prefix, for instance).  Rows outside ``[0, S)`` are not written.

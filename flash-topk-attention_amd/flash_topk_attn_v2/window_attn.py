@@ -117,6 +117,10 @@ def flash_window_attn(
     Returns:
         ``(output [B, N, num_heads * D], lse [B, num_heads, N] float32 natural log)``; lse
         is not differentiable.
+
+    Scores, softmax statistics and sums are float32; probabilities, and in the backward dS,
+    are rounded to the inputs' type for the matrix units.  float16 gradients below 6e-5 lose
+    bits: scale the loss.
     """
     what = "flash_window_attn"
     if not q.is_cuda:
@@ -154,7 +158,8 @@ def flash_window_attn_decode(
     and sees key j when ``j <= p`` and (``j >= p - window_left`` or ``j < num_sinks``);
     one that sees nothing (an idle request) gives o = 0, lse = -inf.  Cache rows that no
     token sees may hold anything.  ``window_left >= S`` is plain causal attention over the
-    cache.  Not differentiable.
+    cache.  Probabilities are rounded to the inputs' type, as in ``flash_window_attn``.  Not
+    differentiable.
 
     Returns ``(output [B, T, num_heads * D], lse [B, num_heads, T] float32)``.
     """

@@ -487,8 +487,9 @@ int fta_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k, 
 
 /*
  * Its backward, from the forward's o and lse: dq [B][N][H][D], dk, dv [B][N][Hk][D].
- * No atomics; the workspace (fta_window_attn_bwd_workspace_size bytes) holds delta =
- * o . dout, the lse in log2 units and the fp32 parts of split dK / dV walks.
+ * No atomics; the workspace (fta_window_attn_bwd_workspace_size bytes) holds delta
+ * (o . dout, or the sum of P dP for rows that see few keys), the lse in log2 units and the
+ * fp32 parts of split dK / dV walks.
  */
 size_t fta_window_attn_bwd_workspace_size(int B, int H, int Hk, int N, int D, int left, int right, int num_sinks);
 int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
@@ -508,7 +509,7 @@ int fta_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k, 
  * request sees whole (k_prefix, v_prefix [P][Hk][D]; strides {unused, stride_h, stride_n}),
  * read once for the batch; it needs left >= S (no window).  q and o are [B][T][H][D]
  * strided, lse [B][H][T]; rows that see nothing give o = 0, lse = -inf.  Cache rows that
- * no token sees may hold anything.  The workspace (fta_cache_attn_workspace_size bytes)
+ * no token sees may hold anything.  0 < scale <= 2e38.  The workspace (fta_cache_attn_workspace_size bytes)
  * holds the parts that the keys are split into.
  */
 size_t fta_cache_attn_workspace_size(int B, int H, int Hk, int T, int S, int D, int P, int left, int num_sinks);
