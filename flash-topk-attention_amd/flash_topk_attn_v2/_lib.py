@@ -203,6 +203,7 @@ def rows_in_place(what: str, x: torch.Tensor, heads: int):
     return at, strides
 
 
+@lru_cache(maxsize=4096)
 def _rows_meet(shape: tuple, stride: tuple, delta: int) -> bool:
     """Whether a row of ``[B, N, C]`` and one of the same layout ``delta`` elements on share an
     element (``delta`` 0: two different rows of the one)."""
