@@ -162,7 +162,7 @@ constexpr int win_dq_waves(int D) { return D <= 64 ? 4 : D <= 128 ? 2 : 1; }
 // Forward.  Four waves of 32 rows: hw query heads that share a K/V head, 4 / hw row
 // tiles each; 64-key tiles of K and V (32 at D = 256), worked on 32 keys at a time so
 // that the half tiles at the band's edges and the sinks' tile cost what they hold.
-// What bounds it at D = 128: power, then neither pipe alone.  N32768, 32 / 8 heads of 128,
+// What bounds it at D = 128: neither pipe alone, at a clock below the card's 2.4 GHz.  N32768, 32 / 8 heads of 128,
 // window 1024, 4 sinks: 680 us, 845 TFLOP/s with the masked scores, 66% of a large library
 // product on the same card; in one pass of 703 us at a clock of 1.88 GHz the matrix units
 // were busy 44% of the cycles, the vector units 44%; more waves per SIMD (three, by 32-key stages)
