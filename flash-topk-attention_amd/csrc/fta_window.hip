@@ -124,7 +124,9 @@ __device__ __forceinline__ uint32_t seen_keys(const WinArgs& a, int len, int i, 
 __device__ __forceinline__ int seen_count(const WinArgs& a, int len, int i) {
     return min(i + a.right, len - 1) - max(i - a.left, 0) + 1 + max(min(a.sinks, i - a.left), 0);
 }
-// Rows that see fewer keys than this take delta from their scores, see the dQ kernel.
+// Rows that see fewer keys than this take delta from their scores, see the dQ kernel.  Where all
+// of them do (16384 tokens, 32 / 8 heads of 128, 41 tokens of window), forward and backward took
+// 460 us without that walk and 462 with it; dQ's error falls from 1.5 to 2.3 roundings to 1.41.
 constexpr int kFewKeys = 64;
 
 // Workgroup -> (K/V head, b, head group, token tile).  An XCD takes an eighth of that order: heads
