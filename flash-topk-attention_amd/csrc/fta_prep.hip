@@ -25,6 +25,13 @@
 
 namespace {
 
+// Codes and scales of a 4-bit cache ([B][Hk][S] rows, see fta_q4.hip); batch and head strides in elements.
+struct Q4Out {
+    uint32_t* codes;
+    uint16_t* scales;
+    int64_t c_sb, c_sh, s_sb, s_sh;
+};
+
 struct PrepArgs {
     const uint16_t *q, *k, *v;      // inputs (v: append only)
     const uint16_t *dqo, *dko;      // backward: gradients of the outputs
@@ -39,6 +46,8 @@ struct PrepArgs {
     int64_t pos_sb;
     const int32_t* lens;            // append: tokens in the cache, the new ones included
     int S, pos_off;                 // append: rows of the cache, table row of cache row 0
+    const int32_t* pos_offs;        // append: the same for each request, or null
+    Q4Out qk, qv;                   // append to a 4-bit cache: in place of ko and vo
     float* part;                    // backward: [workgroup][2][D] partial weight gradients, or null
     int N, H, Hk, D, R, P, inter;
     int parts, per;                 // parts of a token's row groups, groups in each
@@ -158,16 +167,45 @@ __device__ __forceinline__ void load_angles(const PrepArgs& a, const LaneCols& c
     }
 }
 
+// Four bits of a row's values, this lane's eight columns of them: four lanes hold a group of 32,
+// whose value of largest magnitude over -8 is its scale d (rounded to float16; the negative of two
+// equal ones), and a value's code is round(x / d) + 8, ties to even, held to 0 .. 15.  x / d is
+// an IEEE division: a border between two codes falls where the quotient's formula says.
+__device__ __forceinline__ uint32_t quant8(const float* x, uint16_t& scale) {
+    float hi = x[0], lo = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        hi = fmaxf(hi, x[e]);
+        lo = fminf(lo, x[e]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
+        lo = fminf(lo, __shfl_xor(lo, o, 64));
+    }
+    const float top = (-lo >= hi ? lo : hi) * -0.125f;
+    const _Float16 h = (_Float16)fminf(fmaxf(top, -65504.f), 65504.f);
+    scale = __builtin_bit_cast(uint16_t, h);
+    const float d = (float)h;
+    if (d == 0.f) return 0x88888888u;
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= (uint32_t)(int)fminf(fmaxf(rintf(x[e] / d) + 8.f, 0.f), 15.f) << (4 * e);
+    return w;
+}
+
 // ----------------------------------------------------------------------------
 // Forward.  A wave strides over (token, part) pairs; a part is U groups of 64 / LG
 // rows of one token, whose loads are issued together and share the token's angles.
 // The weights (the lane's own and its partners') stay in registers.
 // APPEND: rows past the query and key heads copy V; K and V go to cache row
-// lens[b] - N + n (not written outside [0, S)).
+// lens[b] - N + n (not written outside [0, S)).  Q4: into a 4-bit cache, K as its 16-bit values,
+// so that a cache holds the same whether or not it was written in one pass with the norm.
 // ----------------------------------------------------------------------------
-template <int DT, int LG, int U, bool APPEND, bool NT>
+template <int DT, int LG, int U, bool APPEND, bool NT, bool Q4 = false>
 __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
     constexpr int RW = 64 / LG;
+    static_assert(!Q4 || (APPEND && LG >= 4), "a group of 32 columns within a row's lanes");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const LaneCols c = lane_cols<LG>(a, lane);
@@ -191,7 +229,7 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
         if constexpr (APPEND) {
             const int64_t at = (int64_t)a.lens[b] - a.N + n;
             crow = (at < 0 || at >= a.S) ? -1 : (int)at;
-            pos = (int)min(max(at + a.pos_off, (int64_t)0), (int64_t)a.P - 1);
+            pos = (int)min(max(at + (a.pos_offs ? a.pos_offs[b] : a.pos_off), (int64_t)0), (int64_t)a.P - 1);
         } else {
             pos = a.positions ? a.positions[b * a.pos_sb + n] : n;
             pos = min(max(pos, 0), a.P - 1);
@@ -226,6 +264,49 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
             for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
             const float r = rsqrtf(fmaf(row_sum<LG>(ss), inv_d, a.eps));
             const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
+            if constexpr (Q4) {
+                // every lane takes part: those behind D hold zeros, and write them behind D
+                const bool isv = row >= a.H + a.Hk;
+                if (!isv) {
+                    float g[8];
+                    unpack8<DT>(xp, g);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] *= r * (isq ? wq[e] : wk[e]);
+                        g[e] *= r * (isq ? pq[e] : pk[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        if (a.inter) {
+                            y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
+                            y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
+                        } else {
+                            y[e] = fmaf(g[e], sn[e], f[e] * cs[e]);
+                            y[e + 1] = fmaf(g[e + 1], sn[e + 1], f[e + 1] * cs[e + 1]);
+                        }
+                    }
+                    if (!c.live) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) y[e] = 0.f;
+                    }
+                }
+                const uint4 out = isv ? x[u] : pack8<DT>(y);
+                unpack8<DT>(out, y);
+                uint16_t scale;
+                const uint32_t w = quant8(y, scale);
+                if (row >= rows || u >= a.per) continue;
+                if (isq) {
+                    if (c.live) store16<NT>(a.qo + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn + c.d0, out);
+                    continue;
+                }
+                const int ng = (a.D + 31) >> 5, g = c.d0 >> 5, o = (c.d0 >> 3) & 3;
+                if (crow < 0 || g >= ng) continue;
+                const Q4Out& t = isv ? a.qv : a.qk;
+                const int hk = isv ? row - a.H - a.Hk : row - a.H;
+                t.codes[b * t.c_sb + hk * t.c_sh + (int64_t)crow * 4 * ng + (isv ? 4 * g + o : o * ng + g)] = w;
+                if (o == 0) t.scales[b * t.s_sb + hk * t.s_sh + (int64_t)crow * ng + g] = scale;
+                continue;
+            }
             if (!c.live || row >= rows || u >= a.per) continue;
             uint16_t* out;
             if (APPEND && row >= a.H + a.Hk) {
@@ -427,8 +508,8 @@ int prep_geometry(int B, int H, int Hk, int N, int D, int R, int P) {
 }
 
 // The (token, part) pairs: the 64 / LG-row groups of a token in even parts of at most U.
-void set_units(PrepArgs& a, int B, int U, int rows) {
-    const int rw = 64 / lanes_per_row(a.D);
+void set_units(PrepArgs& a, int B, int U, int rows, int lanes = 0) {
+    const int rw = 64 / (lanes > 0 ? lanes : lanes_per_row(a.D));
     const int groups = (rows + rw - 1) / rw;
     a.parts = (groups + U - 1) / U;
     a.per = (groups + a.parts - 1) / a.parts;
@@ -490,6 +571,23 @@ int launch_fwd(PrepArgs& a, int B, hipStream_t st) {
 }
 
 template <int DT>
+int launch_append_q4(PrepArgs& a, int B, hipStream_t st) {
+    const int rows = a.H + 2 * a.Hk;
+    return with_lanes(std::max(a.D, 32), [&](auto lg) {
+        constexpr int LG = decltype(lg)::value < 4 ? 4 : decltype(lg)::value;
+        set_units(a, B, 1, rows, LG);
+        const bool few = a.units <= 4 * kFwdGrid;
+        if (!few) set_units(a, B, kFwdGroups, rows, LG);
+        const dim3 g(grid_of(a.units, kFwdGrid)), t(256);
+        if (few)
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, true, false, true>), g, t, 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, kFwdGroups, true, false, true>), g, t, 0, st, a);
+        return fta::check_launch("fta_norm_rope_fwd_kernel");
+    });
+}
+
+template <int DT>
 int launch_bwd(PrepArgs& a, int B, void* dqw, void* dkw, hipStream_t st) {
     return with_lanes(a.D, [&](auto lg) {
         constexpr int LG = decltype(lg)::value;
@@ -517,6 +615,33 @@ int check_types(int dtype, int w_dtype) {
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16)
         return fta::arg_error("qk_norm_rope: dtype must be bf16 or fp16");
     if (w_dtype < 0 || w_dtype > FTA_DTYPE_F32) return fta::arg_error("qk_norm_rope: weights must be bf16, fp16 or fp32");
+    return FTA_OK;
+}
+
+// What the appends to either cache have in common.
+int append_args(PrepArgs& a, const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D, const void* q_weight,
+                const void* k_weight, int weight_dtype, const float* cos, const float* sin, int P, int R, int position_offset,
+                const int32_t* position_offsets, float eps, int interleaved, const int32_t* cache_lens, int S, void* q_out,
+                const int64_t* qo_strides) {
+    int rc = prep_geometry(B, H, Hk, T, D, R, P);
+    if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
+    if (!(eps > 0.f) || eps > 3.0e38f) return fta::arg_error("qk_norm_rope: eps must be positive and finite");
+    if (S <= 0) return fta::arg_error("qk_norm_rope_append: the caches must have rows");
+    if (!fta::all_set(q, q_strides, k, k_strides, v, v_strides, cos, sin, cache_lens, q_out, qo_strides))
+        return fta::arg_error("qk_norm_rope_append: a required pointer is null");
+    a.q = (const uint16_t*)q;
+    a.k = (const uint16_t*)k;
+    a.v = (const uint16_t*)v;
+    a.qo = (uint16_t*)q_out;
+    set3(a.q_sb, a.q_sh, a.q_sn, q_strides);
+    set3(a.k_sb, a.k_sh, a.k_sn, k_strides);
+    set3(a.v_sb, a.v_sh, a.v_sn, v_strides);
+    set3(a.qo_sb, a.qo_sh, a.qo_sn, qo_strides);
+    a.qw = q_weight, a.kw = k_weight, a.w_dtype = weight_dtype;
+    a.cos = cos, a.sin = sin, a.P = P, a.R = R;
+    a.lens = cache_lens, a.S = S, a.pos_off = position_offset, a.pos_offs = position_offsets;
+    a.N = T, a.H = H, a.Hk = Hk, a.D = D, a.inter = interleaved != 0, a.eps = eps;
     return FTA_OK;
 }
 
@@ -607,33 +732,55 @@ int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void*
                             const float* sin, int P, int R, int position_offset, float eps, int interleaved,
                             const int32_t* cache_lens, int S, void* q_out, const int64_t* qo_strides, void* k_cache,
                             const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides, void* stream) {
+    return fta_qk_norm_rope_append_at(q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, T, D, q_weight, k_weight,
+                                      weight_dtype, cos, sin, P, R, position_offset, nullptr, eps, interleaved, cache_lens, S,
+                                      q_out, qo_strides, k_cache, kc_strides, v_cache, vc_strides, stream);
+}
+
+int fta_qk_norm_rope_append_at(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                               const float* sin, int P, int R, int position_offset, const int32_t* position_offsets,
+                               float eps, int interleaved, const int32_t* cache_lens, int S, void* q_out,
+                               const int64_t* qo_strides, void* k_cache, const int64_t* kc_strides, void* v_cache,
+                               const int64_t* vc_strides, void* stream) {
     FTA_TRY_BEGIN
-    int rc = prep_geometry(B, H, Hk, T, D, R, P);
-    if (rc != FTA_OK || (rc = check_types(dtype, weight_dtype)) != FTA_OK) return rc;
-    if (!(eps > 0.f) || eps > 3.0e38f) return fta::arg_error("qk_norm_rope: eps must be positive and finite");
-    if (S <= 0) return fta::arg_error("qk_norm_rope_append: the caches must have rows");
-    if (!fta::all_set(q, q_strides, k, k_strides, v, v_strides, cos, sin, cache_lens, q_out, qo_strides, k_cache, kc_strides,
-                      v_cache, vc_strides))
-        return fta::arg_error("qk_norm_rope_append: a required pointer is null");
     PrepArgs a = {};
-    a.q = (const uint16_t*)q;
-    a.k = (const uint16_t*)k;
-    a.v = (const uint16_t*)v;
-    a.qo = (uint16_t*)q_out;
+    int rc = append_args(a, q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, T, D, q_weight, k_weight, weight_dtype,
+                         cos, sin, P, R, position_offset, position_offsets, eps, interleaved, cache_lens, S, q_out, qo_strides);
+    if (rc != FTA_OK) return rc;
+    if (!fta::all_set(k_cache, kc_strides, v_cache, vc_strides))
+        return fta::arg_error("qk_norm_rope_append: a required pointer is null");
     a.ko = (uint16_t*)k_cache;
     a.vo = (uint16_t*)v_cache;
-    set3(a.q_sb, a.q_sh, a.q_sn, q_strides);
-    set3(a.k_sb, a.k_sh, a.k_sn, k_strides);
-    set3(a.v_sb, a.v_sh, a.v_sn, v_strides);
-    set3(a.qo_sb, a.qo_sh, a.qo_sn, qo_strides);
     set3(a.ko_sb, a.ko_sh, a.ko_sn, kc_strides);
     set3(a.vo_sb, a.vo_sh, a.vo_sn, vc_strides);
-    a.qw = q_weight, a.kw = k_weight, a.w_dtype = weight_dtype;
-    a.cos = cos, a.sin = sin, a.P = P, a.R = R;
-    a.lens = cache_lens, a.S = S, a.pos_off = position_offset;
-    a.N = T, a.H = H, a.Hk = Hk, a.D = D, a.inter = interleaved != 0, a.eps = eps;
     hipStream_t st = (hipStream_t)stream;
     return dtype == FTA_DTYPE_BF16 ? launch_fwd<FTA_DTYPE_BF16, true>(a, B, st) : launch_fwd<FTA_DTYPE_F16, true>(a, B, st);
+    FTA_TRY_END
+}
+
+int fta_qk_norm_rope_append_q4(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                               const float* sin, int P, int R, int position_offset, const int32_t* position_offsets,
+                               float eps, int interleaved, const int32_t* cache_lens, int S, void* q_out,
+                               const int64_t* qo_strides, void* k_codes, const int64_t* kc_strides, void* k_scales,
+                               const int64_t* ks_strides, void* v_codes, const int64_t* vc_strides, void* v_scales,
+                               const int64_t* vs_strides, void* stream) {
+    FTA_TRY_BEGIN
+    PrepArgs a = {};
+    int rc = append_args(a, q, q_strides, k, k_strides, v, v_strides, dtype, B, H, Hk, T, D, q_weight, k_weight, weight_dtype,
+                         cos, sin, P, R, position_offset, position_offsets, eps, interleaved, cache_lens, S, q_out, qo_strides);
+    if (rc != FTA_OK) return rc;
+    if (!fta::all_set(k_codes, kc_strides, k_scales, ks_strides, v_codes, vc_strides, v_scales, vs_strides))
+        return fta::arg_error("qk_norm_rope_append_q4: a required pointer is null");
+    if ((((uintptr_t)k_codes | (uintptr_t)v_codes) & 3) != 0 || ((kc_strides[0] | kc_strides[1] | vc_strides[0] | vc_strides[1]) & 3) != 0)
+        return fta::arg_error("qk_norm_rope_append_q4: codes must be 4-byte aligned");
+    a.qk = {(uint32_t*)k_codes, (uint16_t*)k_scales, kc_strides[0] / 4, kc_strides[1] / 4, ks_strides[0], ks_strides[1]};
+    a.qv = {(uint32_t*)v_codes, (uint16_t*)v_scales, vc_strides[0] / 4, vc_strides[1] / 4, vs_strides[0], vs_strides[1]};
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == FTA_DTYPE_BF16 ? launch_append_q4<FTA_DTYPE_BF16>(a, B, st) : launch_append_q4<FTA_DTYPE_F16>(a, B, st);
     FTA_TRY_END
 }
 

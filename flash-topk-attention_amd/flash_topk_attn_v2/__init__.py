@@ -23,6 +23,13 @@ import torch.nn.functional as F
 from . import _lib
 from .block_score import _parse_block_score_args, _prepare_qk, flash_block_score
 from .cache_attn import flash_prefix_attn_decode
+from .q4_cache import (
+    Q4Cache,
+    flash_q4_cache,
+    flash_q4_cache_read,
+    flash_qk_norm_rope_append_q4,
+    flash_window_attn_decode_q4,
+)
 from .qblock_merge import flash_qblock_merge
 from .qk_prep import flash_qk_norm_rope, flash_qk_norm_rope_append
 from .sparse_attn import FlashSparseAttnFunc, flash_sparse_attn
@@ -241,4 +248,9 @@ __all__ = [
     "flash_window_attn",
     "flash_window_attn_decode",
     "flash_prefix_attn_decode",
+    "Q4Cache",
+    "flash_q4_cache",
+    "flash_q4_cache_read",
+    "flash_qk_norm_rope_append_q4",
+    "flash_window_attn_decode_q4",
 ]

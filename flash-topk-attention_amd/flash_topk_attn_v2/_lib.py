@@ -79,6 +79,15 @@ _SIGNATURES = {
                                   _p, _i, _i, _p, _i64, _f, _i, _p, _i64p, _p, _i64p, _p, _p, _p, _sz, _p]),
     "fta_qk_norm_rope_append": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
                                      _i, _i, _f, _i, _p, _i, _p, _i64p, _p, _i64p, _p, _i64p, _p]),
+    "fta_qk_norm_rope_append_at": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
+                                        _i, _i, _p, _f, _i, _p, _i, _p, _i64p, _p, _i64p, _p, _i64p, _p]),
+    "fta_qk_norm_rope_append_q4": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _p, _i, _p, _p, _i,
+                                        _i, _i, _p, _f, _i, _p, _i, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p,
+                                        _i64p, _p]),
+    "fta_q4_read": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _p, _p, _p]),
+    "fta_q4_attn_workspace_size": (_sz, [_i] * 8),
+    "fta_q4_attn": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _f,
+                         _p, _i64p, _p, _p, _sz, _p]),
     "fta_window_attn_fwd": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _i, _i, _i, _f, _p,
                                  _i64p, _p, _p]),
     "fta_window_attn_bwd_workspace_size": (_sz, [_i] * 8),

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import warnings
 from functools import lru_cache
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -70,6 +70,32 @@ def _warn_of_short_tables(what, P, S, offset):
     if offset < 0 or S + offset > P:
         warnings.warn(f"{what}: cos and sin have rows for positions 0 .. {P - 1}, rows of the cache stand at {offset} .. "
                       f"{S + offset - 1}: tokens outside the tables are turned as the nearest row", stacklevel=3)
+
+
+def offsets(what, position_offset, B, device, P, S):
+    """``(offset for all, offset of each request or None)`` of an append, checked."""
+    if isinstance(position_offset, torch.Tensor):
+        if position_offset.dtype != torch.int32 or position_offset.shape != (B,):
+            raise ValueError(f"{what}: position_offset must be a whole number or int32 [B] = [{B}]")
+        _lib.check_device(what, device, position_offset)
+        return 0, position_offset.contiguous()
+    position_offset = _lib.whole(what, position_offset)
+    if not -(1 << 31) <= position_offset < (1 << 31):
+        raise ValueError(f"{what}: position_offset out of range")
+    _warn_of_short_tables(what, P, S, position_offset)
+    return position_offset, None
+
+
+def check_lens(what, cache_lens, B):
+    if cache_lens.dtype != torch.int32 or cache_lens.shape != (B,):
+        raise ValueError(f"{what}: cache_lens must be int32 [B] = [{B}]")
+
+
+def written(*tensors):
+    """Marks tensors as changed in place (inference tensors keep no version)."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 class _QKNormRopeFunc(torch.autograd.Function):
@@ -184,7 +210,7 @@ def flash_qk_norm_rope_append(
     k_weight: Optional[torch.Tensor] = None,
     eps: float = 1e-6,
     num_kv_heads: Optional[int] = None,
-    position_offset: int = 0,
+    position_offset: Union[int, torch.Tensor] = 0,
     interleaved: bool = False,
 ) -> torch.Tensor:
     """``flash_qk_norm_rope`` of the T new tokens of each request, their keys and values
@@ -196,9 +222,10 @@ def flash_qk_norm_rope_append(
     may lie in them only where a row is written to itself).  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host)
     counts each request's cached tokens with these T: token t is written to row
     ``cache_lens[b] - T + t`` and turned as position ``row + position_offset`` (the
-    length of a shared prefix, for instance).  Rows outside ``[0, S)`` are not written.
+    length of a shared prefix, for instance, or, as int32 ``[B]`` on the device, how many rows
+    of each request ``flash_cache_evict`` took).  Rows outside ``[0, S)`` are not written.
     Positions outside the tables take their nearest row, which turns those tokens wrongly; a
-    call whose cache has such rows (tables of fewer than ``S + position_offset``) warns once.
+    call whose cache has such rows (tables of fewer than ``S + position_offset``, a number) warns once.
     Other arguments as for ``flash_qk_norm_rope``.  Not differentiable.
 
     Returns the prepared q ``[B, T, num_heads * D]``.
@@ -214,23 +241,18 @@ def flash_qk_norm_rope_append(
     kca, kcs = _lib.rows_in_place(what, k_cache, Hk)
     vca, vcs = _lib.rows_in_place(what, v_cache, Hk)
     _lib.check_written(what, k_cache, v_cache)
-    position_offset = _lib.whole(what, position_offset)
-    if not -(1 << 31) <= position_offset < (1 << 31):
-        raise ValueError(f"{what}: position_offset out of range")
-    _warn_of_short_tables(what, cos.shape[0], k_cache.shape[1], position_offset)
+    offset, offs = offsets(what, position_offset, B, q.device, cos.shape[0], k_cache.shape[1])
     q, qa, qs = _lib.rows(q, H)
     k, ka, ks = _lib.rows(k, Hk)
     v, va, vs = _lib.rows(v, Hk)
     qw, kw = (None if w is None else _lib.flat(w) for w in (q_weight, k_weight))
     cos, sin, lens = _lib.flat(cos), _lib.flat(sin), cache_lens.contiguous()
     qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-    _lib.call("fta_qk_norm_rope_append", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, D,
-              _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, position_offset,
-              float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),
+    _lib.call("fta_qk_norm_rope_append_at", q.device, qa, qs, ka, ks, va, vs, _lib.DTYPE_CODES[q.dtype], B, H, Hk, T, D,
+              _lib.ptr(qw), _lib.ptr(kw), wt, cos.data_ptr(), sin.data_ptr(), cos.shape[0], R, offset,
+              _lib.ptr(offs), float(eps), int(bool(interleaved)), lens.data_ptr(), k_cache.shape[1], qo.data_ptr(),
               _lib.dense_strides(q.shape, H), kca, kcs, vca, vcs)
-    for c in (k_cache, v_cache):
-        if not c.is_inference():  # written in place (inference tensors keep no version)
-            torch.autograd.graph.increment_version(c)
+    written(k_cache, v_cache)
     return qo
 
 
@@ -244,8 +266,7 @@ def check_cache(what, q, k_cache, v_cache, cache_lens, B, width):
         raise ValueError(f"{what}: v_cache must have k_cache's shape")
     if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
         raise ValueError(f"{what}: the caches must have q's type")
-    if cache_lens.dtype != torch.int32 or cache_lens.shape != (B,):
-        raise ValueError(f"{what}: cache_lens must be int32 [B] = [{B}]")
+    check_lens(what, cache_lens, B)
     _lib.check_device(what, q.device, k_cache, v_cache, cache_lens)
 
 

@@ -470,6 +470,19 @@ int fta_qk_norm_rope_append(const void* q, const int64_t* q_strides, const void*
                             const int32_t* cache_lens, int S, void* q_out, const int64_t* qo_strides, void* k_cache,
                             const int64_t* kc_strides, void* v_cache, const int64_t* vc_strides, void* stream);
 
+/*
+ * The same, the position offset of each request in position_offsets[b] (int32, device) or, where
+ * that is null, position_offset for all: a cache whose rows no longer stand at their positions,
+ * after fta_cache_evict.
+ */
+int fta_qk_norm_rope_append_at(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                               const float* sin, int P, int R, int position_offset, const int32_t* position_offsets,
+                               float eps, int interleaved, const int32_t* cache_lens, int S, void* q_out,
+                               const int64_t* qo_strides, void* k_cache, const int64_t* kc_strides, void* v_cache,
+                               const int64_t* vc_strides, void* stream);
+
 /* ---------------------------------------------------------------- window attention */
 
 /*
@@ -518,6 +531,47 @@ int fta_cache_attn(const void* q, const int64_t* q_strides, const void* k_cache,
                    const int32_t* cache_lens, const void* k_prefix, const int64_t* kp_strides, const void* v_prefix,
                    const int64_t* vp_strides, int P, int left, int num_sinks, float scale, void* o,
                    const int64_t* o_strides, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- 4-bit caches */
+
+/*
+ * Keys and values in 4 bits (no counterpart in the reference).  A row is one head of one token,
+ * NG = ceil(D / 32) groups of 32 columns, the last one filled up with zeros.  A group has a
+ * float16 scale d and a code n = 0 .. 15 per column, which stands for d (n - 8).  Codes are
+ * [B][Hk][S][16 NG] bytes, eight to a little-endian 32-bit word: column 8 o + i of group g is bits
+ * 4 i .. 4 i + 3 of word 4 g + o of a value row, of word o NG + g of a key row.  Scales are
+ * [B][Hk][S][NG].  The rows of one head follow each other; strides are {stride_b, stride_h} in
+ * elements (bytes for codes), 16-byte steps for fta_q4_attn, fta_q4_read and fta_cache_weights.
+ *
+ * fta_qk_norm_rope_append_q4 is fta_qk_norm_rope_append_at into such a cache: d is the group's
+ * value of largest magnitude over -8 (the negative of two equal ones; rounded to float16, at most
+ * 65504 in magnitude), the code round(x / d) + 8, ties to even, held to 0 .. 15 (8 where d is 0).
+ * x is k as fta_qk_norm_rope_append writes it, rounded to its 16-bit type, and v.
+ */
+int fta_qk_norm_rope_append_q4(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, int dtype, int B, int H, int Hk, int T, int D,
+                               const void* q_weight, const void* k_weight, int weight_dtype, const float* cos,
+                               const float* sin, int P, int R, int position_offset, const int32_t* position_offsets,
+                               float eps, int interleaved, const int32_t* cache_lens, int S, void* q_out,
+                               const int64_t* qo_strides, void* k_codes, const int64_t* kc_strides, void* k_scales,
+                               const int64_t* ks_strides, void* v_codes, const int64_t* vc_strides, void* v_scales,
+                               const int64_t* vs_strides, void* stream);
+
+/* Every row of a 4-bit cache in 16 bits (dtype), rounded once: k, v [B][S][Hk][D] contiguous. */
+int fta_q4_read(const void* k_codes, const int64_t* kc_strides, const void* k_scales, const int64_t* ks_strides,
+                const void* v_codes, const int64_t* vc_strides, const void* v_scales, const int64_t* vs_strides, int dtype,
+                int B, int Hk, int S, int D, void* k, void* v, void* stream);
+
+/*
+ * fta_cache_attn (without a prefix) over a 4-bit cache: visibility, rows that see nothing, unseen
+ * rows and the workspace (fta_q4_attn_workspace_size bytes) as there.
+ */
+size_t fta_q4_attn_workspace_size(int B, int H, int Hk, int T, int S, int D, int left, int num_sinks);
+int fta_q4_attn(const void* q, const int64_t* q_strides, const void* k_codes, const int64_t* kc_strides, const void* k_scales,
+                const int64_t* ks_strides, const void* v_codes, const int64_t* vc_strides, const void* v_scales,
+                const int64_t* vs_strides, int dtype, int B, int H, int Hk, int T, int S, int D, const int32_t* cache_lens,
+                int left, int num_sinks, float scale, void* o, const int64_t* o_strides, float* lse, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
