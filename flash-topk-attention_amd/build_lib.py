@@ -21,7 +21,7 @@ HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
 
 SOURCES = ["fta_api.cpp", "fta_score.hip", "fta_index.hip", "fta_attn.hip", "fta_prep.hip", "fta_window.hip", "fta_cache.hip",
-           "fta_q4.hip"]
+           "fta_q4.hip", "fta_weights.hip", "fta_evict.hip"]
 
 # Packed fp32 VALU ops are disabled: hipcc -O3 would otherwise form
 # v_pk_{add,mul,fma}_f32 from ordinary float code.

@@ -169,8 +169,11 @@ __device__ __forceinline__ void load_angles(const PrepArgs& a, const LaneCols& c
 
 // Four bits of a row's values, this lane's eight columns of them: four lanes hold a group of 32,
 // whose value of largest magnitude over -8 is its scale d (rounded to float16; the negative of two
-// equal ones), and a value's code is round(x / d) + 8, ties to even, held to 0 .. 15.  x / d is
-// an IEEE division: a border between two codes falls where the quotient's formula says.
+// equal ones), and a value's code is round(x / d) + 8, ties to even, held to 0 .. 15.  x has at most 11
+// bits and d as many, so a quotient that is no border between two codes is 2^-12 or more from
+// the next, and the borders themselves are float32 numbers: x / d by a reciprocal and one
+// step of correction, which is right to less than 2^-20 and exact on them, gives the same codes
+// as an exact division.
 __device__ __forceinline__ uint32_t quant8(const float* x, uint16_t& scale) {
     float hi = x[0], lo = x[0];
 #pragma unroll
@@ -188,10 +191,15 @@ __device__ __forceinline__ uint32_t quant8(const float* x, uint16_t& scale) {
     scale = __builtin_bit_cast(uint16_t, h);
     const float d = (float)h;
     if (d == 0.f) return 0x88888888u;
-    uint32_t w = 0;
+    const float r = __builtin_amdgcn_rcpf(d);
+    float n[2] = {34952.f, 34952.f};  // 8 in each of four digits to base 16
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w |= (uint32_t)(int)fminf(fmaxf(rintf(x[e] / d) + 8.f, 0.f), 15.f) << (4 * e);
-    return w;
+    for (int e = 0; e < 8; ++e) {
+        const float q = x[e] * r;
+        const float y = fmaf(fmaf(-q, d, x[e]), r, q);
+        n[e >> 2] = fmaf(rintf(fminf(fmaxf(y, -8.f), 7.f)), (float)(1 << (4 * (e & 3))), n[e >> 2]);
+    }
+    return (uint32_t)n[0] | (uint32_t)n[1] << 16;
 }
 
 // ----------------------------------------------------------------------------
@@ -291,14 +299,14 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
                     }
                 }
                 const uint4 out = isv ? x[u] : pack8<DT>(y);
-                unpack8<DT>(out, y);
-                uint16_t scale;
-                const uint32_t w = quant8(y, scale);
                 if (row >= rows || u >= a.per) continue;
                 if (isq) {
                     if (c.live) store16<NT>(a.qo + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn + c.d0, out);
                     continue;
                 }
+                unpack8<DT>(out, y);
+                uint16_t scale;
+                const uint32_t w = quant8(y, scale);  // a row's lanes are here together
                 const int ng = (a.D + 31) >> 5, g = c.d0 >> 5, o = (c.d0 >> 3) & 3;
                 if (crow < 0 || g >= ng) continue;
                 const Q4Out& t = isv ? a.qv : a.qk;

@@ -483,9 +483,11 @@ int launch_q4_groups(Q4Args& A, hipStream_t st) {
     }
 }
 
-// 16-byte steps of the codes, and of the scales
-bool q4_aligned(const void* codes, const int64_t* cs, const void* scales, const int64_t* ss) {
-    return (((uintptr_t)codes | (uintptr_t)scales) & 15) == 0 && ((cs[0] | cs[1]) & 15) == 0 && ((ss[0] | ss[1]) & 7) == 0;
+// 16-byte steps of the codes; of the scales 4-byte steps where a row has an even number of them
+bool q4_aligned(const void* codes, const int64_t* cs, const void* scales, const int64_t* ss, int D) {
+    const int even = (D + 31) / 32 % 2 == 0;
+    return ((uintptr_t)codes & 15) == 0 && ((cs[0] | cs[1]) & 15) == 0 && ((uintptr_t)scales & (even ? 3 : 1)) == 0 &&
+           ((ss[0] | ss[1]) & even) == 0;
 }
 
 }  // namespace
@@ -516,8 +518,8 @@ int fta_q4_attn(const void* q, const int64_t* q_strides, const void* k_codes, co
     if (!fta::all_set(q, q_strides, k_codes, kc_strides, k_scales, ks_strides, v_codes, vc_strides, v_scales, vs_strides,
                       cache_lens, o, o_strides, lse))
         return fta::arg_error("q4_attn: a required pointer is null");
-    if (!q4_aligned(k_codes, kc_strides, k_scales, ks_strides) || !q4_aligned(v_codes, vc_strides, v_scales, vs_strides))
-        return fta::arg_error("q4_attn: the cache's heads must be 16-byte aligned");
+    if (!q4_aligned(k_codes, kc_strides, k_scales, ks_strides, D) || !q4_aligned(v_codes, vc_strides, v_scales, vs_strides, D))
+        return fta::arg_error("q4_attn: the heads' codes must be 16-byte aligned, their scales 4-byte");
     a.q = (const uint16_t*)q, a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sn = q_strides[2];
     A.kc = (const uint8_t*)k_codes, A.kc_sb = kc_strides[0], A.kc_sh = kc_strides[1];
     A.vc = (const uint8_t*)v_codes, A.vc_sb = vc_strides[0], A.vc_sh = vc_strides[1];
@@ -543,8 +545,8 @@ int fta_q4_read(const void* k_codes, const int64_t* kc_strides, const void* k_sc
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("q4_read: dtype must be bf16 or fp16");
     if (!fta::all_set(k_codes, kc_strides, k_scales, ks_strides, v_codes, vc_strides, v_scales, vs_strides, k, v))
         return fta::arg_error("q4_read: a required pointer is null");
-    if (!q4_aligned(k_codes, kc_strides, k_scales, ks_strides) || !q4_aligned(v_codes, vc_strides, v_scales, vs_strides))
-        return fta::arg_error("q4_read: the cache's heads must be 16-byte aligned");
+    if (!q4_aligned(k_codes, kc_strides, k_scales, ks_strides, D) || !q4_aligned(v_codes, vc_strides, v_scales, vs_strides, D))
+        return fta::arg_error("q4_read: the heads' codes must be 16-byte aligned, their scales 4-byte");
     Q4Read a = {};
     a.kc = (const uint8_t*)k_codes, a.kc_sb = kc_strides[0], a.kc_sh = kc_strides[1];
     a.vc = (const uint8_t*)v_codes, a.vc_sb = vc_strides[0], a.vc_sh = vc_strides[1];

@@ -1,0 +1,329 @@
+// How much attention each cached key received, added to a running sum:
+//   w[b][hk][j] += sum over new tokens t and the query heads of hk of exp(scale q_t . k_j - lse_t)
+// for the tokens that see key j (as in fta_cache_attn: the last T of len_b tokens, token t at
+// p = len_b - T + t sees j <= p with j >= p - left or j < sinks).  lse is the attention's own
+// log-sum, so nothing is normalised here.  T is 1 for a step of a serving batch and the prompt's
+// length for a prompt; keys are 16-bit rows or rows of a 4-bit cache (see fta_q4.hip).
+//
+// S = Q K^T with the keys as columns: a wave keeps 32 keys in registers, one to a lane and its
+// mirror, and walks over all the rows that see them, 32 at a time; a key's sum stays in its lane.
+// So a key is read once, no sum crosses lanes, and there are no atomics (the same bits every run).
+// The rows come through LDS, shared by the four waves: TT tokens x GG query heads of the group,
+// as many heads as it takes to fill 32 rows where there are few tokens.
+#include "fta_common.h"
+#include "fta_host.h"
+#include "fta_tile.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WeighArgs {
+    const uint16_t* q;
+    int64_t q_sb, q_sh, q_sn;
+    const uint8_t* k;  // 16-bit rows, or codes
+    int64_t k_sb, k_sh, k_sn;  // bytes
+    const uint16_t* ks;  // scales of 4-bit rows
+    int64_t ks_sb, ks_sh;
+    const float* lse;  // [B][H][T]
+    const int32_t* lens;
+    float* w;
+    int64_t w_sb, w_sh;
+    float* part;  // [part][B * Hk][S]
+    int B, T, H, Hk, G, S, Dreal, left, sinks;
+    int GG, TT, groups;  // query heads and tokens of 32 rows; head groups of a K/V head
+    int tiles, np, total;
+    float c;
+};
+
+constexpr int kWeighWaves = 4, kWeighKeys = 32 * kWeighWaves;
+
+// KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
+template <int DT, int KD, bool Q4>
+__global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache_weights_kernel(WeighArgs a) {
+    constexpr int QSEG = KD / 8, KS = KD / 16, NG = KD / 32, BLOCKS = QSEG / 2, TILE_B = 32 * QSEG * 16;
+    using SW = FtaSwz<QSEG>;
+    using E = Elem<DT>;
+    __shared__ __align__(1024) unsigned char sQ[2][TILE_B];
+    __shared__ __align__(16) float sL[2][32];  // -lse log2(e), -inf for rows that do not count
+    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wgi = fta_xcd_remap(blockIdx.x, a.total);
+    const int u = fta_scalar(wgi / a.np), sp = wgi - u * a.np;
+    const int bhk = fta_scalar(u / a.tiles), tile = u - bhk * a.tiles;  // the first keys, which most rows see, first
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
+    const int k_lo = kWeighKeys * tile, kt = k_lo + 32 * wave, key = kt + (lane & 31);
+    const int p0 = len - a.T;  // position of the first new token
+
+    // chunks [s0, s1) of the walk: token chunks that see any of the workgroup's keys, for each head group
+    int c_lo = 0, nct = 0;
+    if (k_lo < len) {
+        const int t_lo = max(0, k_lo - p0);
+        const int64_t far = (int64_t)min(k_lo + kWeighKeys, len) - 1 + a.left - p0;
+        const int t_hi = k_lo < a.sinks ? a.T - 1 : (int)min(far, (int64_t)a.T - 1);
+        c_lo = fta_scalar(t_lo / a.TT);
+        if (t_hi >= t_lo) nct = fta_scalar(t_hi / a.TT) + 1 - c_lo;
+    }
+    const int64_t all = (int64_t)nct * a.groups;
+    const int s0 = fta_scalar((int)(all * sp / a.np)), s1 = fta_scalar((int)(all * (sp + 1) / a.np));
+
+    float sum = 0.f;
+    if (s0 < s1) {
+        // this wave's keys as B operands
+        fta_frag kf[KS];
+        float ds[NG];  // 4-bit keys: the key's scales
+        const bool kok = key < a.S;
+        const int64_t krow = kok ? key : 0;
+        if constexpr (Q4) {
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
+            const uint16_t* sp_ = a.ks + b * a.ks_sb + hk * a.ks_sh + krow * NG;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                ds[g] = (float)__builtin_bit_cast(_Float16, sp_[g]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {  // octet 2 hf + m of the group: the first or second product's
+                    const uint32_t w = kp[(2 * hf + m) * NG + g];
+                    float n[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) n[e] = (float)((int)((w >> (4 * e)) & 15u) - 8);
+                    kf[2 * g + m] = 32 * g + 16 * hf + 8 * m < a.Dreal ? fta_pack_frag<DT>(n) : fta_frag{0u, 0u, 0u, 0u};
+                }
+            }
+        } else {
+            const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
+            FtaTile<DT, KD>::load_rows(kp, kok, a.Dreal, lane, kf);
+        }
+        const uint16_t* qp = a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
+        const float* lp = a.lse + ((int64_t)b * a.H + (int64_t)hk * a.G) * a.T;
+        // this lane's rows of a chunk: token and head within it, 16-byte slot
+        constexpr int MINE = (BLOCKS + kWeighWaves - 1) / kWeighWaves;
+        int tt[MINE], gg[MINE], col[MINE];
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            const int s = (i * kWeighWaves + wave) * 64 + lane, row = (s / QSEG) & 31;
+            const int j = SW::slot(row, s - (s / QSEG) * QSEG);
+            tt[i] = row / a.GG;
+            gg[i] = row - tt[i] * a.GG;
+            col[i] = j * 8 < a.Dreal ? j * 8 : 0;  // columns past D: they meet zero key columns
+        }
+        const int ltt = (lane & 31) / a.GG, lgg = (lane & 31) - ltt * a.GG;
+        const uint32_t ldq = fta_lds_addr(&sQ[0][0]);
+        float lv = 0.f;  // lse of the next chunk's row `lane` (wave 0)
+        auto issue = [&](int ct, int cg, int st) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int blk = i * kWeighWaves + wave;
+                if (blk >= BLOCKS) break;  // wave-uniform
+                const int64_t t = min(ct * a.TT + tt[i], a.T - 1), g = min(cg * a.GG + gg[i], a.G - 1);
+                fta_dma16_at(qp + t * a.q_sn + g * a.q_sh + col[i], ldq + st * TILE_B + blk * 1024);
+            }
+            if (wave == 0) {
+                const int t = ct * a.TT + ltt, g = cg * a.GG + lgg;
+                const bool ok = t < a.T && g < a.G && ltt < a.TT;
+                const float x = lp[ok ? (int64_t)g * a.T + t : 0];
+                lv = ok ? x : FTA_INF;
+            }
+        };
+        const uint32_t ro = ldq + (lane & 31) * QSEG * 16u;
+        auto frag = [&](int st, int slot) { return fta_lds_frag(ro + st * TILE_B + 16u * (slot ^ SW::x(lane & 31))); };
+        const int g0 = fta_scalar(s0 / nct);
+        int ct = c_lo + s0 - g0 * nct, cg = g0;
+        fta_wait_vmcnt<0>();  // the keys: the DMAs are invisible to the compiler's wait counting
+        issue(ct, cg, 0);
+        float run = 0.f;
+        int st = 0;
+        for (int s = s0; s < s1; ++s, st ^= 1) {
+            fta_wait_vmcnt<0>();
+            // a row that saw nothing (lse = -inf) gives nothing, as one that does not exist
+            if (wave == 0 && lane < 32) sL[st][lane] = (lv == -FTA_INF) ? -FTA_INF : -lv * kLog2e;
+            __syncthreads();  // this chunk visible; every wave is past the last one
+            const int c = ct;
+            if (++ct == c_lo + nct) {
+                ct = c_lo;
+                ++cg;
+            }
+            if (s + 1 < s1) issue(ct, cg, st ^ 1);
+            const int q_lo = p0 + c * a.TT, q_hi = min(q_lo + a.TT, len) - 1;  // positions of the chunk's tokens
+            if (q_hi < kt || (kt + 31 < q_lo - a.left && kt >= a.sinks)) continue;  // wave-uniform
+            f32x16 x;
+            if constexpr (Q4) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    f32x16 y;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                    y = fta_mma<DT>(frag(st, 4 * g + 2 * hf), kf[2 * g], y);
+                    y = fta_mma<DT>(frag(st, 4 * g + 2 * hf + 1), kf[2 * g + 1], y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = fmaf(ds[g], y[i], x[i]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) x = fta_mma<DT>(frag(st, 2 * ks + hf), kf[ks], x);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(&sL[st][c_row(i, lane)]);
+                x[i] = fta_exp2(fmaf(x[i], a.c, l.x));
+                x[i + 1] = fta_exp2(fmaf(x[i + 1], a.c, l.y));
+                x[i + 2] = fta_exp2(fmaf(x[i + 2], a.c, l.z));
+                x[i + 3] = fta_exp2(fmaf(x[i + 3], a.c, l.w));
+            }
+            if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
+                // the rows of the tokens that see this lane's key
+                const int64_t t_hi = key < a.sinks ? a.TT : min((int64_t)key + a.left - q_lo, (int64_t)a.TT);
+                const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
+                const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int r = c_row(i, lane);
+                    x[i] = (r >= rlo && r < rhi) ? x[i] : 0.f;
+                }
+            }
+            // sums of a chunk, of 64 chunks, of all: their rounding errors stay small on long walks
+            run += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) +
+                   (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+            if (((s - s0) & 63) == 63) {
+                sum += run;
+                run = 0.f;
+            }
+        }
+        sum += run;
+        sum += fta_xor32(sum);
+    }
+    if (lane >= 32) return;
+    if (a.np > 1) {
+        if (key < a.S) a.part[((int64_t)sp * a.B * a.Hk + bhk) * a.S + key] = sum;
+    } else if (key < len) {
+        a.w[b * a.w_sb + hk * a.w_sh + key] += sum;
+    }
+}
+
+__global__ __launch_bounds__(256) void fta_cache_weights_join_kernel(WeighArgs a) {
+    const int64_t n = (int64_t)a.B * a.Hk * a.S;
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (e >= n) return;
+    const int64_t bhk = e / a.S;
+    const int b = (int)(bhk / a.Hk), hk = (int)(bhk - (int64_t)b * a.Hk), j = (int)(e - bhk * a.S);
+    if (j >= min(max(a.lens[b], 0), a.S)) return;
+    float s = 0.f;
+    for (int p = 0; p < a.np; ++p) s += a.part[p * n + e];
+    a.w[b * a.w_sb + hk * a.w_sh + j] += s;
+}
+
+// ---------------------------------------------------------------------- host
+
+int weigh_plan(WeighArgs& a, int B, int H, int Hk, int T, int S, int D, int left, int sinks) {
+    if (B <= 0 || H <= 0 || Hk <= 0 || T <= 0 || S <= 0 || D <= 0) return fta::arg_error("cache_weights: dims must be positive");
+    if (H % Hk != 0) return fta::arg_error("cache_weights: num_heads must be a multiple of num_kv_heads");
+    if (D % 16 != 0 || D > 256) return fta::arg_error("cache_weights: D must be a multiple of 16 up to 256");
+    if (left < 0 || sinks < 0) return fta::arg_error("cache_weights: window and num_sinks must be non-negative");
+    if (S > (1 << 29) || T > (1 << 29) || H > (1 << 20))
+        return fta::unsupported("cache_weights: sizes past 2^29 tokens or 2^20 heads");
+    if (!fta::size_fits(B, T, H, D) || !fta::size_fits(B, S, Hk, D)) return fta::unsupported("cache_weights: 2^60 elements and more");
+    a = WeighArgs{};
+    a.B = B, a.T = T, a.H = H, a.Hk = Hk, a.G = H / Hk, a.S = S, a.Dreal = D;
+    a.left = std::min(left, S);
+    a.sinks = a.left >= S - 1 ? 0 : std::min(sinks, S);
+    a.GG = std::min(a.G, std::max(1, 32 / std::min(T, 32)));
+    a.TT = 32 / a.GG;
+    a.groups = (a.G + a.GG - 1) / a.GG;
+    a.tiles = (S + kWeighKeys - 1) / kWeighKeys;
+    const int64_t wgs = (int64_t)B * Hk * a.tiles;
+    // the longest walk, in chunks
+    const int64_t span = std::min<int64_t>(T, a.sinks > 0 ? T : (int64_t)a.left + kWeighKeys + 1);
+    const int64_t chunks = ((span + a.TT - 1) / a.TT + 1) * a.groups;
+    if (chunks > (1 << 30)) return fta::unsupported("cache_weights: too many rows");
+    a.np = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + wgs - 1) / wgs, chunks / 8));
+    const int64_t most = (1 << 24) - 1;
+    if (wgs * a.np > most || (int64_t)B * Hk * ((S + 255) / 256) > most)
+        return fta::unsupported("cache_weights: too many keys");
+    a.total = (int)(wgs * a.np);
+    return FTA_OK;
+}
+
+size_t weigh_bytes(const WeighArgs& a) { return a.np <= 1 ? 0 : fta::align_up((size_t)a.np * a.B * a.Hk * a.S * sizeof(float)); }
+
+template <int DT, int KD, bool Q4>
+int launch_weigh(const WeighArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((fta_cache_weights_kernel<DT, KD, Q4>), dim3((unsigned)a.total), dim3(kWeighWaves * 64), 0, st, a);
+    int rc = fta::check_launch("fta_cache_weights_kernel");
+    if (rc != FTA_OK || a.np <= 1) return rc;
+    const int64_t n = (int64_t)a.B * a.Hk * a.S;
+    hipLaunchKernelGGL(fta_cache_weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    return fta::check_launch("fta_cache_weights_join_kernel");
+}
+
+template <int DT>
+int launch_weigh_dims(const WeighArgs& a, bool q4, hipStream_t st) {
+    if (!q4) {
+        if (a.Dreal <= 64) return launch_weigh<DT, 64, false>(a, st);
+        if (a.Dreal <= 128) return launch_weigh<DT, 128, false>(a, st);
+        return launch_weigh<DT, 256, false>(a, st);
+    }
+    switch ((a.Dreal + 31) / 32) {
+        case 1: return launch_weigh<DT, 32, true>(a, st);
+        case 2: return launch_weigh<DT, 64, true>(a, st);
+        case 3: return launch_weigh<DT, 96, true>(a, st);
+        case 4: return launch_weigh<DT, 128, true>(a, st);
+        case 5: return launch_weigh<DT, 160, true>(a, st);
+        case 6: return launch_weigh<DT, 192, true>(a, st);
+        case 7: return launch_weigh<DT, 224, true>(a, st);
+        default: return launch_weigh<DT, 256, true>(a, st);
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fta_cache_weights_workspace_size(int B, int H, int Hk, int T, int S, int D, int left, int num_sinks) {
+    WeighArgs a;
+    if (weigh_plan(a, B, H, Hk, T, S, D, left, num_sinks) != FTA_OK) return 0;
+    return weigh_bytes(a);
+}
+
+int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* k_scales,
+                      const int64_t* ks_strides, int dtype, int B, int H, int Hk, int T, int S, int D,
+                      const int32_t* cache_lens, int left, int num_sinks, float scale, const float* lse, float* weights,
+                      const int64_t* w_strides, void* workspace, size_t workspace_bytes, void* stream) {
+    FTA_TRY_BEGIN
+    WeighArgs a;
+    int rc = weigh_plan(a, B, H, Hk, T, S, D, left, num_sinks);
+    if (rc != FTA_OK) return rc;
+    if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("cache_weights: dtype must be bf16 or fp16");
+    if (!(scale > 0.f) || scale > 2.0e38f)  // times log2(e) still finite
+        return fta::arg_error("cache_weights: scale must be positive and at most 2e38");
+    const size_t need = weigh_bytes(a);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fta::arg_error("cache_weights: workspace too small");
+    if (!fta::all_set(q, q_strides, k, k_strides, cache_lens, lse, weights, w_strides) || (k_scales != nullptr && ks_strides == nullptr))
+        return fta::arg_error("cache_weights: a required pointer is null");
+    const bool q4 = k_scales != nullptr;
+    a.q = (const uint16_t*)q, a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sn = q_strides[2];
+    a.k = (const uint8_t*)k;
+    if (q4) {
+        if ((((uintptr_t)k) & 15) != 0 || ((k_strides[0] | k_strides[1]) & 15) != 0)
+            return fta::arg_error("cache_weights: the heads' codes must be 16-byte aligned");
+        a.k_sb = k_strides[0], a.k_sh = k_strides[1], a.k_sn = (D + 31) / 32 * 16;
+        a.ks = (const uint16_t*)k_scales, a.ks_sb = ks_strides[0], a.ks_sh = ks_strides[1];
+    } else {
+        a.k_sb = 2 * k_strides[0], a.k_sh = 2 * k_strides[1], a.k_sn = 2 * k_strides[2];
+    }
+    a.lse = lse;
+    a.lens = cache_lens;
+    a.w = weights, a.w_sb = w_strides[0], a.w_sh = w_strides[1];
+    a.part = (float*)workspace;
+    a.c = scale * kLog2e;
+    hipStream_t st = (hipStream_t)stream;
+    return dtype == FTA_DTYPE_BF16 ? launch_weigh_dims<FTA_DTYPE_BF16>(a, q4, st) : launch_weigh_dims<FTA_DTYPE_F16>(a, q4, st);
+    FTA_TRY_END
+}
+
+}  // extern "C"

@@ -23,6 +23,7 @@ import torch.nn.functional as F
 from . import _lib
 from .block_score import _parse_block_score_args, _prepare_qk, flash_block_score
 from .cache_attn import flash_prefix_attn_decode
+from .cache_evict import flash_cache_evict, flash_cache_weights
 from .q4_cache import (
     Q4Cache,
     flash_q4_cache,
@@ -253,4 +254,6 @@ __all__ = [
     "flash_q4_cache_read",
     "flash_qk_norm_rope_append_q4",
     "flash_window_attn_decode_q4",
+    "flash_cache_weights",
+    "flash_cache_evict",
 ]

@@ -88,6 +88,10 @@ _SIGNATURES = {
     "fta_q4_attn_workspace_size": (_sz, [_i] * 8),
     "fta_q4_attn": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _f,
                          _p, _i64p, _p, _p, _sz, _p]),
+    "fta_cache_weights_workspace_size": (_sz, [_i] * 8),
+    "fta_cache_weights": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _i, _f, _p, _p, _i64p, _p,
+                               _sz, _p]),
+    "fta_cache_evict": (_i, [_i, _p, _i64p, _p, _i64p, _p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _i, _p, _p, _p, _p]),
     "fta_window_attn_fwd": (_i, [_p, _i64p, _p, _i64p, _p, _i64p, _i, _i, _i, _i, _i, _i, _p, _i, _i, _i, _f, _p,
                                  _i64p, _p, _p]),
     "fta_window_attn_bwd_workspace_size": (_sz, [_i] * 8),

@@ -28,7 +28,7 @@ class Q4Cache(NamedTuple):
 
     ``k_codes`` and ``v_codes`` are uint8 ``[B, num_kv_heads, S, 16 * groups]``,
     ``k_scales`` and ``v_scales`` float16 ``[B, num_kv_heads, S, groups]``; the rows of a
-    head follow each other, heads start at 16-byte steps.
+    head follow each other, the codes of heads start at 16-byte steps.
     """
 
     k_codes: torch.Tensor
@@ -43,10 +43,9 @@ def flash_q4_cache(batch: int, tokens: int, num_kv_heads: int, head_dim: int, de
     B, S, Hk, D = (_lib.whole(what, x) for x in (batch, tokens, num_kv_heads, head_dim))
     if min(B, S, Hk, D) <= 0 or D % 16 != 0 or D > 256:
         raise ValueError(f"{what}: sizes must be positive, head_dim a multiple of 16 up to 256")
-    groups, room = -(-D // 32), -(-S // 8) * 8  # eight rows of scales: 16-byte steps for any number of groups
-    made = (torch.zeros(B, Hk, room, n, device=device, dtype=t)[:, :, :S]
-            for n, t in ((16 * groups, torch.uint8), (groups, torch.float16)) * 2)
-    return Q4Cache(*made)
+    groups = -(-D // 32)
+    return Q4Cache(*(torch.zeros(B, Hk, S, n, device=device, dtype=t)
+                     for n, t in ((16 * groups, torch.uint8), (groups, torch.float16)) * 2))
 
 
 @lru_cache(maxsize=1024)
@@ -63,9 +62,9 @@ def _layout(what, shapes, strides, types, B, Hk, groups):
         if tuple(shape) != (B, Hk, S, w) or S == 0:
             raise ValueError(f"{what}: {name} must be {[B, Hk, 'S', w]}")
         sb, sh = stride[0] if B > 1 else 0, stride[1] if Hk > 1 else 0
-        step = 15 if name.endswith("codes") else 7
+        step = 15 if name.endswith("codes") else 1 - groups % 2  # bytes; elements, two where rows are read by pairs
         if (w > 1 and stride[3] != 1) or (S > 1 and stride[2] != w) or (sb | sh) & step:
-            raise ValueError(f"{what}: the rows of a head of {name} must follow each other, heads at 16-byte steps")
+            raise ValueError(f"{what}: the rows of a head of {name} must follow each other, heads at aligned steps")
         found.append(_lib.i64arr((sb, sh)))
     return S, tuple(found)
 
@@ -81,8 +80,8 @@ def q4_args(what, cache, B, Hk, D, device):
     args = []
     for t, st in zip(cache, strides):
         at = t.data_ptr()
-        if at & 15:
-            raise ValueError(f"{what}: the cache's tensors must be 16-byte aligned")
+        if at & (15 if t.dtype == torch.uint8 else 3):
+            raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte")
         args += (at, st)
     return S, args
 

@@ -541,7 +541,8 @@ int fta_cache_attn(const void* q, const int64_t* q_strides, const void* k_cache,
  * [B][Hk][S][16 NG] bytes, eight to a little-endian 32-bit word: column 8 o + i of group g is bits
  * 4 i .. 4 i + 3 of word 4 g + o of a value row, of word o NG + g of a key row.  Scales are
  * [B][Hk][S][NG].  The rows of one head follow each other; strides are {stride_b, stride_h} in
- * elements (bytes for codes), 16-byte steps for fta_q4_attn, fta_q4_read and fta_cache_weights.
+ * elements (bytes for codes).  fta_q4_attn and fta_q4_read take 16-byte steps of codes, and 4-byte
+ * steps of scales where NG is even.
  *
  * fta_qk_norm_rope_append_q4 is fta_qk_norm_rope_append_at into such a cache: d is the group's
  * value of largest magnitude over -8 (the negative of two equal ones; rounded to float16, at most
@@ -572,6 +573,38 @@ int fta_q4_attn(const void* q, const int64_t* q_strides, const void* k_codes, co
                 const int64_t* vs_strides, int dtype, int B, int H, int Hk, int T, int S, int D, const int32_t* cache_lens,
                 int left, int num_sinks, float scale, void* o, const int64_t* o_strides, float* lse, void* workspace,
                 size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- eviction */
+
+/*
+ * weights[b][hk][j] += sum over the T tokens and the H / Hk query heads of hk of
+ * exp(scale q . k_j - lse), for tokens that see key j as in fta_cache_attn, where j <
+ * cache_lens[b] (no counterpart in the reference).  k: 16-bit keys [B][S][Hk][D] strided, and
+ * k_scales null; or the key codes of a 4-bit cache ({stride_b, stride_h} in bytes) with their
+ * scales.  lse [B][H][T]; rows of -inf add nothing.  w_strides {b, head} in elements, rows
+ * follow each other.  No atomics; the workspace (fta_cache_weights_workspace_size bytes) holds
+ * the parts of split walks.
+ */
+size_t fta_cache_weights_workspace_size(int B, int H, int Hk, int T, int S, int D, int left, int num_sinks);
+int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* k_scales,
+                      const int64_t* ks_strides, int dtype, int B, int H, int Hk, int T, int S, int D,
+                      const int32_t* cache_lens, int left, int num_sinks, float scale, const float* lse, float* weights,
+                      const int64_t* w_strides, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Of the len = cache_lens[b] rows (clamped into [0, S]) of every request and K/V head keeps
+ * min(len, budget): the first num_sinks, the last `recent` and, of those between, the ones of
+ * largest weight (of equal ones the lower rows, NaN below every number), in their order, moved to
+ * the front.  `tensors` (1 to 4) arrays are moved and the weights; array i has rows of
+ * row_bytes[i] bytes (even, up to 512) at byte strides {b, head, row} 3 i .. 3 i + 2.  Either every
+ * dst is its src and weights_out is weights, or none (they must not overlap then).
+ * Behind the rows that stayed weights are set to zero: up to len in place, up to S_out otherwise.
+ * new_lens [B]; kept [B][Hk][budget]: the former row of each row, -1 behind them.
+ */
+int fta_cache_evict(int tensors, const void* const* src, const int64_t* src_strides, void* const* dst,
+                    const int64_t* dst_strides, const int32_t* row_bytes, const float* weights, const int64_t* w_strides,
+                    float* weights_out, const int64_t* wo_strides, int B, int Hk, int S, int S_out, int budget, int recent,
+                    int num_sinks, const int32_t* cache_lens, int32_t* new_lens, int32_t* kept, void* stream);
 
 #ifdef __cplusplus
 }

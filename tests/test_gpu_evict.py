@@ -1,0 +1,181 @@
+"""The attention that cached keys receive, and the eviction by it, against their definitions."""
+
+import math
+
+import pytest
+import torch
+
+import _operators_ref as R
+import _q4_ref as Q
+from _helpers import rand, say
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def _weights(q, keys, lse, lens, H, Hk, left, sinks, scale):
+    """``flash_cache_weights`` of keys [B, Hk, S, D] in float64.
+
+    Every term is off by at most F4 of it (the exponent's fp32 arithmetic; 4-bit keys the more of the
+    two kinds) and by the lse's own rounding; sums of n positive terms by n 2^-24 of the sum at most,
+    here in chunks of 32 rows, runs of 64 chunks and their sum.
+    """
+    B, T, C = q.shape
+    D, G, S, dev = C // H, H // Hk, keys.shape[2], q.device
+    w, tol = (torch.zeros(B, Hk, S, device=dev, dtype=torch.float64) for _ in range(2))
+    for b in range(B):
+        n = max(0, min(S, int(lens[b])))
+        if n == 0:
+            continue
+        see = R.window_mask(T, n, n - T, left, 0, sinks, dev)
+        for h in range(H):
+            s = (q[b].view(T, H, D)[:, h].double() @ keys[b, h // G, :n].T * scale).masked_fill(~see, -math.inf)
+            x = torch.exp(s - lse[b, h, :, None].double().masked_fill(lse[b, h, :, None] == -math.inf, math.inf))
+            w[b, h // G, :n] += x.sum(0)
+            tol[b, h // G, :n] += (x * (Q.F4 + 2.0 ** -22 * lse[b, h, :, None].double().abs().nan_to_num(posinf=0))).sum(0)
+    sums = (32 + 64 + T * G / 2048 + 16) * 2.0 ** -24
+    return w, tol + sums * w + T * G * R.FLUSH
+
+
+# dtype, B, T, H, Hk, D, S, left, sinks, lens
+WEIGHTS = [
+    (BF, 1, 1, 1, 1, 64, 1, 0, 0, [1]),
+    (BF, 4, 1, 8, 2, 128, 300, 20, 4, [300, 1, 0, 157]),
+    (FP, 3, 2, 4, 4, 64, 333, 100, 0, [333, 200, 64]),
+    (BF, 2, 1, 8, 1, 256, 700, 10000, 3, [700, 129]),
+    (FP, 2, 5, 16, 2, 80, 300, 31, 33, [3, 300]),       # fewer tokens than new ones
+    (BF, 1, 3, 12, 2, 128, 260, 255, 0, [259]),         # groups of six heads: 30 rows of 32
+    (FP, 2, 7, 33, 1, 96, 200, 200, 0, [200, 64]),      # 33 heads on one K/V head
+    (BF, 2, 100, 4, 2, 64, 100, 100, 0, [100, 60]),     # a prompt, padded batch
+    (BF, 1, 700, 8, 2, 128, 700, 700, 0, [700]),        # parts
+    (FP, 1, 700, 6, 2, 64, 700, 99, 10, [700]),         # with a window and sinks
+    (BF, 2, 33, 4, 4, 256, 500, 500, 0, [500, 40]),
+    (BF, 2, 1, 4, 2, 16, 50, 0, 0, [-4, 1000]),
+    (BF, 1, 20, 40, 1, 48, 129, 60, 2, [129]),
+    (FP, 1, 40, 4, 4, 160, 140, 140, 0, [140]),
+]
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+@pytest.mark.parametrize("case", WEIGHTS, ids=lambda c: "-".join(str(x) for x in c[1:9]))
+def test_weights(gpu, case, q4):
+    import flash_topk_attn_v2 as fta
+
+    dtype, B, T, H, Hk, D, S, left, sinks, lens = case
+    say("weights", case, q4)
+    q = rand((B, T, H * D), 3, dtype, gpu)
+    ln = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    if q4:
+        cache = Q.cache(B, S, Hk, D, gpu, 4)
+        keys = Q.values(cache.k_codes, cache.k_scales, True, D)[0]
+        _, lse = fta.flash_window_attn_decode_q4(q, cache, ln, H, left, sinks, num_kv_heads=Hk)
+    else:
+        cache = rand((B, S, Hk * D), 4, dtype, gpu)
+        keys = cache.view(B, S, Hk, D).transpose(1, 2).double()
+        _, lse = fta.flash_window_attn_decode(q, cache, cache, ln, H, left, sinks, num_kv_heads=Hk)
+    start = torch.rand(B, Hk, S, generator=torch.Generator().manual_seed(1)).to(gpu)
+    w = start.clone()
+    assert fta.flash_cache_weights(q, cache, lse, ln, w, H, left, sinks, num_kv_heads=Hk) is w
+    want, tol = _weights(q, keys, lse, lens, H, Hk, left, sinks, D ** -0.5)
+    assert ((w.double() - start.double() - want).abs() <= tol + 2.0 ** -23 * (w.double() + start.double())).all()
+    for b in range(B):  # rows behind the length
+        assert torch.equal(w[b, :, max(0, lens[b]):], start[b, :, max(0, lens[b]):])
+    # every token that sees something gives 1 per head, in all
+    live = (lse > -math.inf).sum((1, 2)).double()
+    assert ((want.sum((1, 2)) - live).abs() <= 1e-3 * live + 1e-12).all()
+
+
+def _evicted(w, n, budget, recent, sinks):
+    """Rows of one head that stay."""
+    if n <= budget:
+        return list(range(n))
+    val = [(math.isnan(x), 0.0 if math.isnan(x) else -x) for x in w.tolist()]  # NaN last
+    best = sorted(range(sinks, n - recent), key=lambda j: (val[j], j))[:budget - sinks - recent]
+    return sorted([*range(sinks), *best, *range(n - recent, n)])
+
+
+# B, Hk, D, S, budget, recent, sinks, lens
+EVICT = [
+    (1, 1, 64, 1, 1, 0, 0, [1]),
+    (2, 2, 64, 40, 10, 3, 2, [40, 9]),
+    (3, 2, 128, 300, 100, 0, 0, [300, 101, 0]),
+    (2, 3, 80, 257, 64, 64, 0, [257, 64]),              # recent rows alone
+    (2, 1, 16, 257, 64, 0, 64, [200, 65]),              # sinks alone
+    (1, 2, 256, 1030, 1029, 17, 4, [1030]),             # one row goes
+    (2, 2, 96, 700, 600, 30, 4, [5000, -3]),            # lengths outside the cache
+    (1, 2, 64, 9000, 2000, 100, 4, [8999]),             # more rows than a thread's eight
+    (1, 1, 32, 40000, 777, 10, 1, [39000]),             # more than its 32
+    (20, 8, 128, 500, 123, 20, 4, None),
+]
+
+
+@pytest.mark.parametrize("out", [False, True], ids=["in_place", "out"])
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+@pytest.mark.parametrize("case", EVICT, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_evict(gpu, case, q4, out):
+    import flash_topk_attn_v2 as fta
+
+    B, Hk, D, S, budget, recent, sinks, lens = case
+    say("evict", case, q4, out)
+    gen = torch.Generator().manual_seed(7)
+    if lens is None:
+        lens = torch.randint(0, S + 1, (B,), generator=gen).tolist()
+    w = torch.randn(B, Hk, S, generator=gen).exp()
+    w = torch.where(torch.rand(B, Hk, S, generator=gen) < 0.4, (w * 4).round() / 4, w)  # ties
+    w[torch.rand(B, Hk, S, generator=gen) < 0.1] = 0.0
+    w[:, 0, S // 3:S // 2] = 0.25                                                    # a run of equal ones
+    ln = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    if q4:
+        cache = Q.cache(B, S, Hk, D, gpu, 4)
+        rows = list(cache)
+    else:
+        cache = tuple(rand((B, S, Hk * D), 5 + i, BF, gpu) for i in (0, 1))
+        rows = [x.view(B, S, Hk, D).transpose(1, 2) for x in cache]
+    old = [x.clone() for x in rows]
+    wg = w.to(gpu)
+    to, to_rows, room = None, rows, S
+    if out:
+        room = budget + 5
+        if q4:
+            to = Q.cache(B, room, Hk, D, gpu, 9)
+            to_rows = list(to)
+        else:
+            to = tuple(rand((B, room, Hk * D), 9 + i, BF, gpu) for i in (0, 1))
+            to_rows = [x.view(B, room, Hk, D).transpose(1, 2) for x in to]
+        to = (to, torch.ones(B, Hk, room, device=gpu))
+    before = [x.clone() for x in to_rows]
+    new, kept = fta.flash_cache_evict(cache, wg, ln, budget, recent, sinks, out=to)
+    got_w = wg if to is None else to[1]
+    assert new.dtype == kept.dtype == torch.int32 and kept.shape == (B, Hk, budget)
+    for b in range(B):
+        n = max(0, min(S, lens[b]))
+        assert int(new[b]) == min(n, budget)
+        for h in range(Hk):
+            stay = _evicted(w[b, h], n, budget, recent, sinks)
+            m = len(stay)
+            assert kept[b, h, :m].tolist() == stay and (kept[b, h, m:] == -1).all()
+            at = torch.tensor(stay, dtype=torch.long, device=gpu)
+            for x, o, f in zip(to_rows, old, before):
+                assert torch.equal(x[b, h, :m], o[b, h, at]) and torch.equal(x[b, h, m:], f[b, h, m:])
+            want = w[b, h].to(gpu).clone() if to is None else torch.zeros(room, device=gpu)
+            if to is None:
+                want[m:n] = 0
+            want[:m] = w[b, h].to(gpu)[at]
+            assert torch.equal(got_w[b, h], want)
+    if out:  # the inputs are as they were
+        assert torch.equal(wg.cpu(), w) and all(torch.equal(x, o) for x, o in zip(rows, old))
+
+
+def test_evict_of_special_weights(gpu):
+    """NaN below everything, infinities, zeros of both signs, negative and subnormal numbers."""
+    import flash_topk_attn_v2 as fta
+
+    vals = [0.0, -0.0, math.nan, math.inf, -math.inf, -1.0, 1e-40, -1e-40, 1.0, 3.0e38, -math.nan, 2.0 ** -149]
+    S = 4 * len(vals)
+    w = torch.tensor(vals * 4)[None, None]
+    cache = tuple(rand((1, S, 16), i, BF, gpu) for i in (0, 1))
+    for budget in range(1, S, 5):
+        c = tuple(x.clone() for x in cache)
+        _, kept = fta.flash_cache_evict(c, w.to(gpu), torch.tensor([S], dtype=torch.int32, device=gpu), budget)
+        assert kept[0, 0].tolist() == _evicted(w[0, 0], S, budget, 0, 0)
