@@ -19,6 +19,7 @@
 // formed in fp32 and rounded once, when it is stored.
 #include "fta_common.h"
 #include "fta_host.h"
+#include "fta_tile.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -167,53 +168,16 @@ __device__ __forceinline__ void load_angles(const PrepArgs& a, const LaneCols& c
     }
 }
 
-// Four bits of a row's values, this lane's eight columns of them: four lanes hold a group of 32,
-// whose value of largest magnitude over -8 is its scale d (rounded to float16; the negative of two
-// equal ones), and a value's code is round(x / d) + 8, ties to even, held to 0 .. 15.  x has at most 11
-// bits and d as many, so a quotient that is no border between two codes is 2^-12 or more from
-// the next, and the borders themselves are float32 numbers: x / d by a reciprocal and one
-// step of correction, which is right to less than 2^-20 and exact on them, gives the same codes
-// as an exact division.
-__device__ __forceinline__ uint32_t quant8(const float* x, uint16_t& scale) {
-    float hi = x[0], lo = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; ++e) {
-        hi = fmaxf(hi, x[e]);
-        lo = fminf(lo, x[e]);
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-        lo = fminf(lo, __shfl_xor(lo, o, 64));
-    }
-    const float top = (-lo >= hi ? lo : hi) * -0.125f;
-    const _Float16 h = (_Float16)fminf(fmaxf(top, -65504.f), 65504.f);
-    scale = __builtin_bit_cast(uint16_t, h);
-    const float d = (float)h;
-    if (d == 0.f) return 0x88888888u;
-    const float r = __builtin_amdgcn_rcpf(d);
-    float n[2] = {34952.f, 34952.f};  // 8 in each of four digits to base 16
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float q = x[e] * r;
-        const float y = fmaf(fmaf(-q, d, x[e]), r, q);
-        n[e >> 2] = fmaf(rintf(fminf(fmaxf(y, -8.f), 7.f)), (float)(1 << (4 * (e & 3))), n[e >> 2]);
-    }
-    return (uint32_t)n[0] | (uint32_t)n[1] << 16;
-}
-
 // ----------------------------------------------------------------------------
 // Forward.  A wave strides over (token, part) pairs; a part is U groups of 64 / LG
 // rows of one token, whose loads are issued together and share the token's angles.
 // The weights (the lane's own and its partners') stay in registers.
 // APPEND: rows past the query and key heads copy V; K and V go to cache row
-// lens[b] - N + n (not written outside [0, S)).  Q4: into a 4-bit cache, K as its 16-bit values,
-// so that a cache holds the same whether or not it was written in one pass with the norm.
+// lens[b] - N + n (not written outside [0, S)).
 // ----------------------------------------------------------------------------
-template <int DT, int LG, int U, bool APPEND, bool NT, bool Q4 = false>
+template <int DT, int LG, int U, bool APPEND, bool NT>
 __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
     constexpr int RW = 64 / LG;
-    static_assert(!Q4 || (APPEND && LG >= 4), "a group of 32 columns within a row's lanes");
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const LaneCols c = lane_cols<LG>(a, lane);
@@ -272,49 +236,6 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
             for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
             const float r = rsqrtf(fmaf(row_sum<LG>(ss), inv_d, a.eps));
             const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
-            if constexpr (Q4) {
-                // every lane takes part: those behind D hold zeros, and write them behind D
-                const bool isv = row >= a.H + a.Hk;
-                if (!isv) {
-                    float g[8];
-                    unpack8<DT>(xp, g);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        f[e] *= r * (isq ? wq[e] : wk[e]);
-                        g[e] *= r * (isq ? pq[e] : pk[e]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        if (a.inter) {
-                            y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
-                            y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
-                        } else {
-                            y[e] = fmaf(g[e], sn[e], f[e] * cs[e]);
-                            y[e + 1] = fmaf(g[e + 1], sn[e + 1], f[e + 1] * cs[e + 1]);
-                        }
-                    }
-                    if (!c.live) {
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) y[e] = 0.f;
-                    }
-                }
-                const uint4 out = isv ? x[u] : pack8<DT>(y);
-                if (row >= rows || u >= a.per) continue;
-                if (isq) {
-                    if (c.live) store16<NT>(a.qo + b * a.qo_sb + row * a.qo_sh + n * a.qo_sn + c.d0, out);
-                    continue;
-                }
-                unpack8<DT>(out, y);
-                uint16_t scale;
-                const uint32_t w = quant8(y, scale);  // a row's lanes are here together
-                const int ng = (a.D + 31) >> 5, g = c.d0 >> 5, o = (c.d0 >> 3) & 3;
-                if (crow < 0 || g >= ng) continue;
-                const Q4Out& t = isv ? a.qv : a.qk;
-                const int hk = isv ? row - a.H - a.Hk : row - a.H;
-                t.codes[b * t.c_sb + hk * t.c_sh + (int64_t)crow * 4 * ng + (isv ? 4 * g + o : o * ng + g)] = w;
-                if (o == 0) t.scales[b * t.s_sb + hk * t.s_sh + (int64_t)crow * ng + g] = scale;
-                continue;
-            }
             if (!c.live || row >= rows || u >= a.per) continue;
             uint16_t* out;
             if (APPEND && row >= a.H + a.Hk) {
@@ -346,6 +267,209 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
                 out = a.ko + b * a.ko_sb + (row - a.H) * a.ko_sh + n * a.ko_sn;
             }
             store16<NT>(out + c.d0, pack8<DT>(y));
+        }
+    }
+}
+
+// ----------------------------------------------------------------------------
+// Append to a 4-bit cache: the forward's tiling, K and V quantized.  K is rounded to its 16-bit type
+// first, so that a cache holds the same whether its rows came prepared or not.  The groups of a part
+// are of one kind (queries, keys, values) but where the kinds meet, and each kind has its own body.
+// What bounds it: vector instructions, 190 a group of four rows and 69% of the cycles (32768 tokens, 32 / 8
+// heads of 128: 198 us, 708 MB).  One body for any row 227 us; held to four waves a SIMD 198, three 206;
+// through the caches 209; the queries by the forward's kernel and the rest by this one 121 + 84; one
+// group at a time with the next one asked for ahead 373.
+// ----------------------------------------------------------------------------
+
+// x of lane ^ 1, ^ 2, and of lanes that hold the other halves of 8 and of 16 (equal within 4 and 8).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xb1, kXor2 = 0x4e, kHalfMirror = 0x141, kMirror = 0x140;
+
+// row_sum without LDS: the same additions
+template <int LG>
+__device__ __forceinline__ float row_sum_dpp(float x) {
+    static_assert(LG >= 4, "");
+    x += dpp<kXor1>(x);
+    x += dpp<kXor2>(x);
+    if constexpr (LG >= 8) x += dpp<kHalfMirror>(x);
+    if constexpr (LG >= 16) x += dpp<kMirror>(x);
+    if constexpr (LG >= 32) x += __shfl_xor(x, 16, 64);
+    return x;
+}
+
+// Four bits of a row's values, this lane's eight columns of them: four lanes hold a group of 32,
+// whose value of largest magnitude over -8 is its scale d (rounded to float16; the negative of two
+// equal ones), and a value's code is round(x / d) + 8, ties to even, held to 0 .. 15.  x has at most 11
+// bits and d as many, so a quotient that is no border between two codes is 2^-12 or more from
+// the next, and the borders themselves are float32 numbers: x / d by a reciprocal and one
+// step of correction, which is right to less than 2^-20 and exact on them, gives the same codes
+// as an exact division.
+__device__ __forceinline__ uint32_t quant8(const float* x, uint16_t& scale) {
+    float hi = x[0], lo = x[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) {
+        hi = fmaxf(hi, x[e]);
+        lo = fminf(lo, x[e]);
+    }
+    hi = fmaxf(hi, dpp<kXor1>(hi));
+    lo = fminf(lo, dpp<kXor1>(lo));
+    hi = fmaxf(hi, dpp<kXor2>(hi));
+    lo = fminf(lo, dpp<kXor2>(lo));
+    const float top = (-lo >= hi ? lo : hi) * -0.125f;
+    const _Float16 h = (_Float16)fminf(fmaxf(top, -65504.f), 65504.f);
+    scale = __builtin_bit_cast(uint16_t, h);
+    const float d = (float)h;
+    if (d == 0.f) return 0x88888888u;
+    const float r = __builtin_amdgcn_rcpf(d);
+    float n[2] = {34952.f, 34952.f};  // 8 in each of four digits to base 16
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float q = x[e] * r;
+        const float y = fmaf(fmaf(-q, d, x[e]), r, q);
+        n[e >> 2] = fmaf(rintf(__builtin_amdgcn_fmed3f(y, -8.f, 7.f)), (float)(1 << (4 * (e & 3))), n[e >> 2]);
+    }
+    return (uint32_t)n[0] | (uint32_t)n[1] << 16;
+}
+
+template <int DT, int LG, int U, bool NT>
+__global__ __launch_bounds__(256, 4) void fta_norm_rope_append_q4_kernel(PrepArgs a) {
+    constexpr int RW = 64 / LG;
+    static_assert(LG >= 4, "a group of 32 columns within a row's lanes");
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const LaneCols c = lane_cols<LG>(a, lane);
+    const int rows = a.H + 2 * a.Hk, ng = (a.D + 31) >> 5;
+    const float inv_d = 1.f / (float)a.D;
+    float wq[8], wk[8], pq[8], pk[8];
+    {
+        const int d = c.live ? c.d0 : 0, dp = c.live ? (c.src & (LG - 1)) * 8 : 0;
+        load_w8(a.qw, a.w_dtype, d, wq);
+        load_w8(a.kw, a.w_dtype, d, wk);
+        load_w8(a.qw, a.w_dtype, dp, pq);
+        load_w8(a.kw, a.w_dtype, dp, pk);
+    }
+    const int oct = (c.d0 >> 3) & 3, grp = c.d0 >> 5;
+    // rows of neighbouring tokens share cache lines: an XCD takes neighbouring tokens
+    for (int64_t unit = (int64_t)fta_xcd_remap(blockIdx.x, gridDim.x) * 4 + wave; unit < a.units;
+         unit += (int64_t)gridDim.x * 4) {
+        int part, b, n;
+        if (a.units <= 0x7fffffff) {  // 64-bit divisions were a third of the scalar instructions
+            const uint32_t tok = (uint32_t)unit / (uint32_t)a.parts;
+            part = (int)((uint32_t)unit - tok * (uint32_t)a.parts);
+            b = (int)(tok / (uint32_t)a.N), n = (int)(tok - (uint32_t)b * (uint32_t)a.N);
+        } else {
+            const int64_t tok = unit / a.parts;
+            part = (int)(unit - tok * a.parts);
+            b = (int)(tok / a.N), n = (int)(tok - (int64_t)b * a.N);
+        }
+        part = fta_scalar(part), b = fta_scalar(b), n = fta_scalar(n);
+        const int first = part * a.per * RW;
+        const int64_t at = (int64_t)a.lens[b] - a.N + n;
+        const bool in = at >= 0 && at < a.S;  // wave-uniform
+        const int pos = (int)min(max(at + (a.pos_offs ? a.pos_offs[b] : a.pos_off), (int64_t)0), (int64_t)a.P - 1);
+        // the token's rows of each kind, and the cache's
+        const uint16_t* qp = a.q + b * a.q_sb + n * a.q_sn;
+        const uint16_t* kp = a.k + b * a.k_sb + n * a.k_sn;
+        const uint16_t* vp = a.v + b * a.v_sb + n * a.v_sn;
+        uint16_t* op = a.qo + b * a.qo_sb + n * a.qo_sn;
+        const int64_t crow = in ? at : 0;
+        uint32_t* kc = a.qk.codes + b * a.qk.c_sb + crow * 4 * ng;
+        uint32_t* vc = a.qv.codes + b * a.qv.c_sb + crow * 4 * ng;
+        uint16_t* ks = a.qk.scales + b * a.qk.s_sb + crow * ng;
+        uint16_t* vs = a.qv.scales + b * a.qv.s_sb + crow * ng;
+
+        uint4 x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int row = first + u * RW + lane / LG;
+            x[u] = fta_zero4();
+            const int lo = first + u * RW, hi = lo + RW - 1;  // wave-uniform
+            if (u >= a.per || lo >= rows) continue;
+            if (c.live && row < rows) {
+                const uint16_t* p;
+                if (hi < a.H)
+                    p = qp + row * a.q_sh;
+                else if (lo >= a.H && hi < a.H + a.Hk)
+                    p = kp + (row - a.H) * a.k_sh;
+                else if (lo >= a.H + a.Hk)
+                    p = vp + (row - a.H - a.Hk) * a.v_sh;
+                else
+                    p = row < a.H ? qp + row * a.q_sh : row < a.H + a.Hk ? kp + (row - a.H) * a.k_sh
+                                                                         : vp + (row - a.H - a.Hk) * a.v_sh;
+                x[u] = load16<NT>(p + c.d0);
+            }
+        }
+        float cs[8], sn[8];
+        load_angles(a, c, pos, cs, sn);
+        if (!a.inter) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sn[e] *= c.sgn;
+        }
+        // one group of rows.  KIND 0, 1, 2: queries, keys, values alone; 3: any of them
+        auto group = [&](auto kind, int u) __attribute__((always_inline)) {
+            constexpr int KIND = decltype(kind)::value;
+            const int row = first + u * RW + lane / LG;
+            const bool isq = KIND == 3 ? row < a.H : KIND == 0;
+            const bool isv = KIND == 3 ? row >= a.H + a.Hk : KIND == 2;
+            uint4 out = x[u];
+            if constexpr (KIND != 2) {
+                float f[8], g[8], y[8];
+                unpack8<DT>(x[u], f);
+                float ss = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) ss = fmaf(f[e], f[e], ss);
+                const float r = rsqrtf(fmaf(row_sum_dpp<LG>(ss), inv_d, a.eps));
+                const uint4 xp = a.inter ? x[u] : shfl4(x[u], c.src);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] *= r * (isq ? wq[e] : wk[e]);
+                if (a.inter) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
+                        y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
+                    }
+                } else {
+                    unpack8<DT>(xp, g);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) y[e] = fmaf(g[e] * (r * (isq ? pq[e] : pk[e])), sn[e], f[e] * cs[e]);
+                }
+                const uint4 turned = pack8<DT>(y);
+                if (KIND != 3 || !isv) out = turned;
+            }
+            if (row >= rows || u >= a.per) return;
+            if (KIND == 0 || (KIND == 3 && isq)) {
+                if (c.live) store16<NT>(op + row * a.qo_sh + c.d0, out);
+                return;
+            }
+            float y[8];
+            unpack8<DT>(out, y);  // columns behind D hold zeros
+            if (!c.live) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = 0.f;
+            }
+            uint16_t scale;
+            const uint32_t w = quant8(y, scale);  // a row's lanes are here together
+            if (!in || grp >= ng) return;
+            const int hk = row - a.H - (isv ? a.Hk : 0);
+            uint32_t* codes = isv ? vc + hk * a.qv.c_sh + 4 * grp + oct : kc + hk * a.qk.c_sh + oct * ng + grp;
+            *codes = w;
+            if (oct == 0) *(isv ? vs + hk * a.qv.s_sh + grp : ks + hk * a.qk.s_sh + grp) = scale;
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int lo = first + u * RW, hi = lo + RW - 1;  // wave-uniform
+            if (u >= a.per || lo >= rows) break;
+            if (hi < a.H)
+                group(std::integral_constant<int, 0>{}, u);
+            else if (lo >= a.H && hi < a.H + a.Hk)
+                group(std::integral_constant<int, 1>{}, u);
+            else if (lo >= a.H + a.Hk)
+                group(std::integral_constant<int, 2>{}, u);
+            else
+                group(std::integral_constant<int, 3>{}, u);
         }
     }
 }
@@ -588,10 +712,12 @@ int launch_append_q4(PrepArgs& a, int B, hipStream_t st) {
         if (!few) set_units(a, B, kFwdGroups, rows, LG);
         const dim3 g(grid_of(a.units, kFwdGrid)), t(256);
         if (few)
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, 1, true, false, true>), g, t, 0, st, a);
+            hipLaunchKernelGGL((fta_norm_rope_append_q4_kernel<DT, LG, 1, false>), g, t, 0, st, a);
+        else if (streams(a, B))
+            hipLaunchKernelGGL((fta_norm_rope_append_q4_kernel<DT, LG, kFwdGroups, true>), g, t, 0, st, a);
         else
-            hipLaunchKernelGGL((fta_norm_rope_fwd_kernel<DT, LG, kFwdGroups, true, false, true>), g, t, 0, st, a);
-        return fta::check_launch("fta_norm_rope_fwd_kernel");
+            hipLaunchKernelGGL((fta_norm_rope_append_q4_kernel<DT, LG, kFwdGroups, false>), g, t, 0, st, a);
+        return fta::check_launch("fta_norm_rope_append_q4_kernel");
     });
 }
 

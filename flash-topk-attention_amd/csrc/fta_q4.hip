@@ -71,13 +71,19 @@ __device__ __forceinline__ f32x4 mma16(fta_frag a, fta_frag b, f32x4 c) {
 // Eight codes as 16-bit numbers 16 + n: the code is the upper half of the mantissa of a number whose
 // exponent says 16.  Two codes take a shift and an and-or.  Pairs (0, 4), (1, 5), (2, 6), (3, 7).
 template <int DT>
-__device__ __forceinline__ fta_frag codes16(uint32_t w) {
+constexpr uint32_t kSixteen = DT == FTA_DTYPE_BF16 ? 0x41804180u : 0x4c004c00u;
+// A constant held in a vector register: an and-or takes one scalar operand, and has the mask for it.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+template <int DT>
+__device__ __forceinline__ fta_frag codes16(uint32_t w, uint32_t sixteen) {
     constexpr uint32_t mask = DT == FTA_DTYPE_BF16 ? 0x00780078u : 0x03c003c0u;
-    constexpr uint32_t one = DT == FTA_DTYPE_BF16 ? 0x41804180u : 0x4c004c00u;  // 16
     constexpr int up = DT == FTA_DTYPE_BF16 ? 3 : 6;
     fta_frag f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = ((up >= 4 * i ? w << (up - 4 * i) : w >> (4 * i - up)) & mask) | one;
+    for (int i = 0; i < 4; ++i) f[i] = ((up >= 4 * i ? w << (up - 4 * i) : w >> (4 * i - up)) & mask) | sixteen;
     return f;
 }
 // Eight 16-bit values in that order of pairs.
@@ -112,14 +118,17 @@ __device__ __forceinline__ float max_quarters(float x) {
 template <int NG>
 struct Q4Shape {
     static constexpr int NW = 4, KEYS = 64, ROWS = 16;
-    static constexpr int ROW_B = 16 * NG, V_B = KEYS * ROW_B, SC_B = KEYS * NG * 2;
-    static constexpr int STAGE_B = 2 * V_B + ((2 * SC_B + 1023) & ~1023);  // two tiles of value codes, one of either's scales
+    static constexpr int ROW_B = 16 * NG, TILE_B = KEYS * ROW_B, SC_B = 2 * KEYS * NG * 2;
+    static constexpr int STAGE_B = 2 * TILE_B + 2 * SC_B;  // a tile of key and of value codes, both's scales twice
     static constexpr int OROW = 32 * NG + 4;
-    static constexpr int MERGE_B = NW * ROWS * OROW * 4;
-    static constexpr int LDS_B = NW * STAGE_B > MERGE_B ? NW * STAGE_B : MERGE_B;
-    // The value rows' 16-byte slots are exchanged by row so that the transpose reads of 16 rows
-    // (one slot each) spread over the banks.
-    __device__ static __forceinline__ int slot(int row, int p) {
+    static constexpr int MERGE_B = NW * ROWS * OROW * 4, ML_B = NW * ROWS * 8;
+    static constexpr int LDS_B = NW * STAGE_B > MERGE_B + ML_B ? NW * STAGE_B : MERGE_B + ML_B;
+    // waves per SIMD that LDS and registers leave room for
+    static constexpr int WAVES = NG <= 2 ? 4 : NG <= 4 ? 3 : 2;
+    // A row's 16-byte slots are exchanged by row so that the reads of 16 rows (one slot each) spread
+    // over the banks: transpose reads take rows 16 q + e of the values, operand reads rows
+    // 16 a + 4 t + e (a, e = 0 .. 3) of the keys.
+    __device__ static __forceinline__ int vslot(int row, int p) {
         if constexpr (NG == 2 || NG == 6)
             return p ^ ((row >> 3) & 1);
         else if constexpr (NG == 4)
@@ -128,6 +137,16 @@ struct Q4Shape {
             return p ^ ((row >> 1) & 7);
         else
             return p;  // an odd number of slots spreads by itself
+    }
+    __device__ static __forceinline__ int kslot(int row, int p) {
+        if constexpr (NG == 2)
+            return p ^ ((row >> 4) & 1);
+        else if constexpr (NG == 4)
+            return p ^ ((row >> 4) & 3);
+        else if constexpr (NG == 8)
+            return p ^ (((row >> 1) & 1) | ((row >> 3) & 6));
+        else
+            return p;
     }
 };
 
@@ -138,18 +157,19 @@ struct Q4Shape {
 //   S^T = K Q^T: lane (r, q) = (l & 15, l >> 4) holds row r's scores of keys 16 q + 4 t + i
 //   (register i of product t; the key rows are handed to the products in that order), and so the
 //   16 keys whose value codes one transpose read gives lane (c, q) for its column c.
-// The codes enter as 16 + n; -24 sum_{c in g} q_c is the key products' first addend, and for the
-// values sum_j p_j d_jg is formed by one more product with a column of ones, from the same rounded
-// numbers, and taken 24 times from the result.
+// The codes enter as 16 + n; -24 sum_{c in g} q_c is the key products' first addend, and every value
+// product is followed by one of the same p d with -24 in every column.
 // bf16: p d is rounded to bf16 as P is in the 16-bit kernels.  fp16: it would leave fp16's range for
 // the scales that caches hold, so it goes as two bf16 numbers, hi + lo, 16 bits of it.
+// A wave has one stage for a tile's key codes and one for its value codes: the next tile's keys are
+// asked for before this one's values are multiplied, the next values after it.  Three waves per
+// SIMD cover the rest of the wait.
 // ----------------------------------------------------------------------------
 template <int DT, int NG>
-__global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_attn_kernel(Q4Args A) {
+__global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4Args A) {
     using Sh = Q4Shape<NG>;
-    constexpr int NW = Sh::NW, ROW_B = Sh::ROW_B, V_B = Sh::V_B, NS = (NG + 1) / 2;
+    constexpr int NW = Sh::NW, ROW_B = Sh::ROW_B, TILE_B = Sh::TILE_B, NS = (NG + 1) / 2;
     __shared__ __align__(1024) unsigned char sStage[Sh::LDS_B];
-    __shared__ float2 sML[NW][16];
     const CacheArgs& a = A.c;
     const int lane = threadIdx.x & 63, r16 = lane & 15, qt = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -171,11 +191,9 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
     const int all = max(ns + c_hi - c_lo, 0);
     const int it0 = fta_scalar((int)((int64_t)all * sp / a.ns)), it1 = fta_scalar((int)((int64_t)all * (sp + 1) / a.ns));
 
-    f32x4 oacc[2 * NG], wacc[NG];
+    f32x4 oacc[2 * NG];
 #pragma unroll
     for (int i = 0; i < 2 * NG; ++i) oacc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int g = 0; g < NG; ++g) wacc[g] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m_run = -FTA_INF, l_run = 0.f;
 
     if (it0 + wave < it1) {  // wave-uniform
@@ -184,9 +202,8 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
         const uint16_t* ks = A.ks + b * A.ks_sb + hk * A.ks_sh;
         const uint16_t* vs = A.vs + b * A.vs_sb + hk * A.vs_sh;
         unsigned char* stage = sStage + wave * Sh::STAGE_B;
-        uint16_t* sks = reinterpret_cast<uint16_t*>(stage + 2 * V_B);  // [64][NG]
-        uint16_t* svs = sks + 64 * NG;
-        const uint32_t lds0 = fta_lds_addr(stage);
+        uint16_t* sc0 = reinterpret_cast<uint16_t*>(stage + 2 * TILE_B);  // [tile parity][keys, values][NG][64]
+        const uint32_t ldk = fta_lds_addr(stage), ldv = ldk + TILE_B;
 
         fta_frag qf[NG];
         f32x4 first[NG];  // -24 sum q over the group, the key products' first addend
@@ -204,82 +221,95 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
                 qf[g] = paired(x);
             }
         }
-        struct Regs {
-            Words<NG> k[4];
-            Words<NS> ks, vs;
-        };
         auto key = [&](int it) { return 64 * (it < ns ? it : c_lo + it - ns); };
-        const int krow = 16 * (r16 >> 2) + (r16 & 3);  // key of product 0's row r16; 4 t further for product t
-        const uint32_t koff = krow * ROW_B + qt * 4 * NG;
-        uint32_t voff[NG];
+        auto whole = [&](int kb) { return kb + 64 <= ke && (kb >= kb0 || kb + 64 <= a.sinks); };
+        // keys that no row sees are taken from one that is seen (masked)
+        auto seen = [&](int t) -> int64_t { return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t; };
+        uint32_t koff[NG], voff[NG];  // of this lane's 16 bytes of a tile
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            const int s = i * 64 + lane, row = s / NG;
-            voff[i] = row * ROW_B + Sh::slot(row, s - row * NG) * 16;
+            const int s = i * 64 + lane, row = s / NG, p = s - row * NG;
+            koff[i] = row * ROW_B + Sh::kslot(row, p) * 16;
+            voff[i] = row * ROW_B + Sh::vslot(row, p) * 16;
         }
-        auto issue = [&](int it, Regs& x, int st) __attribute__((always_inline)) {
-            const int kb = key(it);
-            const uint32_t lds = lds0 + st * V_B;
-            if (kb + 64 <= ke && (kb >= kb0 || kb + 64 <= a.sinks)) {
-                const uint8_t* kt = kc + (int64_t)kb * ROW_B;
-                const uint8_t* vt = vc + (int64_t)kb * ROW_B;
+        auto codes = [&](const uint8_t* base, const uint32_t* off, int kb, uint32_t lds) __attribute__((always_inline)) {
+            if (whole(kb)) {
+                const uint8_t* tile = base + (int64_t)kb * ROW_B;
 #pragma unroll
-                for (int i = 0; i < NG; ++i) fta_dma16_so(vt, voff[i], lds + i * 1024);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) x.k[t] = load_words<NG>(kt + koff + t * 4 * ROW_B);
-                x.ks = load_scales<NG>(ks + (int64_t)kb * NG + lane * NG);
-                x.vs = load_scales<NG>(vs + (int64_t)kb * NG + lane * NG);
-            } else {  // keys that no row sees are taken from one that is seen (masked)
-                auto seen = [&](int t) -> int64_t { return t >= ke ? ke - 1 : (t < kb0 && t >= a.sinks) ? kb0 : t; };
+                for (int i = 0; i < NG; ++i) fta_dma16_so(tile, off[i], lds + i * 1024);
+            } else {
 #pragma unroll
                 for (int i = 0; i < NG; ++i) {
                     const int row = (i * 64 + lane) / NG;
-                    fta_dma16_at(vc + seen(kb + row) * ROW_B + (voff[i] - row * ROW_B), lds + i * 1024);
+                    fta_dma16_at(base + seen(kb + row) * ROW_B + (off[i] - row * ROW_B), lds + i * 1024);
                 }
-#pragma unroll
-                for (int t = 0; t < 4; ++t) x.k[t] = load_words<NG>(kc + seen(kb + krow + 4 * t) * ROW_B + qt * 4 * NG);
-                const int64_t row = seen(kb + lane);
-                x.ks = load_scales<NG>(ks + row * NG);
-                x.vs = load_scales<NG>(vs + row * NG);
             }
         };
-        const uint32_t vrow = lds0 + (16 * qt + r16) * ROW_B;
-        const fta_frag ones = fta_frag{0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16
+        struct Scales {
+            Words<NS> k, v;
+        };
+        auto scales = [&](int kb) __attribute__((always_inline)) {  // of key kb + lane
+            const int64_t row = whole(kb) ? kb + lane : seen(kb + lane);
+            return Scales{load_scales<NG>(ks + row * NG), load_scales<NG>(vs + row * NG)};
+        };
+        auto put_scales = [&](const Scales& x, uint16_t* sc) __attribute__((always_inline)) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                sc[64 * g + lane] = (uint16_t)(x.k.w[g / 2] >> (16 * (g & 1)));
+                sc[64 * (NG + g) + lane] = (uint16_t)(x.v.w[g / 2] >> (16 * (g & 1)));
+            }
+        };
+        // this lane's key words: row 16 (r16 >> 2) + 4 t + (r16 & 3) of product t, its words qt NG ..
+        const int krow = 16 * (r16 >> 2) + (r16 & 3);
+        auto key_words = [&](int t) __attribute__((always_inline)) {
+            const unsigned char* row = stage + (krow + 4 * t) * ROW_B;
+            Words<NG> x;
+            if constexpr (NG == 8) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    __builtin_memcpy(&x.w[4 * h], __builtin_assume_aligned(row + Sh::kslot(krow + 4 * t, 2 * qt + h) * 16, 16), 16);
+            } else if constexpr (NG == 4) {
+                __builtin_memcpy(&x, __builtin_assume_aligned(row + Sh::kslot(krow + 4 * t, qt) * 16, 16), 16);
+            } else if constexpr (NG == 2) {
+                __builtin_memcpy(&x, __builtin_assume_aligned(row + Sh::kslot(krow + 4 * t, qt >> 1) * 16 + 8 * (qt & 1), 8), 8);
+            } else {
+                __builtin_memcpy(&x, __builtin_assume_aligned(row + qt * 4 * NG, 4), 4 * NG);
+            }
+            return x;
+        };
+        const uint32_t vrow = ldv + (16 * qt + r16) * ROW_B;
+        const uint32_t sixteen_k = in_vgpr(kSixteen<DT>), sixteen_v = in_vgpr(kSixteen<FTA_DTYPE_BF16>);
+        const float zero = __builtin_bit_cast(float, in_vgpr(0u));  // products of fp16 and fp32 numbers are one instruction as multiply-adds
+        const fta_frag less24 = fta_frag{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};  // bf16
 
-        auto tile = [&](int it, Regs& cur, Regs& nxt, int st) __attribute__((always_inline)) {
-            // this tile's codes and scales are there, and every LDS read of the last tile has returned
-            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+        fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
+        int it = it0 + wave, kb = key(it);
+        Scales sreg = scales(kb);
+        codes(kc, koff, kb, ldk);
+        codes(vc, voff, kb, ldv);
+        put_scales(sreg, sc0);
+        if (it + NW < it1) sreg = scales(key(it + NW));
+        fta_wait_vmcnt<0>();
+        int odd = 0;
+        while (true) {
+            fta_wait_vmcnt<NG>();  // the key codes are there; the last NG, the value codes, may be on their way
             __builtin_amdgcn_sched_barrier(0);
             asm volatile("" ::: "memory");
-            if constexpr (NG % 2 == 0) {
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    reinterpret_cast<uint32_t*>(sks)[lane * NS + i] = cur.ks.w[i];
-                    reinterpret_cast<uint32_t*>(svs)[lane * NS + i] = cur.vs.w[i];
-                }
-            } else {
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    sks[lane * NG + g] = (uint16_t)(cur.ks.w[g / 2] >> (16 * (g & 1)));
-                    svs[lane * NG + g] = (uint16_t)(cur.vs.w[g / 2] >> (16 * (g & 1)));
-                }
-            }
-            if (it + NW < it1) issue(it + NW, nxt, st ^ 1);
-            __builtin_amdgcn_wave_barrier();
-            const int kb = key(it);
+            const uint16_t* sks = sc0 + odd * (Sh::SC_B / 2);
+            const uint16_t* svs = sks + 64 * NG;
             f32x4 s[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) {
-                Words<2 * NG> sc;  // scales of keys 16 qt + 4 t + i, group g: element i NG + g
-                __builtin_memcpy(&sc, __builtin_assume_aligned(sks + (16 * qt + 4 * t) * NG, 8), 8 * NG);
+                const Words<NG> kw = key_words(t);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[t][i] = zero;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const f32x4 x = mma16<DT>(codes16<DT>(cur.k[t].w[g]), qf[g], first[g]);
+                    const f32x4 x = mma16<DT>(codes16<DT>(kw.w[g], sixteen_k), qf[g], first[g]);
+                    Words<2> d;  // scales of keys 16 qt + 4 t + i
+                    __builtin_memcpy(&d, __builtin_assume_aligned(sks + 64 * g + 16 * qt + 4 * t, 8), 8);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float d = half_of(sc.w[(i * NG + g) >> 1], (i * NG + g) & 1);
-                        s[t][i] = g == 0 ? d * x[i] : fmaf(d, x[i], s[t][i]);
-                    }
+                    for (int i = 0; i < 4; ++i) s[t][i] = fmaf(half_of(d.w[i >> 1], i & 1), x[i], s[t][i]);
                 }
             }
             if (!(kb + 63 <= p0 && (kb >= p1 - a.left || kb + 63 < a.sinks))) {  // (rows past R are never written)
@@ -300,10 +330,6 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
                 for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) oacc[i][e] *= alpha;
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wacc[g][e] *= alpha;
                 l_run *= alpha;
                 if (grow) m_run = mn;
             }
@@ -315,21 +341,29 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
                     s[t][i] = fta_exp2(fmaf(s[t][i], a.c, -mc));
                     l_run += s[t][i];
                 }
-            // the scales of the lane's 16 keys: of keys 16 qt + 4 t + i, group g at element i NG + g of sc[t]
-            Words<2 * NG> sc[4];
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                __builtin_memcpy(&sc[t], __builtin_assume_aligned(svs + (16 * qt + 4 * t) * NG, 8), 8 * NG);
+            // the value codes and the next tile's scales are there, and every read of the key codes has returned
+            const bool more = it + NW < it1;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0x0070);  // vmcnt(0) lgkmcnt(0)
+            asm volatile("" ::: "memory");
+            const int kn = key(it + NW);
+            if (more) {
+                put_scales(sreg, sc0 + (odd ^ 1) * (Sh::SC_B / 2));
+                if (it + 2 * NW < it1) sreg = scales(key(it + 2 * NW));
+                codes(kc, koff, kn, ldk);
+            }
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
+                Words<8> d;  // scales of the lane's keys 16 qt + 4 t + i
+                __builtin_memcpy(&d, __builtin_assume_aligned(svs + 64 * g + 16 * qt, 16), 32);
                 fta_frag hi[2], lo[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int e = i * NG + g;
-                        const float x = s[2 * h][i] * half_of(sc[2 * h].w[e >> 1], e & 1);
-                        const float y = s[2 * h + 1][i] * half_of(sc[2 * h + 1].w[e >> 1], e & 1);
+                        const float x = fmaf(half_of(d.w[4 * h + (i >> 1)], i & 1), s[2 * h][i], zero);
+                        const float y = fmaf(half_of(d.w[4 * h + 2 + (i >> 1)], i & 1), s[2 * h + 1][i], zero);
                         hi[h][i] = Elem<FTA_DTYPE_BF16>::pack2(x, y);
                         if constexpr (DT == FTA_DTYPE_F16)
                             lo[h][i] = Elem<FTA_DTYPE_BF16>::pack2(x - __builtin_bit_cast(float, hi[h][i] << 16),
@@ -338,28 +372,29 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
 #pragma unroll
                 for (int ct = 0; ct < 2; ++ct) {  // 16 columns
                     typedef int v2i __attribute__((ext_vector_type(2)));
-                    const uint32_t at = vrow + st * V_B + Sh::slot(16 * qt + r16, g) * 16 + 8 * ct;
+                    const uint32_t at = vrow + Sh::vslot(16 * qt + r16, g) * 16 + 8 * ct;
                     const v2i w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) v2i*)at);
+                    f32x4& o = oacc[2 * g + ct];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const fta_frag v = codes16<FTA_DTYPE_BF16>((uint32_t)w[h]);
-                        oacc[2 * g + ct] = mma16<FTA_DTYPE_BF16>(v, hi[h], oacc[2 * g + ct]);
-                        if constexpr (DT == FTA_DTYPE_F16) oacc[2 * g + ct] = mma16<FTA_DTYPE_BF16>(v, lo[h], oacc[2 * g + ct]);
+                        const fta_frag v = codes16<FTA_DTYPE_BF16>((uint32_t)w[h], sixteen_v);
+                        o = mma16<FTA_DTYPE_BF16>(v, hi[h], o);
+                        o = mma16<FTA_DTYPE_BF16>(less24, hi[h], o);
+                        if constexpr (DT == FTA_DTYPE_F16) {
+                            o = mma16<FTA_DTYPE_BF16>(v, lo[h], o);
+                            o = mma16<FTA_DTYPE_BF16>(less24, lo[h], o);
+                        }
                     }
                 }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    wacc[g] = mma16<FTA_DTYPE_BF16>(ones, hi[h], wacc[g]);
-                    if constexpr (DT == FTA_DTYPE_F16) wacc[g] = mma16<FTA_DTYPE_BF16>(ones, lo[h], wacc[g]);
-                }
             }
-        };
-        Regs x0, x1;
-        fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
-        issue(it0 + wave, x0, 0);
-        for (int it = it0 + wave; it < it1; it += 2 * NW) {
-            tile(it, x0, x1, 0);
-            if (it + NW < it1) tile(it + NW, x1, x0, 1);
+            if (!more) break;
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): every read of the value codes has returned
+            asm volatile("" ::: "memory");
+            codes(vc, voff, kn, ldv);
+            kb = kn;
+            it += NW;
+            odd ^= 1;
         }
     }
 
@@ -367,16 +402,14 @@ __global__ __launch_bounds__(256, NG <= 2 ? 3 : NG <= 4 ? 2 : 1) void fta_q4_att
     const float L = sum_quarters(l_run);
     __syncthreads();
     float* so = reinterpret_cast<float*>(sStage);
-    if (lane < 16) sML[wave][lane] = make_float2(m_run, L);
+    float2* sml = reinterpret_cast<float2*>(sStage + Sh::MERGE_B);
+    if (lane < 16) sml[wave * 16 + lane] = make_float2(m_run, L);
 #pragma unroll
-    for (int i = 0; i < 2 * NG; ++i) {
-        const f32x4 w = wacc[i >> 1];
+    for (int i = 0; i < 2 * NG; ++i)
         *reinterpret_cast<float4*>(so + (wave * 16 + r16) * Sh::OROW + 16 * i + 4 * qt) =
-            make_float4(fmaf(-24.f, w[0], oacc[i][0]), fmaf(-24.f, w[1], oacc[i][1]), fmaf(-24.f, w[2], oacc[i][2]),
-                        fmaf(-24.f, w[3], oacc[i][3]));
-    }
+            make_float4(oacc[i][0], oacc[i][1], oacc[i][2], oacc[i][3]);
     __syncthreads();
-    cache_merge<DT, 32 * NG, (NG <= 2 ? 64 : NG <= 4 ? 128 : 256), 16, Sh::OROW, NW>(a, bhk, b, hk, r_lo, r_n, sp, so, &sML[0][0]);
+    cache_merge<DT, 32 * NG, (NG <= 2 ? 64 : NG <= 4 ? 128 : 256), 16, Sh::OROW, NW>(a, bhk, b, hk, r_lo, r_n, sp, so, sml);
 }
 
 // ----------------------------------------------------------------------------
@@ -450,7 +483,14 @@ int q4_plan(CacheArgs& a, int B, int H, int Hk, int T, int S, int D, int left, i
     const int64_t wgs = (int64_t)B * Hk * a.row_tiles;
     const int64_t span = std::min<int64_t>(S, (int64_t)a.left + T + a.sinks);
     const int64_t tiles = (span + 63) / 64;
-    a.ns = (int)std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, tiles / 4));
+    // At least 512 workgroups, down to a tile for each wave and part; and about 2048, where a wave still
+    // has eight tiles of its own: three workgroups of 128 columns fit a CU, and 768 at a time leave a
+    // long tail of a call of, say, 1024.  Target 512 / 1024 / 2048 / 4096, us of both kernels, 32 / 8 heads of
+    // 128, 4096 to 8192 tokens: 8 requests 24 / 26 / 30 / 29, 64 requests 100 / 117 / 104 / 109, 100 requests 168 /
+    // 156 / 150 / 154, 128 requests 218 / 212 / 189 / 185; 64 requests of 2048 to 4096, 16 / 4 heads of 256 118 /
+    // 131 / 157 / 197.
+    auto parts = [&](int64_t target, int64_t least) { return std::min<int64_t>((target + wgs - 1) / wgs, tiles / least); };
+    a.ns = (int)std::max<int64_t>(1, std::max(parts(512, 4), parts(2048, 32)));
     // workgroups of 256 threads: fewer than 2^32 threads a launch
     const int64_t most = (1 << 24) - 1;
     if (a.rows > most || wgs * a.ns > most) return fta::unsupported("q4_attn: too many rows");

@@ -73,17 +73,16 @@ def q4_args(what, cache, B, Hk, D, device):
     """``(S, address and strides of the four tensors)`` of a ``Q4Cache``, checked."""
     if not isinstance(cache, Q4Cache):
         raise ValueError(f"{what}: cache must be a Q4Cache")
-    S, strides = _layout(what, tuple(t.shape for t in cache), tuple(t.stride() for t in cache),
-                         tuple(t.dtype for t in cache), B, Hk, -(-D // 32))
-    _lib.check_device(what, device, *cache)
-    _lib.no_grad_inputs(what, cache.k_scales, cache.v_scales)
-    args = []
-    for t, st in zip(cache, strides):
-        at = t.data_ptr()
-        if at & (15 if t.dtype == torch.uint8 else 3):
-            raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte")
-        args += (at, st)
-    return S, args
+    kc, ks, vc, vs = cache
+    S, (kcs, kss, vcs, vss) = _layout(what, (kc.shape, ks.shape, vc.shape, vs.shape),
+                                      (kc.stride(), ks.stride(), vc.stride(), vs.stride()),
+                                      (kc.dtype, ks.dtype, vc.dtype, vs.dtype), B, Hk, -(-D // 32))
+    _lib.check_device(what, device, kc, ks, vc, vs)
+    _lib.no_grad_inputs(what, ks, vs)
+    kca, ksa, vca, vsa = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
+    if (kca | vca) & 15 or (ksa | vsa) & 3:
+        raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte")
+    return S, (kca, kcs, ksa, kss, vca, vcs, vsa, vss)
 
 
 @lru_cache(maxsize=1024)

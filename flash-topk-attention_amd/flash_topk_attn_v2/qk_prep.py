@@ -69,7 +69,7 @@ def _warn_of_short_tables(what, P, S, offset):
     once per geometry."""
     if offset < 0 or S + offset > P:
         warnings.warn(f"{what}: cos and sin have rows for positions 0 .. {P - 1}, rows of the cache stand at {offset} .. "
-                      f"{S + offset - 1}: tokens outside the tables are turned as the nearest row", stacklevel=3)
+                      f"{S + offset - 1}: tokens outside the tables are turned as the nearest row", stacklevel=4)
 
 
 def offsets(what, position_offset, B, device, P, S):
