@@ -17,6 +17,7 @@
 //   o_c = sum_j (p_j d_jg) (n_jc - 8)               for c in group g,
 // so that what 4 bits hold is multiplied without a further rounding, but for that of p d.
 #include "fta_cache.h"
+#include "fta_q4.h"
 #include "fta_tile.h"
 
 #include <algorithm>
@@ -56,63 +57,6 @@ __device__ __forceinline__ Words<(NG + 1) / 2> load_scales(const uint16_t* p) {
 }
 __device__ __forceinline__ float half_of(uint32_t w, int hi) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(hi ? w >> 16 : w & 0xffffu));
-}
-
-template <int DT>
-__device__ __forceinline__ f32x4 mma16(fta_frag a, fta_frag b, f32x4 c) {
-    if constexpr (DT == FTA_DTYPE_BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(fta_bf16x8, a), __builtin_bit_cast(fta_bf16x8, b), c,
-                                                       0, 0, 0);
-    else
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(fta_f16x8, a), __builtin_bit_cast(fta_f16x8, b), c, 0,
-                                                      0, 0);
-}
-
-// Eight codes as 16-bit numbers 16 + n: the code is the upper half of the mantissa of a number whose
-// exponent says 16.  Two codes take a shift and an and-or.  Pairs (0, 4), (1, 5), (2, 6), (3, 7).
-template <int DT>
-constexpr uint32_t kSixteen = DT == FTA_DTYPE_BF16 ? 0x41804180u : 0x4c004c00u;
-// A constant held in a vector register: an and-or takes one scalar operand, and has the mask for it.
-__device__ __forceinline__ uint32_t in_vgpr(uint32_t x) {
-    asm volatile("" : "+v"(x));
-    return x;
-}
-template <int DT>
-__device__ __forceinline__ fta_frag codes16(uint32_t w, uint32_t sixteen) {
-    constexpr uint32_t mask = DT == FTA_DTYPE_BF16 ? 0x00780078u : 0x03c003c0u;
-    constexpr int up = DT == FTA_DTYPE_BF16 ? 3 : 6;
-    fta_frag f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = ((up >= 4 * i ? w << (up - 4 * i) : w >> (4 * i - up)) & mask) | sixteen;
-    return f;
-}
-// Eight 16-bit values in that order of pairs.
-__device__ __forceinline__ fta_frag paired(fta_frag x) {
-    return fta_frag{(x[0] & 0xffffu) | x[2] << 16, x[0] >> 16 | (x[2] & 0xffff0000u), (x[1] & 0xffffu) | x[3] << 16,
-                    x[1] >> 16 | (x[3] & 0xffff0000u)};
-}
-
-// Lanes 16 .. 31 of a with 0 .. 15 of b, 48 .. 63 with 32 .. 47 (v_permlane16_swap on two
-// registers; through asm with its waits, as fta_swap32).
-__device__ __forceinline__ void swap16(float& a, float& b) {
-    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
-}
-// Sum and maximum over lanes l, l ^ 16, l ^ 32, l ^ 48.
-__device__ __forceinline__ float sum_quarters(float x) {
-    float y = x;
-    swap16(x, y);
-    x += y;
-    y = x;
-    fta_swap32(x, y);
-    return x + y;
-}
-__device__ __forceinline__ float max_quarters(float x) {
-    float y = x;
-    swap16(x, y);
-    x = fmaxf(x, y);
-    y = x;
-    fta_swap32(x, y);
-    return fmaxf(x, y);
 }
 
 template <int NG>
@@ -216,9 +160,9 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
                 float s = 0.f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s += Elem<DT>::to_f32((uint16_t)(x[e] & 0xffffu)) + Elem<DT>::to_f32((uint16_t)(x[e] >> 16));
-                s = -24.f * sum_quarters(s);
+                s = -24.f * fta_sum_quarters(s);
                 first[g] = f32x4{s, s, s, s};
-                qf[g] = paired(x);
+                qf[g] = fta_paired(x);
             }
         }
         auto key = [&](int it) { return 64 * (it < ns ? it : c_lo + it - ns); };
@@ -278,8 +222,8 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
             return x;
         };
         const uint32_t vrow = ldv + (16 * qt + r16) * ROW_B;
-        const uint32_t sixteen_k = in_vgpr(kSixteen<DT>), sixteen_v = in_vgpr(kSixteen<FTA_DTYPE_BF16>);
-        const float zero = __builtin_bit_cast(float, in_vgpr(0u));  // products of fp16 and fp32 numbers are one instruction as multiply-adds
+        const uint32_t sixteen_k = fta_in_vgpr(kFtaSixteen<DT>), sixteen_v = fta_in_vgpr(kFtaSixteen<FTA_DTYPE_BF16>);
+        const float zero = __builtin_bit_cast(float, fta_in_vgpr(0u));  // products of fp16 and fp32 numbers are one instruction as multiply-adds
         const fta_frag less24 = fta_frag{0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u, 0xc1c0c1c0u};  // bf16
 
         fta_wait_vmcnt<0>();  // the Q loads: the DMAs are invisible to the compiler's wait counting
@@ -305,7 +249,7 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
                 for (int i = 0; i < 4; ++i) s[t][i] = zero;
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const f32x4 x = mma16<DT>(codes16<DT>(kw.w[g], sixteen_k), qf[g], first[g]);
+                    const f32x4 x = fta_mma16<DT>(fta_codes16<DT>(kw.w[g], sixteen_k), qf[g], first[g]);
                     Words<2> d;  // scales of keys 16 qt + 4 t + i
                     __builtin_memcpy(&d, __builtin_assume_aligned(sks + 64 * g + 16 * qt + 4 * t, 8), 8);
 #pragma unroll
@@ -321,7 +265,7 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
             float mx = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
             for (int t = 1; t < 4; ++t) mx = fmaxf(mx, fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])));
-            mx = max_quarters(mx);
+            mx = fta_max_quarters(mx);
             const float mn = fmaxf(m_run, mx);
             const bool grow = (mn - m_run) * a.c > 8.f;  // rescaled only where P could pass 2^8
             if (__ballot(grow) != 0ull) {
@@ -377,12 +321,12 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
                     f32x4& o = oacc[2 * g + ct];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const fta_frag v = codes16<FTA_DTYPE_BF16>((uint32_t)w[h], sixteen_v);
-                        o = mma16<FTA_DTYPE_BF16>(v, hi[h], o);
-                        o = mma16<FTA_DTYPE_BF16>(less24, hi[h], o);
+                        const fta_frag v = fta_codes16<FTA_DTYPE_BF16>((uint32_t)w[h], sixteen_v);
+                        o = fta_mma16<FTA_DTYPE_BF16>(v, hi[h], o);
+                        o = fta_mma16<FTA_DTYPE_BF16>(less24, hi[h], o);
                         if constexpr (DT == FTA_DTYPE_F16) {
-                            o = mma16<FTA_DTYPE_BF16>(v, lo[h], o);
-                            o = mma16<FTA_DTYPE_BF16>(less24, lo[h], o);
+                            o = fta_mma16<FTA_DTYPE_BF16>(v, lo[h], o);
+                            o = fta_mma16<FTA_DTYPE_BF16>(less24, lo[h], o);
                         }
                     }
                 }
@@ -399,7 +343,7 @@ __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4
     }
 
     // merge of the waves through LDS (the stages are done with)
-    const float L = sum_quarters(l_run);
+    const float L = fta_sum_quarters(l_run);
     __syncthreads();
     float* so = reinterpret_cast<float*>(sStage);
     float2* sml = reinterpret_cast<float2*>(sStage + Sh::MERGE_B);

@@ -12,6 +12,7 @@
 // as many heads as it takes to fill 32 rows where there are few tokens.
 #include "fta_common.h"
 #include "fta_host.h"
+#include "fta_q4.h"
 #include "fta_tile.h"
 
 #include <algorithm>
@@ -34,18 +35,41 @@ struct WeighArgs {
     float* part;  // [part][B * Hk][S]
     int B, T, H, Hk, G, S, Dreal, left, sinks;
     int GG, TT, groups;  // query heads and tokens of 32 rows; head groups of a K/V head
-    int tiles, np, total;
+    int tiles, per, np, total;  // key tiles; chunks of 32 rows in a part, parts of the longest walk
     float c;
+    bool few;     // the rows stay in registers
+    bool narrow;  // a chunk's rows are within 32-bit offsets
 };
 
 constexpr int kWeighWaves = 4, kWeighKeys = 32 * kWeighWaves;
 
-// KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
+// The walk of a workgroup's keys from k_lo: chunks [c_lo, c_lo + nct) of TT tokens that see any of them,
+// for each head group.
+struct WeighWalk {
+    int c_lo = 0, nct = 0;
+    __device__ __forceinline__ WeighWalk(const WeighArgs& a, int len, int k_lo) {
+        if (k_lo >= len) return;
+        const int p0 = len - a.T;  // position of the first new token
+        const int t_lo = max(0, k_lo - p0);
+        const int64_t far = (int64_t)min(k_lo + kWeighKeys, len) - 1 + a.left - p0;
+        const int t_hi = k_lo < a.sinks ? a.T - 1 : (int)min(far, (int64_t)a.T - 1);
+        c_lo = fta_scalar(t_lo / a.TT);
+        if (t_hi >= t_lo) nct = fta_scalar(t_hi / a.TT) + 1 - c_lo;
+    }
+};
+
+// ----------------------------------------------------------------------------
+// Many rows.  KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
+// What bounds it: matrix and vector instructions (of these the 16 exp2 of a tile most), at a clock that
+// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 360 us, 764 TFLOP/s at 2.0 GHz, the
+// matrix units busy 39% of the cycles, the vector units 57%.  Four stages with all of a part's lse loaded
+// ahead (367), two key tiles a wave (411), and the last chunk's exp2 between this one's products (357 to
+// 374) changed nothing: what overlaps more runs at a lower clock.
+// ----------------------------------------------------------------------------
 template <int DT, int KD, bool Q4>
 __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache_weights_kernel(WeighArgs a) {
     constexpr int QSEG = KD / 8, KS = KD / 16, NG = KD / 32, BLOCKS = QSEG / 2, TILE_B = 32 * QSEG * 16;
     using SW = FtaSwz<QSEG>;
-    using E = Elem<DT>;
     __shared__ __align__(1024) unsigned char sQ[2][TILE_B];
     __shared__ __align__(16) float sL[2][32];  // -lse log2(e), -inf for rows that do not count
     const int lane = threadIdx.x & 63, hf = lane >> 5;
@@ -55,166 +79,302 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     const int bhk = fta_scalar(u / a.tiles), tile = u - bhk * a.tiles;  // the first keys, which most rows see, first
     const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
     const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
-    const int k_lo = kWeighKeys * tile, kt = k_lo + 32 * wave, key = kt + (lane & 31);
-    const int p0 = len - a.T;  // position of the first new token
-
-    // chunks [s0, s1) of the walk: token chunks that see any of the workgroup's keys, for each head group
-    int c_lo = 0, nct = 0;
-    if (k_lo < len) {
-        const int t_lo = max(0, k_lo - p0);
-        const int64_t far = (int64_t)min(k_lo + kWeighKeys, len) - 1 + a.left - p0;
-        const int t_hi = k_lo < a.sinks ? a.T - 1 : (int)min(far, (int64_t)a.T - 1);
-        c_lo = fta_scalar(t_lo / a.TT);
-        if (t_hi >= t_lo) nct = fta_scalar(t_hi / a.TT) + 1 - c_lo;
-    }
+    const int kt = kWeighKeys * tile + 32 * wave, key = kt + (lane & 31);  // this wave's first key, this lane's
+    const int p0 = len - a.T;                                             // position of the first new token
+    const WeighWalk walk(a, len, kWeighKeys * tile);
+    const int c_lo = walk.c_lo, nct = walk.nct;
     const int64_t all = (int64_t)nct * a.groups;
-    const int s0 = fta_scalar((int)(all * sp / a.np)), s1 = fta_scalar((int)(all * (sp + 1) / a.np));
+    if ((int64_t)sp * a.per >= all) return;  // a walk of fewer parts
+    const int s0 = sp * a.per, s1 = (int)min(all, (int64_t)s0 + a.per);
 
-    float sum = 0.f;
-    if (s0 < s1) {
-        // this wave's keys as B operands
-        fta_frag kf[KS];
-        float ds[NG];  // 4-bit keys: the key's scales
-        const bool kok = key < a.S;
-        const int64_t krow = kok ? key : 0;
-        if constexpr (Q4) {
-            const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
-            const uint16_t* sp_ = a.ks + b * a.ks_sb + hk * a.ks_sh + krow * NG;
+    const uint16_t* qp = a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
+    const float* lp = a.lse + ((int64_t)b * a.H + (int64_t)hk * a.G) * a.T;
+    // this lane's rows of a chunk: token and head within it, 16-byte slot
+    constexpr int MINE = (BLOCKS + kWeighWaves - 1) / kWeighWaves;
+    int tt[MINE], gg[MINE], col[MINE];
+    uint32_t off[MINE];  // bytes, where strides let 32 bits hold them
 #pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                ds[g] = (float)__builtin_bit_cast(_Float16, sp_[g]);
-#pragma unroll
-                for (int m = 0; m < 2; ++m) {  // octet 2 hf + m of the group: the first or second product's
-                    const uint32_t w = kp[(2 * hf + m) * NG + g];
-                    float n[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) n[e] = (float)((int)((w >> (4 * e)) & 15u) - 8);
-                    kf[2 * g + m] = 32 * g + 16 * hf + 8 * m < a.Dreal ? fta_pack_frag<DT>(n) : fta_frag{0u, 0u, 0u, 0u};
-                }
-            }
-        } else {
-            const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
-            FtaTile<DT, KD>::load_rows(kp, kok, a.Dreal, lane, kf);
-        }
-        const uint16_t* qp = a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
-        const float* lp = a.lse + ((int64_t)b * a.H + (int64_t)hk * a.G) * a.T;
-        // this lane's rows of a chunk: token and head within it, 16-byte slot
-        constexpr int MINE = (BLOCKS + kWeighWaves - 1) / kWeighWaves;
-        int tt[MINE], gg[MINE], col[MINE];
-#pragma unroll
-        for (int i = 0; i < MINE; ++i) {
-            const int s = (i * kWeighWaves + wave) * 64 + lane, row = (s / QSEG) & 31;
-            const int j = SW::slot(row, s - (s / QSEG) * QSEG);
-            tt[i] = row / a.GG;
-            gg[i] = row - tt[i] * a.GG;
-            col[i] = j * 8 < a.Dreal ? j * 8 : 0;  // columns past D: they meet zero key columns
-        }
-        const int ltt = (lane & 31) / a.GG, lgg = (lane & 31) - ltt * a.GG;
-        const uint32_t ldq = fta_lds_addr(&sQ[0][0]);
-        float lv = 0.f;  // lse of the next chunk's row `lane` (wave 0)
-        auto issue = [&](int ct, int cg, int st) __attribute__((always_inline)) {
+    for (int i = 0; i < MINE; ++i) {
+        const int s = (i * kWeighWaves + wave) * 64 + lane, row = (s / QSEG) & 31;
+        const int j = SW::slot(row, s - (s / QSEG) * QSEG);
+        tt[i] = row / a.GG;
+        gg[i] = row - tt[i] * a.GG;
+        col[i] = j * 8 < a.Dreal ? j * 8 : 0;  // columns past D: they meet zero key columns
+        off[i] = 2u * (tt[i] * (uint32_t)a.q_sn + gg[i] * (uint32_t)a.q_sh + col[i]);
+    }
+    const int ltt = (lane & 31) / a.GG, lgg = (lane & 31) - ltt * a.GG;
+    const int64_t loff = (int64_t)lgg * a.T + ltt;
+    const int t_last = 31 / a.GG;  // the last row's token in its chunk
+    const uint32_t ldq = fta_lds_addr(&sQ[0][0]);
+    float lv = 0.f;  // lse of the next chunk's row `lane` (wave 0)
+    auto issue = [&](int ct, int cg, int st) __attribute__((always_inline)) {
+        const int t0 = ct * a.TT, g0 = cg * a.GG;
+        if (a.narrow && t0 + t_last < a.T && g0 + a.GG <= a.G) {  // every row is there
+            const uint16_t* base = qp + t0 * a.q_sn + g0 * a.q_sh;
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
                 const int blk = i * kWeighWaves + wave;
-                if (blk >= BLOCKS) break;  // wave-uniform
-                const int64_t t = min(ct * a.TT + tt[i], a.T - 1), g = min(cg * a.GG + gg[i], a.G - 1);
-                fta_dma16_at(qp + t * a.q_sn + g * a.q_sh + col[i], ldq + st * TILE_B + blk * 1024);
+                if (blk < BLOCKS) fta_dma16_so(base, off[i], ldq + st * TILE_B + blk * 1024);  // wave-uniform
             }
             if (wave == 0) {
-                const int t = ct * a.TT + ltt, g = cg * a.GG + lgg;
-                const bool ok = t < a.T && g < a.G && ltt < a.TT;
-                const float x = lp[ok ? (int64_t)g * a.T + t : 0];
+                const float x = lp[(int64_t)g0 * a.T + t0 + loff];
+                lv = ltt < a.TT ? x : FTA_INF;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < MINE; ++i) {
+                const int blk = i * kWeighWaves + wave;
+                const int64_t t = min(t0 + tt[i], a.T - 1), g = min(g0 + gg[i], a.G - 1);
+                if (blk < BLOCKS) fta_dma16_at(qp + t * a.q_sn + g * a.q_sh + col[i], ldq + st * TILE_B + blk * 1024);
+            }
+            if (wave == 0) {
+                const bool ok = t0 + ltt < a.T && g0 + lgg < a.G && ltt < a.TT;
+                const float x = lp[ok ? (int64_t)g0 * a.T + t0 + loff : 0];
                 lv = ok ? x : FTA_INF;
             }
-        };
-        const uint32_t ro = ldq + (lane & 31) * QSEG * 16u;
-        auto frag = [&](int st, int slot) { return fta_lds_frag(ro + st * TILE_B + 16u * (slot ^ SW::x(lane & 31))); };
-        const int g0 = fta_scalar(s0 / nct);
-        int ct = c_lo + s0 - g0 * nct, cg = g0;
-        fta_wait_vmcnt<0>();  // the keys: the DMAs are invisible to the compiler's wait counting
-        issue(ct, cg, 0);
-        float run = 0.f;
-        int st = 0;
-        for (int s = s0; s < s1; ++s, st ^= 1) {
-            fta_wait_vmcnt<0>();
-            // a row that saw nothing (lse = -inf) gives nothing, as one that does not exist
-            if (wave == 0 && lane < 32) sL[st][lane] = (lv == -FTA_INF) ? -FTA_INF : -lv * kLog2e;
-            __syncthreads();  // this chunk visible; every wave is past the last one
-            const int c = ct;
-            if (++ct == c_lo + nct) {
-                ct = c_lo;
-                ++cg;
-            }
-            if (s + 1 < s1) issue(ct, cg, st ^ 1);
-            const int q_lo = p0 + c * a.TT, q_hi = min(q_lo + a.TT, len) - 1;  // positions of the chunk's tokens
-            if (q_hi < kt || (kt + 31 < q_lo - a.left && kt >= a.sinks)) continue;  // wave-uniform
-            f32x16 x;
-            if constexpr (Q4) {
+        }
+    };
+    const uint32_t ro = ldq + (lane & 31) * QSEG * 16u;
+    auto frag = [&](int st, int slot) { return fta_lds_frag(ro + st * TILE_B + 16u * (slot ^ SW::x(lane & 31))); };
+    int cg = fta_scalar(s0 / nct), ct = c_lo + s0 - cg * nct;
+    issue(ct, cg, 0);
+    // this wave's keys as B operands
+    fta_frag kf[KS];
+    float ds[NG];  // 4-bit keys: the key's scales
+    const bool kok = key < a.S;
+    const int64_t krow = kok ? key : 0;
+    if constexpr (Q4) {
+        const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
+        const uint16_t* scales = a.ks + b * a.ks_sb + hk * a.ks_sh + krow * NG;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0.f;
+        for (int g = 0; g < NG; ++g) {
+            ds[g] = (float)__builtin_bit_cast(_Float16, scales[g]);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    f32x16 y;
+            for (int m = 0; m < 2; ++m) {  // octet 2 hf + m of the group: the first or second product's
+                const uint32_t word = kp[(2 * hf + m) * NG + g];
+                float n[8];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) y[i] = 0.f;
-                    y = fta_mma<DT>(frag(st, 4 * g + 2 * hf), kf[2 * g], y);
-                    y = fta_mma<DT>(frag(st, 4 * g + 2 * hf + 1), kf[2 * g + 1], y);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) x[i] = fmaf(ds[g], y[i], x[i]);
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) x = fta_mma<DT>(frag(st, 2 * ks + hf), kf[ks], x);
-            }
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(&sL[st][c_row(i, lane)]);
-                x[i] = fta_exp2(fmaf(x[i], a.c, l.x));
-                x[i + 1] = fta_exp2(fmaf(x[i + 1], a.c, l.y));
-                x[i + 2] = fta_exp2(fmaf(x[i + 2], a.c, l.z));
-                x[i + 3] = fta_exp2(fmaf(x[i + 3], a.c, l.w));
-            }
-            if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
-                // the rows of the tokens that see this lane's key
-                const int64_t t_hi = key < a.sinks ? a.TT : min((int64_t)key + a.left - q_lo, (int64_t)a.TT);
-                const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
-                const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int r = c_row(i, lane);
-                    x[i] = (r >= rlo && r < rhi) ? x[i] : 0.f;
-                }
-            }
-            // sums of a chunk, of 64 chunks, of all: their rounding errors stay small on long walks
-            run += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) +
-                   (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
-            if (((s - s0) & 63) == 63) {
-                sum += run;
-                run = 0.f;
+                for (int e = 0; e < 8; ++e) n[e] = (float)((int)((word >> (4 * e)) & 15u) - 8);
+                kf[2 * g + m] = 32 * g + 16 * hf + 8 * m < a.Dreal ? fta_pack_frag<DT>(n) : fta_frag{0u, 0u, 0u, 0u};
             }
         }
-        sum += run;
-        sum += fta_xor32(sum);
+    } else {
+        const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
+        FtaTile<DT, KD>::load_rows(kp, kok, a.Dreal, lane, kf);
     }
-    if (lane >= 32) return;
-    if (a.np > 1) {
-        if (key < a.S) a.part[((int64_t)sp * a.B * a.Hk + bhk) * a.S + key] = sum;
-    } else if (key < len) {
+    float run = 0.f, sum = 0.f;
+    int st = 0;
+    for (int s = s0; s < s1; ++s, st ^= 1) {
+        fta_wait_vmcnt<0>();
+        // a row that saw nothing (lse = -inf) gives nothing, as one that does not exist
+        if (wave == 0 && lane < 32) sL[st][lane] = (lv == -FTA_INF) ? -FTA_INF : -lv * kLog2e;
+        __syncthreads();  // this chunk visible; every wave is past the last one
+        const int c = ct;
+        if (++ct == c_lo + nct) {
+            ct = c_lo;
+            ++cg;
+        }
+        if (s + 1 < s1) issue(ct, cg, st ^ 1);
+        // sums of a chunk, of 64 chunks, of all: their rounding errors stay small on long walks
+        if (((s - s0) & 63) == 63) {
+            sum += run;
+            run = 0.f;
+        }
+        const int q_lo = p0 + c * a.TT, q_hi = min(q_lo + a.TT, len) - 1;  // positions of the chunk's tokens
+        if (q_hi < kt || (kt + 31 < q_lo - a.left && kt >= a.sinks)) continue;  // wave-uniform
+        f32x16 x;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = 0.f;
+        if constexpr (Q4) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                f32x16 y;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = 0.f;
+                y = fta_mma<DT>(frag(st, 4 * g + 2 * hf), kf[2 * g], y);
+                y = fta_mma<DT>(frag(st, 4 * g + 2 * hf + 1), kf[2 * g + 1], y);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[i] = fmaf(ds[g], y[i], x[i]);
+            }
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) x = fta_mma<DT>(frag(st, 2 * ks + hf), kf[ks], x);
+        }
+        if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
+            asm volatile("");  // an edge: kept apart, or every chunk pays for it
+            // the rows of the tokens that see this lane's key
+            const int64_t t_hi = key < a.sinks ? a.TT : min((int64_t)key + a.left - q_lo, (int64_t)a.TT);
+            const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
+            const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
+            FtaTile<DT, KD>::mask(fta_bits_below(rhi) & ~fta_bits_below(rlo), lane, x);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(&sL[st][c_row(i, lane)]);
+            x[i] = fta_exp2(fmaf(x[i], a.c, l.x));
+            x[i + 1] = fta_exp2(fmaf(x[i + 1], a.c, l.y));
+            x[i + 2] = fta_exp2(fmaf(x[i + 2], a.c, l.z));
+            x[i + 3] = fta_exp2(fmaf(x[i + 3], a.c, l.w));
+        }
+        run += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) +
+               (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+    }
+    sum += run;
+    sum += fta_xor32(sum);
+    if (lane >= 32 || key >= len) return;
+    if (a.np > 1)
+        a.part[((int64_t)sp * a.B * a.Hk + bhk) * a.S + key] = sum;
+    else
         a.w[b * a.w_sb + hk * a.w_sh + key] += sum;
+}
+
+// ----------------------------------------------------------------------------
+// Few rows (T * G of at most 32): a serving step.  A workgroup takes a run of keys, its waves 32-key tiles
+// in turn, the next tile's asked for ahead; the rows, 16 or 32, stay in registers.  16 x 16 x 32 products,
+// S = Q K^T: lane (k, q) = (l & 15, l >> 4) holds rows 4 q + i of its key k.  4-bit keys enter as 16 + n,
+// after a product of the rows with -24 (see fta_q4.hip).
+// What bounds it: memory.
+// ----------------------------------------------------------------------------
+template <int KD, bool Q4>
+struct KeyTile {  // 32 keys as B operands: of keys 16 t + k, this lane's words
+    uint32_t w[2][Q4 ? KD / 32 : KD / 8];
+    uint16_t d[2][KD / 32];
+    float before[2];
+};
+
+template <int DT, int KD, bool Q4, int RT>
+__global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_step_kernel(WeighArgs a) {
+    constexpr int NG = KD / 32, NW = 4;
+    const int lane = threadIdx.x & 63, r16 = lane & 15, qt = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bhk = fta_scalar(blockIdx.x / a.np), sp = blockIdx.x - bhk * a.np;
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
+    const int R = a.T * a.G, p0 = len - a.T, p1 = len - 1;  // rows; first and last position
+    // 32-key tiles: the sinks', then the band's
+    const int kb0 = max(0, p0 - a.left);
+    int ns = (min(a.sinks, len) + 31) >> 5, c_lo = kb0 >> 5;
+    const int c_hi = (len + 31) >> 5;
+    if (c_lo <= ns) c_lo = ns = 0;
+    const int all = max(ns + c_hi - c_lo, 0);
+    const int it0 = fta_scalar((int)((int64_t)all * sp / a.np)), it1 = fta_scalar((int)((int64_t)all * (sp + 1) / a.np));
+    if (it0 + wave >= it1) return;
+
+    const uint8_t* kp = a.k + b * a.k_sb + hk * a.k_sh;
+    const uint16_t* ks = a.ks + b * a.ks_sb + hk * a.ks_sh;
+    float* wp = a.w + b * a.w_sb + hk * a.w_sh;
+    auto key = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
+    using Tile = KeyTile<KD, Q4>;
+    auto ask = [&](int it, Tile& x) __attribute__((always_inline)) {
+        const int kb = key(it);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int j = min(kb + 16 * t + r16, len - 1);  // behind the last token: masked, and not written
+            if constexpr (Q4) {
+                __builtin_memcpy(x.w[t], __builtin_assume_aligned(kp + (int64_t)j * (16 * NG) + qt * 4 * NG, 4), 4 * NG);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) x.d[t][g] = ks[(int64_t)j * NG + g];
+            } else {
+                const uint8_t* row = kp + (int64_t)j * a.k_sn;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const int d = 32 * g + 8 * qt;
+                    const fta_frag f = d < a.Dreal ? *reinterpret_cast<const fta_frag*>(row + 2 * d) : fta_frag{0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x.w[t][4 * g + e] = f[e];
+                }
+            }
+            x.before[t] = wp[j];
+        }
+    };
+    Tile cur, nxt;
+    ask(it0 + wave, cur);
+
+    fta_frag qf[RT][NG];
+    float nl[RT][4];  // of rows 4 qt + i
+    int pos[RT][4];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = 16 * rt + r16, t = min(r, R - 1) / a.G, g = min(r, R - 1) - t * a.G;
+        const uint16_t* qp = a.q + b * a.q_sb + (int64_t)(hk * a.G + g) * a.q_sh + t * a.q_sn;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            const int d = 32 * n + 8 * qt;
+            const fta_frag x = (r < R && d < a.Dreal) ? *reinterpret_cast<const fta_frag*>(qp + d) : fta_frag{0u, 0u, 0u, 0u};
+            qf[rt][n] = Q4 ? fta_paired(x) : x;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rr = 16 * rt + 4 * qt + i, tr = min(rr, R - 1) / a.G, gr = min(rr, R - 1) - tr * a.G;
+            const float x = a.lse[((int64_t)b * a.H + hk * a.G + gr) * a.T + tr];
+            nl[rt][i] = rr < R && x != -FTA_INF ? -x * kLog2e : -FTA_INF;  // a row that saw nothing gives nothing
+            pos[rt][i] = p0 + tr;
+        }
+    }
+    f32x4 first[RT][Q4 ? NG : 1];
+    if constexpr (Q4) {
+        constexpr uint32_t m24 = DT == FTA_DTYPE_BF16 ? 0xc1c0c1c0u : 0xce00ce00u;  // -24
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+                first[rt][g] = fta_mma16<DT>(qf[rt][g], fta_frag{m24, m24, m24, m24}, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+    const uint32_t sixteen = fta_in_vgpr(kFtaSixteen<DT>);
+    const float zero = __builtin_bit_cast(float, fta_in_vgpr(0u));
+
+    for (int it = it0 + wave; it < it1; it += NW) {
+        if (it + NW < it1) ask(it + NW, nxt);
+        const int kb = key(it);
+        const bool full = kb + 31 <= p0 && (kb >= p1 - a.left || kb + 31 < a.sinks);
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                f32x4 x = f32x4{zero, zero, zero, zero};
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    if constexpr (Q4) {
+                        const f32x4 y = fta_mma16<DT>(qf[rt][g], fta_codes16<DT>(cur.w[t][g], sixteen), first[rt][g]);
+                        const float d = (float)__builtin_bit_cast(_Float16, cur.d[t][g]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = fmaf(d, y[i], x[i]);
+                    } else {
+                        x = fta_mma16<DT>(qf[rt][g], fta_frag{cur.w[t][4 * g], cur.w[t][4 * g + 1], cur.w[t][4 * g + 2], cur.w[t][4 * g + 3]}, x);
+                    }
+                }
+                const int j = kb + 16 * t + r16;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool seen = full || (j <= pos[rt][i] && (j >= pos[rt][i] - a.left || j < a.sinks));
+                    const float p = fta_exp2(fmaf(x[i], a.c, nl[rt][i]));
+                    sum[t] += seen ? p : 0.f;
+                }
+            }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const float s = fta_sum_quarters(sum[t]);
+            const int j = kb + 16 * t + r16;
+            if (qt == 0 && j < len) wp[j] = cur.before[t] + s;
+        }
+        cur = nxt;
     }
 }
 
+// Sum of the parts that a key's walk has.
 __global__ __launch_bounds__(256) void fta_cache_weights_join_kernel(WeighArgs a) {
+    const int bhk = blockIdx.y, b = bhk / a.Hk, hk = bhk - b * a.Hk;
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    const int len = min(max(a.lens[b], 0), a.S);
+    const int tile = fta_scalar((blockIdx.x * 256 + (threadIdx.x & ~63)) / kWeighKeys);  // a wave's 64 keys lie in one tile
+    if (j >= len) return;
+    const WeighWalk w(a, len, kWeighKeys * tile);
+    const int parts = (int)(((int64_t)w.nct * a.groups + a.per - 1) / a.per);
     const int64_t n = (int64_t)a.B * a.Hk * a.S;
-    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (e >= n) return;
-    const int64_t bhk = e / a.S;
-    const int b = (int)(bhk / a.Hk), hk = (int)(bhk - (int64_t)b * a.Hk), j = (int)(e - bhk * a.S);
-    if (j >= min(max(a.lens[b], 0), a.S)) return;
+    const float* p = a.part + (int64_t)bhk * a.S + j;
     float s = 0.f;
-    for (int p = 0; p < a.np; ++p) s += a.part[p * n + e];
+    for (int i = 0; i < parts; ++i) s += p[i * n];
     a.w[b * a.w_sb + hk * a.w_sh + j] += s;
 }
 
@@ -235,29 +395,55 @@ int weigh_plan(WeighArgs& a, int B, int H, int Hk, int T, int S, int D, int left
     a.GG = std::min(a.G, std::max(1, 32 / std::min(T, 32)));
     a.TT = 32 / a.GG;
     a.groups = (a.G + a.GG - 1) / a.GG;
+    const int64_t most = (1 << 24) - 1, heads = (int64_t)B * Hk;
+    a.few = (int64_t)T * a.G <= 32;
+    if (a.few) {
+        // parts cost nothing (every key is its own): about 2048 workgroups, down to four tiles of a wave, and
+        // enough to fill the chip down to one
+        const int64_t tiles = (std::min<int64_t>(S, (int64_t)a.left + T + a.sinks + 62) + 31) / 32;
+        auto parts = [&](int64_t target, int64_t least) { return std::min<int64_t>((target + heads - 1) / heads, tiles / least); };
+        const int64_t np = std::max<int64_t>(1, std::max(parts(1024, 4), parts(2048, 16)));
+        if (heads * np > most) return fta::unsupported("cache_weights: too many heads");
+        a.np = (int)np;
+        a.total = (int)(heads * np);
+        return FTA_OK;
+    }
     a.tiles = (S + kWeighKeys - 1) / kWeighKeys;
-    const int64_t wgs = (int64_t)B * Hk * a.tiles;
-    // the longest walk, in chunks
-    const int64_t span = std::min<int64_t>(T, a.sinks > 0 ? T : (int64_t)a.left + kWeighKeys + 1);
-    const int64_t chunks = ((span + a.TT - 1) / a.TT + 1) * a.groups;
-    if (chunks > (1 << 30)) return fta::unsupported("cache_weights: too many rows");
-    a.np = (int)std::max<int64_t>(1, std::min<int64_t>((1024 + wgs - 1) / wgs, chunks / 8));
-    const int64_t most = (1 << 24) - 1;
-    if (wgs * a.np > most || (int64_t)B * Hk * ((S + 255) / 256) > most)
+    const int64_t wgs = heads * a.tiles;
+    // walks in chunks: the longest, and all of them, of sequences that fill the cache
+    const int64_t span = (int64_t)a.left + kWeighKeys + 1;
+    auto chunks = [&](int64_t tokens) { return ((tokens + a.TT - 1) / a.TT + 1) * a.groups; };
+    const int64_t longest = chunks(std::min<int64_t>(T, a.sinks > 0 ? T : span));
+    if (longest > (1 << 30)) return fta::unsupported("cache_weights: too many rows");
+    const int64_t mean = chunks(std::min<int64_t>(span, T - std::max<int64_t>(0, T - ((int64_t)S - T)) / 2));
+    // Parts of 32 chunks and more, about 4096 of them: causal walks shorten with the key, and tiles of sinks
+    // walk every token.  Target 1024 / 2048 / 4096 / 8192, us: 8192 tokens 523 / 440 / 361 / 361; least 32 / 64
+    // chunks: 2048 tokens 46 / 66.
+    a.per = (int)std::min<int64_t>(longest, std::max<int64_t>(32, wgs * mean / 4096));
+    a.np = (int)((longest + a.per - 1) / a.per);
+    if (wgs * a.np > most || heads > 65535 || heads * ((S + 255) / 256) > most)
         return fta::unsupported("cache_weights: too many keys");
     a.total = (int)(wgs * a.np);
     return FTA_OK;
 }
 
-size_t weigh_bytes(const WeighArgs& a) { return a.np <= 1 ? 0 : fta::align_up((size_t)a.np * a.B * a.Hk * a.S * sizeof(float)); }
+size_t weigh_bytes(const WeighArgs& a) { return a.few || a.np <= 1 ? 0 : fta::align_up((size_t)a.np * a.B * a.Hk * a.S * sizeof(float)); }
 
 template <int DT, int KD, bool Q4>
 int launch_weigh(const WeighArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL((fta_cache_weights_kernel<DT, KD, Q4>), dim3((unsigned)a.total), dim3(kWeighWaves * 64), 0, st, a);
+    const dim3 grid((unsigned)a.total), t(256);
+    if (a.few) {
+        if (a.T * a.G <= 16)
+            hipLaunchKernelGGL((fta_cache_weights_step_kernel<DT, KD, Q4, 1>), grid, t, 0, st, a);
+        else
+            hipLaunchKernelGGL((fta_cache_weights_step_kernel<DT, KD, Q4, 2>), grid, t, 0, st, a);
+        return fta::check_launch("fta_cache_weights_step_kernel");
+    }
+    hipLaunchKernelGGL((fta_cache_weights_kernel<DT, KD, Q4>), grid, t, 0, st, a);
     int rc = fta::check_launch("fta_cache_weights_kernel");
     if (rc != FTA_OK || a.np <= 1) return rc;
-    const int64_t n = (int64_t)a.B * a.Hk * a.S;
-    hipLaunchKernelGGL(fta_cache_weights_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    const dim3 g((unsigned)((a.S + 255) / 256), (unsigned)(a.B * a.Hk));
+    hipLaunchKernelGGL(fta_cache_weights_join_kernel, g, t, 0, st, a);
     return fta::check_launch("fta_cache_weights_join_kernel");
 }
 
@@ -321,6 +507,8 @@ int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, co
     a.w = weights, a.w_sb = w_strides[0], a.w_sh = w_strides[1];
     a.part = (float*)workspace;
     a.c = scale * kLog2e;
+    auto fits = [](int64_t stride, int n) { return stride >= 0 && stride <= (1 << 29) / n; };
+    a.narrow = fits(a.q_sn, 32) && fits(a.q_sh, 32);
     hipStream_t st = (hipStream_t)stream;
     return dtype == FTA_DTYPE_BF16 ? launch_weigh_dims<FTA_DTYPE_BF16>(a, q4, st) : launch_weigh_dims<FTA_DTYPE_F16>(a, q4, st);
     FTA_TRY_END
