@@ -22,7 +22,7 @@ struct CacheArgs {
     int B, T, H, Hk, G, R, S, P, Dreal;  // R = T * G rows per (b, K/V head); row (b * Hk + hk) * R + t * G + g
     int left, sinks;
     float c;
-    int row_tiles, ns;        // own keys: 32-row tiles of R, parts
+    int row_tiles, ns;        // own keys: tiles of R rows (32, or 16 over 4-bit caches), parts
     int pre_tiles, pre_ns;    // prefix: row tiles of B * R, parts
     int64_t rows;             // B * Hk * R
     int total, pre_total;     // workgroups of either

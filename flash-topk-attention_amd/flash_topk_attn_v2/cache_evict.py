@@ -78,7 +78,7 @@ def flash_cache_weights(
     if isinstance(cache, Q4Cache):
         S, (ka, ks, sa, ss, *_) = q4_args(what, cache, B, Hk, D, dev)
     else:
-        if cache.ndim != 3 or cache.shape[0] != B or cache.shape[2] != Hk * D or cache.shape[1] == 0:
+        if not isinstance(cache, torch.Tensor) or cache.ndim != 3 or cache.shape[0] != B or cache.shape[2] != Hk * D or cache.shape[1] == 0:
             raise ValueError(f"{what}: cache must be keys [B, S, num_kv_heads * D] = [{B}, S, {Hk * D}] or a Q4Cache")
         if cache.dtype != q.dtype:
             raise ValueError(f"{what}: the keys must have q's type")
@@ -214,7 +214,7 @@ def flash_cache_evict(
     check_lens(what, cache_lens, B)
     _lib.check_device(what, dev, cache_lens)
     q4 = isinstance(cache, Q4Cache)
-    if not q4 and (not isinstance(cache, (tuple, list)) or len(cache) != 2):
+    if not q4 and (not isinstance(cache, (tuple, list)) or len(cache) != 2 or not all(isinstance(t, torch.Tensor) for t in cache)):
         raise ValueError(f"{what}: cache must be (k_cache, v_cache) or a Q4Cache")
     tensors = (*cache, weights)
     if out is None:
