@@ -233,7 +233,8 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
 // in turn, the next tile's asked for ahead; the rows, 16 or 32, stay in registers.  16 x 16 x 32 products,
 // S = Q K^T: lane (k, q) = (l & 15, l >> 4) holds rows 4 q + i of its key k.  4-bit keys enter as 16 + n,
 // after a product of the rows with -24 (see fta_q4.hip).
-// What bounds it: memory.
+// What bounds it: memory.  64 requests of 4096 to 8192 tokens, 32 / 8 heads of 128: 154 us, 5.4 TB/s; with 4-bit keys
+// 66 us, 3.4 TB/s, where vector instructions weigh as much.
 // ----------------------------------------------------------------------------
 template <int KD, bool Q4>
 struct KeyTile {  // 32 keys as B operands: of keys 16 t + k, this lane's words
@@ -380,7 +381,7 @@ __global__ __launch_bounds__(256) void fta_cache_weights_join_kernel(WeighArgs a
 
 // ---------------------------------------------------------------------- host
 
-int weigh_plan(WeighArgs& a, int B, int H, int Hk, int T, int S, int D, int left, int sinks) {
+int weigh_plan(WeighArgs& a, bool q4, int B, int H, int Hk, int T, int S, int D, int left, int sinks) {
     if (B <= 0 || H <= 0 || Hk <= 0 || T <= 0 || S <= 0 || D <= 0) return fta::arg_error("cache_weights: dims must be positive");
     if (H % Hk != 0) return fta::arg_error("cache_weights: num_heads must be a multiple of num_kv_heads");
     if (D % 16 != 0 || D > 256) return fta::arg_error("cache_weights: D must be a multiple of 16 up to 256");
@@ -398,11 +399,14 @@ int weigh_plan(WeighArgs& a, int B, int H, int Hk, int T, int S, int D, int left
     const int64_t most = (1 << 24) - 1, heads = (int64_t)B * Hk;
     a.few = (int64_t)T * a.G <= 32;
     if (a.few) {
-        // parts cost nothing (every key is its own): about 2048 workgroups, down to four tiles of a wave, and
-        // enough to fill the chip down to one
+        // Parts cost nothing but a workgroup's start (every key is its own): enough to fill the chip, down to one
+        // tile of a wave, and about 16384 of two tiles and more, whose starts overlap with others' ends; 4-bit tiles
+        // are shorter, 2048 of four.  Target 2048 / 8192 / 16384 / 65536 (the last down to one tile), us, 64 requests
+        // of 4096 to 8192 tokens, 32 / 8 heads: of 128 193 / 161 / 154 / 158, of 64 123 / 89 / 85 / 90, of 128 in 4
+        // bits 66 / 71 / 83 / 113.
         const int64_t tiles = (std::min<int64_t>(S, (int64_t)a.left + T + a.sinks + 62) + 31) / 32;
         auto parts = [&](int64_t target, int64_t least) { return std::min<int64_t>((target + heads - 1) / heads, tiles / least); };
-        const int64_t np = std::max<int64_t>(1, std::max(parts(1024, 4), parts(2048, 16)));
+        const int64_t np = std::max<int64_t>(1, std::max(parts(1024, 4), q4 ? parts(2048, 16) : parts(16384, 8)));
         if (heads * np > most) return fta::unsupported("cache_weights: too many heads");
         a.np = (int)np;
         a.total = (int)(heads * np);
@@ -472,7 +476,7 @@ extern "C" {
 
 size_t fta_cache_weights_workspace_size(int B, int H, int Hk, int T, int S, int D, int left, int num_sinks) {
     WeighArgs a;
-    if (weigh_plan(a, B, H, Hk, T, S, D, left, num_sinks) != FTA_OK) return 0;
+    if (weigh_plan(a, false, B, H, Hk, T, S, D, left, num_sinks) != FTA_OK) return 0;
     return weigh_bytes(a);
 }
 
@@ -482,7 +486,8 @@ int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, co
                       const int64_t* w_strides, void* workspace, size_t workspace_bytes, void* stream) {
     FTA_TRY_BEGIN
     WeighArgs a;
-    int rc = weigh_plan(a, B, H, Hk, T, S, D, left, num_sinks);
+    const bool q4 = k_scales != nullptr;
+    int rc = weigh_plan(a, q4, B, H, Hk, T, S, D, left, num_sinks);
     if (rc != FTA_OK) return rc;
     if (dtype != FTA_DTYPE_BF16 && dtype != FTA_DTYPE_F16) return fta::arg_error("cache_weights: dtype must be bf16 or fp16");
     if (!(scale > 0.f) || scale > 2.0e38f)  // times log2(e) still finite
@@ -491,7 +496,6 @@ int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, co
     if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return fta::arg_error("cache_weights: workspace too small");
     if (!fta::all_set(q, q_strides, k, k_strides, cache_lens, lse, weights, w_strides) || (k_scales != nullptr && ks_strides == nullptr))
         return fta::arg_error("cache_weights: a required pointer is null");
-    const bool q4 = k_scales != nullptr;
     a.q = (const uint16_t*)q, a.q_sb = q_strides[0], a.q_sh = q_strides[1], a.q_sn = q_strides[2];
     a.k = (const uint8_t*)k;
     if (q4) {
