@@ -74,7 +74,7 @@ def _warn_of_short_tables(what, P, S, offset):
 
 def offsets(what, position_offset, B, device, P, S):
     """``(offset for all, offset of each request or None)`` of an append, checked."""
-    if isinstance(position_offset, torch.Tensor):
+    if isinstance(position_offset, torch.Tensor) and position_offset.ndim > 0:
         if position_offset.dtype != torch.int32 or position_offset.shape != (B,):
             raise ValueError(f"{what}: position_offset must be a whole number or int32 [B] = [{B}]")
         _lib.check_device(what, device, position_offset)

@@ -135,3 +135,17 @@ def test_what_is_written_lies_apart():
         with pytest.raises(ValueError):
             apart((0, 256, 512), to)
     assert to_metas is not metas
+
+
+def test_position_offset_of_no_dimensions_is_a_number():
+    """Only int32 [B] is an offset for each request; a tensor of no dimensions is a whole number, as any other is."""
+    from flash_topk_attn_v2.qk_prep import offsets
+
+    cpu = torch.device("cpu")
+    for x in (5, 5.0, torch.tensor(5), torch.tensor(5, dtype=torch.int32)):
+        assert offsets("x", x, 2, cpu, 64, 8) == (5, None)
+    number, each = offsets("x", torch.tensor([3, 4], dtype=torch.int32), 2, cpu, 64, 8)
+    assert number == 0 and each.tolist() == [3, 4]
+    for x in (torch.tensor(0.5), torch.tensor([3], dtype=torch.int32), torch.tensor([3, 4]), torch.tensor([[3, 4]], dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            offsets("x", x, 2, cpu, 64, 8)
