@@ -97,19 +97,20 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     for (int i = 0; i < MINE; ++i) {
         const int s = (i * kWeighWaves + wave) * 64 + lane, row = (s / QSEG) & 31;
         const int j = SW::slot(row, s - (s / QSEG) * QSEG);
-        tt[i] = row / a.GG;
-        gg[i] = row - tt[i] * a.GG;
+        const bool has = row < a.TT * a.GG;  // the last rows of a chunk that heads do not fill repeat its first
+        tt[i] = has ? row / a.GG : 0;
+        gg[i] = has ? row - tt[i] * a.GG : 0;
         col[i] = j * 8 < a.Dreal ? j * 8 : 0;  // columns past D: they meet zero key columns
         off[i] = 2u * (tt[i] * (uint32_t)a.q_sn + gg[i] * (uint32_t)a.q_sh + col[i]);
     }
-    const int ltt = (lane & 31) / a.GG, lgg = (lane & 31) - ltt * a.GG;
+    const bool lhas = (lane & 31) < a.TT * a.GG;
+    const int ltt = lhas ? (lane & 31) / a.GG : 0, lgg = lhas ? (lane & 31) - ltt * a.GG : 0;
     const int64_t loff = (int64_t)lgg * a.T + ltt;
-    const int t_last = 31 / a.GG;  // the last row's token in its chunk
     const uint32_t ldq = fta_lds_addr(&sQ[0][0]);
     float lv = 0.f;  // lse of the next chunk's row `lane` (wave 0)
     auto issue = [&](int ct, int cg, int st) __attribute__((always_inline)) {
         const int t0 = ct * a.TT, g0 = cg * a.GG;
-        if (a.narrow && t0 + t_last < a.T && g0 + a.GG <= a.G) {  // every row is there
+        if (a.narrow && t0 + a.TT <= a.T && g0 + a.GG <= a.G) {  // every row is there
             const uint16_t* base = qp + t0 * a.q_sn + g0 * a.q_sh;
 #pragma unroll
             for (int i = 0; i < MINE; ++i) {
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
             }
             if (wave == 0) {
                 const float x = lp[(int64_t)g0 * a.T + t0 + loff];
-                lv = ltt < a.TT ? x : FTA_INF;
+                lv = lhas ? x : FTA_INF;
             }
         } else {
 #pragma unroll
@@ -128,7 +129,7 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
                 if (blk < BLOCKS) fta_dma16_at(qp + t * a.q_sn + g * a.q_sh + col[i], ldq + st * TILE_B + blk * 1024);
             }
             if (wave == 0) {
-                const bool ok = t0 + ltt < a.T && g0 + lgg < a.G && ltt < a.TT;
+                const bool ok = t0 + ltt < a.T && g0 + lgg < a.G && lhas;
                 const float x = lp[ok ? (int64_t)g0 * a.T + t0 + loff : 0];
                 lv = ok ? x : FTA_INF;
             }
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
         if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
             asm volatile("");  // an edge: kept apart, or every chunk pays for it
             // the rows of the tokens that see this lane's key
-            const int64_t t_hi = key < a.sinks ? a.TT : min((int64_t)key + a.left - q_lo, (int64_t)a.TT);
+            const int64_t t_hi = key < a.sinks ? a.TT - 1 : min((int64_t)key + a.left - q_lo, (int64_t)a.TT - 1);
             const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
             const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
             FtaTile<DT, KD>::mask(fta_bits_below(rhi) & ~fta_bits_below(rlo), lane, x);

@@ -179,3 +179,27 @@ def test_evict_of_special_weights(gpu):
         c = tuple(x.clone() for x in cache)
         _, kept = fta.flash_cache_evict(c, w.to(gpu), torch.tensor([S], dtype=torch.int32, device=gpu), budget)
         assert kept[0, 0].tolist() == _evicted(w[0, 0], S, budget, 0, 0)
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+@pytest.mark.parametrize("T,H,Hk,left,sinks", [(8, 3, 1, 5, 0), (64, 3, 1, 5, 0), (64, 12, 2, 40, 3), (70, 5, 5, 9, 0), (45, 33, 1, 7, 0)])
+def test_a_token_that_is_not_finite_stays_with_its_keys(gpu, T, H, Hk, left, sinks, q4):
+    """A query of NaN reaches the keys that its token sees and no others, whose sums keep every bit."""
+    import flash_topk_attn_v2 as fta
+
+    S, D = 200, 64
+    q = rand((1, T, H * D), 3, BF, gpu)
+    cache = Q.cache(1, S, Hk, D, gpu, 4) if q4 else rand((1, S, Hk * D), 4, BF, gpu)
+    ln = torch.tensor([S - 9], dtype=torch.int32, device=gpu)
+    lse = torch.full((1, H, T), 3.0, device=gpu)
+    zero = torch.zeros(1, Hk, S, device=gpu)
+    want = fta.flash_cache_weights(q, cache, lse, ln, zero.clone(), H, left, sinks, num_kv_heads=Hk)
+    for t in (0, T // 2, T - 1):
+        bad = q.clone()
+        bad[:, t] = math.nan
+        got = fta.flash_cache_weights(bad, cache, lse, ln, zero.clone(), H, left, sinks, num_kv_heads=Hk)
+        p = S - 9 - T + t
+        sees = torch.zeros(S, dtype=torch.bool, device=gpu)
+        sees[max(0, p - left):p + 1] = True
+        sees[:sinks] = True
+        assert got[0, :, sees].isnan().all() and torch.equal(got[0, :, ~sees], want[0, :, ~sees])
