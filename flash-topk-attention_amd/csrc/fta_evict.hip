@@ -195,7 +195,7 @@ __global__ __launch_bounds__(kSelThreads) void fta_evict_select_kernel(EvictArgs
 // What bounds it: memory, and in place for few heads the latency of its blocks, which follow each
 // other.  16 x 8 heads of 128 bf16, 8192 rows to 4096: 146 us in place, 117 into another cache (537 MB:
 // 3.7 and 4.6 TB/s); 64 x 8 heads of 128 in 4 bits, 16384 to 4096: 176 us (604 MB; single rows of 64 and 8
-// bytes out of 128-byte lines); 1 x 8 heads, 32768 to 8192: 35 us.  In place with 512 threads instead of
+// bytes out of 128-byte lines); 1 x 8 heads, 32768 to 8192: 34 us.  In place with 512 threads instead of
 // 1024 152 / 184 / 42 us, with eight rows a thread 174 / 194 / 39.
 // ----------------------------------------------------------------------------
 constexpr int kMove = 4;

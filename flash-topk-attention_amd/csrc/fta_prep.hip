@@ -277,8 +277,8 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
 // are of one kind (queries, keys, values) but where the kinds meet, and each kind has its own body.
 // What bounds it: vector instructions, 190 a group of four rows and 69% of the cycles (32768 tokens, 32 / 8
 // heads of 128: 198 us, 708 MB).  One body for any row 227 us; held to four waves a SIMD 198, three 206;
-// through the caches 209; the queries by the forward's kernel and the rest by this one 121 + 84; one
-// group at a time with the next one asked for ahead 373.
+// through the caches 209; rows at 32-bit offsets 264 (more registers than there are); the queries by the
+// forward's kernel and the rest by this one 121 + 84; one group at a time with the next one asked for ahead 373.
 // ----------------------------------------------------------------------------
 
 // x of lane ^ 1, ^ 2, and of lanes that hold the other halves of 8 and of 16 (equal within 4 and 8).

@@ -61,10 +61,12 @@ struct WeighWalk {
 // ----------------------------------------------------------------------------
 // Many rows.  KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
 // What bounds it: matrix and vector instructions (of these the 16 exp2 of a tile most), at a clock that
-// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 360 us, 764 TFLOP/s at 2.0 GHz, the
+// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 345 us, 797 TFLOP/s at 2.0 GHz, the
 // matrix units busy 39% of the cycles, the vector units 57%.  Four stages with all of a part's lse loaded
-// ahead (367), two key tiles a wave (411), and the last chunk's exp2 between this one's products (357 to
-// 374) changed nothing: what overlaps more runs at a lower clock.
+// ahead (367 beside 360), two key tiles a wave (411), and the last chunk's exp2 between this one's products
+// (357 to 374) gained nothing: what overlaps more runs at a lower clock.  Short walks wait for their starts:
+// the last 32 tokens of two requests of up to 32768, 16 / 4 heads of 64 in 4 bits, 19 us, four chunks a
+// workgroup; the weights so far loaded with the keys instead of at the end changed nothing.
 // ----------------------------------------------------------------------------
 template <int DT, int KD, bool Q4>
 __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache_weights_kernel(WeighArgs a) {
