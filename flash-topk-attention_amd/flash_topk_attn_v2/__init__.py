@@ -10,7 +10,10 @@ Beside it, without counterpart in the reference, what a model puts around such
 attention: ``flash_qk_norm_rope`` in front of it, ``flash_window_attn`` for its local
 layers (both differentiable), and the serving forms over K/V caches
 ``flash_qk_norm_rope_append``, ``flash_window_attn_decode`` and
-``flash_prefix_attn_decode``.
+``flash_prefix_attn_decode``.  For long caches: ``Q4Cache``, keys and values in 4 bits, with
+``flash_qk_norm_rope_append_q4``, ``flash_window_attn_decode_q4`` and
+``flash_q4_cache_read``; and ``flash_cache_weights`` with ``flash_cache_evict``, which cut a cache to
+the rows that received most attention.
 """
 
 from __future__ import annotations

@@ -52,8 +52,10 @@ def flash_cache_weights(
     keys, ``[B, S, num_kv_heads * D]`` of q's type with rows 16-byte aligned, or a
     ``Q4Cache``.  ``cache_lens`` (int32 ``[B]`` on the device, not read by the host) counts the
     cached tokens with these T; token t sees key j as in ``flash_window_attn_decode``; tokens
-    that see nothing (lse = -inf) add nothing.  ``weights`` is float32 ``[B, num_kv_heads, S]``,
-    written in place where ``j < cache_lens[b]``.  Unseen rows of the cache may hold anything.
+    that see nothing (lse = -inf) add nothing.  (Tokens are the last T of each request: prompts of
+    different lengths that are padded behind their ends go one by one.)  ``weights`` is float32
+    ``[B, num_kv_heads, S]``, written in place where ``j < cache_lens[b]``, and overlaps no other
+    argument.  Unseen rows of the cache may hold anything.
     Sums are float32 in a fixed order.  Not differentiable.
 
     Returns ``weights``.

@@ -131,7 +131,8 @@ def flash_qk_norm_rope_append_q4(
     ``round(x / scale) + 8``, ties to even, held to 0 .. 15.  A column is off by at most half
     a scale, a sixteenth of its group's largest magnitude, but for values near the largest
     one's opposite, which are off by up to a whole scale.  Groups of magnitudes below 2.4e-7
-    are held as zeros.  Other arguments as for ``flash_qk_norm_rope_append``.  Not
+    are held as zeros.  Values must be finite: infinities and NaN leave finite
+    values of no meaning in their group.  Other arguments as for ``flash_qk_norm_rope_append``.  Not
     differentiable.
 
     Returns the prepared q ``[B, T, num_heads * D]``, which is not quantized.

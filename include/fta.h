@@ -582,7 +582,7 @@ int fta_q4_attn(const void* q, const int64_t* q_strides, const void* k_codes, co
  * cache_lens[b] (no counterpart in the reference).  k: 16-bit keys [B][S][Hk][D] strided, and
  * k_scales null; or the key codes of a 4-bit cache ({stride_b, stride_h} in bytes) with their
  * scales.  lse [B][H][T]; rows of -inf add nothing.  w_strides {b, head} in elements, rows
- * follow each other.  No atomics; the workspace (fta_cache_weights_workspace_size bytes) holds
+ * follow each other; weights overlap no other argument.  No atomics; the workspace (fta_cache_weights_workspace_size bytes) holds
  * the parts of split walks.
  */
 size_t fta_cache_weights_workspace_size(int B, int H, int Hk, int T, int S, int D, int left, int num_sinks);
@@ -599,7 +599,8 @@ int fta_cache_weights(const void* q, const int64_t* q_strides, const void* k, co
  * row_bytes[i] bytes (even, up to 512) at byte strides {b, head, row} 3 i .. 3 i + 2.  Either every
  * dst is its src and weights_out is weights, or none (they must not overlap then).
  * Behind the rows that stayed weights are set to zero: up to len in place, up to S_out otherwise.
- * new_lens [B]; kept [B][Hk][budget]: the former row of each row, -1 behind them.
+ * new_lens [B]; kept [B][Hk][budget]: the former row of each row, -1 behind them; they overlap no
+ * other argument, cache_lens included.
  */
 int fta_cache_evict(int tensors, const void* const* src, const int64_t* src_strides, void* const* dst,
                     const int64_t* dst_strides, const int32_t* row_bytes, const float* weights, const int64_t* w_strides,
