@@ -8,7 +8,7 @@
 // S = Q K^T with the keys as columns: a wave keeps 32 keys in registers, one to a lane and its
 // mirror, and walks over all the rows that see them, 32 at a time; a key's sum stays in its lane.
 // So a key is read once, no sum crosses lanes, and there are no atomics (the same bits every run).
-// The rows come through LDS, shared by the four waves: TT tokens x GG query heads of the group,
+// Many rows come through LDS, shared by the four waves: TT tokens x GG query heads of the group,
 // as many heads as it takes to fill 32 rows where there are few tokens.
 #include "fta_common.h"
 #include "fta_host.h"
@@ -37,6 +37,7 @@ struct WeighArgs {
     int GG, TT, groups;  // query heads and tokens of 32 rows; head groups of a K/V head
     int tiles, per, np, total;  // key tiles; chunks of 32 rows in a part, parts of the longest walk
     float c;
+    int chunks;   // of 32 rows, where they all stay in LDS; else 0
     bool few;     // the rows stay in registers
     bool narrow;  // a chunk's rows are within 32-bit offsets
 };
@@ -58,15 +59,111 @@ struct WeighWalk {
     }
 };
 
+// 32 keys, one to a lane and its mirror, as they are loaded, and as B operands.
+template <int DT, int KD, bool Q4>
+struct KeyRows {
+    static constexpr int KS = KD / 16, NG = KD / 32;
+    uint32_t w[Q4 ? 2 * NG : 4 * KS];
+    uint16_t d[Q4 ? NG : 1];
+    __device__ __forceinline__ void load(const WeighArgs& a, int b, int hk, int64_t row, bool ok, int lane) {
+        const int hf = lane >> 5;
+        const uint8_t* p = a.k + b * a.k_sb + hk * a.k_sh + row * a.k_sn;
+        if constexpr (Q4) {
+            const uint32_t* kp = reinterpret_cast<const uint32_t*>(p);
+            const uint16_t* scales = a.ks + b * a.ks_sb + hk * a.ks_sh + row * NG;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                d[g] = scales[g];
+#pragma unroll
+                for (int m = 0; m < 2; ++m) w[2 * g + m] = kp[(2 * hf + m) * NG + g];  // octet 2 hf + m of the group
+            }
+        } else {
+            fta_frag f[KS];
+            FtaTile<DT, KD>::load_rows(reinterpret_cast<const uint16_t*>(p), ok, a.Dreal, lane, f);
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[4 * i + e] = f[i][e];
+        }
+    }
+    __device__ __forceinline__ void operands(const WeighArgs& a, int lane, fta_frag (&kf)[KS], float (&ds)[NG]) const {
+        const int hf = lane >> 5;
+        if constexpr (Q4) {
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                ds[g] = (float)__builtin_bit_cast(_Float16, d[g]);
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {  // the group's first or second product
+                    float n[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) n[e] = (float)((int)((w[2 * g + m] >> (4 * e)) & 15u) - 8);
+                    kf[2 * g + m] = 32 * g + 16 * hf + 8 * m < a.Dreal ? fta_pack_frag<DT>(n) : fta_frag{0u, 0u, 0u, 0u};
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) kf[i] = fta_frag{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        }
+    }
+};
+
+// What chunk c's 32 rows, in LDS at `rows` with -lse log2(e) at sl, add to this lane's key kt + (lane & 31).
+template <int DT, int KD, bool Q4>
+__device__ __forceinline__ float chunk_sum(const WeighArgs& a, const fta_frag (&kf)[KD / 16], const float (&ds)[KD / 32],
+                                           uint32_t rows, const float* sl, int c, int kt, int len, int lane) {
+    constexpr int QSEG = KD / 8, KS = KD / 16, NG = KD / 32;
+    using SW = FtaSwz<QSEG>;
+    const int hf = lane >> 5, key = kt + (lane & 31);
+    const int q_lo = len - a.T + c * a.TT, q_hi = min(q_lo + a.TT, len) - 1;  // positions of the chunk's tokens
+    if (q_hi < kt || (kt + 31 < q_lo - a.left && kt >= a.sinks)) return 0.f;  // wave-uniform
+    const uint32_t ro = rows + (lane & 31) * QSEG * 16u;
+    auto frag = [&](int slot) { return fta_lds_frag(ro + 16u * (slot ^ SW::x(lane & 31))); };
+    f32x16 x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = 0.f;
+    if constexpr (Q4) {
+#pragma unroll
+        for (int g = 0; g < NG; ++g) {
+            f32x16 y;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = 0.f;
+            y = fta_mma<DT>(frag(4 * g + 2 * hf), kf[2 * g], y);
+            y = fta_mma<DT>(frag(4 * g + 2 * hf + 1), kf[2 * g + 1], y);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = fmaf(ds[g], y[i], x[i]);
+        }
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) x = fta_mma<DT>(frag(2 * ks + hf), kf[ks], x);
+    }
+    if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
+        asm volatile("");  // an edge: kept apart, or every chunk pays for it
+        // the rows of the tokens that see this lane's key
+        const int64_t t_hi = key < a.sinks ? a.TT - 1 : min((int64_t)key + a.left - q_lo, (int64_t)a.TT - 1);
+        const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
+        const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
+        FtaTile<DT, KD>::mask(fta_bits_below(rhi) & ~fta_bits_below(rlo), lane, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 l = *reinterpret_cast<const float4*>(&sl[c_row(i, lane)]);
+        x[i] = fta_exp2(fmaf(x[i], a.c, l.x));
+        x[i + 1] = fta_exp2(fmaf(x[i + 1], a.c, l.y));
+        x[i + 2] = fta_exp2(fmaf(x[i + 2], a.c, l.z));
+        x[i + 3] = fta_exp2(fmaf(x[i + 3], a.c, l.w));
+    }
+    return ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) +
+           (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+}
+
 // ----------------------------------------------------------------------------
 // Many rows.  KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
 // What bounds it: matrix and vector instructions (of these the 16 exp2 of a tile most), at a clock that
 // their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 345 us, 797 TFLOP/s at 2.0 GHz, the
 // matrix units busy 39% of the cycles, the vector units 57%.  Four stages with all of a part's lse loaded
 // ahead (367 beside 360), two key tiles a wave (411), and the last chunk's exp2 between this one's products
-// (357 to 374) gained nothing: what overlaps more runs at a lower clock.  Short walks wait for their starts:
-// the last 32 tokens of two requests of up to 32768, 16 / 4 heads of 64 in 4 bits, 19 us, four chunks a
-// workgroup; the weights so far loaded with the keys instead of at the end changed nothing.
+// (357 to 374) gained nothing: what overlaps more runs at a lower clock.  The weights so far
+// loaded with the keys instead of at the end changed nothing.
 // ----------------------------------------------------------------------------
 template <int DT, int KD, bool Q4>
 __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache_weights_kernel(WeighArgs a) {
@@ -74,7 +171,7 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     using SW = FtaSwz<QSEG>;
     __shared__ __align__(1024) unsigned char sQ[2][TILE_B];
     __shared__ __align__(16) float sL[2][32];  // -lse log2(e), -inf for rows that do not count
-    const int lane = threadIdx.x & 63, hf = lane >> 5;
+    const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wgi = fta_xcd_remap(blockIdx.x, a.total);
     const int u = fta_scalar(wgi / a.np), sp = wgi - u * a.np;
@@ -82,7 +179,6 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
     const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
     const int kt = kWeighKeys * tile + 32 * wave, key = kt + (lane & 31);  // this wave's first key, this lane's
-    const int p0 = len - a.T;                                             // position of the first new token
     const WeighWalk walk(a, len, kWeighKeys * tile);
     const int c_lo = walk.c_lo, nct = walk.nct;
     const int64_t all = (int64_t)nct * a.groups;
@@ -137,33 +233,15 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
             }
         }
     };
-    const uint32_t ro = ldq + (lane & 31) * QSEG * 16u;
-    auto frag = [&](int st, int slot) { return fta_lds_frag(ro + st * TILE_B + 16u * (slot ^ SW::x(lane & 31))); };
     int cg = fta_scalar(s0 / nct), ct = c_lo + s0 - cg * nct;
     issue(ct, cg, 0);
-    // this wave's keys as B operands
     fta_frag kf[KS];
-    float ds[NG];  // 4-bit keys: the key's scales
-    const bool kok = key < a.S;
-    const int64_t krow = kok ? key : 0;
-    if constexpr (Q4) {
-        const uint32_t* kp = reinterpret_cast<const uint32_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
-        const uint16_t* scales = a.ks + b * a.ks_sb + hk * a.ks_sh + krow * NG;
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            ds[g] = (float)__builtin_bit_cast(_Float16, scales[g]);
-#pragma unroll
-            for (int m = 0; m < 2; ++m) {  // octet 2 hf + m of the group: the first or second product's
-                const uint32_t word = kp[(2 * hf + m) * NG + g];
-                float n[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) n[e] = (float)((int)((word >> (4 * e)) & 15u) - 8);
-                kf[2 * g + m] = 32 * g + 16 * hf + 8 * m < a.Dreal ? fta_pack_frag<DT>(n) : fta_frag{0u, 0u, 0u, 0u};
-            }
-        }
-    } else {
-        const uint16_t* kp = reinterpret_cast<const uint16_t*>(a.k + b * a.k_sb + hk * a.k_sh + krow * a.k_sn);
-        FtaTile<DT, KD>::load_rows(kp, kok, a.Dreal, lane, kf);
+    float ds[NG];
+    {
+        KeyRows<DT, KD, Q4> keys;
+        const bool kok = key < a.S;
+        keys.load(a, b, hk, kok ? key : 0, kok, lane);
+        keys.operands(a, lane, kf, ds);
     }
     float run = 0.f, sum = 0.f;
     int st = 0;
@@ -183,44 +261,7 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
             sum += run;
             run = 0.f;
         }
-        const int q_lo = p0 + c * a.TT, q_hi = min(q_lo + a.TT, len) - 1;  // positions of the chunk's tokens
-        if (q_hi < kt || (kt + 31 < q_lo - a.left && kt >= a.sinks)) continue;  // wave-uniform
-        f32x16 x;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.f;
-        if constexpr (Q4) {
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                f32x16 y;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = 0.f;
-                y = fta_mma<DT>(frag(st, 4 * g + 2 * hf), kf[2 * g], y);
-                y = fta_mma<DT>(frag(st, 4 * g + 2 * hf + 1), kf[2 * g + 1], y);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = fmaf(ds[g], y[i], x[i]);
-            }
-        } else {
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) x = fta_mma<DT>(frag(st, 2 * ks + hf), kf[ks], x);
-        }
-        if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
-            asm volatile("");  // an edge: kept apart, or every chunk pays for it
-            // the rows of the tokens that see this lane's key
-            const int64_t t_hi = key < a.sinks ? a.TT - 1 : min((int64_t)key + a.left - q_lo, (int64_t)a.TT - 1);
-            const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
-            const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
-            FtaTile<DT, KD>::mask(fta_bits_below(rhi) & ~fta_bits_below(rlo), lane, x);
-        }
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 l = *reinterpret_cast<const float4*>(&sL[st][c_row(i, lane)]);
-            x[i] = fta_exp2(fmaf(x[i], a.c, l.x));
-            x[i + 1] = fta_exp2(fmaf(x[i + 1], a.c, l.y));
-            x[i + 2] = fta_exp2(fmaf(x[i + 2], a.c, l.z));
-            x[i + 3] = fta_exp2(fmaf(x[i + 3], a.c, l.w));
-        }
-        run += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7])) +
-               (((x[8] + x[9]) + (x[10] + x[11])) + ((x[12] + x[13]) + (x[14] + x[15])));
+        run += chunk_sum<DT, KD, Q4>(a, kf, ds, ldq + st * TILE_B, sL[st], c, kt, len, lane);
     }
     sum += run;
     sum += fta_xor32(sum);
@@ -229,6 +270,85 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
         a.part[((int64_t)sp * a.B * a.Hk + bhk) * a.S + key] = sum;
     else
         a.w[b * a.w_sb + hk * a.w_sh + key] += sum;
+}
+
+// ----------------------------------------------------------------------------
+// Rows that stay in LDS, up to kHeld chunks of 32: the last tokens of a prompt, or several tokens of a step. They are
+// loaded once, and the keys stream past: a workgroup takes a run of keys, its waves 32-key tiles in turn, the
+// next tile's asked for ahead.
+// What bounds it: memory for 16-bit keys (64 requests x 12 tokens on 4096 to 8192, 32 / 8 heads of 128: 196 us, 4.2
+// TB/s), vector instructions for 4-bit ones (156 us).  The kernel of many rows, which starts anew for every 128
+// keys, takes 216 and 273; 2 x 32 tokens on up to 32768 4-bit keys, 16 / 4 heads of 64, 17.5 and 19.5.  Eight chunks,
+// which leave two waves a SIMD at 128 columns, are slower than it: 64 tokens, 40 us and 32.
+// ----------------------------------------------------------------------------
+constexpr int kHeld = 4;
+template <int DT, int KD, bool Q4>
+__global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows_kernel(WeighArgs a) {
+    constexpr int QSEG = KD / 8, KS = KD / 16, NG = KD / 32, BLOCKS = QSEG / 2, TILE_B = 32 * QSEG * 16, NW = 4;
+    using SW = FtaSwz<QSEG>;
+    __shared__ __align__(1024) unsigned char sQ[kHeld][TILE_B];
+    __shared__ __align__(16) float sL[kHeld][32];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int bhk = fta_scalar(blockIdx.x / a.np), sp = blockIdx.x - bhk * a.np;
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
+    // 32-key tiles: the sinks', then the band's
+    const int kb0 = max(0, len - a.T - a.left);
+    int ns = (min(a.sinks, len) + 31) >> 5, c_lo = kb0 >> 5;
+    const int c_hi = (len + 31) >> 5;
+    if (c_lo <= ns) c_lo = ns = 0;
+    const int all = max(ns + c_hi - c_lo, 0);
+    const int it0 = fta_scalar((int)((int64_t)all * sp / a.np)), it1 = fta_scalar((int)((int64_t)all * (sp + 1) / a.np));
+    if (it0 >= it1) return;  // all waves
+
+    const uint16_t* qp = a.q + b * a.q_sb + (int64_t)hk * a.G * a.q_sh;
+    const float* lp = a.lse + ((int64_t)b * a.H + (int64_t)hk * a.G) * a.T;
+    const uint32_t ldq = fta_lds_addr(&sQ[0][0]);
+    const int nct = a.chunks / a.groups;  // chunk = head group * nct + tokens / TT
+    for (int i = wave; i < a.chunks * BLOCKS; i += NW) {
+        const int ch = i / BLOCKS, blk = i - ch * BLOCKS, cg = ch / nct, ct = ch - cg * nct;  // wave-uniform
+        const int s = blk * 64 + lane, row = s / QSEG, j = SW::slot(row, s - row * QSEG);
+        const bool has = row < a.TT * a.GG;
+        const int tt = has ? row / a.GG : 0, gg = has ? row - tt * a.GG : 0;  // rows that are not there repeat others
+        const int64_t t = min(ct * a.TT + tt, a.T - 1), g = min(cg * a.GG + gg, a.G - 1);
+        fta_dma16_at(qp + t * a.q_sn + g * a.q_sh + (j * 8 < a.Dreal ? j * 8 : 0), ldq + i * 1024);
+    }
+    for (int i = threadIdx.x; i < a.chunks * 32; i += 256) {
+        const int ch = i >> 5, row = i & 31, cg = ch / nct, ct = ch - cg * nct;
+        const int t = ct * a.TT + row / a.GG, g = cg * a.GG + row % a.GG;
+        const bool ok = row < a.TT * a.GG && t < a.T && g < a.G;
+        const float x = lp[ok ? (int64_t)g * a.T + t : 0];
+        sL[ch][row] = ok && x != -FTA_INF ? -x * kLog2e : -FTA_INF;  // a row that saw nothing gives nothing
+    }
+    float* wp = a.w + b * a.w_sb + hk * a.w_sh;
+    auto tile = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
+    struct Tile {
+        KeyRows<DT, KD, Q4> keys;
+        float before;
+    };
+    auto ask = [&](int it, Tile& x) __attribute__((always_inline)) {
+        const int j = min(tile(it) + (lane & 31), len - 1);  // behind the last token: masked, and not written
+        x.keys.load(a, b, hk, j, true, lane);
+        x.before = wp[j];
+    };
+    Tile cur, nxt;
+    if (it0 + wave < it1) ask(it0 + wave, cur);
+    fta_wait_vmcnt<0>();
+    __syncthreads();
+    for (int it = it0 + wave; it < it1; it += NW) {
+        if (it + NW < it1) ask(it + NW, nxt);
+        fta_frag kf[KS];
+        float ds[NG];
+        cur.keys.operands(a, lane, kf, ds);
+        const int kt = tile(it), key = kt + (lane & 31);
+        float sum = 0.f;
+        for (int cg = 0, ch = 0; cg < a.groups; ++cg)
+            for (int ct = 0; ct < nct; ++ct, ++ch) sum += chunk_sum<DT, KD, Q4>(a, kf, ds, ldq + ch * TILE_B, sL[ch], ct, kt, len, lane);
+        sum += fta_xor32(sum);
+        if (lane < 32 && key < len) wp[key] = cur.before + sum;
+        cur = nxt;
+    }
 }
 
 // ----------------------------------------------------------------------------
@@ -401,16 +521,28 @@ int weigh_plan(WeighArgs& a, bool q4, int B, int H, int Hk, int T, int S, int D,
     a.groups = (a.G + a.GG - 1) / a.GG;
     const int64_t most = (1 << 24) - 1, heads = (int64_t)B * Hk;
     a.few = (int64_t)T * a.G <= 32;
+    const int64_t tiles = (std::min<int64_t>(S, (int64_t)a.left + T + a.sinks + 62) + 31) / 32;  // of 32 keys
+    auto parts = [&](int64_t target, int64_t least) { return std::min<int64_t>((target + heads - 1) / heads, tiles / least); };
     if (a.few) {
         // Parts cost nothing but a workgroup's start (every key is its own): enough to fill the chip, down to one
         // tile of a wave, and about 16384 of two tiles and more, whose starts overlap with others' ends; 4-bit tiles
         // are shorter, 2048 of four.  Target 2048 / 8192 / 16384 / 65536 (the last down to one tile), us, 64 requests
         // of 4096 to 8192 tokens, 32 / 8 heads: of 128 193 / 161 / 154 / 158, of 64 123 / 89 / 85 / 90, of 128 in 4
         // bits 66 / 71 / 83 / 113.
-        const int64_t tiles = (std::min<int64_t>(S, (int64_t)a.left + T + a.sinks + 62) + 31) / 32;
-        auto parts = [&](int64_t target, int64_t least) { return std::min<int64_t>((target + heads - 1) / heads, tiles / least); };
         const int64_t np = std::max<int64_t>(1, std::max(parts(1024, 4), q4 ? parts(2048, 16) : parts(16384, 8)));
         if (heads * np > most) return fta::unsupported("cache_weights: too many heads");
+        a.np = (int)np;
+        a.total = (int)(heads * np);
+        return FTA_OK;
+    }
+    const int64_t held = (int64_t)((T + a.TT - 1) / a.TT) * a.groups;
+    if (held <= kHeld) {
+        // Parts as above, of two tiles a wave and more.  Target 1024 / 2048 / 4096 / 16384, us, 32 / 8 heads of 128, 4096
+        // to 8192 tokens: 64 requests x 12 246 / 243 / 226 / 196, 16 x 16 69 / 63 / 62 / 61; 64 x 12 in 4 bits
+        // 177 / 156 / 155 / 205, 18 x 16 of up to 16028, 16 / 4 heads of 256 in 4 bits, 126 / 132 / 149 / 149.
+        const int64_t np = std::max<int64_t>(1, std::max(parts(1024, 8), q4 ? parts(2048, 16) : parts(16384, 8)));
+        if (heads * np > most) return fta::unsupported("cache_weights: too many heads");
+        a.chunks = (int)held;
         a.np = (int)np;
         a.total = (int)(heads * np);
         return FTA_OK;
@@ -434,7 +566,7 @@ int weigh_plan(WeighArgs& a, bool q4, int B, int H, int Hk, int T, int S, int D,
     return FTA_OK;
 }
 
-size_t weigh_bytes(const WeighArgs& a) { return a.few || a.np <= 1 ? 0 : fta::align_up((size_t)a.np * a.B * a.Hk * a.S * sizeof(float)); }
+size_t weigh_bytes(const WeighArgs& a) { return a.few || a.chunks > 0 || a.np <= 1 ? 0 : fta::align_up((size_t)a.np * a.B * a.Hk * a.S * sizeof(float)); }
 
 template <int DT, int KD, bool Q4>
 int launch_weigh(const WeighArgs& a, hipStream_t st) {
@@ -445,6 +577,10 @@ int launch_weigh(const WeighArgs& a, hipStream_t st) {
         else
             hipLaunchKernelGGL((fta_cache_weights_step_kernel<DT, KD, Q4, 2>), grid, t, 0, st, a);
         return fta::check_launch("fta_cache_weights_step_kernel");
+    }
+    if (a.chunks > 0) {
+        hipLaunchKernelGGL((fta_cache_weights_rows_kernel<DT, KD, Q4>), grid, t, 0, st, a);
+        return fta::check_launch("fta_cache_weights_rows_kernel");
     }
     hipLaunchKernelGGL((fta_cache_weights_kernel<DT, KD, Q4>), grid, t, 0, st, a);
     int rc = fta::check_launch("fta_cache_weights_kernel");

@@ -203,3 +203,22 @@ def test_a_token_that_is_not_finite_stays_with_its_keys(gpu, T, H, Hk, left, sin
         sees[max(0, p - left):p + 1] = True
         sees[:sinks] = True
         assert got[0, :, sees].isnan().all() and torch.equal(got[0, :, ~sees], want[0, :, ~sees])
+
+
+# rows that stay in LDS while keys stream past: windows, sinks, lengths under T, several tiles of a wave
+HELD = [
+    (BF, 5, 24, 8, 2, 128, 3001, 1500, 40, [3001, 2000, 24, 10, 0]),
+    (FP, 2, 128, 2, 2, 64, 5000, 5000, 0, [5000, 127]),
+    (BF, 1, 12, 40, 4, 80, 2100, 300, 100, [2099]),          # ten heads: 30 rows of 32
+    (FP, 3, 33, 6, 2, 256, 1200, 1200, 3, [1200, 33, 1]),
+    (BF, 40, 9, 8, 2, 96, 4000, 2000, 0, None),
+    (FP, 1, 64, 4, 2, 16, 70, 5, 1, [70]),
+]
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+@pytest.mark.parametrize("case", HELD, ids=lambda c: "-".join(str(x) for x in c[1:9]))
+def test_weights_of_held_rows(gpu, case, q4):
+    if case[-1] is None:
+        case = (*case[:-1], torch.randint(0, case[6] + 1, (case[1],), generator=torch.Generator().manual_seed(2)).tolist())
+    test_weights(gpu, case, q4)
