@@ -159,7 +159,7 @@ __device__ __forceinline__ float chunk_sum(const WeighArgs& a, const fta_frag (&
 // ----------------------------------------------------------------------------
 // Many rows.  KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
 // What bounds it: matrix and vector instructions (of these the 16 exp2 of a tile most), at a clock that
-// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 345 us, 797 TFLOP/s at 2.0 GHz, the
+// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 334 to 364 us by run, 797 TFLOP/s at 2.0 GHz, the
 // matrix units busy 39% of the cycles, the vector units 57%.  Four stages with all of a part's lse loaded
 // ahead (367 beside 360), two key tiles a wave (411), and the last chunk's exp2 between this one's products
 // (357 to 374) gained nothing: what overlaps more runs at a lower clock.  The weights so far
@@ -557,8 +557,10 @@ int weigh_plan(WeighArgs& a, bool q4, int B, int H, int Hk, int T, int S, int D,
     const int64_t mean = chunks(std::min<int64_t>(span, T - std::max<int64_t>(0, T - ((int64_t)S - T)) / 2));
     // Parts of 32 chunks and more, about 4096 of them: causal walks shorten with the key, and tiles of sinks
     // walk every token.  Target 1024 / 2048 / 4096 / 8192, us: 8192 tokens 523 / 440 / 361 / 361; least 32 / 64
-    // chunks: 2048 tokens 46 / 66.
-    a.per = (int)std::min<int64_t>(longest, std::max<int64_t>(32, wgs * mean / 4096));
+    // chunks: 2048 tokens 46 / 66.  Down to 8 chunks where they would not be 1024 parts, least 32 / 16 / 8 / 4, us of
+    // both kernels: 6 x 456 tokens, 8 heads on one, 39 / 24 / 19 / 21, 8 x 512, 32 / 8 heads, 41 / 35 / 35 / 36.
+    const int64_t work = wgs * mean;
+    a.per = (int)std::min(longest, std::max(std::clamp<int64_t>(work / 1024, 8, 32), work / 4096));
     a.np = (int)((longest + a.per - 1) / a.per);
     if (wgs * a.np > most || heads > 65535 || heads * ((S + 255) / 256) > most)
         return fta::unsupported("cache_weights: too many keys");
