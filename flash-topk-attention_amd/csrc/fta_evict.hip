@@ -8,7 +8,8 @@
 //  * fta_evict_select_kernel, one workgroup of 1024 threads per (b, K/V head): the weight of the
 //    last row to stay is found digit by digit (11, 11 and 10 bits of the weights as ordered
 //    integers, a histogram in LDS for each), then every wave counts what it keeps of its own run
-//    of rows and writes their numbers behind those of the waves in front of it.
+//    of rows and writes their numbers behind those of the waves in front of it.  Up to 1024 rows
+//    take one wave each instead, fta_evict_select_wave_kernel.
 //  * fta_evict_move_kernel moves the rows.  In place, destinations never lie behind their sources
 //    and both ascend, so a workgroup that reads a block of rows, waits, and then writes it may go
 //    on to the next block: nothing that later blocks read has been written.  What can run side by
@@ -189,6 +190,62 @@ __global__ __launch_bounds__(kSelThreads) void fta_evict_select_kernel(EvictArgs
     });
 }
 
+// The same by one wave for up to 64 PT rows: the weight of the last row to stay is found bit by bit, by the
+// number of rows at or above it, until that number is the budget.  No LDS and no barriers.
+// What bounds it: latency, a compare, a count and an addition that wait for each other for every 64 rows.  481 rows, 512
+// heads: 7.8 us, the workgroup's kernel 14; 704 rows, 404 heads: 12.3 and 15.3.  2048 rows, 8 heads, would be 17 and 10.
+template <int PT>
+__global__ __launch_bounds__(256) void fta_evict_select_wave_kernel(EvictArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int bhk = fta_scalar(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (bhk >= a.B * a.Hk) return;
+    const int b = fta_scalar(bhk / a.Hk), hk = bhk - b * a.Hk;
+    const int len = __builtin_amdgcn_readfirstlane(min(max(a.lens[b], 0), a.S));
+    int32_t* kept = a.kept + (int64_t)bhk * a.budget;
+    if (hk == 0 && lane == 0) a.new_lens[b] = min(len, a.budget);
+    if (len <= a.budget) {
+        for (int i = lane; i < a.budget; i += 64) kept[i] = i < len ? i : -1;
+        return;
+    }
+    const float* w = a.w + b * a.w_sb + hk * a.w_sh;
+    const int hi = len - a.recent;
+    float x[PT];
+    uint32_t held[PT];
+#pragma unroll
+    for (int i = 0; i < PT; ++i) x[i] = w[min(64 * i + lane, len - 1)];
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+        const int j = 64 * i + lane;
+        held[i] = j >= len ? 0u : (j < a.sinks || j >= hi) ? kAlways : ordered(x[i]);
+    }
+    auto count = [&](auto f) __attribute__((always_inline)) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < PT; ++i) n += __popcll(__ballot(f(held[i])));
+        return n;
+    };
+    uint32_t last = 0;  // more than `budget` rows are there, so it ends above 0, which stands for none
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t c = last | 1u << bit;
+        const int n = count([&](uint32_t v) { return v >= c; });
+        if (n >= a.budget) last = c;
+        if (n == a.budget) break;
+    }
+    const int need = a.budget - count([&](uint32_t v) { return v > last; });
+    const uint64_t below = (1ull << lane) - 1;
+    int eqs = 0, at = 0;
+#pragma unroll
+    for (int i = 0; i < PT; ++i) {
+        const uint64_t ties = __ballot(held[i] == last);
+        const bool stay = held[i] > last || (held[i] == last && eqs + __popcll(ties & below) < need);
+        const uint64_t all = __ballot(stay);
+        const int p = at + __popcll(all & below);
+        if (stay && p < a.budget) kept[p] = 64 * i + lane;
+        at += __popcll(all);
+        eqs += __popcll(ties);
+    }
+}
+
 // ----------------------------------------------------------------------------
 // The move: workgroup = (b, K/V head, slice) in place, (b, K/V head, slice, block of rows) into
 // another cache.  A thread moves one access of a row, kMove rows at a time.
@@ -196,10 +253,11 @@ __global__ __launch_bounds__(kSelThreads) void fta_evict_select_kernel(EvictArgs
 // other.  16 x 8 heads of 128 bf16, 8192 rows to 4096: 146 us in place, 117 into another cache (537 MB:
 // 3.7 and 4.6 TB/s); 64 x 8 heads of 128 in 4 bits, 16384 to 4096: 176 us (604 MB; single rows of 64 and 8
 // bytes out of 128-byte lines); 1 x 8 heads, 32768 to 8192: 34 us.  In place with 512 threads instead of
-// 1024 152 / 184 / 42 us, with eight rows a thread 174 / 194 / 39.
+// 1024 152 / 184 / 42 us, with eight rows a thread 174 / 194 / 39.  Where few rows stay most of 1024 threads have
+// none, and 256 move them: 346 rows of 64 x 8 heads bf16 45 -> 27 us, 345 rows of 101 x 4 heads in 4 bits 26 -> 11, 1024
+// rows of 128 x 8 in 4 bits 100 -> 75; but of 8 heads 1024 rows 6.8 -> 11.5, 4096 of 16 x 8 155 -> 171.
 // ----------------------------------------------------------------------------
 constexpr int kMove = 4;
-constexpr int move_threads(bool in_place) { return in_place ? 1024 : 512; }
 // Bytes of a row that one workgroup moves: the fewest that memory reads at once.  32 / 64 / 128 / 256, us of
 // the kernel: in place, 8192 rows to 4096, 16 x 8 heads of 128 bf16 (537 MB moved) 244 / 153 / 155 / 174,
 // 32768 to 8192, 1 x 8 heads 46 / 42 / 75 / 141; into another cache, 16 x 8 heads 202 / 121 / 119 / 125.
@@ -214,12 +272,12 @@ __device__ __forceinline__ void arrived(uint16_t& x) { asm volatile("" : "+v"(x)
 // Rows [first, last) of (b, hk), this slice of them, kMove accesses of a thread in a block of rows.
 // The next block's rows are asked for before this one's are written: they lie behind everything
 // that this one writes.
-template <typename V, bool IN_PLACE>
+template <typename V, bool IN_PLACE, int NT>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, const Moved& t, int b, int hk, int slice, int first, int last,
                                           const int32_t* kept) {
     const int u0 = slice * t.slice, un = min(t.slice, t.units - u0);  // this slice's accesses
     const int row0 = threadIdx.x / t.slice, u = threadIdx.x - row0 * t.slice;
-    const int rows = move_threads(IN_PLACE) / t.slice;  // rows of one access of the workgroup
+    const int rows = NT / t.slice;  // rows of one access of the workgroup
     const bool mine = u < un && row0 < rows;
     const uint8_t* src = t.src + b * t.s_sb + hk * t.s_sh + (int64_t)(u0 + u) * sizeof(V);
     uint8_t* dst = t.dst + b * t.d_sb + hk * t.d_sh + (int64_t)(u0 + u) * sizeof(V);
@@ -258,8 +316,8 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Moved& t, in
     }
 }
 
-template <bool IN_PLACE>
-__global__ __launch_bounds__(move_threads(IN_PLACE)) void fta_evict_move_kernel(EvictArgs a) {
+template <bool IN_PLACE, int NT>
+__global__ __launch_bounds__(NT) void fta_evict_move_kernel(EvictArgs a) {
     const int wgi = blockIdx.x;
     const int rest = wgi / a.blocks, block = wgi - rest * a.blocks;
     const int bhk = rest / a.jobs;
@@ -275,10 +333,10 @@ __global__ __launch_bounds__(move_threads(IN_PLACE)) void fta_evict_move_kernel(
         const int first = min(block * per, n), last = min(n, first + per);
         if (first < last) {
             switch (t.unit) {
-                case 16: move_rows<uint4, IN_PLACE>(a, t, b, hk, job, first, last, kept); break;
-                case 8: move_rows<uint2, IN_PLACE>(a, t, b, hk, job, first, last, kept); break;
-                case 4: move_rows<uint32_t, IN_PLACE>(a, t, b, hk, job, first, last, kept); break;
-                default: move_rows<uint16_t, IN_PLACE>(a, t, b, hk, job, first, last, kept);
+                case 16: move_rows<uint4, IN_PLACE, NT>(a, t, b, hk, job, first, last, kept); break;
+                case 8: move_rows<uint2, IN_PLACE, NT>(a, t, b, hk, job, first, last, kept); break;
+                case 4: move_rows<uint32_t, IN_PLACE, NT>(a, t, b, hk, job, first, last, kept); break;
+                default: move_rows<uint16_t, IN_PLACE, NT>(a, t, b, hk, job, first, last, kept);
             }
         }
     }
@@ -286,11 +344,17 @@ __global__ __launch_bounds__(move_threads(IN_PLACE)) void fta_evict_move_kernel(
     // weights of the rows behind those that stayed start again at zero (in place every weight has
     // been read: the last block's are waited for before it is written)
     const int end = IN_PLACE ? len : a.S_out;
-    for (int j = n + block * move_threads(IN_PLACE) + threadIdx.x; j < end; j += a.blocks * move_threads(IN_PLACE))
+    for (int j = n + block * NT + threadIdx.x; j < end; j += a.blocks * NT)
         *reinterpret_cast<float*>(t.dst + b * t.d_sb + hk * t.d_sh + j * t.d_sn) = 0.f;
 }
 
 // ---------------------------------------------------------------------- host
+
+template <int PT>
+int launch_select_wave(const EvictArgs& a, hipStream_t st) {
+    hipLaunchKernelGGL((fta_evict_select_wave_kernel<PT>), dim3((unsigned)((a.B * a.Hk + 3) / 4)), dim3(256), 0, st, a);
+    return fta::check_launch("fta_evict_select_wave_kernel");
+}
 
 template <int PT>
 int launch_select(const EvictArgs& a, hipStream_t st) {
@@ -349,16 +413,20 @@ int fta_cache_evict(int tensors, const void* const* src, const int64_t* src_stri
     a.blocks = a.in_place ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>((budget + 255) / 256, (8192 + heads * a.jobs - 1) / (heads * a.jobs)));
     if (heads * a.jobs * a.blocks > (1 << 22) - 1 || heads > (1 << 22) - 1) return fta::unsupported("cache_evict: too many heads");
     hipStream_t st = (hipStream_t)stream;
-    int rc = S <= 8 * kSelThreads    ? launch_select<8>(a, st)
+    int rc = S <= 8 * 64             ? launch_select_wave<8>(a, st)
+             : S <= 16 * 64          ? launch_select_wave<16>(a, st)
+             : S <= 8 * kSelThreads  ? launch_select<8>(a, st)
              : S <= 16 * kSelThreads ? launch_select<16>(a, st)
              : S <= 32 * kSelThreads ? launch_select<32>(a, st)
                                      : launch_select<0>(a, st);
     if (rc != FTA_OK) return rc;
     const dim3 g((unsigned)(heads * a.jobs * a.blocks));
-    if (a.in_place)
-        hipLaunchKernelGGL((fta_evict_move_kernel<true>), g, dim3(move_threads(true)), 0, st, a);
+    if (!a.in_place)
+        hipLaunchKernelGGL((fta_evict_move_kernel<false, 512>), g, dim3(512), 0, st, a);
+    else if (budget <= 512 || (budget <= 1024 && heads * a.jobs >= 2048))
+        hipLaunchKernelGGL((fta_evict_move_kernel<true, 256>), g, dim3(256), 0, st, a);
     else
-        hipLaunchKernelGGL((fta_evict_move_kernel<false>), g, dim3(move_threads(false)), 0, st, a);
+        hipLaunchKernelGGL((fta_evict_move_kernel<true, 1024>), g, dim3(1024), 0, st, a);
     return fta::check_launch("fta_evict_move_kernel");
     FTA_TRY_END
 }

@@ -222,3 +222,34 @@ def test_weights_of_held_rows(gpu, case, q4):
     if case[-1] is None:
         case = (*case[:-1], torch.randint(0, case[6] + 1, (case[1],), generator=torch.Generator().manual_seed(2)).tolist())
     test_weights(gpu, case, q4)
+
+
+# caches of more than 1024 rows (a workgroup selects, not a wave), and few rows of many heads (fewer threads move them)
+EVICT_LONG = [
+    (2, 3, 80, 1300, 64, 64, 0, [1300, 64]),
+    (2, 1, 16, 1100, 64, 0, 64, [1100, 65]),
+    (2, 2, 96, 2100, 600, 30, 4, [5000, -3]),
+    (3, 2, 128, 1025, 1024, 0, 0, [1025, 1024, 7]),
+    (1, 1, 64, 1024, 1000, 3, 1, [1024]),
+    (64, 8, 64, 1100, 1000, 20, 4, None),
+]
+
+
+@pytest.mark.parametrize("out", [False, True], ids=["in_place", "out"])
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+@pytest.mark.parametrize("case", EVICT_LONG, ids=lambda c: "-".join(str(x) for x in c[:7]))
+def test_evict_of_long_caches(gpu, case, q4, out):
+    test_evict(gpu, case, q4, out)
+
+
+@pytest.mark.parametrize("S", [1024, 1100])
+def test_evict_of_special_weights_in_long_caches(gpu, S):
+    import flash_topk_attn_v2 as fta
+
+    vals = [0.0, -0.0, math.nan, math.inf, -math.inf, -1.0, 1e-40, -1e-40, 1.0, 3.0e38, -math.nan, 2.0 ** -149]
+    w = torch.tensor(vals * (S // len(vals) + 1))[None, None, :S].contiguous()
+    cache = tuple(rand((1, S, 16), i, BF, gpu) for i in (0, 1))
+    for budget in range(1, S, 85):
+        c = tuple(x.clone() for x in cache)
+        _, kept = fta.flash_cache_evict(c, w.to(gpu), torch.tensor([S], dtype=torch.int32, device=gpu), budget)
+        assert kept[0, 0].tolist() == _evicted(w[0, 0], S, budget, 0, 0)
