@@ -116,7 +116,7 @@ def _moved_layout(what, q4, metas, B, Hk, budget):
         groups = shape[3] if len(shape) == 4 else 0
         if not 1 <= groups <= 8:
             raise ValueError(f"{what}: k_scales must be [B, num_kv_heads, S, groups], up to 8 groups")
-        S, strides = _layout(what, *zip(*cache), B, Hk, groups)
+        S, strides, _ = _layout(what, *zip(*cache), B, Hk, groups)
         for (shape, _, dtype), st in zip(cache, strides):
             size = dtype.itemsize
             found += [size * st[0], size * st[1], size * shape[3]]

@@ -50,7 +50,8 @@ def flash_q4_cache(batch: int, tokens: int, num_kv_heads: int, head_dim: int, de
 
 @lru_cache(maxsize=1024)
 def _layout(what, shapes, strides, types, B, Hk, groups):
-    """The strides that the library takes of each tensor of a ``Q4Cache``, checked (calls of one shape are checked once)."""
+    """``(rows S, the strides that the library takes of each tensor of a Q4Cache, distances between the tensors that
+    check_q4_written has passed)``, checked (calls of one shape are checked once)."""
     S = shapes[0][2] if len(shapes[0]) == 4 else 0
     widths = (16 * groups, groups) * 2
     names = Q4Cache._fields
@@ -66,22 +67,29 @@ def _layout(what, shapes, strides, types, B, Hk, groups):
         if (w > 1 and stride[3] != 1) or (S > 1 and stride[2] != w) or (sb | sh) & step:
             raise ValueError(f"{what}: the rows of a head of {name} must follow each other, heads at aligned steps")
         found.append(_lib.i64arr((sb, sh)))
-    return S, tuple(found)
+    return S, tuple(found), set()
 
 
-def q4_args(what, cache, B, Hk, D, device):
-    """``(S, address and strides of the four tensors)`` of a ``Q4Cache``, checked."""
+def q4_args(what, cache, B, Hk, D, device, write=False):
+    """``(S, address and strides of the four tensors)`` of a ``Q4Cache``, checked; with ``write`` by ``check_q4_written`` too."""
     if not isinstance(cache, Q4Cache):
         raise ValueError(f"{what}: cache must be a Q4Cache")
     kc, ks, vc, vs = cache
-    S, (kcs, kss, vcs, vss) = _layout(what, (kc.shape, ks.shape, vc.shape, vs.shape),
-                                      (kc.stride(), ks.stride(), vc.stride(), vs.stride()),
-                                      (kc.dtype, ks.dtype, vc.dtype, vs.dtype), B, Hk, -(-D // 32))
+    S, (kcs, kss, vcs, vss), apart = _layout(what, (kc.shape, ks.shape, vc.shape, vs.shape),
+                                             (kc.stride(), ks.stride(), vc.stride(), vs.stride()),
+                                             (kc.dtype, ks.dtype, vc.dtype, vs.dtype), B, Hk, -(-D // 32))
     _lib.check_device(what, device, kc, ks, vc, vs)
     _lib.no_grad_inputs(what, ks, vs)
     kca, ksa, vca, vsa = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
     if (kca | vca) & 15 or (ksa | vsa) & 3:
         raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte")
+    if write:
+        distances = (ksa - kca, vca - kca, vsa - kca)
+        if distances not in apart:
+            check_q4_written(what, cache)
+            if len(apart) >= 1024:
+                apart.clear()
+            apart.add(distances)
     return S, (kca, kcs, ksa, kss, vca, vcs, vsa, vss)
 
 
@@ -145,8 +153,7 @@ def flash_qk_norm_rope_append_q4(
         raise ValueError(f"{what}: v must have k's shape and type")
     check_lens(what, cache_lens, B)
     _lib.check_device(what, q.device, v, cache_lens)
-    S, args = q4_args(what, cache, B, Hk, D, q.device)
-    check_q4_written(what, cache)
+    S, args = q4_args(what, cache, B, Hk, D, q.device, write=True)
     offset, offs = offsets(what, position_offset, B, q.device, cos.shape[0], S)
     q, qa, qs = _lib.rows(q, H)
     k, ka, ks = _lib.rows(k, Hk)

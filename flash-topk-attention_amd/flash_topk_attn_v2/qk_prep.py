@@ -93,9 +93,7 @@ def check_lens(what, cache_lens, B):
 
 def written(*tensors):
     """Marks tensors as changed in place (inference tensors keep no version)."""
-    for t in tensors:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 class _QKNormRopeFunc(torch.autograd.Function):
