@@ -108,7 +108,8 @@ def _metas(tensors):
 @lru_cache(maxsize=1024)
 def _moved_layout(what, q4, metas, B, Hk, budget):
     """``(rows S, byte strides {b, head, row} and row bytes of the cache's tensors, strides of the
-    weights)`` of a cache and its weights, checked (calls of one shape are checked once)."""
+    weights, places that _check_apart has passed)`` of a cache and its weights, checked (calls of one
+    shape are checked once)."""
     *cache, (w_shape, w_stride, w_type) = metas
     found, nbytes = [], []
     if q4:
@@ -142,7 +143,7 @@ def _moved_layout(what, q4, metas, B, Hk, budget):
         raise ValueError(f"{what}: weights must have the cache's {S} rows, not {w_shape[2]}")
     if budget > S:
         raise ValueError(f"{what}: budget ({budget}) must not pass the cache's rows ({S})")
-    return S, _lib.i64arr(found), (ctypes.c_int32 * len(nbytes))(*nbytes), w_strides
+    return S, _lib.i64arr(found), (ctypes.c_int32 * len(nbytes))(*nbytes), w_strides, set()
 
 
 def _span(meta, at):
@@ -150,21 +151,25 @@ def _span(meta, at):
     return at, at + dtype.itemsize * (1 + sum((n - 1) * s for n, s in zip(shape, stride)))
 
 
-@lru_cache(maxsize=1024)
-def _check_apart(what, q4, metas, to_metas, at, to_at):
-    """Refuses what is written where rows share memory, and ``out`` that overlaps the inputs
-    (addresses are given as distances; calls of one layout are checked once)."""
+def _check_aligned(what, q4, at):
+    wide, narrow = (at[0] | at[2], at[1] | at[3] | at[4]) if q4 else (at[0] | at[1], at[2])
+    if wide & 15 or narrow & 3:
+        raise ValueError(f"{what}: cache rows must be 16-byte aligned (scales 4-byte)")
+
+
+def _check_apart(what, q4, metas, to_metas, at, to_at, in_place=False):
+    """Refuses what is written where rows share memory, and ``out`` that overlaps the inputs."""
     *cache, _ = to_metas
     shapes, strides = tuple(m[0] for m in cache), tuple(m[1] for m in cache)
     if q4:
-        if _q4_meet(shapes, strides, to_at[:4]):
+        if _q4_meet(shapes, strides, tuple(a - to_at[0] for a in to_at[:4])):
             raise ValueError(f"{what}: rows of the cache share memory (an expanded cache, or tensors that overlap)")
     elif _lib._caches_meet(shapes[0], strides[0], strides[1], (to_at[1] - to_at[0]) // 2):
         raise ValueError(f"{what}: rows of the caches share memory (an expanded cache, or one that overlaps the other)")
     spans = [_span(m, a) for m, a in zip(to_metas, to_at)]
     if any(spans[-1][0] < end and spans[-1][1] > a for a, end in spans[:-1]):
         raise ValueError(f"{what}: the weights overlap the cache")
-    if metas is not to_metas:
+    if not in_place:
         for a, end in (_span(m, x) for m, x in zip(metas, at)):
             if any(a < e and end > b for b, e in spans):
                 raise ValueError(f"{what}: out overlaps the inputs")
@@ -231,22 +236,26 @@ def flash_cache_evict(
     _lib.check_device(what, dev, *tensors)
     _lib.no_grad_inputs(what, *tensors)
     metas = _metas(tensors)
-    S, strides, nbytes, w_strides = _moved_layout(what, q4, metas, B, Hk, budget)
+    S, strides, nbytes, w_strides, apart = _moved_layout(what, q4, metas, B, Hk, budget)
     at = [t.data_ptr() for t in tensors]
+    _check_aligned(what, q4, at)
+    base = at[0]
     if out is None:
         to_metas, to_at = metas, at
         S_out, to_strides, to_w_strides = S, strides, w_strides
+        places = tuple([a - base for a in at])
     else:
         to_metas, to_at = _metas(to), [t.data_ptr() for t in to]
-        S_out, to_strides, to_bytes, to_w_strides = _moved_layout(what, q4, to_metas, B, Hk, budget)
+        S_out, to_strides, to_bytes, to_w_strides, _ = _moved_layout(what, q4, to_metas, B, Hk, budget)
+        _check_aligned(what, q4, to_at)
+        places = to_metas, tuple([a - base for a in (*at, *to_at)])
         if to_metas[0][2] != metas[0][2] or list(to_bytes) != list(nbytes):
             raise ValueError(f"{what}: out must have the cache's type and head dim")
-    for i, a in enumerate((*at, *to_at)):
-        i %= len(at)
-        if a & (3 if i + 1 == len(at) or (q4 and i % 2) else 15):
-            raise ValueError(f"{what}: cache rows must be 16-byte aligned (scales 4-byte)")
-    base = min(*at, *to_at)
-    _check_apart(what, q4, metas, to_metas, tuple(a - base for a in at), tuple(a - base for a in to_at))
+    if places not in apart:
+        _check_apart(what, q4, metas, to_metas, at, to_at, out is None)
+        if len(apart) >= 1024:
+            apart.clear()
+        apart.add(places)
     n = len(cache)
     lens = cache_lens.contiguous()
     new_lens = torch.empty(B, device=dev, dtype=torch.int32)

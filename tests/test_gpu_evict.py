@@ -253,3 +253,19 @@ def test_evict_of_special_weights_in_long_caches(gpu, S):
         c = tuple(x.clone() for x in cache)
         _, kept = fta.flash_cache_evict(c, w.to(gpu), torch.tensor([S], dtype=torch.int32, device=gpu), budget)
         assert kept[0, 0].tolist() == _evicted(w[0, 0], S, budget, 0, 0)
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+def test_out_that_is_the_input_is_refused_every_time(gpu, q4):
+    """Also behind calls in place and into another cache of the same layout."""
+    import flash_topk_attn_v2 as fta
+
+    cache, other = (Q.cache(1, 40, 2, 64, gpu, 4 + i) if q4 else tuple(rand((1, 40, 128), 2 * i + j, BF, gpu) for j in (0, 1)) for i in (0, 1))
+    w, w2 = (torch.rand(1, 2, 40, device=gpu) for _ in range(2))
+    ln = torch.tensor([40], dtype=torch.int32, device=gpu)
+    for _ in range(2):
+        fta.flash_cache_evict(cache, w, ln, 10)
+        fta.flash_cache_evict(cache, w, ln, 10, out=(other, w2))
+        for out in ((cache, w), (cache, w2), (other, w)):
+            with pytest.raises(ValueError, match="overlap"):
+                fta.flash_cache_evict(cache, w, ln, 10, out=out)
