@@ -63,7 +63,9 @@ def attend(q, c, lens, H, Hk, left, sinks, scale):
     B, T, C = q.shape
     D, G, S, dev, dt = C // H, H // Hk, c.k_codes.shape[2], q.device, q.dtype
     u, t = R.half_step(dt), R.tiny(dt)
-    up = 2.0 ** -17 if dt == torch.float16 else 2.0 ** -9  # of p d, half a step
+    # Of p d.  bf16 keeps 8 bits, 2^e (1 + m / 128): half a step is 2^(e - 8), at most 2^-8 of a value of 2^e and more.
+    # Two of them, hi + lo: |lo| is at most 2^-8 |x|, and its own rounding 2^-8 of that, 2^-16 |x|.
+    up = 2.0 ** -16 if dt == torch.float16 else 2.0 ** -8
     out = {"o": torch.zeros(B, T, H, D, device=dev, dtype=torch.float64),
            "lse": torch.full((B, H, T), -math.inf, device=dev, dtype=torch.float64)}
     out |= {n + "_tol": torch.zeros_like(x) for n, x in list(out.items())}
