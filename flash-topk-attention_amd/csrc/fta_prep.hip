@@ -248,9 +248,9 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
             for (int e = 0; e < 8; ++e) f[e] *= r * (isq ? wq[e] : wk[e]);
             if (a.inter) {
 #pragma unroll
-                for (int e = 0; e < 8; e += 2) {
-                    y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
-                    y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
+                for (int e = 0; e < 8; e += 2) {  // written out: the append to a 4-bit cache forms the same bits
+                    y[e] = fmaf(f[e], cs[e], -(f[e + 1] * sn[e]));
+                    y[e + 1] = fmaf(f[e], sn[e], f[e + 1] * cs[e]);
                 }
             } else {
                 float g[8];
@@ -428,8 +428,8 @@ __global__ __launch_bounds__(256, 4) void fta_norm_rope_append_q4_kernel(PrepArg
                 if (a.inter) {
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
-                        y[e] = f[e] * cs[e] - f[e + 1] * sn[e];
-                        y[e + 1] = f[e + 1] * cs[e] + f[e] * sn[e];
+                        y[e] = fmaf(f[e], cs[e], -(f[e + 1] * sn[e]));
+                        y[e + 1] = fmaf(f[e], sn[e], f[e + 1] * cs[e]);
                     }
                 } else {
                     unpack8<DT>(xp, g);

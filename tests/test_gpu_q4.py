@@ -178,3 +178,19 @@ def test_values_of_any_size(gpu, dtype, scale):
     ln = torch.tensor([S, 1500], dtype=torch.int32, device=gpu)
     o, lse = fta.flash_window_attn_decode_q4(q, c, ln, H, S, num_kv_heads=Hk)
     R.check({"o": o, "lse": lse}, Q.attend(q, c, ln.tolist(), H, Hk, S, 0, D ** -0.5), ("o", "lse"))
+
+
+# interleaved pairs, tokens enough that a different order of the rotation's two products shows in 16 bits
+INTERLEAVED = [
+    (FP, 3, 386, 900, 3, 1, 16, 16, True, [121, 82, 342]),
+    (FP, 1, 278, 250, 20, 4, 256, 16, True, [250]),
+    (FP, 4, 150, 94, 11, 1, 224, 160, True, [13, 94, 94, 32]),
+    (FP, 4, 97, 39, 64, 4, 96, 64, True, [22, 25, 39, 39]),
+    (BF, 3, 217, 900, 8, 1, 112, 32, True, [174, 426, 541]),
+    (BF, 2, 2000, 2000, 8, 2, 128, 128, True, [2000, 1999]),
+]
+
+
+@pytest.mark.parametrize("case", INTERLEAVED, ids=lambda c: "-".join(str(x) for x in c[1:9]))
+def test_append_of_interleaved_pairs(gpu, case):
+    test_append(gpu, case)
