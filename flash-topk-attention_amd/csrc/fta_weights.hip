@@ -107,7 +107,20 @@ struct KeyRows {
     }
 };
 
-// What chunk c's 32 rows, in LDS at `rows` with -lse log2(e) at sl, add to this lane's key kt + (lane & 31).
+// The rows of a chunk, its first token at position q_lo, whose tokens see a key.
+__device__ __forceinline__ uint32_t rows_that_see(const WeighArgs& a, int q_lo, int key) {
+    const int64_t t_hi = key < a.sinks ? a.TT - 1 : min((int64_t)key + a.left - q_lo, (int64_t)a.TT - 1);
+    const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
+    const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
+    return fta_bits_below(rhi) & ~fta_bits_below(rlo);
+}
+
+// -lse log2(e), or -inf for what gives nothing: a row that saw nothing (lse = -inf) or does not exist (inf).  A NaN
+// would outlast a masked score and reach keys that its token does not see: it gives nothing here, and
+// makes the sums of its own keys NaN in the end.
+__device__ __forceinline__ float row_offset(float lse) { return fabsf(lse) < FTA_INF ? -lse * kLog2e : -FTA_INF; }
+
+// What chunk c's 32 rows, in LDS at `rows` with their row_offset at sl, add to this lane's key kt + (lane & 31).
 template <int DT, int KD, bool Q4>
 __device__ __forceinline__ float chunk_sum(const WeighArgs& a, const fta_frag (&kf)[KD / 16], const float (&ds)[KD / 32],
                                            uint32_t rows, const float* sl, int c, int kt, int len, int lane) {
@@ -138,11 +151,7 @@ __device__ __forceinline__ float chunk_sum(const WeighArgs& a, const fta_frag (&
     }
     if (!(q_lo >= kt + 31 && (q_hi - a.left <= kt || kt + 31 < a.sinks))) {
         asm volatile("");  // an edge: kept apart, or every chunk pays for it
-        // the rows of the tokens that see this lane's key
-        const int64_t t_hi = key < a.sinks ? a.TT - 1 : min((int64_t)key + a.left - q_lo, (int64_t)a.TT - 1);
-        const int rlo = max(key - q_lo, 0) >= a.TT ? 32 : max(key - q_lo, 0) * a.GG;
-        const int rhi = (int)max(t_hi + 1, (int64_t)0) * a.GG;
-        FtaTile<DT, KD>::mask(fta_bits_below(rhi) & ~fta_bits_below(rlo), lane, x);
+        FtaTile<DT, KD>::mask(rows_that_see(a, q_lo, key), lane, x);
     }
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
@@ -170,7 +179,8 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     constexpr int QSEG = KD / 8, KS = KD / 16, NG = KD / 32, BLOCKS = QSEG / 2, TILE_B = 32 * QSEG * 16;
     using SW = FtaSwz<QSEG>;
     __shared__ __align__(1024) unsigned char sQ[2][TILE_B];
-    __shared__ __align__(16) float sL[2][32];  // -lse log2(e), -inf for rows that do not count
+    __shared__ __align__(16) float sL[2][32];  // row_offset
+    __shared__ int sNan;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wgi = fta_xcd_remap(blockIdx.x, a.total);
@@ -244,11 +254,12 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
         keys.operands(a, lane, kf, ds);
     }
     float run = 0.f, sum = 0.f;
+    bool nans = false;  // wave 0: a row's lse was
     int st = 0;
     for (int s = s0; s < s1; ++s, st ^= 1) {
         fta_wait_vmcnt<0>();
-        // a row that saw nothing (lse = -inf) gives nothing, as one that does not exist
-        if (wave == 0 && lane < 32) sL[st][lane] = (lv == -FTA_INF) ? -FTA_INF : -lv * kLog2e;
+        if (wave == 0 && lane < 32) sL[st][lane] = row_offset(lv);
+        nans |= lv != lv;
         __syncthreads();  // this chunk visible; every wave is past the last one
         const int c = ct;
         if (++ct == c_lo + nct) {
@@ -265,6 +276,16 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
     }
     sum += run;
     sum += fta_xor32(sum);
+    if (wave == 0) sNan = __ballot(nans) != 0ull;
+    __syncthreads();
+    if (sNan) {
+        for (int s = s0; s < s1; ++s) {
+            const int g0 = s / nct * a.GG, t0 = (c_lo + s % nct) * a.TT, r = lane & 31, t = t0 + r / a.GG, g = g0 + r % a.GG;
+            const bool ok = r < a.TT * a.GG && t < a.T && g < a.G;
+            const float x = lp[ok ? (int64_t)g * a.T + t : 0];
+            if ((uint32_t)__ballot(ok && x != x) & rows_that_see(a, len - a.T + t0, key)) sum = __builtin_nanf("");
+        }
+    }
     if (lane >= 32 || key >= len) return;
     if (a.np > 1)
         a.part[((int64_t)sp * a.B * a.Hk + bhk) * a.S + key] = sum;
@@ -288,6 +309,7 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
     using SW = FtaSwz<QSEG>;
     __shared__ __align__(1024) unsigned char sQ[kHeld][TILE_B];
     __shared__ __align__(16) float sL[kHeld][32];
+    __shared__ uint32_t sNan[kHeld];  // rows of a chunk whose lse is
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int bhk = fta_scalar(blockIdx.x / a.np), sp = blockIdx.x - bhk * a.np;
@@ -319,7 +341,9 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
         const int t = ct * a.TT + row / a.GG, g = cg * a.GG + row % a.GG;
         const bool ok = row < a.TT * a.GG && t < a.T && g < a.G;
         const float x = lp[ok ? (int64_t)g * a.T + t : 0];
-        sL[ch][row] = ok && x != -FTA_INF ? -x * kLog2e : -FTA_INF;  // a row that saw nothing gives nothing
+        sL[ch][row] = row_offset(ok ? x : FTA_INF);
+        const uint64_t n = __ballot(ok && x != x);  // of two chunks, or of the last
+        if (row == 0) sNan[ch] = (uint32_t)(n >> (lane & 32));
     }
     float* wp = a.w + b * a.w_sb + hk * a.w_sh;
     auto tile = [&](int it) { return 32 * (it < ns ? it : c_lo + it - ns); };
@@ -336,6 +360,9 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
     if (it0 + wave < it1) ask(it0 + wave, cur);
     fta_wait_vmcnt<0>();
     __syncthreads();
+    uint32_t nans = 0;
+    for (int ch = 0; ch < a.chunks; ++ch) nans |= sNan[ch];
+    nans = fta_scalar((int)nans);
     for (int it = it0 + wave; it < it1; it += NW) {
         if (it + NW < it1) ask(it + NW, nxt);
         fta_frag kf[KS];
@@ -346,6 +373,9 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
         for (int cg = 0, ch = 0; cg < a.groups; ++cg)
             for (int ct = 0; ct < nct; ++ct, ++ch) sum += chunk_sum<DT, KD, Q4>(a, kf, ds, ldq + ch * TILE_B, sL[ch], ct, kt, len, lane);
         sum += fta_xor32(sum);
+        if (nans != 0)
+            for (int ch = 0; ch < a.chunks; ++ch)
+                if (sNan[ch] & rows_that_see(a, len - a.T + ch % nct * a.TT, key)) sum = __builtin_nanf("");
         if (lane < 32 && key < len) wp[key] = cur.before + sum;
         cur = nxt;
     }
