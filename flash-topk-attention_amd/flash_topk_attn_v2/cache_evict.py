@@ -13,7 +13,7 @@ from typing import Optional, Tuple, Union
 import torch
 
 from . import _lib
-from .q4_cache import _MAX, Q4Cache, _geometry, _layout, _q4_meet, q4_args
+from .q4_cache import _MAX, Q4Cache, _geometry, _layout, _q4_meet, _scale_step, q4_args
 from .qk_prep import check_lens, written
 
 
@@ -151,10 +151,10 @@ def _span(meta, at):
     return at, at + dtype.itemsize * (1 + sum((n - 1) * s for n, s in zip(shape, stride)))
 
 
-def _check_aligned(what, q4, at):
-    wide, narrow = (at[0] | at[2], at[1] | at[3] | at[4]) if q4 else (at[0] | at[1], at[2])
-    if wide & 15 or narrow & 3:
-        raise ValueError(f"{what}: cache rows must be 16-byte aligned (scales 4-byte)")
+def _check_aligned(what, q4, nbytes, at):
+    wide, scales = (at[0] | at[2], at[1] | at[3]) if q4 else (at[0] | at[1], 0)
+    if wide & 15 or at[-1] & 3 or scales & _scale_step(nbytes[1] // 2):
+        raise ValueError(f"{what}: cache rows must be 16-byte aligned (scales 4-byte where there is an even number of groups)")
 
 
 def _check_apart(what, q4, metas, to_metas, at, to_at, in_place=False):
@@ -238,7 +238,7 @@ def flash_cache_evict(
     metas = _metas(tensors)
     S, strides, nbytes, w_strides, apart = _moved_layout(what, q4, metas, B, Hk, budget)
     at = [t.data_ptr() for t in tensors]
-    _check_aligned(what, q4, at)
+    _check_aligned(what, q4, nbytes, at)
     base = at[0]
     if out is None:
         to_metas, to_at = metas, at
@@ -247,7 +247,7 @@ def flash_cache_evict(
     else:
         to_metas, to_at = _metas(to), [t.data_ptr() for t in to]
         S_out, to_strides, to_bytes, to_w_strides, _ = _moved_layout(what, q4, to_metas, B, Hk, budget)
-        _check_aligned(what, q4, to_at)
+        _check_aligned(what, q4, to_bytes, to_at)
         places = to_metas, tuple([a - base for a in (*at, *to_at)])
         if to_metas[0][2] != metas[0][2] or list(to_bytes) != list(nbytes):
             raise ValueError(f"{what}: out must have the cache's type and head dim")

@@ -28,7 +28,8 @@ class Q4Cache(NamedTuple):
 
     ``k_codes`` and ``v_codes`` are uint8 ``[B, num_kv_heads, S, 16 * groups]``,
     ``k_scales`` and ``v_scales`` float16 ``[B, num_kv_heads, S, groups]``; the rows of a
-    head follow each other, the codes of heads start at 16-byte steps.
+    head follow each other, the codes of heads start at 16-byte steps and, where there is an
+    even number of groups, their scales at 4-byte steps.
     """
 
     k_codes: torch.Tensor
@@ -70,19 +71,25 @@ def _layout(what, shapes, strides, types, B, Hk, groups):
     return S, tuple(found), set()
 
 
+def _scale_step(groups):
+    """Address bits that scales have clear: they are read by pairs where a row has an even number of them."""
+    return 1 if groups % 2 else 3
+
+
 def q4_args(what, cache, B, Hk, D, device, write=False):
     """``(S, address and strides of the four tensors)`` of a ``Q4Cache``, checked; with ``write`` by ``check_q4_written`` too."""
     if not isinstance(cache, Q4Cache):
         raise ValueError(f"{what}: cache must be a Q4Cache")
     kc, ks, vc, vs = cache
+    groups = -(-D // 32)
     S, (kcs, kss, vcs, vss), apart = _layout(what, (kc.shape, ks.shape, vc.shape, vs.shape),
                                              (kc.stride(), ks.stride(), vc.stride(), vs.stride()),
-                                             (kc.dtype, ks.dtype, vc.dtype, vs.dtype), B, Hk, -(-D // 32))
+                                             (kc.dtype, ks.dtype, vc.dtype, vs.dtype), B, Hk, groups)
     _lib.check_device(what, device, kc, ks, vc, vs)
     _lib.no_grad_inputs(what, ks, vs)
     kca, ksa, vca, vsa = kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()
-    if (kca | vca) & 15 or (ksa | vsa) & 3:
-        raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte")
+    if (kca | vca) & 15 or (ksa | vsa) & _scale_step(groups):
+        raise ValueError(f"{what}: the cache's codes must be 16-byte aligned, its scales 4-byte where there is an even number of groups")
     if write:
         distances = (ksa - kca, vca - kca, vsa - kca)
         if distances not in apart:
