@@ -244,6 +244,59 @@ def _caches_meet(shape: tuple, k_stride: tuple, v_stride: tuple, delta: int) -> 
     return any(k_stride[i] != v_stride[i] for i in dims) or _rows_meet(shape, k_stride, delta) or delta == 0
 
 
+def _span(t) -> int:
+    """Bytes from a tensor's first to behind its last."""
+    return t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _runs(shape, stride, size):
+    """A tensor's bytes: the length of its runs, and where they start, {byte stride: how often}."""
+    run, steps = size, {}
+    for s, n in sorted((s * size, n) for n, s in zip(shape, stride) if n > 1 and s > 0):
+        if s <= run:
+            run += s * (n - 1)
+        else:
+            steps[s] = steps.get(s, 0) + n - 1
+    return run, steps
+
+
+@lru_cache(maxsize=4096)
+def tensors_meet(a: tuple, b: tuple, delta: int) -> bool:
+    """Whether two tensors ``(shape, stride, bytes of an element)``, b ``delta`` bytes behind a, share a byte:
+    whether some x - y of the starts of their runs lies in ``(delta - a's run, delta + b's run)``
+    (after 2^16 steps, which nested layouts never take, they are taken to)."""
+    (run_a, steps_a), (run_b, steps_b) = _runs(*a), _runs(*b)
+    dims = sorted({*steps_a, *steps_b}, reverse=True)
+    spans = [(-steps_b.get(s, 0), steps_a.get(s, 0)) for s in dims]
+    low, high = [0], [0]  # what the dims behind each can add
+    for s, (lo, hi) in zip(dims[::-1], spans[::-1]):
+        low.append(low[-1] + lo * s)
+        high.append(high[-1] + hi * s)
+    left = 1 << 16
+
+    def reach(i, lo, hi):  # lo <= sum of the dims from i on <= hi
+        nonlocal left
+        left -= 1
+        if i == len(dims) or left < 0:
+            return left < 0 or lo <= 0 <= hi
+        s, rest = dims[i], len(dims) - i - 1
+        first, last = max(spans[i][0], -((high[rest] - lo) // s)), min(spans[i][1], (hi - low[rest]) // s)
+        return any(reach(i + 1, lo - k * s, hi - k * s) for k in range(first, last + 1))
+
+    return reach(0, delta - run_a + 1, delta + run_b - 1)
+
+
+def check_apart(what: str, name: str, written, *tensors) -> None:
+    """Refuses tensors that share memory with the one that is written in place."""
+    lo = written.data_ptr()
+    hi = lo + (written.nbytes if written.is_contiguous() else _span(written))
+    for t in tensors:
+        at = t.data_ptr()
+        if at < hi and (at + t.nbytes > lo or not t.is_contiguous()) and at + _span(t) > lo and tensors_meet(
+                (written.shape, written.stride(), written.element_size()), (t.shape, t.stride(), t.element_size()), at - lo):
+            raise ValueError(f"{what}: {name} must not overlap any other argument")
+
+
 def check_written(what: str, k: torch.Tensor, v: torch.Tensor) -> None:
     """Refuses caches whose rows share memory: what they would hold depends on which of two
     writes is the last."""

@@ -54,8 +54,8 @@ def flash_cache_weights(
     cached tokens with these T; token t sees key j as in ``flash_window_attn_decode``; tokens
     that see nothing (lse = -inf) add nothing.  (Tokens are the last T of each request: prompts of
     different lengths that are padded behind their ends go one by one.)  ``weights`` is float32
-    ``[B, num_kv_heads, S]``, written in place where ``j < cache_lens[b]``, and overlaps no other
-    argument.  Unseen rows of the cache may hold anything.
+    ``[B, num_kv_heads, S]``, written in place where ``j < cache_lens[b]``, and must overlap no
+    other argument.  Unseen rows of the cache may hold anything.
     Sums are float32 in a fixed order.  Not differentiable.
 
     Returns ``weights``.
@@ -91,6 +91,7 @@ def flash_cache_weights(
         (ka, ks), sa, ss = _lib.rows_in_place(what, cache, Hk), None, None
     if weights.shape[2] != S:
         raise ValueError(f"{what}: weights must be float32 [B, num_kv_heads, S] = {[B, Hk, S]}")
+    _lib.check_apart(what, "weights", weights, q, lse, cache_lens, *(cache if isinstance(cache, Q4Cache) else (cache,)))
     nbytes = _lib.size_of("fta_cache_weights_workspace_size", B, H, Hk, T, S, D, left, sinks)
     q, qa, qs = _lib.rows(q, H)
     lens, lse = cache_lens.contiguous(), lse.contiguous()

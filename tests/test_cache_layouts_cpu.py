@@ -1,10 +1,13 @@
 """Layouts of caches and weights that the calls take, and those that they refuse, by address alone (no GPU)."""
 
+import itertools
+import random
+
 import pytest
 import torch
 
 import flash_topk_attn_v2 as fta
-from flash_topk_attn_v2 import cache_evict, q4_cache
+from flash_topk_attn_v2 import _lib, cache_evict, q4_cache
 
 CPU = torch.device("cpu")
 
@@ -43,3 +46,38 @@ def test_scales_that_are_read_by_pairs_start_at_pairs(D):
         _, _, nbytes, _, _ = cache_evict._moved_layout("evict", True, cache_evict._metas((*bad, w)), 1, 1, 2)
         with pytest.raises(ValueError, match="aligned"):
             cache_evict._check_aligned("evict", True, nbytes, [t.data_ptr() for t in (*bad, w)])
+
+
+def _bytes(shape, stride, size, at):
+    """Every byte of a tensor."""
+    found = set()
+    for i in itertools.product(*map(range, shape)):
+        a = at + size * sum(x * s for x, s in zip(i, stride))
+        found.update(range(a, a + size))
+    return found
+
+
+def test_tensors_that_share_a_byte():
+    """Any strides, runs between each other, types of different sizes: against the sets of their bytes."""
+    rng = random.Random(1)
+    seen = {False: 0, True: 0}
+    for _ in range(4000):
+        a, b = ((tuple(rng.randint(1, 5) for _ in range(d)), tuple(rng.choice([0, 1, 2, 3, 4, 5, 7, 8, 12, 16, 20, 40]) for _ in range(d)),
+                 rng.choice([1, 2, 4])) for d in (rng.randint(1, 3), rng.randint(1, 3)))
+        delta = rng.randint(-150, 150)
+        meet = bool(_bytes(*a, 0) & _bytes(*b, delta))
+        seen[meet] += 1
+        assert _lib.tensors_meet(a, b, delta) == meet, (a, b, delta)
+    assert min(seen.values()) > 500
+
+
+def test_weights_lie_apart_from_what_is_read():
+    B, Hk, S, C = 3, 2, 16, 64
+    raw = torch.zeros(B, 2 * S * C + 2 * Hk * S + 8, dtype=torch.bfloat16)  # a request's keys, values and weights side by side
+    keys = raw[:, :S * C].view(B, S, C)
+    w = raw[:, 2 * S * C:2 * S * C + 2 * Hk * S].view(torch.float32).view(B, Hk, S)
+    apart = lambda *t: _lib.check_apart("weights", "weights", w, *t)  # noqa: E731
+    apart(keys, raw[:, S * C:2 * S * C].view(B, S, C), torch.zeros(B, 4, 1), raw[0, -8:].view(torch.int32)[:B])
+    for bad in (w, w[1:2, 1:], keys[:, :, :1].as_strided((B, S, C), keys.stride(), S * C + 64), raw, raw.view(torch.int32)[2, S * C + 2:][:B]):
+        with pytest.raises(ValueError, match="overlap"):
+            apart(bad)

@@ -47,3 +47,35 @@ def test_scales_of_one_request(gpu, D, T):
     for a, b in zip(*done):
         assert torch.equal(a, b)
     assert all(torch.equal(t[0], x) for t, x in zip(big, other))
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+def test_weights_that_overlap_what_is_read_are_refused(gpu, q4):
+    import flash_topk_attn_v2 as fta
+
+    B, T, H, Hk, D, S = 2, 4, 4, 2, 64, 48
+    buf = torch.zeros(B * T * H * D * 2 + B * S * Hk * D * 2 + 64, dtype=torch.uint8, device=gpu)
+    cache = Q.cache(B, S, Hk, D, gpu, 4) if q4 else rand((B, S, Hk * D), 4, BF, gpu)
+    q = rand((B, T, H * D), 3, BF, gpu)
+    ln = torch.tensor([40, 9], dtype=torch.int32, device=gpu)
+    lse = torch.full((B, H, T), 3.0, device=gpu)
+    want = fta.flash_cache_weights(q, cache, lse, ln, torch.zeros(B, Hk, S, device=gpu), H, S, num_kv_heads=Hk)
+    n = 4 * B * Hk * S
+    w = buf[:n].view(torch.float32).view(B, Hk, S)
+    qs = buf[n - 16:][:B * T * H * D * 2].view(BF).view(B, T, H * D)
+    ls = buf[n - 4:][:4 * B * H * T].view(torch.float32).view(B, H, T)
+    li = buf[n // 2:][:4 * B].view(torch.int32)
+    if q4:
+        held = [cache._replace(v_scales=buf[n - 64:][:2 * cache.v_scales.numel()].view(FP).view_as(cache.v_scales)),
+                cache._replace(k_codes=buf[:cache.k_codes.numel()].view_as(cache.k_codes))]
+    else:
+        held = [buf[n - 16:][:2 * cache.numel()].view(BF).view_as(cache)]
+    for a in (dict(q=qs), dict(lse=ls), dict(cache_lens=li), *(dict(cache=x) for x in held)):
+        with pytest.raises(ValueError, match="overlap"):
+            fta.flash_cache_weights(**{**dict(q=q, cache=cache, lse=lse, cache_lens=ln, weights=w, num_heads=H, window_left=S, num_kv_heads=Hk), **a})
+    assert not buf.any()
+    # parts of one buffer that do not meet
+    both = torch.zeros(B, 2, Hk, S, device=gpu)
+    ls = both[:, 0].reshape(B, -1)[:, :H * T].view(B, H, T)
+    ls.fill_(3.0)
+    assert torch.equal(fta.flash_cache_weights(q, cache, ls, ln, both[:, 1], H, S, num_kv_heads=Hk), want)
