@@ -147,9 +147,10 @@ def _moved_layout(what, q4, metas, B, Hk, budget):
     return S, _lib.i64arr(found), (ctypes.c_int32 * len(nbytes))(*nbytes), w_strides, set()
 
 
-def _span(meta, at):
-    shape, stride, dtype = meta
-    return at, at + dtype.itemsize * (1 + sum((n - 1) * s for n, s in zip(shape, stride)))
+def _meet(a, b, delta):
+    """Whether tensors of two of ``_metas``, the second ``delta`` bytes behind the first, share a byte."""
+    (sa, ta, da), (sb, tb, db) = a, b
+    return _lib.tensors_meet((sa, ta, da.itemsize), (sb, tb, db.itemsize), delta)
 
 
 def _check_aligned(what, q4, nbytes, at):
@@ -167,13 +168,10 @@ def _check_apart(what, q4, metas, to_metas, at, to_at, in_place=False):
             raise ValueError(f"{what}: rows of the cache share memory (an expanded cache, or tensors that overlap)")
     elif _lib._caches_meet(shapes[0], strides[0], strides[1], (to_at[1] - to_at[0]) // 2):
         raise ValueError(f"{what}: rows of the caches share memory (an expanded cache, or one that overlaps the other)")
-    spans = [_span(m, a) for m, a in zip(to_metas, to_at)]
-    if any(spans[-1][0] < end and spans[-1][1] > a for a, end in spans[:-1]):
+    if any(_meet(m, to_metas[-1], to_at[-1] - a) for m, a in zip(to_metas[:-1], to_at)):
         raise ValueError(f"{what}: the weights overlap the cache")
-    if not in_place:
-        for a, end in (_span(m, x) for m, x in zip(metas, at)):
-            if any(a < e and end > b for b, e in spans):
-                raise ValueError(f"{what}: out overlaps the inputs")
+    if not in_place and any(_meet(m, n, b - a) for m, a in zip(metas, at) for n, b in zip(to_metas, to_at)):
+        raise ValueError(f"{what}: out overlaps the inputs")
 
 
 def flash_cache_evict(

@@ -103,16 +103,11 @@ def q4_args(what, cache, B, Hk, D, device, write=False):
 @lru_cache(maxsize=1024)
 def _q4_meet(shapes, strides, at):
     """Whether two rows of the four tensors share memory."""
-    blocks, ends = [], []
-    for shape, stride, a, size in zip(shapes, strides, at, (1, 2) * 2):
-        B, Hk, S, w = shape
-        blocks.append(((B, Hk, S * w), (stride[0], stride[1], 1)))
-        ends.append(a + size * (1 + sum((n - 1) * s for n, s in zip(shape, stride))))
-    for i, size in ((0, 1), (1, 2)):
-        (shape, ks), (_, vs) = blocks[i], blocks[i + 2]
-        if _lib._caches_meet(shape, ks, vs, (at[i + 2] - at[i]) // size):
+    for (B, Hk, S, w), st in zip(shapes, strides):
+        if _lib._rows_meet((B, Hk, S * w), (st[0], st[1], 1), 0):
             return True
-    return any(at[i] < ends[j] and at[j] < ends[i] for i in (0, 2) for j in (1, 3))  # codes and scales
+    tensors = [*zip(shapes, strides, (1, 2) * 2)]
+    return any(_lib.tensors_meet(tensors[i], tensors[j], at[j] - at[i]) for j in range(4) for i in range(j))
 
 
 def check_q4_written(what: str, cache: Q4Cache) -> None:

@@ -81,3 +81,46 @@ def test_weights_lie_apart_from_what_is_read():
     for bad in (w, w[1:2, 1:], keys[:, :, :1].as_strided((B, S, C), keys.stride(), S * C + 64), raw, raw.view(torch.int32)[2, S * C + 2:][:B]):
         with pytest.raises(ValueError, match="overlap"):
             apart(bad)
+
+
+def _arena(B, Hk, S, D):
+    """One buffer a request: its key and value codes, their scales and its weights side by side."""
+    G = -(-D // 32)
+    sizes = [16 * G * Hk * S, -(-2 * G * Hk * S // 16) * 16] * 2 + [4 * Hk * S]
+    raw = torch.zeros(B, -(-sum(sizes) // 16) * 16, dtype=torch.uint8)
+    parts, at = [], 0
+    for n in sizes:
+        parts.append(raw[:, at:at + n])
+        at += n
+    codes = [parts[i].view(B, Hk, S, 16 * G) for i in (0, 2)]
+    scales = [parts[i][:, :2 * G * Hk * S].view(torch.float16).view(B, Hk, S, G) for i in (1, 3)]
+    return fta.Q4Cache(codes[0], scales[0], codes[1], scales[1]), parts[4].view(torch.float32).view(B, Hk, S)
+
+
+@pytest.mark.parametrize("D", [48, 64, 96])
+def test_requests_that_lie_between_each_other(D):
+    """No two rows share memory, whatever the tensors' spans."""
+    B, Hk, S = 3, 2, 16
+    c, w = _arena(B, Hk, S, D)
+    q4_cache.check_q4_written("cache", c)
+    metas, at = cache_evict._metas((*c, w)), [t.data_ptr() for t in (*c, w)]
+    cache_evict._check_apart("evict", True, metas, metas, at, at, True)
+    # and half of the requests into the other half's places
+    c2, w2 = _arena(2 * B, Hk, S, D)
+    halves = [(fta.Q4Cache(*(t[i::2] for t in c2)), w2[i::2]) for i in (0, 1)]
+    m, a = zip(*((cache_evict._metas((*x, y)), [t.data_ptr() for t in (*x, y)]) for x, y in halves))
+    cache_evict._check_apart("evict", True, m[0], m[1], a[0], a[1])
+    pool = torch.zeros(B, 2, 2, S, Hk * D, dtype=torch.bfloat16)
+    kv = [(cache_evict._metas((pool[:, i, 0], pool[:, i, 1], w)), [pool[:, i, j].data_ptr() for j in (0, 1)] + [1 << 40]) for i in (0, 1)]
+    kv[1][1][2] = 1 << 41
+    cache_evict._check_apart("evict", False, kv[0][0], kv[1][0], kv[0][1], kv[1][1])
+    # a byte too many
+    a = list(at)
+    for i, j in ((0, 1), (1, 2), (2, 3), (3, 4)):
+        b = list(at)
+        b[j] -= 16 if j % 2 == 0 else 4
+        with pytest.raises(ValueError, match="share memory|overlap"):
+            cache_evict._check_apart("evict", True, metas, metas, b, b, True)
+    a[4] += 4 * Hk * S  # the weights of one request in the next one's codes
+    with pytest.raises(ValueError, match="weights overlap"):
+        cache_evict._check_apart("evict", True, metas, metas, a, a, True)

@@ -79,3 +79,47 @@ def test_weights_that_overlap_what_is_read_are_refused(gpu, q4):
     ls = both[:, 0].reshape(B, -1)[:, :H * T].view(B, H, T)
     ls.fill_(3.0)
     assert torch.equal(fta.flash_cache_weights(q, cache, ls, ln, both[:, 1], H, S, num_kv_heads=Hk), want)
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+def test_requests_that_lie_between_each_other(gpu, q4):
+    """Keys, values and weights of a request side by side in one buffer, requests behind each other; and an
+    eviction into the caches of the requests between."""
+    import flash_topk_attn_v2 as fta
+
+    B, T, H, Hk, D, S = 3, 2, 4, 2, 64, 96
+    lens = torch.tensor([96, 50, 7], dtype=torch.int32, device=gpu)
+    n = 4 * Hk * S
+    if q4:
+        sizes = [32 * Hk * S, 4 * Hk * S] * 2 + [n]
+        raw = torch.zeros(2 * B, sum(sizes), dtype=torch.uint8, device=gpu)
+        codes, scales = (lambda x: x.view(2 * B, Hk, S, 32)), (lambda x: x.view(FP).view(2 * B, Hk, S, 2))
+        views = (codes, scales, codes, scales)
+    else:
+        sizes = [2 * S * Hk * D] * 2 + [n]
+        raw = torch.zeros(2 * B, sum(sizes), dtype=torch.uint8, device=gpu)
+        views = (lambda x: x.view(BF).view(2 * B, S, Hk * D),) * 2
+    at = [sum(sizes[:i]) for i in range(len(sizes))]
+    parts = [f(raw[:, a:a + s]) for f, a, s in zip((*views, lambda x: x.view(torch.float32).view(2 * B, Hk, S)), at, sizes)]
+    full = Q.cache(2 * B, S, Hk, D, gpu, 3) if q4 else tuple(rand((2 * B, S, Hk * D), 3 + i, BF, gpu) for i in (0, 1))
+    for x, y in zip(parts, full):
+        x.copy_(y)
+    kind = (lambda t: fta.Q4Cache(*t)) if q4 else tuple
+    mine, to = ((kind([t[i::2] for t in parts[:-1]]), parts[-1][i::2]) for i in (0, 1))
+    own, own_to = ((kind([t.clone(memory_format=torch.contiguous_format) for t in c]), w.clone(memory_format=torch.contiguous_format))
+                   for c, w in (mine, to))
+    cos, sin = _tables(S, D // 2, gpu)
+    q, k, v = (rand((B, T, h * D), i, BF, gpu) for i, h in enumerate((H, Hk, Hk)))
+    for c, w in (mine, own):
+        if q4:
+            qr = fta.flash_qk_norm_rope_append_q4(q, k, v, c, lens, H, cos, sin, num_kv_heads=Hk)
+            _, lse = fta.flash_window_attn_decode_q4(qr, c, lens, H, S, num_kv_heads=Hk)
+        else:
+            qr = fta.flash_qk_norm_rope_append(q, k, v, *c, lens, H, cos, sin, num_kv_heads=Hk)
+            _, lse = fta.flash_window_attn_decode(qr, *c, lens, H, S, num_kv_heads=Hk)
+        fta.flash_cache_weights(qr, c if q4 else c[0], lse, lens, w, H, S, num_kv_heads=Hk)
+    got = fta.flash_cache_evict(*mine, lens, 40, 8, 2, out=to)
+    want = fta.flash_cache_evict(*own, lens, 40, 8, 2, out=own_to)
+    got2, want2 = (fta.flash_cache_evict(c, w, lens, 30, 8, 2) for c, w in (mine, own))
+    for a, b in zip((*got, *got2, *mine[0], mine[1], *to[0], to[1]), (*want, *want2, *own[0], own[1], *own_to[0], own_to[1])):
+        assert torch.equal(a, b)
