@@ -18,14 +18,14 @@ from .qk_prep import check_lens, written
 
 
 @lru_cache(maxsize=1024)
-def _weights_layout(what, shape, stride, dtype, B, Hk):
-    """Strides of weights ``[B, Hk, S]``, checked (calls of one shape are checked once)."""
+def _weights_layout(what, shape, stride, dtype, B, Hk, write=True):
+    """Strides of weights ``[B, Hk, S]``, checked (calls of one shape are checked once); rows that are written lie apart."""
     if len(shape) != 3 or tuple(shape[:2]) != (B, Hk) or shape[2] == 0 or dtype != torch.float32:
         raise ValueError(f"{what}: weights must be float32 [B, num_kv_heads, S] = [{B}, {Hk}, S]")
     _lib.int_sizes(what, shape[2])
     if shape[2] > 1 and stride[2] != 1:
         raise ValueError(f"{what}: the weights of a head must follow each other")
-    if _lib._rows_meet(tuple(shape), (stride[0] if B > 1 else 0, stride[1] if Hk > 1 else 0, 1), 0):
+    if write and _lib._rows_meet(tuple(shape), (stride[0] if B > 1 else 0, stride[1] if Hk > 1 else 0, 1), 0):
         raise ValueError(f"{what}: rows of the weights share memory")
     return _lib.i64arr((stride[0] if B > 1 else 0, stride[1] if Hk > 1 else 0))
 
@@ -107,7 +107,7 @@ def _metas(tensors):
 
 
 @lru_cache(maxsize=1024)
-def _moved_layout(what, q4, metas, B, Hk, budget):
+def _moved_layout(what, q4, metas, B, Hk, budget, write):
     """``(rows S, byte strides {b, head, row} and row bytes of the cache's tensors, strides of the
     weights, places that _check_apart has passed)`` of a cache and its weights, checked (calls of one
     shape are checked once)."""
@@ -139,7 +139,7 @@ def _moved_layout(what, q4, metas, B, Hk, budget):
                 raise ValueError(f"{what}: cache rows must be contiguous and 16-byte aligned")
             found += [2 * st[0], 2 * st[1], 2 * st[2]]
             nbytes.append(2 * D)
-    w_strides = _weights_layout(what, w_shape, w_stride, w_type, B, Hk)
+    w_strides = _weights_layout(what, w_shape, w_stride, w_type, B, Hk, write)
     if w_shape[2] != S:
         raise ValueError(f"{what}: weights must have the cache's {S} rows, not {w_shape[2]}")
     if budget > S:
@@ -235,7 +235,7 @@ def flash_cache_evict(
     _lib.check_device(what, dev, *tensors)
     _lib.no_grad_inputs(what, *tensors)
     metas = _metas(tensors)
-    S, strides, nbytes, w_strides, apart = _moved_layout(what, q4, metas, B, Hk, budget)
+    S, strides, nbytes, w_strides, apart = _moved_layout(what, q4, metas, B, Hk, budget, out is None)
     at = [t.data_ptr() for t in tensors]
     _check_aligned(what, q4, nbytes, at)
     base = at[0]
@@ -245,7 +245,7 @@ def flash_cache_evict(
         places = tuple([a - base for a in at])
     else:
         to_metas, to_at = _metas(to), [t.data_ptr() for t in to]
-        S_out, to_strides, to_bytes, to_w_strides, _ = _moved_layout(what, q4, to_metas, B, Hk, budget)
+        S_out, to_strides, to_bytes, to_w_strides, _ = _moved_layout(what, q4, to_metas, B, Hk, budget, True)
         _check_aligned(what, q4, to_bytes, to_at)
         places = to_metas, tuple([a - base for a in (*at, *to_at)])
         if to_metas[0][2] != metas[0][2] or list(to_bytes) != list(nbytes):

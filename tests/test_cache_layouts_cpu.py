@@ -24,7 +24,7 @@ def test_scales_of_an_odd_number_of_groups_start_anywhere(D):
     assert S == 75 and args[2] == c.k_scales.data_ptr() and args[2] % 4 == 2
     at = [t.data_ptr() for t in c] + [64]
     w = torch.zeros(1, 1, 75)
-    _, _, nbytes, _, _ = cache_evict._moved_layout("evict", True, cache_evict._metas((*c, w)), 1, 1, 10)
+    _, _, nbytes, _, _ = cache_evict._moved_layout("evict", True, cache_evict._metas((*c, w)), 1, 1, 10, True)
     cache_evict._check_aligned("evict", True, nbytes, at)
 
 
@@ -43,7 +43,7 @@ def test_scales_that_are_read_by_pairs_start_at_pairs(D):
     for bad in (c._replace(k_scales=scales), c._replace(v_scales=scales), c._replace(k_codes=codes), c._replace(v_codes=codes)):
         with pytest.raises(ValueError, match="aligned"):
             q4_cache.q4_args("cache", bad, 1, 1, D, CPU)
-        _, _, nbytes, _, _ = cache_evict._moved_layout("evict", True, cache_evict._metas((*bad, w)), 1, 1, 2)
+        _, _, nbytes, _, _ = cache_evict._moved_layout("evict", True, cache_evict._metas((*bad, w)), 1, 1, 2, True)
         with pytest.raises(ValueError, match="aligned"):
             cache_evict._check_aligned("evict", True, nbytes, [t.data_ptr() for t in (*bad, w)])
 
@@ -124,3 +124,12 @@ def test_requests_that_lie_between_each_other(D):
     a[4] += 4 * Hk * S  # the weights of one request in the next one's codes
     with pytest.raises(ValueError, match="weights overlap"):
         cache_evict._check_apart("evict", True, metas, metas, a, a, True)
+
+
+def test_weights_that_are_read_may_be_shared():
+    """By heads, for instance, of an eviction into another cache; where they are written they may not."""
+    c, w = fta.flash_q4_cache(3, 16, 2, 64, "cpu"), torch.zeros(3, 1, 16).expand(3, 2, 16)
+    layout = cache_evict._moved_layout("evict", True, cache_evict._metas((*c, w)), 3, 2, 5, False)
+    assert list(layout[3]) == [16, 0]
+    with pytest.raises(ValueError, match="share memory"):
+        cache_evict._moved_layout("evict", True, cache_evict._metas((*c, w)), 3, 2, 5, True)

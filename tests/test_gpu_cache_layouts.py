@@ -123,3 +123,26 @@ def test_requests_that_lie_between_each_other(gpu, q4):
     got2, want2 = (fta.flash_cache_evict(c, w, lens, 30, 8, 2) for c, w in (mine, own))
     for a, b in zip((*got, *got2, *mine[0], mine[1], *to[0], to[1]), (*want, *want2, *own[0], own[1], *own_to[0], own_to[1])):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("q4", [False, True], ids=["16bit", "4bit"])
+def test_an_eviction_reads_what_requests_and_heads_share(gpu, q4):
+    """Into another cache: one prompt's cache for every request, one row of weights for every head."""
+    import flash_topk_attn_v2 as fta
+
+    B, Hk, D, S = 3, 2, 96, 150
+    one = Q.cache(1, S, Hk, D, gpu, 3) if q4 else tuple(rand((1, S, Hk * D), 3 + i, BF, gpu) for i in (0, 1))
+    w = torch.rand(B, 1, S, device=gpu).expand(B, Hk, S)
+    lens = torch.tensor([150, 99, 20], dtype=torch.int32, device=gpu)
+    kind = (lambda t: fta.Q4Cache(*t)) if q4 else tuple
+    shared = kind([t.expand(B, *t.shape[1:]) for t in one])
+    done = []
+    for c, x in ((shared, w), (kind([t.contiguous() for t in shared]), w.contiguous())):
+        to = Q.cache(B, 70, Hk, D, gpu, 5) if q4 else tuple(rand((B, 70, Hk * D), 7 + i, BF, gpu) for i in (0, 1))
+        to = to, torch.ones(B, Hk, 70, device=gpu)
+        done.append((*fta.flash_cache_evict(c, x, lens, 60, 8, 2, out=to), *to[0], to[1]))
+    for a, b in zip(*done):
+        assert torch.equal(a, b)
+    for bad in (dict(cache=shared, weights=w.contiguous()), dict(cache=kind([t.contiguous() for t in shared]), weights=w)):
+        with pytest.raises(ValueError, match="share memory"):
+            fta.flash_cache_evict(**bad, cache_lens=lens, budget=60)
