@@ -75,10 +75,12 @@ def _warn_of_short_tables(what, P, S, offset):
 def offsets(what, position_offset, B, device, P, S):
     """``(offset for all, offset of each request or None)`` of an append, checked."""
     if isinstance(position_offset, torch.Tensor) and position_offset.ndim > 0:
-        if position_offset.dtype != torch.int32 or position_offset.shape != (B,):
+        each = position_offset.dtype == torch.int32 and position_offset.ndim == 1
+        if each and position_offset.shape == (B,) and (B > 1 or position_offset.device == device):
+            _lib.check_device(what, device, position_offset)
+            return 0, position_offset.contiguous()
+        if position_offset.numel() != 1 or (each and B > 1):  # any other tensor of one element is a number
             raise ValueError(f"{what}: position_offset must be a whole number or int32 [B] = [{B}]")
-        _lib.check_device(what, device, position_offset)
-        return 0, position_offset.contiguous()
     position_offset = _lib.whole(what, position_offset)
     if not -(1 << 31) <= position_offset < (1 << 31):
         raise ValueError(f"{what}: position_offset out of range")
