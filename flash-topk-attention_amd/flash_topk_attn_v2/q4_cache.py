@@ -140,7 +140,9 @@ def flash_qk_norm_rope_append_q4(
     negative; rounded to float16, at most 65504 in magnitude), a column's code
     ``round(x / scale) + 8``, ties to even, held to 0 .. 15.  A column is off by at most half
     a scale, a sixteenth of its group's largest magnitude, but for values near the largest
-    one's opposite, which are off by up to a whole scale.  Groups of magnitudes below 2.4e-7
+    one's opposite, which are off by up to a whole scale and a 256th of it.  Where the largest
+    magnitude is below 2^-11 (4.9e-4) the scale is a subnormal float16, off by up to 2^-25
+    itself, and a column by up to 2^-22 (2.4e-7) more; groups of magnitudes up to 2^-22
     are held as zeros.  Values must be finite: infinities and NaN leave finite
     values of no meaning in their group.  Other arguments as for ``flash_qk_norm_rope_append``.  Not
     differentiable.
