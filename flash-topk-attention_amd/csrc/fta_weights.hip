@@ -360,9 +360,6 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
     if (it0 + wave < it1) ask(it0 + wave, cur);
     fta_wait_vmcnt<0>();
     __syncthreads();
-    uint32_t nans = 0;
-    for (int ch = 0; ch < a.chunks; ++ch) nans |= sNan[ch];
-    nans = fta_scalar((int)nans);
     for (int it = it0 + wave; it < it1; it += NW) {
         if (it + NW < it1) ask(it + NW, nxt);
         fta_frag kf[KS];
@@ -373,11 +370,16 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
         for (int cg = 0, ch = 0; cg < a.groups; ++cg)
             for (int ct = 0; ct < nct; ++ct, ++ch) sum += chunk_sum<DT, KD, Q4>(a, kf, ds, ldq + ch * TILE_B, sL[ch], ct, kt, len, lane);
         sum += fta_xor32(sum);
-        if (nans != 0)
-            for (int ch = 0; ch < a.chunks; ++ch)
-                if (sNan[ch] & rows_that_see(a, len - a.T + ch % nct * a.TT, key)) sum = __builtin_nanf("");
         if (lane < 32 && key < len) wp[key] = cur.before + sum;
         cur = nxt;
+    }
+    for (int ch = 0; ch < a.chunks; ++ch) {
+        const uint32_t n = fta_scalar((int)sNan[ch]);
+        if (n == 0) continue;
+        for (int it = it0 + wave; it < it1; it += NW) {
+            const int key = tile(it) + (lane & 31);
+            if (lane < 32 && key < len && (n & rows_that_see(a, len - a.T + ch % nct * a.TT, key))) wp[key] = __builtin_nanf("");
+        }
     }
 }
 
