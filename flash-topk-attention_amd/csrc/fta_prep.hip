@@ -275,10 +275,11 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
 // Append to a 4-bit cache: the forward's tiling, K and V quantized.  K is rounded to its 16-bit type
 // first, so that a cache holds the same whether its rows came prepared or not.  The groups of a part
 // are of one kind (queries, keys, values) but where the kinds meet, and each kind has its own body.
-// What bounds it: vector instructions, 190 a group of four rows and 69% of the cycles (32768 tokens, 32 / 8
-// heads of 128: 198 us, 708 MB).  One body for any row 227 us; held to four waves a SIMD 198, three 206;
-// through the caches 209; rows at 32-bit offsets 264 (more registers than there are); the queries by the
-// forward's kernel and the rest by this one 121 + 84; one group at a time with the next one asked for ahead 373.
+// What bounds it: vector instructions, 190 a group of four rows; they take 63% of the cycles, 72% of those in which a CU
+// has waves (32768 tokens, 32 / 8 heads of 128: 184 to 192 us, 708 MB).  One body for any row 227 us.  Held to four waves
+// a SIMD 198 (128 vector registers, of which five groups spill 8 or 9; 67 scalar ones go to lanes), to three, with no vector register
+// spilled, 206; through the caches 209; rows at 32-bit offsets 264 (more registers than there are); the queries by
+// the forward's kernel and the rest by this one 121 + 84; one group at a time with the next one asked for ahead 373.
 // ----------------------------------------------------------------------------
 
 // x of lane ^ 1, ^ 2, and of lanes that hold the other halves of 8 and of 16 (equal within 4 and 8).
@@ -702,13 +703,20 @@ int launch_fwd(PrepArgs& a, int B, hipStream_t st) {
     });
 }
 
+// One group a wave for as many waves as run at once (four a SIMD), five for more.  One / five, us of the kernel: 32 / 8
+// heads of 128, 16 tokens 5.2 / 7.3, 256 6.0 / 7.9, 512 (6144 groups) 9.5 / 9.0, 1000 13.9 / 11.2, 2000 22.3 / 19.0,
+// 8000 67.9 / 49.3; 8 / 8 heads of 64, 1000 tokens (3000 groups) 6.2 / 7.0, 2000 9.2 / 8.1; 12 / 4 of 80, 512
+// tokens (2560) 6.0 / 7.7, 1000 (5000) 8.3 / 8.1, 4000 20.2 / 12.4; 16 / 2 of 256, 256 tokens (2560) 5.9 / 7.8, 512
+// (5120) 8.7 / 8.3, 2000 21.2 / 15.0.
+constexpr int kQ4Few = 4 * 1024;
+
 template <int DT>
 int launch_append_q4(PrepArgs& a, int B, hipStream_t st) {
     const int rows = a.H + 2 * a.Hk;
     return with_lanes(std::max(a.D, 32), [&](auto lg) {
         constexpr int LG = decltype(lg)::value < 4 ? 4 : decltype(lg)::value;
         set_units(a, B, 1, rows, LG);
-        const bool few = a.units <= 4 * kFwdGrid;
+        const bool few = a.units <= kQ4Few;
         if (!few) set_units(a, B, kFwdGroups, rows, LG);
         const dim3 g(grid_of(a.units, kFwdGrid)), t(256);
         if (few)
