@@ -67,7 +67,7 @@ struct Q4Shape {
     static constexpr int OROW = 32 * NG + 4;
     static constexpr int MERGE_B = NW * ROWS * OROW * 4, ML_B = NW * ROWS * 8;
     static constexpr int LDS_B = NW * STAGE_B > MERGE_B + ML_B ? NW * STAGE_B : MERGE_B + ML_B;
-    // waves per SIMD that LDS and registers leave room for
+    // waves per SIMD that LDS leaves room for, and registers but for eight groups: they want more than 256, and spill 16
     static constexpr int WAVES = NG <= 2 ? 4 : NG <= 4 ? 3 : 2;
     // A row's 16-byte slots are exchanged by row so that the reads of 16 rows (one slot each) spread
     // over the banks: transpose reads take rows 16 q + e of the values, operand reads rows
@@ -103,16 +103,20 @@ struct Q4Shape {
 //   16 keys whose value codes one transpose read gives lane (c, q) for its column c.
 // The codes enter as 16 + n; -24 sum_{c in g} q_c is the key products' first addend, and every value
 // product is followed by one of the same p d with -24 in every column.
-// bf16: p d is rounded to bf16 as P is in the 16-bit kernels.  fp16: it would leave fp16's range for
-// the scales that caches hold, so it goes as two bf16 numbers, hi + lo, 16 bits of it.
+// bf16: p d is rounded to bf16 as P is in the 16-bit kernels; o is off by 0.0023 of itself (root mean square) where
+// its own rounding alone is 0.0017.  fp16: it would leave fp16's range for the scales that caches hold, so it goes
+// as two bf16 numbers, hi + lo, 16 bits of it, which takes about a tenth of the time for what bf16 could not hold.
 // A wave has one stage for a tile's key codes and one for its value codes: the next tile's keys are
 // asked for before this one's values are multiplied, the next values after it.  Three waves per
 // SIMD cover the rest of the wait.
 // What bounds it: memory where there are many requests.  128 of 4096 to 8192 tokens, 32 / 8 heads of 128,
-// bf16: 183 us, 906 MB, 5.0 TB/s (a large copy 5.1); with two stages each and two waves per SIMD 245.
-// 64 requests: bf16 108 us, fp16, whose values take twice the products, 118.  One request of 4096: 8 us, the
+// bf16: 185 us, 906 MB, 5.0 TB/s (a large copy 5.1); with two stages each and two waves per SIMD 245.
+// 64 requests: bf16 98 to 109 us, fp16, whose values take twice the products, 114 to 122.  One request of 4096: 9.5 us, the
 // latency of a wave's start, its one tile and the merge.  Four requests of a window of 2000, three tokens each,
-// 16 / 2 heads of 256, fp16: 23 us, latency again.
+// 16 / 2 heads of 256, fp16: 24 us, latency again (a wave's one tile is 2480 vector and 167 matrix instructions).
+// Many tokens: vector and matrix instructions, since each 16 rows unpack their keys and values anew and half of the
+// value products take the 24 off again.  One request, 32 / 8 heads of 128, a call, bf16 / fp16: 128 tokens on 8192 73 / 85
+// us, 512 on 8192 201 / 251, a prompt of 2048 140 / 165, of 8192 1252 / 1621 (window attention of 16-bit rows: 68 and 556).
 // ----------------------------------------------------------------------------
 template <int DT, int NG>
 __global__ __launch_bounds__(256, Q4Shape<NG>::WAVES) void fta_q4_attn_kernel(Q4Args A) {

@@ -6,8 +6,9 @@
 // length for a prompt; keys are 16-bit rows or rows of a 4-bit cache (see fta_q4.hip).
 //
 // S = Q K^T with the keys as columns: a wave keeps 32 keys in registers, one to a lane and its
-// mirror, and walks over all the rows that see them, 32 at a time; a key's sum stays in its lane.
-// So a key is read once, no sum crosses lanes, and there are no atomics (the same bits every run).
+// mirror, and walks over all the rows that see them, 32 at a time; a key's terms stay in these lanes, two
+// (of few rows, four), whose sums are added in a fixed order at the end of a walk or tile.
+// So a key is read once and there are no atomics (the same bits every run).
 // Many rows come through LDS, shared by the four waves: TT tokens x GG query heads of the group,
 // as many heads as it takes to fill 32 rows where there are few tokens.
 #include "fta_common.h"
@@ -168,11 +169,14 @@ __device__ __forceinline__ float chunk_sum(const WeighArgs& a, const fta_frag (&
 // ----------------------------------------------------------------------------
 // Many rows.  KD: columns (16-bit keys: 64, 128 or 256; 4-bit keys: 32 per group).
 // What bounds it: matrix and vector instructions (of these the 16 exp2 of a tile most), at a clock that
-// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 334 to 364 us by run, 797 TFLOP/s at 2.0 GHz, the
-// matrix units busy 39% of the cycles, the vector units 57%.  Four stages with all of a part's lse loaded
-// ahead (367 beside 360), two key tiles a wave (411), and the last chunk's exp2 between this one's products
-// (357 to 374) gained nothing: what overlaps more runs at a lower clock.  The weights so far
-// loaded with the keys instead of at the end changed nothing.
+// their power lowers.  A prompt of 8192 tokens, 32 / 8 heads of 128: 334 to 364 us by run, 750 to 820 TFLOP/s at 2.0 GHz, the
+// matrix units busy 36% of the cycles, the vector units 56%: 104% together of the cycles in which a CU has waves,
+// so they hardly overlap.  Four stages with all of a part's lse loaded ahead (367 beside 360), two key tiles a
+// wave (411), and the last chunk's exp2 between this one's products (357 to 374) gained nothing: what overlaps
+// more runs at a lower clock.  The weights so far loaded with the keys instead of at the end changed nothing.
+// 4-bit keys are expanded once for a walk, and every group's product is scaled by itself: 64 more multiply-adds a tile
+// at 128 columns, 456 us for the same prompt; 4096 tokens, 16 / 4 heads of 256, 318 us beside 130 on 16-bit keys (256
+// registers, 9 more spilled).
 // ----------------------------------------------------------------------------
 template <int DT, int KD, bool Q4>
 __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache_weights_kernel(WeighArgs a) {
@@ -297,8 +301,9 @@ __global__ __launch_bounds__(kWeighWaves * 64, KD <= 128 ? 3 : 2) void fta_cache
 // Rows that stay in LDS, up to kHeld chunks of 32: the last tokens of a prompt, or several tokens of a step. They are
 // loaded once, and the keys stream past: a workgroup takes a run of keys, its waves 32-key tiles in turn, the
 // next tile's asked for ahead.
-// What bounds it: memory for 16-bit keys (64 requests x 12 tokens on 4096 to 8192, 32 / 8 heads of 128: 196 us, 4.2
-// TB/s), vector instructions for 4-bit ones (156 us).  The kernel of many rows, which starts anew for every 128
+// What bounds it: memory for 16-bit keys (64 requests x 12 tokens on 4096 to 8192, 32 / 8 heads of 128: 190 to 207 us, 4.2
+// TB/s), vector instructions for 4-bit ones (153 to 161 us; more than a third of them turn codes into 16-bit numbers
+// one by one; at 256 columns 45 registers are spilled).  The kernel of many rows, which starts anew for every 128
 // keys, takes 216 and 273; 2 x 32 tokens on up to 32768 4-bit keys, 16 / 4 heads of 64, 17.5 and 19.5.  Eight chunks,
 // which leave two waves a SIMD at 128 columns, are slower than it: 64 tokens, 40 us and 32.
 // ----------------------------------------------------------------------------
@@ -389,7 +394,9 @@ __global__ __launch_bounds__(256, KD <= 128 ? 3 : 2) void fta_cache_weights_rows
 // S = Q K^T: lane (k, q) = (l & 15, l >> 4) holds rows 4 q + i of its key k.  4-bit keys enter as 16 + n,
 // after a product of the rows with -24 (see fta_q4.hip).
 // What bounds it: memory.  64 requests of 4096 to 8192 tokens, 32 / 8 heads of 128: 154 us, 5.4 TB/s; with 4-bit keys
-// 66 us, 3.4 TB/s, where vector instructions weigh as much.
+// 61 to 68 us, 3.4 TB/s, where vector instructions weigh as much.  Two tiles of rows: 64 requests x 8 tokens 207 us, with
+// 4-bit keys 117 (12 registers spilled); 32 x 8 tokens, 16 / 4 heads of 256 in 4 bits, 176 (68 spilled; 35 at 224
+// columns).
 // ----------------------------------------------------------------------------
 template <int KD, bool Q4>
 struct KeyTile {  // 32 keys as B operands: of keys 16 t + k, this lane's words
@@ -548,6 +555,10 @@ int weigh_plan(WeighArgs& a, bool q4, int B, int H, int Hk, int T, int S, int D,
     a.B = B, a.T = T, a.H = H, a.Hk = Hk, a.G = H / Hk, a.S = S, a.Dreal = D;
     a.left = std::min(left, S);
     a.sinks = a.left >= S - 1 ? 0 : std::min(sinks, S);
+    // Heads x tokens of a chunk, so that rows and the mask are a division by GG away.  T = 17 .. 31 leaves up to 15 of
+    // 32 rows unused, T = 33 gives every head a second chunk of one token, and such rows may take the kernel of many where
+    // as many others are held: 16 requests of 4096 to 8192 tokens, four K/V heads of 128, 32 tokens x 4 heads (held) 41 us,
+    // 20 x 5 53, 33 x 3 57.
     a.GG = std::min(a.G, std::max(1, 32 / std::min(T, 32)));
     a.TT = 32 / a.GG;
     a.groups = (a.G + a.GG - 1) / a.GG;
