@@ -226,7 +226,8 @@ def flash_window_attn_decode_q4(
     keys a token sees, rows that see nothing (o = 0, lse = -inf) and unseen rows (which may
     hold anything) as there.  The codes are multiplied as they stand, scales are applied
     in float32; probabilities times the values' scales are rounded to 8 bits of mantissa in
-    bfloat16, to 16 in float16.  Not differentiable.
+    bfloat16, to 16 in float16.  Made for few new tokens: from about 128 on,
+    ``flash_q4_cache_read`` and a 16-bit attention take less time.  Not differentiable.
 
     Returns ``(output [B, T, num_heads * D], lse [B, num_heads, T] float32)``.
     """

@@ -5,6 +5,7 @@ import torch
 
 import _operators_ref as R
 import _q4_ref as Q
+import test_gpu_evict as E
 from _helpers import rand, say
 
 pytestmark = pytest.mark.gpu
@@ -47,3 +48,28 @@ def test_a_prompt_in_parts(gpu):
         o, lse = fta.flash_window_attn_decode_q4(q[:, t:t + P], c, ln, H, N, num_kv_heads=Hk)
         part = {n: (x[..., t:t + P] if n.startswith("lse") else x[:, t:t + P]) for n, x in ref.items()}
         R.check({"o": o, "lse": lse}, part, ("o", "lse"), f"part {t}")
+
+
+@pytest.mark.parametrize("dtype", [BF, FP], ids=["bf16", "fp16"])
+def test_a_prompt_over_the_rows_read_back(gpu, dtype):
+    """A prompt into a 4-bit cache, its attention over what the cache gives back in 16 bits, and the weights of the 4-bit
+    keys by that attention's lse; a part of a prompt by the cache attention."""
+    import flash_topk_attn_v2 as fta
+
+    B, T, H, Hk, D, left = 2, 300, 8, 2, 64, 120
+    say("read back", dtype)
+    q, k, v = (rand((B, T, h * D), 3 + i, dtype, gpu) for i, h in enumerate((H, Hk, Hk)))
+    c = fta.flash_q4_cache(B, T, Hk, D, gpu)
+    lens = torch.full((B,), T, dtype=torch.int32, device=gpu)
+    ang = torch.arange(T, dtype=torch.float64)[:, None] * 10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))
+    q = fta.flash_qk_norm_rope_append_q4(q, k, v, c, lens, H, ang.cos().float().to(gpu), ang.sin().float().to(gpu), num_kv_heads=Hk)
+    k16, v16 = fta.flash_q4_cache_read(c, D, dtype)
+    o, lse = fta.flash_window_attn(q, k16, v16, H, (left, 0), num_kv_heads=Hk)
+    R.check({"o": o, "lse": lse}, R.cache(q, k16, v16, [T] * B, H, Hk, left, 0, D ** -0.5), ("o", "lse"))
+    part = torch.tensor([200, 300], dtype=torch.int32, device=gpu)
+    got = fta.flash_window_attn_decode(q[:, 150:200], k16, v16, part, H, left, num_kv_heads=Hk)
+    R.check(dict(zip(("o", "lse"), got)), R.cache(q[:, 150:200], k16, v16, part.tolist(), H, Hk, left, 0, D ** -0.5), ("o", "lse"))
+    w = fta.flash_cache_weights(q, c, lse, lens, torch.zeros(B, Hk, T, device=gpu), H, left, num_kv_heads=Hk)
+    keys = Q.values(c.k_codes, c.k_scales, True, D)[0]
+    want, tol = E._weights(q, keys, lse, [T] * B, H, Hk, left, 0, D ** -0.5)
+    assert ((w.double() - want).abs() <= tol + 2.0 ** -23 * w.double()).all()
