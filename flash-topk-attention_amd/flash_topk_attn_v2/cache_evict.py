@@ -255,6 +255,7 @@ def flash_cache_evict(
         if len(apart) >= 1024:
             apart.clear()
         apart.add(places)
+    _lib.check_apart(what, "weights", to[-1], cache_lens)
     n = len(cache)
     lens = cache_lens.contiguous()
     new_lens = torch.empty(B, device=dev, dtype=torch.int32)

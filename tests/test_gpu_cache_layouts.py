@@ -146,3 +146,27 @@ def test_an_eviction_reads_what_requests_and_heads_share(gpu, q4):
     for bad in (dict(cache=shared, weights=w.contiguous()), dict(cache=kind([t.contiguous() for t in shared]), weights=w)):
         with pytest.raises(ValueError, match="share memory"):
             fta.flash_cache_evict(**bad, cache_lens=lens, budget=60)
+
+
+@pytest.mark.parametrize("out", [False, True], ids=["in_place", "out"])
+def test_an_eviction_whose_weights_hold_the_lengths_is_refused(gpu, out):
+    """The lengths are read while weights are written."""
+    import flash_topk_attn_v2 as fta
+
+    B, Hk, D, S = 2, 2, 64, 40
+    cache, other = (tuple(rand((B, S, Hk * D), 2 * i + j, BF, gpu) for j in (0, 1)) for i in (0, 1))
+    w, free = torch.rand(B, Hk, S, device=gpu), torch.rand(B, Hk, S, device=gpu)
+    held = [x.clone() for x in (*cache, w)]
+    lens = w.view(torch.int32)[1, 1, 5:5 + B]
+    with pytest.raises(ValueError, match="overlap"):
+        fta.flash_cache_evict(cache, free if out else w, lens, 10, out=(other, w) if out else None)
+    assert all(torch.equal(x, y) for x, y in zip(held, (*cache, w)))
+    # lengths between the rows of weights
+    wide = torch.zeros(B, Hk, S + 8, device=gpu)
+    lens = wide.view(torch.int32)[0, 0, S:S + B]
+    lens.copy_(torch.tensor([40, 33], dtype=torch.int32))
+    part = wide[:, :, :S]
+    part.copy_(w)
+    got = fta.flash_cache_evict(cache, part, lens, 10)
+    want = fta.flash_cache_evict(tuple(x.clone() for x in held[:2]), w, torch.tensor([40, 33], dtype=torch.int32, device=gpu), 10)
+    assert torch.equal(got[1], want[1]) and torch.equal(part, w) and lens.tolist() == [40, 33]
