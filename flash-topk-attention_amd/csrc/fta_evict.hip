@@ -249,13 +249,13 @@ __global__ __launch_bounds__(256) void fta_evict_select_wave_kernel(EvictArgs a)
 // ----------------------------------------------------------------------------
 // The move: workgroup = (b, K/V head, slice) in place, (b, K/V head, slice, block of rows) into
 // another cache.  A thread moves one access of a row, kMove rows at a time.
-// What bounds it: memory, and in place for few heads the latency of its blocks, which follow each
-// other.  16 x 8 heads of 128 bf16, 8192 rows to 4096: 146 to 152 us in place, 118 into another cache
-// (537 MB: 3.5 to 3.7 and 4.6 TB/s); 64 x 8 heads of 128 in 4 bits, 16384 to 4096: 176 to 180 us (604 MB; single rows of 64 and 8
-// bytes out of 128-byte lines); 1 x 8 heads, 32768 to 8192: 34 us.  In place, of one run, 146 / 176 / 35 us,
-// with 512 threads instead of 1024 152 / 184 / 42, with eight rows a thread 174 / 194 / 39.  Where few rows stay most of 1024 threads have
-// none, and 256 move them: 346 rows of 64 x 8 heads bf16 45 -> 27 us, 345 rows of 101 x 4 heads in 4 bits 26 -> 11, 1024
-// rows of 128 x 8 in 4 bits 100 -> 75; but of 8 heads 1024 rows 6.8 -> 11.5, 4096 of 16 x 8 155 -> 171.
+// What bounds it: memory, and in place for few heads the latency of its blocks, which follow each other.  16 x 8
+// heads of 128 bf16, 8192 rows to 4096: 146 to 152 us in place, 118 into another cache (537 MB: 3.5 to 3.7 and 4.6
+// TB/s); 64 x 8 heads of 128 in 4 bits, 16384 to 4096: 176 to 180 us (604 MB; single rows of 64 and 8 bytes out of
+// 128-byte lines); 1 x 8 heads, 32768 to 8192: 34 us.  In place, of one run, 146 / 176 / 35 us, with 512 threads
+// instead of 1024 152 / 184 / 42, with eight rows a thread 174 / 194 / 39.  Where few rows stay most of 1024 threads
+// have none, and 256 move them: 346 rows of 64 x 8 heads bf16 45 -> 27 us, 345 rows of 101 x 4 heads in 4 bits 26 ->
+// 11, 1024 rows of 128 x 8 in 4 bits 100 -> 75; but of 8 heads 1024 rows 6.8 -> 11.5, 4096 of 16 x 8 155 -> 171.
 // ----------------------------------------------------------------------------
 constexpr int kMove = 4;
 // Bytes of a row that one workgroup moves: the fewest that memory reads at once.  32 / 64 / 128 / 256, us of

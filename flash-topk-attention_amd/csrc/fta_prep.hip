@@ -275,11 +275,12 @@ __global__ __launch_bounds__(256) void fta_norm_rope_fwd_kernel(PrepArgs a) {
 // Append to a 4-bit cache: the forward's tiling, K and V quantized.  K is rounded to its 16-bit type
 // first, so that a cache holds the same whether its rows came prepared or not.  The groups of a part
 // are of one kind (queries, keys, values) but where the kinds meet, and each kind has its own body.
-// What bounds it: vector instructions, 190 a group of four rows; they take 63% of the cycles, 72% of those in which a CU
-// has waves (32768 tokens, 32 / 8 heads of 128: 184 to 192 us, 708 MB).  One body for any row 227 us.  Held to four waves
-// a SIMD 198 (128 vector registers, of which five groups spill 8 or 9; 67 scalar ones go to lanes), to three, with no vector register
-// spilled, 206; through the caches 209; rows at 32-bit offsets 264 (more registers than there are); the queries by
-// the forward's kernel and the rest by this one 121 + 84; one group at a time with the next one asked for ahead 373.
+// What bounds it: vector instructions, 190 a group of four rows; they take 63% of the cycles, 72% of those in which a
+// CU has waves (32768 tokens, 32 / 8 heads of 128: 184 to 192 us, 708 MB).  One body for any row 227 us.  Held to
+// four waves a SIMD 198 (128 vector registers, of which five groups spill 8 or 9; 67 scalar ones go to lanes), to
+// three, with no vector register spilled, 206; through the caches 209; rows at 32-bit offsets 264 (more registers
+// than there are); the queries by the forward's kernel and the rest by this one 121 + 84; one group at a time with
+// the next one asked for ahead 373.
 // ----------------------------------------------------------------------------
 
 // x of lane ^ 1, ^ 2, and of lanes that hold the other halves of 8 and of 16 (equal within 4 and 8).
